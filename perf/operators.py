@@ -251,7 +251,7 @@ def _own_distill(s, case):
     from myflows_amd import logits as ops
     r = ops.distill_loss_forward(s["logits"], s["ids"], s["teacher"], temperature=case["temperature"],
                                  row_weights=s["weights"])
-    grad = ops.distill_loss_backward(s["logits"], s["ids"], s["teacher"], r, s["seed"], temperature=case["temperature"])
+    grad = ops.distill_loss_backward(s["logits"], s["ids"], r, s["seed"], temperature=case["temperature"])
     return {"loss": r.loss, "row_loss": r.row_loss, "grad": grad}
 
 
