@@ -512,6 +512,86 @@ typedef struct mfh_adam_tensor {
 MFH_API int mfh_adam_step(const mfh_adam_tensor* tensors, int count, float grad_scale, float beta1,
                           float one_minus_beta1, float beta2, float one_minus_beta2, float eps, uint64_t stream);
 
+/* ---- rows of logits -------------------------------------------------------------------------- */
+
+/* Element types of the calls below that take more than float: 0 float32, 1 bfloat16, 2 float16. `logits`
+ * holds `rows` rows of `vocab` contiguous elements, row_stride elements apart (offsets between rows are 64
+ * bits; at most 2^22 rows of at most 2^24 logits). Tokens and ids are int32, or int64 with their flag; a
+ * negative one is none. No counterpart in the reference, whose only loss is the mean squared error. */
+
+/* Bytes of workspace of mfh_log_probs (0: none), -1 when the sizes are out of range. */
+MFH_API int64_t mfh_log_probs_workspace(int64_t rows, int vocab, int type, int top);
+
+/* Per row, float32, with m = max z and s = sum e^(z - m):
+ *   log_sum = m + ln s; entropy = ln s - (1/s) sum e^(z - m) (z - m); log_prob = z[token] - log_sum (0 where
+ *   token < 0, NaN where token >= vocab; log_prob may be 0 with tokens then unused); stats (2 x rows) = m, s;
+ *   top_log_probs / top_ids (rows x top, top <= 64 and <= vocab): the largest logits in falling order, equal
+ *   ones in rising order of their ids.
+ * A logit of -inf has probability 0. A row of nothing else: log_sum, log_prob and the alternatives -inf,
+ * entropy 0. A NaN or +inf makes its row NaN; a NaN is no alternative (ids that are then missing are -1). */
+MFH_API int mfh_log_probs(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
+                          int tokens_int64, uint64_t log_prob, uint64_t entropy, uint64_t log_sum, uint64_t stats, int top,
+                          uint64_t top_log_probs, uint64_t top_ids, uint64_t workspace, int64_t workspace_bytes,
+                          uint64_t stream);
+
+/* grad[r][j] (grad_stride elements a row, of the logits' type) = g ([j = token] - p) - h p (ln p + entropy), or
+ * grad += that when add != 0, with g = scale * factor[0] * log_prob_grad[r * log_prob_grad_stride] (0 where
+ * token < 0) and h = factor[0] * entropy_grad[r * entropy_grad_stride]. factor (one float on the device, 1
+ * when 0), log_prob_grad and entropy_grad are optional; strides may be 0. stats and entropy are those of
+ * mfh_log_probs. A row whose g and h are 0 gets 0 whatever its logits hold. */
+MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
+                                   int tokens_int64, uint64_t stats, uint64_t entropy, uint64_t log_prob_grad,
+                                   int64_t log_prob_grad_stride, uint64_t entropy_grad, int64_t entropy_grad_stride,
+                                   uint64_t factor, float scale, uint64_t grad, int64_t grad_stride, int add,
+                                   uint64_t stream);
+
+/* Bytes of workspace of mfh_distill_loss (0: none), -1 when the sizes are out of range. */
+MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
+
+/* The distillation loss of a student's logits against a teacher's record of `held` (1..256) ids and float32
+ * logits a row: with p = softmax(teacher / temperature) over the ids >= 0 and q = softmax(logits / temperature),
+ *   row_loss = temperature^2 sum p (ln p - ln q[id]),  loss[0] = sum w row_loss / sum w,  loss[1] = 1 / sum w
+ * over the rows that count: w = row_weights[r] (optional, else 1), 0 without an id. A row that does not count
+ * has row_loss 0 whatever its logits hold; without any, loss is 0. An id >= vocab makes a counting row NaN.
+ * For the backward: weights (rows), stats (2 x rows) and targets (rows x held, p summed over equal ids). */
+MFH_API int mfh_distill_loss(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,
+                             int ids_int64, uint64_t teacher, int held, uint64_t row_weights, float temperature,
+                             uint64_t row_loss, uint64_t weights, uint64_t stats, uint64_t targets, uint64_t loss,
+                             uint64_t workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* grad[r][j] = seed[0] w loss[1] temperature (q[j] - sum over k of p[k] [ids[k] = j]), or grad += that. */
+MFH_API int mfh_distill_loss_backward(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,
+                                      int ids_int64, int held, uint64_t targets, uint64_t stats, uint64_t weights,
+                                      uint64_t loss, uint64_t seed, float temperature, uint64_t grad, int64_t grad_stride,
+                                      int add, uint64_t stream);
+
+/* out[0] = scale * mean of the values whose token is >= 0 (of all, when tokens is 0), out[1] = 1 / their
+ * number (both 0 without any): FP64 sums in a fixed order. */
+MFH_API int mfh_row_mean(uint64_t values, uint64_t tokens, int tokens_int64, int64_t rows, float scale, uint64_t out,
+                         uint64_t stream);
+
+/* ---- group norm ------------------------------------------------------------------------------ */
+
+/* Bytes of workspace of mfh_group_norm_forward (backward 0) or mfh_group_norm_backward (backward 1), -1 when
+ * the sizes are out of range (a sample of at most 2^31 - 1 elements, n * channels at most 2^23). */
+MFH_API int64_t mfh_group_norm_workspace(int64_t n, int positions, int channels, int groups, int type, int backward);
+
+/* Group norm over (positions, channels / groups) of each sample and group of a channels-last tensor
+ * (n, positions, channels) of an element type, with float32 gamma and beta (channels):
+ *   y = act(gamma (x - mean) inv_std + beta), inv_std = (biased variance + eps)^(-1/2)
+ * activation 0 none, 1 ReLU, 3 SiLU (u / (1 + e^-u)). mean and inv_std (n x groups, float32) are written.
+ * No counterpart in the reference, whose only norm is the batch norm. */
+MFH_API int mfh_group_norm_forward(uint64_t x, int type, int64_t n, int positions, int channels, int groups, uint64_t gamma,
+                                   uint64_t beta, int activation, float eps, uint64_t y, uint64_t mean, uint64_t inv_std,
+                                   uint64_t workspace, int64_t workspace_bytes, uint64_t stream);
+
+/* The gradients of mfh_group_norm_forward, each optional (0) and written, or added with its add flag: x_grad of
+ * x's type, gamma_grad and beta_grad float32. u is formed again from x, mean and inv_std. */
+MFH_API int mfh_group_norm_backward(uint64_t x, uint64_t dy, int type, int64_t n, int positions, int channels, int groups,
+                                    uint64_t gamma, uint64_t beta, uint64_t mean, uint64_t inv_std, int activation,
+                                    uint64_t x_grad, uint64_t gamma_grad, uint64_t beta_grad, int add_x, int add_gamma,
+                                    int add_beta, uint64_t workspace, int64_t workspace_bytes, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

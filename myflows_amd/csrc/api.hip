@@ -1,6 +1,7 @@
 // The C ABI of libmfhip (declared in include/mfhip.h): initialisation, error reporting, argument
 // validation, and the launch sequences behind each entry point. Invalid calls return status 2 with
 // a message naming the reason, before anything is launched.
+#include <cfloat>
 #include <chrono>
 #include <cstdio>
 #include <cstdlib>
@@ -9,6 +10,7 @@
 
 #include "../../include/mfhip.h"
 #include "common.h"
+#include "typed.h"
 
 namespace mfh {
 namespace {
@@ -98,6 +100,27 @@ int require_ready() {
     const hipError_t rc = hipGetDevice(&device);
     if (rc != hipSuccess) return MFH_FAIL(ERR_HIP, std::string("hipGetDevice: ") + hipGetErrorString(rc));
     if (device != s.device) return MFH_FAIL(ERR_DEVICE, "called on a different HIP device than the one mfh_init used");
+    return OK;
+}
+
+int require_rows(int type, std::int64_t rows, int vocab, std::int64_t row_stride) {
+    MFH_REQUIRE(type_valid(type), "unknown element type");
+    MFH_REQUIRE(rows >= 0 && rows <= LOGIT_ROWS_LIMIT, "rows out of range");
+    MFH_REQUIRE(vocab > 0 && vocab <= LOGIT_VOCAB_LIMIT, "vocabulary out of range");
+    MFH_REQUIRE(row_stride >= vocab, "rows of logits must not overlap");
+    return OK;
+}
+
+int require_group_norm(const GroupNormShape& s, int type, int activation) {
+    MFH_REQUIRE(type_valid(type), "unknown element type");
+    MFH_REQUIRE(s.n >= 0 && s.positions > 0 && s.channels > 0 && s.groups > 0, "group norm sizes must be positive");
+    MFH_REQUIRE(s.channels % s.groups == 0, "the channels must divide into the groups");
+    MFH_REQUIRE(static_cast<std::int64_t>(s.positions) * s.channels <= INDEX_LIMIT,
+                "a sample of the group norm exceeds int32 indexing");
+    MFH_REQUIRE(s.channels <= GROUP_NORM_CHANNELS_LIMIT && s.n <= INDEX_LIMIT && s.n * s.channels <= GROUP_NORM_COLUMNS_LIMIT,
+                "samples or channels of the group norm out of range");
+    MFH_REQUIRE(activation == ACT_NONE || activation == ACT_RELU || activation == ACT_SILU,
+                "unknown activation of the group norm");
     return OK;
 }
 
@@ -1141,6 +1164,162 @@ MFH_API int mfh_adam_step(const mfh_adam_tensor* tensors, int count, float grad_
     }
     const AdamScalars s{grad_scale, beta1, one_minus_beta1, beta2, one_minus_beta2, eps};
     return launch_adam(table.data(), count, s, as_stream(stream));
+}
+
+// ---- rows of logits ---------------------------------------------------------------------------
+MFH_API std::int64_t mfh_log_probs_workspace(std::int64_t rows, int vocab, int type, int top) {
+    if (require_rows(type, rows, vocab, vocab) != OK) return -1;
+    if (top < 0 || top > TOP_MAX || top > vocab) return MFH_FAIL(ERR_ARG, "number of alternatives out of range"), -1;
+    return log_probs_workspace(rows, vocab, type, top);
+}
+
+MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
+                          std::uint64_t tokens, int tokens_int64, std::uint64_t log_prob, std::uint64_t entropy,
+                          std::uint64_t log_sum, std::uint64_t stats, int top, std::uint64_t top_log_probs,
+                          std::uint64_t top_ids, std::uint64_t workspace, std::int64_t workspace_bytes,
+                          std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_rows(type, rows, vocab, row_stride));
+    MFH_REQUIRE(top >= 0 && top <= TOP_MAX && top <= vocab, "number of alternatives out of range");
+    MFH_REQUIRE(rows == 0 || (logits && entropy && log_sum && stats && (!log_prob || tokens) &&
+                              (top == 0 || (top_log_probs && top_ids))),
+                "log probabilities received a null buffer");
+    const std::int64_t bytes = log_probs_workspace(rows, vocab, type, top);
+    MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "log probabilities workspace too small");
+    LogProbsForward f{};
+    f.rows = rows, f.stride = row_stride, f.vocab = vocab, f.top = top;
+    f.tokens = as_ptr<const void>(tokens), f.tokens_wide = tokens_int64 != 0;
+    f.log_prob = as_ptr<float>(log_prob), f.entropy = as_ptr<float>(entropy), f.log_sum = as_ptr<float>(log_sum);
+    f.stats = as_ptr<float>(stats);
+    f.top_log_probs = as_ptr<float>(top_log_probs), f.top_ids = as_ptr<int>(top_ids);
+    f.workspace = as_ptr<void>(workspace);
+    return launch_log_probs(as_ptr<const void>(logits), type, f, as_stream(stream));
+}
+
+MFH_API int mfh_log_probs_backward(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
+                                   std::uint64_t tokens, int tokens_int64, std::uint64_t stats, std::uint64_t entropy,
+                                   std::uint64_t log_prob_grad, std::int64_t log_prob_grad_stride,
+                                   std::uint64_t entropy_grad, std::int64_t entropy_grad_stride, std::uint64_t factor,
+                                   float scale, std::uint64_t grad, std::int64_t grad_stride, int add,
+                                   std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_rows(type, rows, vocab, row_stride));
+    MFH_REQUIRE(grad_stride >= vocab, "rows of the gradient must not overlap");
+    MFH_REQUIRE(rows == 0 || (logits && stats && grad && (!log_prob_grad || tokens) && (!entropy_grad || entropy)),
+                "log probabilities backward received a null buffer");
+    LogProbsBackward b{};
+    b.rows = rows, b.stride = row_stride, b.grad_stride = grad_stride, b.vocab = vocab;
+    b.tokens = as_ptr<const void>(tokens), b.tokens_wide = tokens_int64 != 0;
+    b.stats = as_ptr<const float>(stats), b.entropy = as_ptr<const float>(entropy);
+    b.log_prob_grad = as_ptr<const float>(log_prob_grad), b.log_prob_step = log_prob_grad_stride;
+    b.entropy_grad = as_ptr<const float>(entropy_grad), b.entropy_step = entropy_grad_stride;
+    b.factor = as_ptr<const float>(factor), b.scale = scale, b.add = add != 0;
+    return launch_log_probs_backward(as_ptr<const void>(logits), as_ptr<void>(grad), type, b, as_stream(stream));
+}
+
+MFH_API std::int64_t mfh_distill_workspace(std::int64_t rows, int vocab, int type) {
+    if (require_rows(type, rows, vocab, vocab) != OK) return -1;
+    return distill_workspace(rows, vocab, type);
+}
+
+MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
+                             std::uint64_t ids, int ids_int64, std::uint64_t teacher, int held,
+                             std::uint64_t row_weights, float temperature, std::uint64_t row_loss, std::uint64_t weights,
+                             std::uint64_t stats, std::uint64_t targets, std::uint64_t loss, std::uint64_t workspace,
+                             std::int64_t workspace_bytes, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_rows(type, rows, vocab, row_stride));
+    MFH_REQUIRE(held > 0 && held <= DISTILL_HELD_MAX, "number of teacher logits a row out of range");
+    MFH_REQUIRE(temperature > 0.0f && temperature <= FLT_MAX, "the temperature must be positive and finite");
+    MFH_REQUIRE(loss && (rows == 0 || (logits && ids && teacher && row_loss && weights && stats && targets)),
+                "distillation loss received a null buffer");
+    const std::int64_t bytes = distill_workspace(rows, vocab, type);
+    MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "distillation loss workspace too small");
+    DistillForward f{};
+    f.rows = rows, f.stride = row_stride, f.vocab = vocab, f.held = held;
+    f.ids = as_ptr<const void>(ids), f.ids_wide = ids_int64 != 0;
+    f.teacher = as_ptr<const float>(teacher), f.row_weights = as_ptr<const float>(row_weights);
+    f.temperature = temperature;
+    f.row_loss = as_ptr<float>(row_loss), f.weights = as_ptr<float>(weights), f.stats = as_ptr<float>(stats);
+    f.targets = as_ptr<float>(targets), f.loss = as_ptr<float>(loss), f.workspace = as_ptr<void>(workspace);
+    return launch_distill(as_ptr<const void>(logits), type, f, as_stream(stream));
+}
+
+MFH_API int mfh_distill_loss_backward(std::uint64_t logits, int type, std::int64_t rows, int vocab,
+                                      std::int64_t row_stride, std::uint64_t ids, int ids_int64, int held,
+                                      std::uint64_t targets, std::uint64_t stats, std::uint64_t weights,
+                                      std::uint64_t loss, std::uint64_t seed, float temperature, std::uint64_t grad,
+                                      std::int64_t grad_stride, int add, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_rows(type, rows, vocab, row_stride));
+    MFH_REQUIRE(grad_stride >= vocab, "rows of the gradient must not overlap");
+    MFH_REQUIRE(held > 0 && held <= DISTILL_HELD_MAX, "number of teacher logits a row out of range");
+    MFH_REQUIRE(temperature > 0.0f && temperature <= FLT_MAX, "the temperature must be positive and finite");
+    MFH_REQUIRE(rows == 0 || (logits && ids && targets && stats && weights && loss && seed && grad),
+                "distillation loss backward received a null buffer");
+    DistillBackward b{};
+    b.rows = rows, b.stride = row_stride, b.grad_stride = grad_stride, b.vocab = vocab, b.held = held;
+    b.ids = as_ptr<const void>(ids), b.ids_wide = ids_int64 != 0;
+    b.targets = as_ptr<const float>(targets), b.stats = as_ptr<const float>(stats);
+    b.weights = as_ptr<const float>(weights), b.loss = as_ptr<const float>(loss), b.seed = as_ptr<const float>(seed);
+    b.temperature = temperature, b.add = add != 0;
+    return launch_distill_backward(as_ptr<const void>(logits), as_ptr<void>(grad), type, b, as_stream(stream));
+}
+
+MFH_API int mfh_row_mean(std::uint64_t values, std::uint64_t tokens, int tokens_int64, std::int64_t rows, float scale,
+                         std::uint64_t out, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_REQUIRE(rows >= 0, "rows out of range");
+    MFH_REQUIRE(out && (rows == 0 || values), "row mean received a null buffer");
+    return launch_row_mean(as_ptr<const float>(values), nullptr, as_ptr<const void>(tokens), tokens_int64 != 0, rows,
+                           scale, as_ptr<float>(out), as_stream(stream));
+}
+
+// ---- group norm -------------------------------------------------------------------------------
+MFH_API std::int64_t mfh_group_norm_workspace(std::int64_t n, int positions, int channels, int groups, int type,
+                                              int backward) {
+    const GroupNormShape s{n, positions, channels, groups};
+    if (require_group_norm(s, type, ACT_NONE) != OK) return -1;
+    return group_norm_workspace(s, type, backward != 0);
+}
+
+MFH_API int mfh_group_norm_forward(std::uint64_t x, int type, std::int64_t n, int positions, int channels, int groups,
+                                   std::uint64_t gamma, std::uint64_t beta, int activation, float eps, std::uint64_t y,
+                                   std::uint64_t mean, std::uint64_t inv_std, std::uint64_t workspace,
+                                   std::int64_t workspace_bytes, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    const GroupNormShape s{n, positions, channels, groups};
+    MFH_TRY(require_group_norm(s, type, activation));
+    MFH_REQUIRE(eps >= 0.0f, "eps must not be negative");
+    if (n == 0) return OK;
+    MFH_REQUIRE(x && gamma && beta && y && mean && inv_std, "group norm received a null buffer");
+    const std::int64_t bytes = group_norm_workspace(s, type, false);
+    MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "group norm workspace too small");
+    const GroupNormForward f{as_ptr<const float>(gamma), as_ptr<const float>(beta), activation, eps,
+                             as_ptr<float>(mean), as_ptr<float>(inv_std), as_ptr<void>(workspace)};
+    return launch_group_norm_forward(s, type, as_ptr<const void>(x), as_ptr<void>(y), f, as_stream(stream));
+}
+
+MFH_API int mfh_group_norm_backward(std::uint64_t x, std::uint64_t dy, int type, std::int64_t n, int positions,
+                                    int channels, int groups, std::uint64_t gamma, std::uint64_t beta,
+                                    std::uint64_t mean, std::uint64_t inv_std, int activation, std::uint64_t x_grad,
+                                    std::uint64_t gamma_grad, std::uint64_t beta_grad, int add_x, int add_gamma,
+                                    int add_beta, std::uint64_t workspace, std::int64_t workspace_bytes,
+                                    std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    const GroupNormShape s{n, positions, channels, groups};
+    MFH_TRY(require_group_norm(s, type, activation));
+    MFH_REQUIRE(gamma && beta && (n == 0 || (x && dy && mean && inv_std)), "group norm backward received a null buffer");
+    const std::int64_t bytes = group_norm_workspace(s, type, true);
+    MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "group norm workspace too small");
+    GroupNormBackward b{};
+    b.gamma = as_ptr<const float>(gamma), b.beta = as_ptr<const float>(beta);
+    b.mean = as_ptr<const float>(mean), b.inv_std = as_ptr<const float>(inv_std), b.act = activation;
+    b.gamma_grad = as_ptr<float>(gamma_grad), b.beta_grad = as_ptr<float>(beta_grad);
+    b.add_x = add_x != 0, b.add_gamma = add_gamma != 0, b.add_beta = add_beta != 0;
+    b.workspace = as_ptr<void>(workspace);
+    return launch_group_norm_backward(s, type, as_ptr<const void>(x), as_ptr<const void>(dy),
+                                      n == 0 ? nullptr : as_ptr<void>(x_grad), b, as_stream(stream));
 }
 
 }  // extern "C"

@@ -459,4 +459,121 @@ int launch_mse_grad(const float* pred, const float* target, const float* seed, f
 // out[j] = float(FP64 sum over r of src[r * cols + j])
 int launch_column_sums(const float* src, float* out, std::int64_t rows, std::int64_t cols, hipStream_t stream);
 
+// ---- logits.hip -----------------------------------------------------------------------------
+// Rows of `vocab` logits, `stride` elements apart; whole numbers (tokens, ids) are int32, or int64 with
+// their `wide` flag. A negative token or id is none.
+constexpr int TOP_MAX = 64;           // alternatives of a row
+constexpr int DISTILL_HELD_MAX = 256;  // teacher ids of a row
+constexpr std::int64_t LOGIT_ROWS_LIMIT = 1 << 22;  // rows of a call
+constexpr int LOGIT_VOCAB_LIMIT = 1 << 24;          // logits of a row
+
+struct LogProbsForward {
+    std::int64_t rows, stride;
+    int vocab, top;
+    const void* tokens;  // optional, with log_prob
+    int tokens_wide;
+    float* log_prob;
+    float* entropy;
+    float* log_sum;
+    float* stats;  // 2 x rows: the row's largest logit m and sum e^(z - m)
+    float* top_log_probs;  // rows x top, with top_ids
+    int* top_ids;
+    void* workspace;
+};
+std::int64_t log_probs_workspace(std::int64_t rows, int vocab, int type, int top);  // bytes
+int launch_log_probs(const void* logits, int type, const LogProbsForward& f, hipStream_t stream);
+
+struct LogProbsBackward {
+    std::int64_t rows, stride, grad_stride;
+    int vocab;
+    const void* tokens;
+    int tokens_wide;
+    const float* stats;
+    const float* entropy;
+    const float* log_prob_grad;  // optional; element r at r * log_prob_step
+    std::int64_t log_prob_step;
+    const float* entropy_grad;  // optional
+    std::int64_t entropy_step;
+    const float* factor;  // optional: one float that multiplies both
+    float scale;          // multiplies log_prob_grad
+    bool add;
+};
+int launch_log_probs_backward(const void* logits, void* grad, int type, const LogProbsBackward& b, hipStream_t stream);
+
+struct DistillForward {
+    std::int64_t rows, stride;
+    int vocab, held;
+    const void* ids;  // rows x held
+    int ids_wide;
+    const float* teacher;      // rows x held logits
+    const float* row_weights;  // optional
+    float temperature;
+    float* row_loss;
+    float* weights;  // the weights that count
+    float* stats;    // as LogProbsForward's, of z / temperature in m's units of z
+    float* targets;  // rows x held: the teacher's probability of each id, summed over its occurrences
+    float* loss;     // sum w row_loss / sum w, 1 / sum w
+    void* workspace;
+};
+std::int64_t distill_workspace(std::int64_t rows, int vocab, int type);  // bytes
+int launch_distill(const void* logits, int type, const DistillForward& f, hipStream_t stream);
+
+struct DistillBackward {
+    std::int64_t rows, stride, grad_stride;
+    int vocab, held;
+    const void* ids;
+    int ids_wide;
+    const float* targets;
+    const float* stats;
+    const float* weights;
+    const float* loss;
+    const float* seed;
+    float temperature;
+    bool add;
+};
+int launch_distill_backward(const void* logits, void* grad, int type, const DistillBackward& b, hipStream_t stream);
+
+// out[0] = scale * (weighted mean of values), out[1] = 1 / sum of the weights; both 0 when nothing counts.
+// A row's weight is weights[r], else whether tokens[r] >= 0, else 1.
+int launch_row_mean(const float* values, const float* weights, const void* tokens, int tokens_wide, std::int64_t rows,
+                    float scale, float* out, hipStream_t stream);
+
+// ---- group_norm.hip ---------------------------------------------------------------------------
+// Group norm over the (positions, channels / groups) of each (sample, group) of a channels-last tensor
+// (n, positions, channels), and an activation.
+constexpr int ACT_SILU = 3;
+constexpr int GROUP_NORM_CHANNELS_LIMIT = 1 << 16;
+constexpr std::int64_t GROUP_NORM_COLUMNS_LIMIT = 1 << 23;  // samples times channels
+struct GroupNormShape {
+    std::int64_t n;
+    int positions, channels, groups;
+};
+std::int64_t group_norm_workspace(const GroupNormShape& s, int type, bool backward);  // bytes
+
+struct GroupNormForward {
+    const float* gamma;
+    const float* beta;
+    int act;
+    float eps;
+    float* mean;  // n x groups
+    float* inv_std;
+    void* workspace;
+};
+int launch_group_norm_forward(const GroupNormShape& s, int type, const void* x, void* y, const GroupNormForward& f,
+                              hipStream_t stream);
+
+struct GroupNormBackward {
+    const float* gamma;
+    const float* beta;
+    const float* mean;
+    const float* inv_std;
+    int act;
+    float* gamma_grad;  // optional, as beta_grad and dx
+    float* beta_grad;
+    bool add_x, add_gamma, add_beta;
+    void* workspace;
+};
+int launch_group_norm_backward(const GroupNormShape& s, int type, const void* x, const void* dy, void* dx,
+                               const GroupNormBackward& b, hipStream_t stream);
+
 }  // namespace mfh

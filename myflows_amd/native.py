@@ -136,6 +136,16 @@ _SIGNATURES = {
     "mfh_mse_loss_split": ("i", "pppqpqp"),
     "mfh_mse_loss_backward": ("i", "ppppqip"),
     "mfh_column_sums": ("i", "ppqqp"),
+    "mfh_log_probs_workspace": ("q", "qiii"),
+    "mfh_log_probs": ("i", "piqiq" + "pi" + "pppp" + "ipp" + "pqp"),
+    "mfh_log_probs_backward": ("i", "piqiq" + "pi" + "pp" + "pqpq" + "pf" + "pqi" + "p"),
+    "mfh_distill_workspace": ("q", "qii"),
+    "mfh_distill_loss": ("i", "piqiq" + "pipi" + "pf" + "ppppp" + "pqp"),
+    "mfh_distill_loss_backward": ("i", "piqiq" + "pii" + "ppppp" + "f" + "pqi" + "p"),
+    "mfh_row_mean": ("i", "ppiqfpp"),
+    "mfh_group_norm_workspace": ("q", "qiiiii"),
+    "mfh_group_norm_forward": ("i", "piqiii" + "ppif" + "ppp" + "pqp"),
+    "mfh_group_norm_backward": ("i", "ppiqiii" + "pppp" + "i" + "ppp" + "iii" + "pqp"),
 }
 EXPORTS = tuple(_SIGNATURES)
 
@@ -290,6 +300,7 @@ def set_debug_sync(enabled=True):
 # argument checks shared by the entry points
 # ---------------------------------------------------------------------------------------------
 _F32 = torch.float32
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # of the calls that take several types
 
 
 def _device_f32(value, name):
@@ -610,6 +621,21 @@ def stream_workspaces():
 
 def _holds_pending_split(block):
     return any(entry[1] is block for entry in _PENDING_SPLITS.values())
+
+
+def workspace_bytes(symbol, *sizes):
+    """The bytes of workspace that a ..._workspace entry point asks for."""
+    count = getattr(_library(), symbol)(*sizes)
+    if count < 0:
+        _raise_for(2, _library())
+    return count
+
+
+def byte_workspace(count):
+    """(address, bytes) of a stream workspace of `count` bytes; (0, 0) for none."""
+    if not count:
+        return 0, 0
+    return stream_workspace((count + 7) // 8, torch.float64).data_ptr(), count
 
 
 def _implicit_workspace(g, *passes):
