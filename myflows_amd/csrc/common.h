@@ -10,6 +10,7 @@
 #include <string>
 
 #include "fastdiv.h"
+#include "group_norm_plan.h"
 #include "launch.h"
 
 namespace mfh {
@@ -543,11 +544,7 @@ int launch_row_mean(const float* values, const float* weights, const void* token
 // (n, positions, channels), and an activation.
 constexpr int ACT_SILU = 3;
 constexpr int GROUP_NORM_CHANNELS_LIMIT = 1 << 16;
-constexpr std::int64_t GROUP_NORM_COLUMNS_LIMIT = 1 << 23;  // samples times channels
-struct GroupNormShape {
-    std::int64_t n;
-    int positions, channels, groups;
-};
+constexpr std::int64_t GROUP_NORM_COLUMNS_LIMIT = 1 << 28;  // samples times channels
 std::int64_t group_norm_workspace(const GroupNormShape& s, int type, bool backward);  // bytes
 
 struct GroupNormForward {

@@ -6,163 +6,781 @@
 // and, with du = dy act'(u) and the averages over the group,
 //   dgamma[c] = sum du xhat,  dbeta[c] = sum du,
 //   dx = inv_std (gamma du - average(gamma du) - xhat average(gamma du xhat)).
-// Sums are float32; the variance is a sum of squares about the mean, never a difference of large sums.
+// Sums are float32; the variance is a sum of squares about a mean, never a difference of large sums. Every
+// sum is formed in one fixed order.
+//
+// Two routes, both bound by HBM (or, in small calls, by latency):
+//   * held: a workgroup reads its groups of a sample into registers, once, forms the sums and writes the
+//     result from there. One launch forward; backward a second one adds the samples' dgamma and dbeta;
+//   * split: groups that no workgroup holds are summed by runs of positions over many workgroups, the runs
+//     joined, and a last launch reads the activations again. It starts with those read last, which a cache
+//     still holds.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
+#include "group_norm_plan.h"
 #include "typed.h"
+#include "wave.h"
 
 namespace mfh {
 namespace {
 
-constexpr int NORM_THREADS = 256;
+// A plan's block as the kernels take it (GroupNormPlan's fields).
+struct Block {
+    int per, groups, parts, width, blocks, lanes_log2;
+    FastDiv per_div;
+};
+constexpr int BLOCK_GROUPS_MAX = GROUP_NORM_BLOCK_GROUPS;
 
-__device__ __forceinline__ float block_sum(float v) {
-    __shared__ float part[NORM_THREADS];
-    __syncthreads();
-    part[threadIdx.x] = v;
-    __syncthreads();
-    for (int half = NORM_THREADS / 2; half > 0; half /= 2) {
-        if (static_cast<int>(threadIdx.x) < half) part[threadIdx.x] += part[threadIdx.x + half];
-        __syncthreads();
-    }
-    return part[0];
+// The place of a block: its first channel, its channels and its first group.
+struct Place {
+    int channel, width, group, part;
+};
+__device__ __forceinline__ Place place_of(const Block& k, int index) {
+    if (k.parts == 1) return {index * k.width, k.width, index * k.groups, 0};
+    const int group = index / k.parts, part = index - group * k.parts;
+    return {group * k.per + part * k.width, min(k.width, k.per - part * k.width), group, part};
 }
 
+// ---- activations -----------------------------------------------------------------------------
+// ReLU and no activation are one form: the larger of u and a floor of 0 or -inf (a NaN stays).
 __device__ __forceinline__ float sigmoid_of(float u) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * u));
 }
-template <int ACT>
-__device__ __forceinline__ float activate(float u) {
-    if constexpr (ACT == ACT_RELU) return u > 0.0f || u != u ? u : 0.0f;
-    if constexpr (ACT == ACT_SILU) return u * sigmoid_of(u);
-    return u;
+template <bool SILU>
+__device__ __forceinline__ float activate(float u, float floor) {
+    if constexpr (SILU) return u * sigmoid_of(u);
+    return u < floor ? floor : u;
 }
 // dy act'(u)
-template <int ACT>
-__device__ __forceinline__ float through(float u, float dy) {
-    if constexpr (ACT == ACT_RELU) return u > 0.0f ? dy : 0.0f;
-    if constexpr (ACT == ACT_SILU) {
+template <bool SILU>
+__device__ __forceinline__ float through(float u, float dy, float floor) {
+    if constexpr (SILU) {
         const float g = sigmoid_of(u);
         return dy * (g * (1.0f + u * (1.0f - g)));
     }
-    return dy;
+    return u <= floor ? 0.0f : dy;
 }
 
-template <typename T, int ACT>
-__global__ __launch_bounds__(NORM_THREADS) void group_norm_kernel(const T* __restrict__ x, T* __restrict__ y,
-                                                                  GroupNormShape s, GroupNormForward f) {
-    const int per = s.channels / s.groups, count = s.positions * per;
-    const long long n = blockIdx.x / s.groups;
-    const int g = blockIdx.x % s.groups;
-    const long long base = n * s.positions * s.channels + g * per;
+// ---- sums over a block -----------------------------------------------------------------------
+// Each thread brings VW columns' sums over its rows. Rows of one wave are joined across its lanes, the rest
+// through LDS, part by part in order.
+template <int THREADS, int VW>
+struct ColumnSums {
+    static constexpr int FLOATS = THREADS * VW;
+
+    // Parts that a column has in LDS, and the floats from one part to the next.
+    static __device__ __forceinline__ int parts(const Block& k) { return THREADS >> max(k.lanes_log2, 6); }
+    static __device__ __forceinline__ int pitch(const Block& k) { return VW << k.lanes_log2; }
+
+    static __device__ __forceinline__ void put(const Block& k, float (&lds)[FLOATS], const float (&mine)[VW]) {
+        const int lanes = 1 << k.lanes_log2;
+        float v[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] = mine[i];
+        for (int o = lanes; o < 64; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) v[i] += __shfl_xor(v[i], o);
+        const int tid = threadIdx.x;
+        if (lanes < 64 && (tid & 63) >= lanes) return;
+        float* to = lds + (tid >> max(k.lanes_log2, 6)) * pitch(k) + (tid & (lanes - 1)) * VW;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) to[i] = v[i];
+    }
+
+    // sums[g] = the sum of group g's columns and parts (a wave a group).
+    static __device__ __forceinline__ void groups(const Block& k, int width, const float (&lds)[FLOATS], float* sums) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x & 63, step = pitch(k);
+        const int per = k.parts == 1 ? k.per : width, count = parts(k) * per;
+        for (int g = wave; g < k.groups; g += THREADS / 64) {
+            float s = 0.0f;
+            for (int i = lane; i < count; i += 64) {
+                const int part = k.parts == 1 ? k.per_div.div(i) : i / per;
+                s += lds[part * step + g * per + (i - part * per)];
+            }
+            s = wave_sum(s);
+            if (lane == 0) sums[g] = s;
+        }
+    }
+};
+
+// The group sums of the threads' column sums, for each thread's columns.
+template <int THREADS, int VW>
+__device__ __forceinline__ void group_sums(const Block& k, int width, float (&lds)[THREADS * VW], float* sums,
+                                           const int (&group)[VW], const float (&mine)[VW], float (&result)[VW]) {
+    __syncthreads();  // what the last call left is read
+    ColumnSums<THREADS, VW>::put(k, lds, mine);
+    __syncthreads();
+    ColumnSums<THREADS, VW>::groups(k, width, lds, sums);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VW; ++i) result[i] = sums[group[i]];
+}
+
+// A thread's place in a block: its columns, first row and the rows from one of its rows to the next.
+template <int THREADS, int VW>
+struct Thread {
+    int column, row, step;
+    bool active;
+    int group[VW];  // of the block's groups
+
+    __device__ __forceinline__ Thread(const Block& k, int width) {
+        const int tid = threadIdx.x, lanes = 1 << k.lanes_log2;
+        column = (tid & (lanes - 1)) * VW;
+        row = tid >> k.lanes_log2;
+        step = THREADS >> k.lanes_log2;
+        active = column < width;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) group[i] = active && k.parts == 1 ? k.per_div.div(column + i) : 0;
+    }
+    // The values of this thread's columns in an array by channel (0 for an idle thread).
+    __device__ __forceinline__ void by_column(const float* __restrict__ values, float (&to)[VW]) const {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) to[i] = active ? values[column + i] : 0.0f;
+    }
+    __device__ __forceinline__ void by_group(const float* __restrict__ values, float (&to)[VW]) const {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) to[i] = active ? values[group[i]] : 0.0f;
+    }
+};
+
+// Keeps held packs packed: without it the compiler holds the floats of the first pass over them for the second,
+// at twice the registers.
+template <typename T, int VW, int HOLD>
+__device__ __forceinline__ void keep_packed(Pack<T, VW> (&held)[HOLD]) {
+    if constexpr (sizeof(T) == 2 && VW > 1) {
+        constexpr int WORDS = VW / 2;
+#pragma unroll
+        for (int h = 0; h < HOLD; ++h) {
+            unsigned w[WORDS];
+            __builtin_memcpy(w, &held[h], sizeof(w));
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
+            __builtin_memcpy(&held[h], w, sizeof(w));
+        }
+    }
+}
+
+// Neighbouring blocks of a sample share cache lines where a block's row is narrower than one: the workgroups
+// are dealt round-robin to the 8 XCDs, so each XCD takes one run of the blocks.
+__device__ __forceinline__ unsigned xcd_run(unsigned total) {
+    return total % 8 ? blockIdx.x : (blockIdx.x & 7) * (total / 8) + blockIdx.x / 8;
+}
+
+// ---- held ------------------------------------------------------------------------------------
+template <typename T, int VW, bool SILU, int THREADS, int HOLD>
+__global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restrict__ x, T* __restrict__ y,
+                                                               GroupNormShape s, Block k, GroupNormForward f) {
+    __shared__ float lds[THREADS * VW], sums[BLOCK_GROUPS_MAX];
+    const unsigned at = xcd_run(gridDim.x), sample = at / static_cast<unsigned>(k.blocks);
+    const long long n = sample;
+    const Place place = place_of(k, static_cast<int>(at - sample * k.blocks));
+    const Thread<THREADS, VW> t(k, place.width);
+    const long long base = n * s.positions * s.channels + place.channel + t.column;
+    Pack<T, VW> held[HOLD];
+    float sum[VW] = {}, mean[VW], squares[VW] = {}, a[VW], beta[VW];
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int row = t.row + h * t.step;
+        if (t.active && row < s.positions) held[h] = load_pack<T, VW>(x + base + row * s.channels);
+    }
+    t.by_column(f.gamma + place.channel, a);
+    t.by_column(f.beta + place.channel, beta);
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (t.active && t.row + h * t.step < s.positions)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) sum[i] += held[h].at(i);
+    keep_packed(held);
+    group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, sum, mean);
+    const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
+#pragma unroll
+    for (int i = 0; i < VW; ++i) mean[i] *= inv_count;
+    if (static_cast<int>(threadIdx.x) < k.groups) f.mean[n * s.groups + place.group + threadIdx.x] = sums[threadIdx.x] * inv_count;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (t.active && t.row + h * t.step < s.positions)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const float d = held[h].at(i) - mean[i];
+                squares[i] += d * d;
+            }
+    float variance[VW];
+    keep_packed(held);
+    group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, squares, variance);
+    if (static_cast<int>(threadIdx.x) < k.groups)
+        f.inv_std[n * s.groups + place.group + threadIdx.x] = 1.0f / sqrtf(sums[threadIdx.x] * inv_count + f.eps);
+#pragma unroll
+    for (int i = 0; i < VW; ++i) a[i] *= 1.0f / sqrtf(variance[i] * inv_count + f.eps);
+    const float floor = f.act == ACT_RELU ? 0.0f : -INFINITY;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int row = t.row + h * t.step;
+        if (t.active && row < s.positions) {
+            Pack<T, VW> out;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) out.set(i, activate<SILU>((held[h].at(i) - mean[i]) * a[i] + beta[i], floor));
+            store_pack(y + base + row * s.channels, out);
+        }
+    }
+}
+
+// What the backward forms of an element: xhat and du.
+template <bool SILU>
+struct Backward {
+    float hat, du;
+    __device__ __forceinline__ Backward(float x, float dy, float mean, float inv, float gamma, float beta, float floor) {
+        hat = (x - mean) * inv;
+        du = through<SILU>(hat * gamma + beta, dy, floor);
+    }
+};
+
+// columns[2 c], columns[2 c + 1] = sum du, sum du xhat of channel c of a sample.
+template <typename T, int VW, bool SILU, int THREADS, int HOLD>
+__global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restrict__ x, const T* __restrict__ dy, T* dx,
+                                                                GroupNormShape s, Block k, GroupNormBackward b,
+                                                                float* __restrict__ columns) {
+    using Sums = ColumnSums<THREADS, VW>;
+    __shared__ float first[THREADS * VW], second[THREADS * VW], sums[2][BLOCK_GROUPS_MAX];
+    const unsigned at = xcd_run(gridDim.x), sample = at / static_cast<unsigned>(k.blocks);
+    const long long n = sample;
+    const Place place = place_of(k, static_cast<int>(at - sample * k.blocks));
+    const Thread<THREADS, VW> t(k, place.width);
+    const long long base = n * s.positions * s.channels + place.channel + t.column;
+    Pack<T, VW> held[HOLD], grad[HOLD];
+    float mean[VW], inv[VW], gamma[VW], beta[VW], sum[VW] = {}, product[VW] = {};
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int row = t.row + h * t.step;
+        if (t.active && row < s.positions) {
+            held[h] = load_pack<T, VW>(x + base + row * s.channels);
+            grad[h] = load_pack<T, VW>(dy + base + row * s.channels);
+        }
+    }
+    t.by_group(b.mean + n * s.groups + place.group, mean);
+    t.by_group(b.inv_std + n * s.groups + place.group, inv);
+    t.by_column(b.gamma + place.channel, gamma);
+    t.by_column(b.beta + place.channel, beta);
+    const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
+    const auto form = [&](int h, int i) {
+        return Backward<SILU>(held[h].at(i), grad[h].at(i), mean[i], inv[i], gamma[i], beta[i], floor);
+    };
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (t.active && t.row + h * t.step < s.positions)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const Backward<SILU> e = form(h, i);
+                sum[i] += e.du;
+                product[i] += e.du * e.hat;
+            }
+    keep_packed(held);
+    keep_packed(grad);
+    Sums::put(k, first, sum);
+    Sums::put(k, second, product);
+    __syncthreads();
+    // The columns' sums, weighted by gamma for the groups, take the first part's place.
+    const int parts = Sums::parts(k), pitch = Sums::pitch(k);
+    for (int c = threadIdx.x; c < place.width; c += THREADS) {
+        float d = first[c], p = second[c];
+        for (int i = 1; i < parts; ++i) {
+            d += first[i * pitch + c];
+            p += second[i * pitch + c];
+        }
+        if (columns) {
+            float* to = columns + 2 * (n * s.channels + place.channel + c);
+            to[0] = d;
+            to[1] = p;
+        }
+        const float g = b.gamma[place.channel + c];
+        first[c] = g * d;
+        second[c] = g * p;
+    }
+    if (!dx) return;
+    __syncthreads();
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
+    for (int g = wave; g < k.groups; g += THREADS / 64) {
+        float d = 0.0f, p = 0.0f;
+        for (int c = lane; c < k.per; c += 64) {
+            d += first[g * k.per + c];
+            p += second[g * k.per + c];
+        }
+        d = wave_sum(d) * inv_count;
+        p = wave_sum(p) * inv_count;
+        if (lane == 0) {
+            sums[0][g] = d;
+            sums[1][g] = p;
+        }
+    }
+    __syncthreads();
+    float mean_d[VW], mean_p[VW];
+    t.by_group(sums[0], mean_d);
+    t.by_group(sums[1], mean_p);
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int row = t.row + h * t.step;
+        if (t.active && row < s.positions) {
+            T* to = dx + base + row * s.channels;
+            Pack<T, VW> out, old;
+            if (b.add_x) old = load_pack<T, VW>(to);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const Backward<SILU> e = form(h, i);
+                const float v = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
+                out.set(i, b.add_x ? old.at(i) + v : v);
+            }
+            store_pack(to, out);
+        }
+    }
+}
+
+// ---- split -----------------------------------------------------------------------------------
+constexpr int SPLIT_THREADS = GROUP_NORM_SPLIT_THREADS, SPLIT_AHEAD = GROUP_NORM_SPLIT_AHEAD;
+
+struct Runs {
+    int count, rows;  // runs of a sample's positions, and positions of a run
+};
+struct RunAt {
+    long long n;
+    int run, begin, end;
+    Place place;
+};
+// The run of a workgroup, forwards through the samples or backwards.
+__device__ __forceinline__ RunAt run_at(const Runs& r, const Block& k, int positions, bool backwards) {
+    unsigned at = backwards ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const unsigned rest = at / static_cast<unsigned>(k.blocks);
+    const int block = static_cast<int>(at - rest * k.blocks);
+    const unsigned n = rest / static_cast<unsigned>(r.count);
+    const int run = static_cast<int>(rest - n * r.count);
+    return {n, run, run * r.rows, min(positions, (run + 1) * r.rows), place_of(k, block)};
+}
+
+// means and squares [sample][run][group and part]: the mean of a run's values and the squares about it. A
+// thread keeps each of its columns' mean and squares, SPLIT_AHEAD rows at a time joined to them by
+//   mean += d k / (n + k),  squares += squares' + d^2 n k / (n + k),  d = mean' - mean
+// (Chan, Golub and LeVeque, 1983); the threads' are joined about the run's mean.
+template <typename T, int VW>
+__global__ __launch_bounds__(SPLIT_THREADS) void run_stats_kernel(const T* __restrict__ x, GroupNormShape s, Block k,
+                                                                  Runs runs, float* __restrict__ means,
+                                                                  float* __restrict__ squares) {
+    __shared__ float lds[SPLIT_THREADS * VW], sums[BLOCK_GROUPS_MAX];
+    const RunAt r = run_at(runs, k, s.positions, false);
+    const Thread<SPLIT_THREADS, VW> t(k, r.place.width);
+    const T* __restrict__ from = x + r.n * s.positions * s.channels + r.place.channel + t.column;
+    float count = 0.0f, mean[VW] = {}, m2[VW] = {};
+    if (t.active) {
+        int row = r.begin + t.row;
+        for (; row + (SPLIT_AHEAD - 1) * t.step < r.end; row += SPLIT_AHEAD * t.step) {
+            Pack<T, VW> packs[SPLIT_AHEAD];
+#pragma unroll
+            for (int u = 0; u < SPLIT_AHEAD; ++u) packs[u] = load_pack<T, VW>(from + (row + u * t.step) * s.channels);
+            const float more = count + SPLIT_AHEAD, share = SPLIT_AHEAD * __builtin_amdgcn_rcpf(more), weight = count * share;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                float sum = 0.0f, about = 0.0f;
+#pragma unroll
+                for (int u = 0; u < SPLIT_AHEAD; ++u) sum += packs[u].at(i);
+                const float here = sum * (1.0f / SPLIT_AHEAD);
+#pragma unroll
+                for (int u = 0; u < SPLIT_AHEAD; ++u) {
+                    const float d = packs[u].at(i) - here;
+                    about += d * d;
+                }
+                const float d = here - mean[i];
+                mean[i] += d * share;
+                m2[i] += about + d * d * weight;
+            }
+            count = more;
+        }
+        for (; row < r.end; row += t.step) {
+            const Pack<T, VW> pack = load_pack<T, VW>(from + row * s.channels);
+            const float more = count + 1.0f, share = __builtin_amdgcn_rcpf(more), weight = count * share;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const float d = pack.at(i) - mean[i];
+                mean[i] += d * share;
+                m2[i] += d * d * weight;
+            }
+            count = more;
+        }
+    }
+    float sum[VW], whole[VW];
+#pragma unroll
+    for (int i = 0; i < VW; ++i) sum[i] = count * mean[i];
+    group_sums<SPLIT_THREADS, VW>(k, r.place.width, lds, sums, t.group, sum, whole);
+    const int per = k.parts == 1 ? k.per : r.place.width;
+    const float inv_count = 1.0f / (static_cast<float>(r.end - r.begin) * static_cast<float>(per));
+    const long long to = (r.n * runs.count + r.run) * s.groups * k.parts + static_cast<long long>(r.place.group) * k.parts + r.place.part;
+    if (static_cast<int>(threadIdx.x) < k.groups) means[to + threadIdx.x] = sums[threadIdx.x] * inv_count;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+        const float d = mean[i] - whole[i] * inv_count;
+        sum[i] = m2[i] + count * (d * d);
+    }
+    group_sums<SPLIT_THREADS, VW>(k, r.place.width, lds, sums, t.group, sum, whole);
+    if (static_cast<int>(threadIdx.x) < k.groups) squares[to + threadIdx.x] = sums[threadIdx.x];
+}
+
+// The runs and parts of each (sample, group) joined: one wave each.
+__global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict__ means, const float* __restrict__ squares,
+                                                         GroupNormShape s, Block k, Runs runs, GroupNormForward f) {
+    const long long at = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 64;
+    if (at >= s.n * s.groups) return;  // the whole wave
+    const int lane = threadIdx.x & 63, g = static_cast<int>(at % s.groups), pieces = runs.count * k.parts;
+    const long long n = at / s.groups;
+    const auto piece = [&](int i, float& count) {
+        const int run = i / k.parts, part = i - run * k.parts;
+        const int rows = min(s.positions - run * runs.rows, runs.rows);
+        const int columns = k.parts == 1 ? k.per : min(k.width, k.per - part * k.width);
+        count = static_cast<float>(rows) * static_cast<float>(columns);
+        return ((n * runs.count + run) * s.groups + g) * k.parts + part;
+    };
     float sum = 0.0f;
-    for (int i = threadIdx.x; i < count; i += NORM_THREADS) sum += static_cast<float>(x[base + (i / per) * static_cast<long long>(s.channels) + i % per]);
-    const float mean = block_sum(sum) / count;
-    float squares = 0.0f;
-    for (int i = threadIdx.x; i < count; i += NORM_THREADS) {
-        const float d = static_cast<float>(x[base + (i / per) * static_cast<long long>(s.channels) + i % per]) - mean;
-        squares += d * d;
+    for (int i = lane; i < pieces; i += 64) {
+        float count;
+        const long long from = piece(i, count);
+        sum += count * means[from];
     }
-    const float inv_std = 1.0f / sqrtf(block_sum(squares) / count + f.eps);
-    if (threadIdx.x == 0) {
-        f.mean[blockIdx.x] = mean;
-        f.inv_std[blockIdx.x] = inv_std;
+    const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
+    const float mean = wave_sum(sum) * inv_count;
+    float about = 0.0f;
+    for (int i = lane; i < pieces; i += 64) {
+        float count;
+        const long long from = piece(i, count);
+        const float d = means[from] - mean;
+        about += squares[from] + count * (d * d);
     }
-    for (int i = threadIdx.x; i < count; i += NORM_THREADS) {
-        const long long at = base + (i / per) * static_cast<long long>(s.channels) + i % per;
-        const int c = g * per + i % per;
-        y[at] = static_cast<T>(activate<ACT>((static_cast<float>(x[at]) - mean) * inv_std * f.gamma[c] + f.beta[c]));
+    about = wave_sum(about);
+    if (lane != 0) return;
+    f.mean[at] = mean;
+    f.inv_std[at] = 1.0f / sqrtf(about * inv_count + f.eps);
+}
+
+template <typename T, int VW, bool SILU>
+__global__ __launch_bounds__(SPLIT_THREADS) void apply_forward_kernel(const T* __restrict__ x, T* __restrict__ y,
+                                                                      GroupNormShape s, Block k, Runs runs,
+                                                                      GroupNormForward f) {
+    const RunAt r = run_at(runs, k, s.positions, true);
+    const Thread<SPLIT_THREADS, VW> t(k, r.place.width);
+    if (!t.active) return;
+    const long long base = r.n * s.positions * s.channels + r.place.channel + t.column;
+    float mean[VW], a[VW], beta[VW], inv[VW];
+    t.by_group(f.mean + r.n * s.groups + r.place.group, mean);
+    t.by_group(f.inv_std + r.n * s.groups + r.place.group, inv);
+    t.by_column(f.gamma + r.place.channel, a);
+    t.by_column(f.beta + r.place.channel, beta);
+    const float floor = f.act == ACT_RELU ? 0.0f : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) a[i] *= inv[i];
+    const auto write = [&](int row, const Pack<T, VW>& in) {
+        Pack<T, VW> out;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) out.set(i, activate<SILU>((in.at(i) - mean[i]) * a[i] + beta[i], floor));
+        store_pack(y + base + row * s.channels, out);
+    };
+    int row = r.begin + t.row;
+    for (; row + (SPLIT_AHEAD - 1) * t.step < r.end; row += SPLIT_AHEAD * t.step) {
+        Pack<T, VW> packs[SPLIT_AHEAD];
+#pragma unroll
+        for (int u = 0; u < SPLIT_AHEAD; ++u) packs[u] = load_pack<T, VW>(x + base + (row + u * t.step) * s.channels);
+#pragma unroll
+        for (int u = 0; u < SPLIT_AHEAD; ++u) write(row + u * t.step, packs[u]);
+    }
+    for (; row < r.end; row += t.step) write(row, load_pack<T, VW>(x + base + row * s.channels));
+}
+
+// run_columns [sample][run][channel][2]: sum du and sum du xhat of a run's positions.
+template <typename T, int VW, bool SILU>
+__global__ __launch_bounds__(SPLIT_THREADS) void run_gradients_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+                                                                      GroupNormShape s, Block k, Runs runs,
+                                                                      GroupNormBackward b, float* __restrict__ run_columns) {
+    using Sums = ColumnSums<SPLIT_THREADS, VW>;
+    __shared__ float first[SPLIT_THREADS * VW], second[SPLIT_THREADS * VW];
+    const RunAt r = run_at(runs, k, s.positions, false);
+    const Thread<SPLIT_THREADS, VW> t(k, r.place.width);
+    const long long base = r.n * s.positions * s.channels + r.place.channel + t.column;
+    float mean[VW], inv[VW], gamma[VW], beta[VW], sum[VW] = {}, product[VW] = {};
+    t.by_group(b.mean + r.n * s.groups + r.place.group, mean);
+    t.by_group(b.inv_std + r.n * s.groups + r.place.group, inv);
+    t.by_column(b.gamma + r.place.channel, gamma);
+    t.by_column(b.beta + r.place.channel, beta);
+    const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
+    const auto take = [&](const Pack<T, VW>& in, const Pack<T, VW>& grad) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], gamma[i], beta[i], floor);
+            sum[i] += e.du;
+            product[i] += e.du * e.hat;
+        }
+    };
+    if (t.active) {
+        int row = r.begin + t.row;
+        for (; row + (SPLIT_AHEAD - 1) * t.step < r.end; row += SPLIT_AHEAD * t.step) {
+            Pack<T, VW> in[SPLIT_AHEAD], grad[SPLIT_AHEAD];
+#pragma unroll
+            for (int u = 0; u < SPLIT_AHEAD; ++u) {
+                in[u] = load_pack<T, VW>(x + base + (row + u * t.step) * s.channels);
+                grad[u] = load_pack<T, VW>(dy + base + (row + u * t.step) * s.channels);
+            }
+#pragma unroll
+            for (int u = 0; u < SPLIT_AHEAD; ++u) take(in[u], grad[u]);
+        }
+        for (; row < r.end; row += t.step)
+            take(load_pack<T, VW>(x + base + row * s.channels), load_pack<T, VW>(dy + base + row * s.channels));
+    }
+    Sums::put(k, first, sum);
+    Sums::put(k, second, product);
+    __syncthreads();
+    const int parts = Sums::parts(k), pitch = Sums::pitch(k);
+    for (int c = threadIdx.x; c < r.place.width; c += SPLIT_THREADS) {
+        float d = first[c], p = second[c];
+        for (int i = 1; i < parts; ++i) {
+            d += first[i * pitch + c];
+            p += second[i * pitch + c];
+        }
+        float* to = run_columns + 2 * ((r.n * runs.count + r.run) * s.channels + r.place.channel + c);
+        to[0] = d;
+        to[1] = p;
     }
 }
 
-template <typename T, int ACT>
-__global__ __launch_bounds__(NORM_THREADS) void group_norm_dx_kernel(const T* __restrict__ x, const T* __restrict__ dy,
-                                                                     T* dx, GroupNormShape s, GroupNormBackward b) {
-    const int per = s.channels / s.groups, count = s.positions * per;
-    const long long n = blockIdx.x / s.groups;
-    const int g = blockIdx.x % s.groups;
-    const long long base = n * s.positions * s.channels + g * per;
-    const float mean = b.mean[blockIdx.x], inv_std = b.inv_std[blockIdx.x];
-    float first = 0.0f, second = 0.0f;
-    for (int i = threadIdx.x; i < count; i += NORM_THREADS) {
-        const long long at = base + (i / per) * static_cast<long long>(s.channels) + i % per;
-        const int c = g * per + i % per;
-        const float hat = (static_cast<float>(x[at]) - mean) * inv_std;
-        const float d = through<ACT>(hat * b.gamma[c] + b.beta[c], static_cast<float>(dy[at])) * b.gamma[c];
-        first += d;
-        second += d * hat;
+// out[outer][j] = the sum over `inner` rows of from[outer][row][j], j < columns: 16 runs of rows a column, each in
+// order, then in run order.
+constexpr int COLUMN_SPAN = 64, COLUMN_RUNS = 16;
+__device__ __forceinline__ float sum_of_rows(const float* __restrict__ from, long long rows, long long columns, long long j,
+                                             float (&lds)[COLUMN_RUNS][COLUMN_SPAN]) {
+    const int c = threadIdx.x % COLUMN_SPAN, g = threadIdx.x / COLUMN_SPAN;
+    const long long each = (rows + COLUMN_RUNS - 1) / COLUMN_RUNS, last = min(rows, (g + 1) * each);
+    float s = 0.0f;
+    if (j < columns) {
+        long long row = g * each;
+        for (; row + 8 <= last; row += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = from[(row + u) * columns + j];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; row < last; ++row) s += from[row * columns + j];
     }
-    first = block_sum(first) / count;
-    second = block_sum(second) / count;
-    for (int i = threadIdx.x; i < count; i += NORM_THREADS) {
-        const long long at = base + (i / per) * static_cast<long long>(s.channels) + i % per;
-        const int c = g * per + i % per;
-        const float hat = (static_cast<float>(x[at]) - mean) * inv_std;
-        const float d = through<ACT>(hat * b.gamma[c] + b.beta[c], static_cast<float>(dy[at])) * b.gamma[c];
-        const float v = inv_std * (d - first - hat * second);
-        dx[at] = static_cast<T>(b.add_x ? static_cast<float>(dx[at]) + v : v);
-    }
+    lds[g][c] = s;
+    __syncthreads();
+    if (g == 0)
+#pragma unroll
+        for (int i = 1; i < COLUMN_RUNS; ++i) s += lds[i][c];
+    return s;  // of the first COLUMN_SPAN threads
 }
 
-template <typename T, int ACT>
-__global__ __launch_bounds__(NORM_THREADS) void group_norm_params_kernel(const T* __restrict__ x,
-                                                                         const T* __restrict__ dy, GroupNormShape s,
-                                                                         GroupNormBackward b) {
-    const int c = blockIdx.x, g = c / (s.channels / s.groups);
-    const float gamma = b.gamma[c], beta = b.beta[c];
-    float first = 0.0f, second = 0.0f;
-    for (long long i = threadIdx.x; i < s.n * s.positions; i += NORM_THREADS) {
-        const long long n = i / s.positions;
-        const float hat = (static_cast<float>(x[i * s.channels + c]) - b.mean[n * s.groups + g]) * b.inv_std[n * s.groups + g];
-        const float d = through<ACT>(hat * gamma + beta, static_cast<float>(dy[i * s.channels + c]));
-        first += d;
-        second += d * hat;
-    }
-    first = block_sum(first);
-    second = block_sum(second);
-    if (threadIdx.x != 0) return;
-    if (b.beta_grad) b.beta_grad[c] = b.add_beta ? b.beta_grad[c] + first : first;
-    if (b.gamma_grad) b.gamma_grad[c] = b.add_gamma ? b.gamma_grad[c] + second : second;
+__global__ __launch_bounds__(COLUMN_SPAN* COLUMN_RUNS) void join_columns_kernel(const float* __restrict__ run_columns,
+                                                                                int runs, int columns, int tiles,
+                                                                                float* __restrict__ out) {
+    __shared__ float lds[COLUMN_RUNS][COLUMN_SPAN];
+    const long long n = blockIdx.x / tiles, j = (blockIdx.x % tiles) * COLUMN_SPAN + threadIdx.x % COLUMN_SPAN;
+    const float s = sum_of_rows(run_columns + n * runs * columns, runs, columns, j, lds);
+    if (threadIdx.x < COLUMN_SPAN && j < columns) out[n * columns + j] = s;
 }
 
-// Calls f with the element type and activation as types.
+// dbeta and dgamma: the sums of columns [sample][channel][2] over the samples.
+__global__ __launch_bounds__(COLUMN_SPAN* COLUMN_RUNS) void parameter_grads_kernel(const float* __restrict__ columns,
+                                                                                   GroupNormShape s, GroupNormBackward b) {
+    __shared__ float lds[COLUMN_RUNS][COLUMN_SPAN];
+    const long long j = static_cast<long long>(blockIdx.x) * COLUMN_SPAN + threadIdx.x % COLUMN_SPAN;
+    const float v = sum_of_rows(columns, s.n, 2LL * s.channels, j, lds);
+    if (threadIdx.x >= COLUMN_SPAN || j >= 2LL * s.channels) return;
+    float* out = j & 1 ? b.gamma_grad : b.beta_grad;
+    if (!out) return;
+    const bool add = j & 1 ? b.add_gamma : b.add_beta;
+    out[j / 2] = add ? out[j / 2] + v : v;
+}
+
+template <typename T, int VW, bool SILU>
+__global__ __launch_bounds__(SPLIT_THREADS) void apply_backward_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+                                                                       T* dx, GroupNormShape s, Block k, Runs runs,
+                                                                       GroupNormBackward b,
+                                                                       const float* __restrict__ columns) {
+    __shared__ float sums[2][BLOCK_GROUPS_MAX];
+    const RunAt r = run_at(runs, k, s.positions, true);
+    const Thread<SPLIT_THREADS, VW> t(k, r.place.width);
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
+    for (int g = wave; g < k.groups; g += SPLIT_THREADS / 64) {
+        const int channel = (r.place.group + g) * k.per;
+        const float* __restrict__ from = columns + 2 * (r.n * s.channels + channel);
+        float d = 0.0f, p = 0.0f;
+        for (int c = lane; c < k.per; c += 64) {
+            const float gamma = b.gamma[channel + c];
+            d += gamma * from[2 * c];
+            p += gamma * from[2 * c + 1];
+        }
+        d = wave_sum(d) * inv_count;
+        p = wave_sum(p) * inv_count;
+        if (lane == 0) {
+            sums[0][g] = d;
+            sums[1][g] = p;
+        }
+    }
+    __syncthreads();
+    if (!t.active) return;
+    const long long base = r.n * s.positions * s.channels + r.place.channel + t.column;
+    float mean[VW], inv[VW], gamma[VW], beta[VW], mean_d[VW], mean_p[VW];
+    t.by_group(b.mean + r.n * s.groups + r.place.group, mean);
+    t.by_group(b.inv_std + r.n * s.groups + r.place.group, inv);
+    t.by_column(b.gamma + r.place.channel, gamma);
+    t.by_column(b.beta + r.place.channel, beta);
+    t.by_group(sums[0], mean_d);
+    t.by_group(sums[1], mean_p);
+    const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
+    const auto write = [&](int row, const Pack<T, VW>& in, const Pack<T, VW>& grad) {
+        T* to = dx + base + row * s.channels;
+        Pack<T, VW> out, old;
+        if (b.add_x) old = load_pack<T, VW>(to);
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], gamma[i], beta[i], floor);
+            const float v = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
+            out.set(i, b.add_x ? old.at(i) + v : v);
+        }
+        store_pack(to, out);
+    };
+    int row = r.begin + t.row;
+    for (; row + (SPLIT_AHEAD - 1) * t.step < r.end; row += SPLIT_AHEAD * t.step) {
+        Pack<T, VW> in[SPLIT_AHEAD], grad[SPLIT_AHEAD];
+#pragma unroll
+        for (int u = 0; u < SPLIT_AHEAD; ++u) {
+            in[u] = load_pack<T, VW>(x + base + (row + u * t.step) * s.channels);
+            grad[u] = load_pack<T, VW>(dy + base + (row + u * t.step) * s.channels);
+        }
+#pragma unroll
+        for (int u = 0; u < SPLIT_AHEAD; ++u) write(row + u * t.step, in[u], grad[u]);
+    }
+    for (; row < r.end; row += t.step)
+        write(row, load_pack<T, VW>(x + base + row * s.channels), load_pack<T, VW>(dy + base + row * s.channels));
+}
+
+// ---- launches --------------------------------------------------------------------------------
+Block block_of(const GroupNormPlan& plan) {
+    return {plan.per, plan.groups, plan.parts, plan.width, plan.blocks, plan.lanes_log2, FastDiv(plan.per)};
+}
+
+constexpr std::int64_t THREADS_LIMIT = (1LL << 32) - 1;  // threads of a launch
+
+int require_grid(const GroupNormShape& s, const GroupNormPlan& plan) {
+    MFH_REQUIRE(s.n * plan.grid() * plan.threads <= THREADS_LIMIT, "too many samples for one group norm");
+    return OK;
+}
+
+// Calls f with the element type, the pack's size and whether the activation is SiLU as types.
 template <typename F>
-void with_type_and_act(int type, int act, F&& f) {
+void with_kernel(int type, int vw, int act, F&& f) {
     with_type(type, [&](auto zero) {
-        if (act == ACT_RELU) f(zero, std::integral_constant<int, ACT_RELU>{});
-        else if (act == ACT_SILU) f(zero, std::integral_constant<int, ACT_SILU>{});
-        else f(zero, std::integral_constant<int, ACT_NONE>{});
+        using T = decltype(zero);
+        constexpr int WIDE = 16 / sizeof(T);
+        const auto packed = [&](auto pack) {
+            if (act == ACT_SILU) f(zero, pack, std::true_type{});
+            else f(zero, pack, std::false_type{});
+        };
+        if (vw == WIDE) return packed(std::integral_constant<int, WIDE>{});
+        if constexpr (sizeof(T) == 2)
+            if (vw == 2) return packed(std::integral_constant<int, 2>{});
+        packed(std::integral_constant<int, 1>{});
     });
 }
+
+std::int64_t columns_floats(const GroupNormShape& s) { return 2 * s.n * s.channels; }
 
 }  // namespace
 
-std::int64_t group_norm_workspace(const GroupNormShape&, int, bool) { return 0; }
+std::int64_t group_norm_workspace(const GroupNormShape& s, int type, bool backward) {
+    if (s.n == 0) return 0;
+    const GroupNormPlan plan = group_norm_plan(s, type_bytes(type), backward);
+    const std::int64_t columns = columns_floats(s);
+    if (plan.held) return backward ? 4 * columns : 0;
+    if (backward) return 4 * columns * (1 + plan.runs);
+    return 4 * 2 * s.n * plan.runs * s.groups * plan.parts;
+}
 
 int launch_group_norm_forward(const GroupNormShape& s, int type, const void* x, void* y, const GroupNormForward& f,
                               hipStream_t stream) {
-    with_type_and_act(type, f.act, [&](auto zero, auto act) {
+    const GroupNormPlan plan = group_norm_plan(s, type_bytes(type), false);
+    MFH_TRY(require_grid(s, plan));
+    const Block block = block_of(plan);
+    const Runs runs{plan.runs, plan.rows};
+    const unsigned groups = static_cast<unsigned>(s.n * plan.grid());
+    float* means = static_cast<float*>(f.workspace);
+    float* squares = plan.held ? nullptr : means + s.n * plan.runs * s.groups * plan.parts;
+    with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
         using T = decltype(zero);
-        launch(group_norm_kernel<T, decltype(act)::value>, static_cast<unsigned>(s.n * s.groups), NORM_THREADS, 0, stream,
-               static_cast<const T*>(x), static_cast<T*>(y), s, f);
+        constexpr int VW = decltype(pack)::value, HOLD = group_norm_hold(sizeof(T), VW, false);
+        constexpr bool SILU = decltype(silu)::value;
+        const T* in = static_cast<const T*>(x);
+        if (plan.held && plan.threads == 256)
+            launch(held_forward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, static_cast<T*>(y), s, block, f);
+        else if (plan.held)
+            launch(held_forward_kernel<T, VW, SILU, 1024, HOLD>, groups, 1024, 0, stream, in, static_cast<T*>(y), s, block, f);
+        else
+            launch(run_stats_kernel<T, VW>, groups, SPLIT_THREADS, 0, stream, in, s, block, runs, means, squares);
     });
-    return MFH_CHECK_LAUNCH("group_norm", stream);
+    MFH_TRY(MFH_CHECK_LAUNCH("group_norm_forward", stream));
+    if (plan.held) return OK;
+    launch(join_stats_kernel, blocks_for(s.n * s.groups, 4), 256, 0, stream, means, squares, s, block, runs, f);
+    MFH_TRY(MFH_CHECK_LAUNCH("group_norm_join", stream));
+    with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
+        using T = decltype(zero);
+        launch(apply_forward_kernel<T, decltype(pack)::value, decltype(silu)::value>, groups, SPLIT_THREADS, 0, stream,
+               static_cast<const T*>(x), static_cast<T*>(y), s, block, runs, f);
+    });
+    return MFH_CHECK_LAUNCH("group_norm_apply", stream);
 }
 
 int launch_group_norm_backward(const GroupNormShape& s, int type, const void* x, const void* dy, void* dx,
                                const GroupNormBackward& b, hipStream_t stream) {
-    with_type_and_act(type, b.act, [&](auto zero, auto act) {
-        using T = decltype(zero);
-        if (dx)
-            launch(group_norm_dx_kernel<T, decltype(act)::value>, static_cast<unsigned>(s.n * s.groups), NORM_THREADS, 0,
-                   stream, static_cast<const T*>(x), static_cast<const T*>(dy), static_cast<T*>(dx), s, b);
-        if (b.gamma_grad || b.beta_grad)
-            launch(group_norm_params_kernel<T, decltype(act)::value>, static_cast<unsigned>(s.channels), NORM_THREADS, 0,
-                   stream, static_cast<const T*>(x), static_cast<const T*>(dy), s, b);
-    });
-    return MFH_CHECK_LAUNCH("group_norm_backward", stream);
+    const bool parameters = b.gamma_grad || b.beta_grad;
+    float* columns = static_cast<float*>(b.workspace);
+    if (s.n > 0) {
+        const GroupNormPlan plan = group_norm_plan(s, type_bytes(type), true);
+        MFH_TRY(require_grid(s, plan));
+        const Block block = block_of(plan);
+        const Runs runs{plan.runs, plan.rows};
+        const unsigned groups = static_cast<unsigned>(s.n * plan.grid());
+        float* run_columns = columns + columns_floats(s);
+        with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
+            using T = decltype(zero);
+            constexpr int VW = decltype(pack)::value, HOLD = group_norm_hold(sizeof(T), VW, true);
+            constexpr bool SILU = decltype(silu)::value;
+            const T *in = static_cast<const T*>(x), *grad = static_cast<const T*>(dy);
+            if (plan.held && plan.threads == 256)
+                launch(held_backward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, grad, static_cast<T*>(dx), s,
+                       block, b, parameters ? columns : nullptr);
+            else if (plan.held)
+                launch(held_backward_kernel<T, VW, SILU, 1024, HOLD>, groups, 1024, 0, stream, in, grad, static_cast<T*>(dx), s,
+                       block, b, parameters ? columns : nullptr);
+            else
+                launch(run_gradients_kernel<T, VW, SILU>, groups, SPLIT_THREADS, 0, stream, in, grad, s, block, runs,
+                       b, run_columns);
+        });
+        MFH_TRY(MFH_CHECK_LAUNCH("group_norm_backward", stream));
+        if (!plan.held) {
+            const int tiles = static_cast<int>(blocks_for(2LL * s.channels, COLUMN_SPAN));
+            launch(join_columns_kernel, static_cast<unsigned>(s.n * tiles), COLUMN_SPAN * COLUMN_RUNS, 0, stream, run_columns,
+                   plan.runs, 2 * s.channels, tiles, columns);
+            MFH_TRY(MFH_CHECK_LAUNCH("group_norm_join_columns", stream));
+            if (dx) {
+                with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
+                    using T = decltype(zero);
+                    launch(apply_backward_kernel<T, decltype(pack)::value, decltype(silu)::value>, groups, SPLIT_THREADS, 0,
+                           stream, static_cast<const T*>(x), static_cast<const T*>(dy), static_cast<T*>(dx), s, block,
+                           runs, b, columns);
+                });
+                MFH_TRY(MFH_CHECK_LAUNCH("group_norm_apply_backward", stream));
+            }
+        }
+    }
+    if (!parameters) return OK;
+    launch(parameter_grads_kernel, blocks_for(2LL * s.channels, COLUMN_SPAN), COLUMN_SPAN * COLUMN_RUNS, 0, stream, columns, s, b);
+    return MFH_CHECK_LAUNCH("group_norm_parameter_grads", stream);
 }
 
 }  // namespace mfh

@@ -1,0 +1,115 @@
+// How the group norm kernels divide their work: pure host arithmetic on sizes.
+#pragma once
+
+#include <algorithm>
+#include <cstdint>
+
+namespace mfh {
+
+struct GroupNormShape {
+    std::int64_t n;
+    int positions, channels, groups;
+};
+
+// A block is what one workgroup takes of a row: `groups` whole groups, or, where a group is wider than a
+// workgroup, one of `parts` pieces of a group. Threads lie over it in `lanes` (a power of two) side by side, a
+// pack of `vw` channels each (those beyond the block idle), threads / lanes rows at a time.
+struct GroupNormPlan {
+    bool held;       // a workgroup holds its block over all positions
+    int threads;
+    int vw;          // channels of a pack: a pack lies within a row and within a block
+    int per;         // channels of a group
+    int groups;      // whole groups of a block (1 when parts > 1)
+    int parts;       // blocks of a group
+    int width;       // channels of a block (the last part of a group may hold fewer)
+    int blocks;      // blocks of a sample
+    int lanes_log2;
+    int runs, rows;  // split: runs of a sample's positions, and positions of a run
+    std::int64_t grid() const { return blocks * static_cast<std::int64_t>(held ? 1 : runs); }  // workgroups of a sample
+};
+
+constexpr int GROUP_NORM_BLOCK_GROUPS = 256;  // at most, so that a thread a group suffices
+constexpr int GROUP_NORM_SPLIT_THREADS = 256, GROUP_NORM_SPLIT_AHEAD = 4;  // rows that a thread reads ahead
+
+// Packs that a thread holds of x (and, backward, of dy): as many as leave 1024 threads their 128 registers
+// without spills beside the statistics of a pack's channels.
+constexpr int group_norm_hold(int type_size, int vw, bool backward) {
+    if (vw * type_size < 16) return backward ? 16 : 24;
+    return type_size == 4 ? 8 : backward ? 4 : 6;
+}
+
+// A pack of 16 bytes, a 4-byte pair of a half type, or one element: the widest that divides `channels`.
+inline int group_norm_pack(int type_size, int channels) {
+    const int wide = 16 / type_size;
+    if (channels % wide == 0) return wide;
+    return type_size == 2 && channels % 2 == 0 ? 2 : 1;
+}
+
+inline int log2_up(int value) {
+    int log2 = 0;
+    while ((1 << log2) < value) ++log2;
+    return log2;
+}
+
+inline void group_norm_block(const GroupNormShape& s, int groups, int vw, GroupNormPlan* plan) {
+    plan->vw = vw, plan->per = s.channels / s.groups, plan->groups = groups, plan->parts = 1;
+    plan->width = groups * plan->per, plan->blocks = s.groups / groups;
+    plan->lanes_log2 = log2_up(plan->width / vw);
+}
+
+// Whether `threads` threads hold a block of `groups` groups over all positions.
+inline bool group_norm_holds(const GroupNormShape& s, int type_size, bool backward, int groups, int threads,
+                             GroupNormPlan* plan) {
+    const int width = groups * (s.channels / s.groups), vw = group_norm_pack(type_size, width);
+    if (width / vw > threads || groups > GROUP_NORM_BLOCK_GROUPS) return false;
+    const int rows = (threads >> log2_up(width / vw)) * group_norm_hold(type_size, vw, backward);
+    if (rows < s.positions) return false;
+    group_norm_block(s, groups, vw, plan);
+    plan->held = true, plan->threads = threads;
+    return true;
+}
+
+inline GroupNormPlan group_norm_plan(const GroupNormShape& s, int type_size, bool backward) {
+    constexpr int FILL = 256;        // workgroups that fill the CUs
+    constexpr int LINE_BYTES = 128;  // a cache line
+    constexpr int RUN_GROUPS = 2048; // workgroups of a split pass: eight a CU
+    GroupNormPlan plan{};
+    const int per = s.channels / s.groups;
+    // Held: whole groups side by side until a block's row fills a cache line and the block two packs a thread of
+    // 256, as long as the blocks fill the CUs.
+    for (int groups = 1; groups <= s.groups; ++groups) {
+        if (s.groups % groups) continue;
+        if (groups > 1 && s.n * (s.groups / groups) < FILL) break;
+        if (!group_norm_holds(s, type_size, backward, groups, 256, &plan) &&
+            !group_norm_holds(s, type_size, backward, groups, 1024, &plan))
+            break;
+        if (groups * per * type_size >= LINE_BYTES && static_cast<std::int64_t>(s.positions) * (plan.width / plan.vw) >= 512)
+            break;
+    }
+    if (plan.held) return plan;
+    // Split: as many whole groups as a workgroup's row takes, in the widest pack that allows one; else parts.
+    plan.threads = GROUP_NORM_SPLIT_THREADS;
+    int groups = 0, vw = 0;
+    for (const int pack : {group_norm_pack(type_size, s.channels), group_norm_pack(type_size, per)}) {
+        if (groups) break;
+        vw = pack;
+        for (int g = 1; g <= std::min(s.groups, GROUP_NORM_BLOCK_GROUPS); ++g)
+            if (s.groups % g == 0 && static_cast<std::int64_t>(g) * per <= plan.threads * vw && (g * per) % vw == 0) groups = g;
+    }
+    group_norm_block(s, std::max(groups, 1), vw, &plan);
+    if (!groups) {
+        plan.width = plan.threads * vw;
+        plan.parts = (per + plan.width - 1) / plan.width;
+        plan.blocks = s.groups * plan.parts;
+        plan.lanes_log2 = log2_up(plan.threads);
+    }
+    const int step = (plan.threads >> plan.lanes_log2) * GROUP_NORM_SPLIT_AHEAD;
+    const std::int64_t most = (s.positions + static_cast<std::int64_t>(step) - 1) / step;
+    const std::int64_t wanted = std::max<std::int64_t>(1, RUN_GROUPS / (s.n * plan.blocks));
+    const std::int64_t count = std::min(most, wanted);
+    plan.rows = static_cast<int>((s.positions + count - 1) / count);
+    plan.runs = (s.positions + plan.rows - 1) / plan.rows;
+    return plan;
+}
+
+}  // namespace mfh

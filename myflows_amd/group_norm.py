@@ -23,7 +23,7 @@ from .layers import Layer, _count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 3}
 CHANNELS_LIMIT = 1 << 16
-COLUMNS_LIMIT = 1 << 23  # samples times channels
+COLUMNS_LIMIT = 1 << 28  # samples times channels
 
 
 def _activations(value, name, like=None):
