@@ -573,7 +573,8 @@ MFH_API int mfh_row_mean(uint64_t values, uint64_t tokens, int tokens_int64, int
 /* ---- group norm ------------------------------------------------------------------------------ */
 
 /* Bytes of workspace of mfh_group_norm_forward (backward 0) or mfh_group_norm_backward (backward 1), -1 when
- * the sizes are out of range (a sample of at most 2^31 - 1 elements, n * channels at most 2^28). */
+ * the sizes are out of range (a sample of at most 2^30 positions and 2^31 - 1 elements, n * channels at most
+ * 2^28). */
 MFH_API int64_t mfh_group_norm_workspace(int64_t n, int positions, int channels, int groups, int type, int backward);
 
 /* Group norm over (positions, channels / groups) of each sample and group of a channels-last tensor

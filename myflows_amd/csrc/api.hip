@@ -115,7 +115,8 @@ int require_group_norm(const GroupNormShape& s, int type, int activation) {
     MFH_REQUIRE(type_valid(type), "unknown element type");
     MFH_REQUIRE(s.n >= 0 && s.positions > 0 && s.channels > 0 && s.groups > 0, "group norm sizes must be positive");
     MFH_REQUIRE(s.channels % s.groups == 0, "the channels must divide into the groups");
-    MFH_REQUIRE(static_cast<std::int64_t>(s.positions) * s.channels <= INDEX_LIMIT,
+    MFH_REQUIRE(s.positions <= GROUP_NORM_POSITIONS_LIMIT &&
+                    static_cast<std::int64_t>(s.positions) * s.channels <= INDEX_LIMIT,
                 "a sample of the group norm exceeds int32 indexing");
     MFH_REQUIRE(s.channels <= GROUP_NORM_CHANNELS_LIMIT && s.n <= INDEX_LIMIT && s.n * s.channels <= GROUP_NORM_COLUMNS_LIMIT,
                 "samples or channels of the group norm out of range");

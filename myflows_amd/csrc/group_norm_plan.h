@@ -6,6 +6,8 @@
 
 namespace mfh {
 
+constexpr int GROUP_NORM_POSITIONS_LIMIT = 1 << 30;  // the kernels' row numbers go a few thousand beyond the last
+
 struct GroupNormShape {
     std::int64_t n;
     int positions, channels, groups;
@@ -108,7 +110,7 @@ inline GroupNormPlan group_norm_plan(const GroupNormShape& s, int type_size, boo
     const std::int64_t wanted = std::max<std::int64_t>(1, RUN_GROUPS / (s.n * plan.blocks));
     const std::int64_t count = std::min(most, wanted);
     plan.rows = static_cast<int>((s.positions + count - 1) / count);
-    plan.runs = (s.positions + plan.rows - 1) / plan.rows;
+    plan.runs = static_cast<int>((s.positions + static_cast<std::int64_t>(plan.rows) - 1) / plan.rows);
     return plan;
 }
 

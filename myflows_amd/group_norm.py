@@ -22,6 +22,7 @@ from .graph import GradientOp, Variable
 from .layers import Layer, _count
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 3}
+POSITIONS_LIMIT = 1 << 30
 CHANNELS_LIMIT = 1 << 16
 COLUMNS_LIMIT = 1 << 28  # samples times channels
 
@@ -46,8 +47,8 @@ def _sizes(shape, groups):
     groups = int(groups)
     if groups < 1 or channels < 1 or channels % groups:
         raise ValueError(f"the {channels} channels must divide into {groups} groups")
-    if positions < 1:
-        raise ValueError("group norm needs at least one position")
+    if not 1 <= positions <= POSITIONS_LIMIT:
+        raise ValueError(f"group norm takes 1 to {POSITIONS_LIMIT} positions")
     native._within_int32(sample=positions * channels)
     if channels > CHANNELS_LIMIT or n * channels > COLUMNS_LIMIT:
         raise ValueError(f"group norm takes at most {CHANNELS_LIMIT} channels and {COLUMNS_LIMIT} channels over all samples")
