@@ -146,21 +146,17 @@ struct Thread {
     }
 };
 
-// Keeps held packs packed: without it the compiler holds the floats of the first pass over them for the second,
-// at twice the registers.
 template <typename T, int VW, int HOLD>
-__device__ __forceinline__ void keep_packed(Pack<T, VW> (&held)[HOLD]) {
-    if constexpr (sizeof(T) == 2 && VW > 1) {
-        constexpr int WORDS = VW / 2;
+__device__ __forceinline__ void stay_packed(Pack<T, VW> (&held)[HOLD]) {
 #pragma unroll
-        for (int h = 0; h < HOLD; ++h) {
-            unsigned w[WORDS];
-            __builtin_memcpy(w, &held[h], sizeof(w));
+    for (int h = 0; h < HOLD; ++h) held[h].stay_packed();
+}
+
+template <typename T, int VW>
+__device__ __forceinline__ void add_pack(float (&out)[VW], const T* from) {
+    const Pack<T, VW> old = load_pack<T, VW>(from);
 #pragma unroll
-            for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
-            __builtin_memcpy(&held[h], w, sizeof(w));
-        }
-    }
+    for (int i = 0; i < VW; ++i) out[i] += old.at(i);
 }
 
 // Neighbouring blocks of a sample share cache lines where a block's row is narrower than one: the workgroups
@@ -193,7 +189,7 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
         if (t.active && t.row + h * t.step < s.positions)
 #pragma unroll
             for (int i = 0; i < VW; ++i) sum[i] += held[h].at(i);
-    keep_packed(held);
+    stay_packed(held);
     group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, sum, mean);
     const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
 #pragma unroll
@@ -208,7 +204,7 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
                 squares[i] += d * d;
             }
     float variance[VW];
-    keep_packed(held);
+    stay_packed(held);
     group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, squares, variance);
     if (static_cast<int>(threadIdx.x) < k.groups)
         f.inv_std[n * s.groups + place.group + threadIdx.x] = 1.0f / sqrtf(sums[threadIdx.x] * inv_count + f.eps);
@@ -219,10 +215,10 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
     for (int h = 0; h < HOLD; ++h) {
         const int row = t.row + h * t.step;
         if (t.active && row < s.positions) {
-            Pack<T, VW> out;
+            float out[VW];
 #pragma unroll
-            for (int i = 0; i < VW; ++i) out.set(i, activate<SILU>((held[h].at(i) - mean[i]) * a[i] + beta[i], floor));
-            store_pack(y + base + row * s.channels, out);
+            for (int i = 0; i < VW; ++i) out[i] = activate<SILU>((held[h].at(i) - mean[i]) * a[i] + beta[i], floor);
+            store_pack(y + base + row * s.channels, Pack<T, VW>::of(out));
         }
     }
 }
@@ -276,8 +272,8 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
                 sum[i] += e.du;
                 product[i] += e.du * e.hat;
             }
-    keep_packed(held);
-    keep_packed(grad);
+    stay_packed(held);
+    stay_packed(grad);
     Sums::put(k, first, sum);
     Sums::put(k, second, product);
     __syncthreads();
@@ -324,15 +320,14 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
         const int row = t.row + h * t.step;
         if (t.active && row < s.positions) {
             T* to = dx + base + row * s.channels;
-            Pack<T, VW> out, old;
-            if (b.add_x) old = load_pack<T, VW>(to);
+            float out[VW];
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 const Backward<SILU> e = form(h, i);
-                const float v = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
-                out.set(i, b.add_x ? old.at(i) + v : v);
+                out[i] = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
             }
-            store_pack(to, out);
+            if (b.add_x) add_pack(out, to);
+            store_pack(to, Pack<T, VW>::of(out));
         }
     }
 }
@@ -476,10 +471,10 @@ __global__ __launch_bounds__(SPLIT_THREADS) void apply_forward_kernel(const T* _
 #pragma unroll
     for (int i = 0; i < VW; ++i) a[i] *= inv[i];
     const auto write = [&](int row, const Pack<T, VW>& in) {
-        Pack<T, VW> out;
+        float out[VW];
 #pragma unroll
-        for (int i = 0; i < VW; ++i) out.set(i, activate<SILU>((in.at(i) - mean[i]) * a[i] + beta[i], floor));
-        store_pack(y + base + row * s.channels, out);
+        for (int i = 0; i < VW; ++i) out[i] = activate<SILU>((in.at(i) - mean[i]) * a[i] + beta[i], floor);
+        store_pack(y + base + row * s.channels, Pack<T, VW>::of(out));
     };
     int row = r.begin + t.row;
     for (; row + (SPLIT_AHEAD - 1) * t.step < r.end; row += SPLIT_AHEAD * t.step) {
@@ -635,15 +630,14 @@ __global__ __launch_bounds__(SPLIT_THREADS) void apply_backward_kernel(const T* 
     const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
     const auto write = [&](int row, const Pack<T, VW>& in, const Pack<T, VW>& grad) {
         T* to = dx + base + row * s.channels;
-        Pack<T, VW> out, old;
-        if (b.add_x) old = load_pack<T, VW>(to);
+        float out[VW];
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
             const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], gamma[i], beta[i], floor);
-            const float v = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
-            out.set(i, b.add_x ? old.at(i) + v : v);
+            out[i] = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
         }
-        store_pack(to, out);
+        if (b.add_x) add_pack(out, to);
+        store_pack(to, Pack<T, VW>::of(out));
     };
     int row = r.begin + t.row;
     for (; row + (SPLIT_AHEAD - 1) * t.step < r.end; row += SPLIT_AHEAD * t.step) {

@@ -37,7 +37,7 @@ constexpr int GROUP_NORM_SPLIT_THREADS = 256, GROUP_NORM_SPLIT_AHEAD = 4;  // ro
 // without spills beside the statistics of a pack's channels.
 constexpr int group_norm_hold(int type_size, int vw, bool backward) {
     if (vw * type_size < 16) return backward ? 16 : 24;
-    return type_size == 4 ? 8 : backward ? 4 : 6;
+    return type_size == 2 && backward ? 5 : 8;
 }
 
 // A pack of 16 bytes, a 4-byte pair of a half type, or one element: the widest that divides `channels`.

@@ -76,17 +76,27 @@ struct RowEnd {
     __device__ __forceinline__ float log_prob(float z) const { return empty ? -INFINITY : (z - m) - ln_s; }
 };
 
-template <typename T>
-__device__ __forceinline__ void finish_log_probs(const LogProbsForward& f, const T* __restrict__ z, long long r,
+// A row's token and its logit, read ahead of the row's end.
+struct GivenToken {
+    long long token;
+    float z;
+    GivenToken() = default;
+    template <typename T>
+    __device__ __forceinline__ GivenToken(const LogProbsForward& f, const T* __restrict__ row, long long r) : token(-1), z(0.0f) {
+        if (!f.log_prob) return;
+        token = whole_at(f.tokens, f.tokens_wide, r);
+        if (token >= 0 && token < f.vocab) z = static_cast<float>(row[token]);
+    }
+};
+
+__device__ __forceinline__ void finish_log_probs(const LogProbsForward& f, long long r, const GivenToken& given,
                                                  const RowStats& row) {
     const RowEnd end(row);
     f.stats[r] = end.m;
     f.stats[f.rows + r] = end.s;
     f.log_sum[r] = end.empty ? -INFINITY : end.m + end.ln_s;
     f.entropy[r] = end.empty ? 0.0f : end.ln_s - row.t / row.s;
-    if (!f.log_prob) return;
-    const long long t = whole_at(f.tokens, f.tokens_wide, r);
-    f.log_prob[r] = t < 0 ? 0.0f : t >= f.vocab ? NOT_A_NUMBER : end.log_prob(static_cast<float>(z[t]));
+    if (f.log_prob) f.log_prob[r] = given.token < 0 ? 0.0f : given.token >= f.vocab ? NOT_A_NUMBER : end.log_prob(given.z);
 }
 
 __device__ __forceinline__ void write_top(const LogProbsForward& f, long long r, int k, unsigned long long key,
@@ -96,79 +106,127 @@ __device__ __forceinline__ void write_top(const LogProbsForward& f, long long r,
     f.top_log_probs[at] = key ? RowEnd(row).log_prob(key_value(key)) : NOT_A_NUMBER;
 }
 
-// The loss of one row, its targets and weight, by all threads of a workgroup. A row that does not count
-// (no id held, weight 0) has loss 0 and weight 0, whatever its logits hold; an id beyond the vocabulary
-// makes a counting row's loss and gradient NaN.
-template <typename T>
-__device__ __forceinline__ void finish_distill(const DistillForward& f, const T* __restrict__ z, long long r,
-                                               const RowStats& row) {
-    __shared__ long long ids[DISTILL_HELD_MAX];
-    __shared__ float probs[DISTILL_HELD_MAX];
-    const int lane = threadIdx.x;
-    const float inv_t = 1.0f / f.temperature;
-    if (lane < 64) {
-        const float ln_s = logf(row.s);
-        float most = -INFINITY, bad = 0.0f;
-        for (int k = lane; k < f.held; k += 64) {
-            const long long id = whole_at(f.ids, f.ids_wide, r * f.held + k);
-            const float u = id < 0 ? -INFINITY : f.teacher[r * f.held + k] * inv_t;
-            ids[k] = id;
-            probs[k] = u;
-            if (id >= f.vocab) bad = 1.0f;
-            most = u > most || u != u ? u : most;
+// The teacher's record of one row, by all threads of a workgroup: `read` loads it with the logits at its ids and
+// forms the teacher's probabilities and the targets, none of which needs the row's statistics; `finish` forms
+// the loss. A row that does not count (no id held, weight 0) has loss 0 and weight 0, whatever its logits hold;
+// an id beyond the vocabulary makes a counting row's loss and gradient NaN.
+template <int THREADS>
+struct TeacherRow {
+    static constexpr int EACH = DISTILL_HELD_MAX / THREADS;
+    static_assert(DISTILL_HELD_MAX % THREADS == 0, "ids are shared evenly");
+    float p[EACH], log_p[EACH], z[EACH];  // of the ids of this thread; p is 0 for none
+    float weight;
+    bool poisoned;
+
+    // The joint result of the threads' values.
+    template <typename Op>
+    static __device__ __forceinline__ float joint(float v, Op op) {
+        v = wave_reduce(v, op);
+        if constexpr (THREADS > 64) {
+            __shared__ float part[THREADS / 64];
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = v;
+            __syncthreads();
+            v = part[0];
+#pragma unroll
+            for (int w = 1; w < THREADS / 64; ++w) v = op(v, part[w]);
         }
-        for (int o = 32; o > 0; o /= 2) {
-            const float other = __shfl_xor(most, o);
-            most = other > most || other != other ? other : most;
-            bad = fmaxf(bad, __shfl_xor(bad, o));
+        return v;
+    }
+
+    template <typename T>
+    __device__ __forceinline__ void read(const DistillForward& f, const T* __restrict__ row, long long r) {
+        __shared__ int ids[DISTILL_HELD_MAX];
+        __shared__ float probs[DISTILL_HELD_MAX];
+        const int tid = threadIdx.x;
+        const float inv_t = 1.0f / f.temperature;
+        float u[EACH], most = -INFINITY, bad = 0.0f;
+        int id[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int k = tid + i * THREADS;
+            u[i] = -INFINITY;
+            z[i] = 0.0f;
+            id[i] = -1;
+            if (k >= f.held) continue;
+            const long long given = whole_at(f.ids, f.ids_wide, r * f.held + k);
+            if (given < 0) continue;
+            u[i] = f.teacher[r * f.held + k] * inv_t;
+            if (given >= f.vocab) {
+                bad = 1.0f;
+                continue;
+            }
+            id[i] = static_cast<int>(given);
+            z[i] = static_cast<float>(row[given]);
         }
+        const auto larger = [](float a, float b) { return b > a || b != b ? b : a; };  // a NaN wins
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) most = larger(most, u[i]);
+        most = joint(most, larger);
+        bad = joint(bad, [](float a, float b) { return fmaxf(a, b); });
         float sum = 0.0f;
-        if (most > -INFINITY || most != most) {
-            for (int k = lane; k < f.held; k += 64) sum += exp2_of((probs[k] - most) * LOG2E);
-            for (int o = 32; o > 0; o /= 2) sum += __shfl_xor(sum, o);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            // Teacher logits of -inf alone leave no target (and -inf - -inf would not be a number).
+            p[i] = most == -INFINITY ? 0.0f : exp2_of((u[i] - most) * LOG2E);
+            sum += p[i];
         }
-        const bool counts = sum != 0.0f && (!f.row_weights || f.row_weights[r] != 0.0f);
+        sum = joint(sum, [](float a, float b) { return a + b; });
+        weight = sum == 0.0f ? 0.0f : f.row_weights ? f.row_weights[r] : 1.0f;
+        poisoned = weight != 0.0f && bad != 0.0f;
         const float ln_sum = logf(sum);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int k = tid + i * THREADS;
+            p[i] = weight == 0.0f ? 0.0f : p[i] / sum;
+            log_p[i] = u[i] - most - ln_sum;
+            if (k < f.held) {
+                ids[k] = id[i];
+                probs[k] = p[i];
+            }
+        }
+        __syncthreads();
+        // An id that the record holds twice has the sum of its probabilities as its target.
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int k = tid + i * THREADS;
+            if (k >= f.held) break;
+            float target = 0.0f;
+            for (int other = 0; other < f.held; ++other) target += ids[other] == id[i] ? probs[other] : 0.0f;
+            f.targets[r * f.held + k] = target;
+        }
+    }
+
+    __device__ __forceinline__ void finish(const DistillForward& f, long long r, const RowStats& row) {
+        const float inv_t = 1.0f / f.temperature, ln_s = logf(row.s);
         float loss = 0.0f;
-        for (int k = lane; k < f.held; k += 64) {
-            const float d = probs[k] - most;
-            const float p = counts ? exp2_of(d * LOG2E) / sum : 0.0f;
-            probs[k] = p;
-            if (p == 0.0f || ids[k] >= f.vocab) continue;
-            const float log_q = row.s == 0.0f ? -INFINITY : (static_cast<float>(z[ids[k]]) - row.m) * inv_t - ln_s;
-            loss += p * (d - ln_sum - log_q);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const float log_q = row.s == 0.0f ? -INFINITY : (z[i] - row.m) * inv_t - ln_s;
+            if (p[i] != 0.0f) loss += p[i] * (log_p[i] - log_q);
         }
-        for (int o = 32; o > 0; o /= 2) loss += __shfl_xor(loss, o);
-        if (lane == 0) {
-            const bool poisoned = counts && bad != 0.0f;
-            f.row_loss[r] = !counts ? 0.0f : poisoned ? NOT_A_NUMBER : f.temperature * f.temperature * loss;
-            f.weights[r] = !counts ? 0.0f : f.row_weights ? f.row_weights[r] : 1.0f;
-            f.stats[r] = row.m;
-            f.stats[f.rows + r] = poisoned ? NOT_A_NUMBER : row.s;
-        }
+        loss = joint(loss, [](float a, float b) { return a + b; });
+        if (threadIdx.x != 0) return;
+        f.row_loss[r] = weight == 0.0f ? 0.0f : poisoned ? NOT_A_NUMBER : f.temperature * f.temperature * loss;
+        f.weights[r] = weight;
+        f.stats[r] = row.m;
+        f.stats[f.rows + r] = poisoned ? NOT_A_NUMBER : row.s;
     }
-    __syncthreads();
-    // An id that the record holds twice has the sum of its probabilities as its target.
-    for (int k = lane; k < f.held; k += blockDim.x) {
-        float p = 0.0f;
-        for (int other = 0; other < f.held; ++other) p += ids[other] == ids[k] ? probs[other] : 0.0f;
-        f.targets[r * f.held + k] = p;
-    }
-}
+};
 
 // ---- the pass over a row --------------------------------------------------------------------
-// A workgroup takes a run of a row's logits tile by tile, in 16-byte packs: each thread keeps the running
-// statistics of its own logits, and the threads' are joined once, at the end of the run. One read of the
-// logits, one exp a logit. Bound by HBM for float32; a bfloat16 or float16 logit costs about as many vector
-// instructions as the time that its two bytes take allows.
+// A workgroup takes a run of a row's logits tile by tile, in 16-byte packs, the next tile's loads in flight:
+// each thread keeps the running statistics of its own logits, and the threads' are joined once, at the end of
+// the run. One read of the logits, one exp a logit. Bound by HBM for float32; a bfloat16 or float16 logit
+// costs about as many vector instructions as the time that its two bytes take allows.
 //
 // The top alternatives come out of the same read. The k-th largest of the threads' own maxima is at most the
 // row's k-th largest logit, so only logits above that threshold can be alternatives: about k of a tile's
-// thousands. They are kept in LDS (a list of CANDIDATES), the threshold is raised as the maxima grow, and at
-// the end each candidate's rank is counted. A list that overflows (all logits equal, or rising logits) is made
+// thousands. Each wave keeps its own in a list in LDS, the threshold is raised as the maxima grow, and at the
+// end each candidate's rank is counted. A list that overflows (all logits equal, or rising logits) is made
 // again by exact_top, which needs no threshold.
 constexpr int TILE_PACKS = 4;
-constexpr int CANDIDATES = 1024;
+constexpr int CANDIDATES = 1024;  // of a workgroup, shared evenly by its waves
 
 struct RowRun {
     long long row;
@@ -183,11 +241,12 @@ struct RowPartials {
 
 template <int THREADS>
 struct TopState {
-    unsigned long long candidates[CANDIDATES];
+    static constexpr int WAVES = THREADS / 64, EACH = CANDIDATES / WAVES;
+    unsigned long long candidates[WAVES][EACH];
     unsigned long long best[2][TOP_MAX];
-    unsigned long long wave_best[THREADS / 64];
+    unsigned long long wave_best[WAVES];
     float maxima[2][THREADS];
-    int count;
+    int counts[WAVES];
 };
 
 template <typename T, int THREADS>
@@ -199,21 +258,17 @@ struct RowTile {
     static __device__ __forceinline__ int index(int base, int p, int e) {
         return base + (p * THREADS + static_cast<int>(threadIdx.x)) * N + e;
     }
-    __device__ __forceinline__ void load(const T* __restrict__ z, int base) {
+    // The tile at base; -inf past a run's end that cuts it.
+    __device__ __forceinline__ void load(const T* __restrict__ z, int base, int end) {
+        if (base + SIZE <= end) {
 #pragma unroll
-        for (int p = 0; p < TILE_PACKS; ++p) packs[p] = load_pack<T, N>(z + index(base, p, 0));
-    }
-    // A tile that the run's end cuts: -inf past the end.
-    __device__ __forceinline__ void load_cut(const T* __restrict__ z, int base, int end) {
+            for (int p = 0; p < TILE_PACKS; ++p) packs[p] = load_pack<T, N>(z + index(base, p, 0));
+            return;
+        }
 #pragma unroll
         for (int p = 0; p < TILE_PACKS; ++p) {
             const int at = index(base, p, 0);
-            if (at + N <= end) {
-                packs[p] = load_pack<T, N>(z + at);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e) packs[p].v[e] = at + e < end ? z[at + e] : static_cast<T>(-INFINITY);
-            }
+            packs[p] = at + N <= end ? load_pack<T, N>(z + at) : load_part<T, N>(z + at, end - at, -INFINITY);
         }
     }
 };
@@ -224,16 +279,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-template <int COUNT>
-__device__ __forceinline__ float largest(const float (&x)[COUNT]) {
-    float m[2] = {x[0], x[1]};
+template <typename T, int N>
+__device__ __forceinline__ float largest(const Pack<T, N>& pack) {
+    static_assert(N % 4 == 0, "two chains of pairs");
+    float a = fmaxf(pack.at(0), pack.at(1)), b = fmaxf(pack.at(2), pack.at(3));
 #pragma unroll
-    for (int i = 2; i + 3 < COUNT; i += 4) {
-        m[0] = max3(m[0], x[i], x[i + 1]);
-        m[1] = max3(m[1], x[i + 2], x[i + 3]);
+    for (int i = 4; i < N; i += 4) {
+        a = max3(a, pack.at(i), pack.at(i + 1));
+        b = max3(b, pack.at(i + 2), pack.at(i + 3));
     }
-    static_assert(COUNT % 4 == 0, "pairs of pairs");
-    return max3(fmaxf(m[0], m[1]), x[COUNT - 2], x[COUNT - 1]);
+    return fmaxf(a, b);
 }
 
 // A float that at least k of the threads' maxima reach (the k-th largest of them, its low 16 bits cleared
@@ -250,6 +305,7 @@ __device__ __forceinline__ float kth_of_maxima(float (&maxima)[THREADS], float m
         order[i] = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
     }
     unsigned found = 0;
+#pragma unroll 1
     for (int bit = 31; bit >= 16; --bit) {
         const unsigned probe = found | (1u << bit);
         int reached = 0;
@@ -268,39 +324,38 @@ __device__ __forceinline__ float just_below(float v) {
     return __uint_as_float(v > 0.0f ? bits - 1 : v == 0.0f ? 0x80000001u : bits + 1);
 }
 
-// The k largest keys of a run in falling order, in best (0 where there are fewer), by k rounds a tile of the
-// largest key below the last, for the tiles that hold a key above the k-th best so far.
+// The k largest keys of a run in falling order (0 where there are fewer), by k rounds a tile of the largest key
+// below the last, for the tiles that hold a key above the k-th best so far. Every round reads the tile again.
 template <typename T, int THREADS>
-__device__ __forceinline__ unsigned long long* exact_top(TopState<THREADS>& top, const T* __restrict__ z,
-                                                         const RowRun& run, int k) {
-    using Tile = RowTile<T, THREADS>;
+__device__ __forceinline__ const unsigned long long* exact_top(TopState<THREADS>& top, const T* __restrict__ z,
+                                                               const RowRun& run, int k) {
+    constexpr int SIZE = THREADS * 16;
+    const int tid = threadIdx.x;
     int side = 0;
     __syncthreads();
-    if (static_cast<int>(threadIdx.x) < k) top.best[0][threadIdx.x] = 0;
+    if (tid < k) top.best[0][tid] = 0;
     __syncthreads();
-    for (int base = run.begin; base < run.end; base += Tile::SIZE) {
-        Tile tile;
-        tile.load_cut(z, base, run.end);
-        const auto key_at = [&](int p, int e) -> unsigned long long {
-            const float x = tile.packs[p].at(e);
-            const int at = Tile::index(base, p, e);
-            return x == x && at < run.end ? key_of(x, at) : 0;
-        };
-        const unsigned long long least = top.best[side][k - 1];
-        bool above = false;
-        for (int p = 0; p < TILE_PACKS; ++p)
-            for (int e = 0; e < Tile::N; ++e) above = above || key_at(p, e) > least;
-        if (!__syncthreads_or(above)) continue;
-        unsigned long long last = ~0ull;
-        for (int i = 0; i < k && last; ++i) {
+#pragma unroll 1
+    for (int base = run.begin; base < run.end; base += SIZE) {
+        const int end = min(run.end, base + SIZE);
+        // The largest key of this thread's part of the tile below `last`.
+        const auto largest_below = [&](unsigned long long last) {
             unsigned long long mine = 0;
-            for (int p = 0; p < TILE_PACKS; ++p)
-                for (int e = 0; e < Tile::N; ++e) {
-                    const unsigned long long key = key_at(p, e);
-                    if (key < last && key > mine) mine = key;
-                }
-            if (static_cast<int>(threadIdx.x) < k) {
-                const unsigned long long key = top.best[side][threadIdx.x];
+#pragma unroll 1
+            for (int at = base + tid; at < end; at += THREADS) {
+                const float x = static_cast<float>(z[at]);
+                const unsigned long long key = x == x ? key_of(x, at) : 0;
+                if (key < last && key > mine) mine = key;
+            }
+            return mine;
+        };
+        if (!__syncthreads_or(largest_below(~0ull) > top.best[side][k - 1])) continue;
+        unsigned long long last = ~0ull;
+#pragma unroll 1
+        for (int i = 0; i < k && last; ++i) {
+            unsigned long long mine = largest_below(last);
+            if (tid < k) {
+                const unsigned long long key = top.best[side][tid];
                 if (key < last && key > mine) mine = key;
             }
             for (int o = 32; o > 0; o /= 2) {
@@ -309,15 +364,14 @@ __device__ __forceinline__ unsigned long long* exact_top(TopState<THREADS>& top,
             }
             if constexpr (THREADS > 64) {
                 __syncthreads();
-                if ((threadIdx.x & 63) == 0) top.wave_best[threadIdx.x / 64] = mine;
+                if ((tid & 63) == 0) top.wave_best[tid / 64] = mine;
                 __syncthreads();
                 for (int w = 0; w < THREADS / 64; ++w)
                     if (top.wave_best[w] > mine) mine = top.wave_best[w];
             }
             last = mine;
-            if (threadIdx.x == 0) top.best[side ^ 1][i] = last;
-            if (last == 0 && static_cast<int>(threadIdx.x) > i && static_cast<int>(threadIdx.x) < k)
-                top.best[side ^ 1][threadIdx.x] = 0;
+            if (tid == 0) top.best[side ^ 1][i] = last;
+            if (last == 0 && tid > i && tid < k) top.best[side ^ 1][tid] = 0;
         }
         side ^= 1;
         __syncthreads();
@@ -327,24 +381,46 @@ __device__ __forceinline__ unsigned long long* exact_top(TopState<THREADS>& top,
 
 // Takes every candidate to its rank: emit(rank, key) for the k largest, emit(rank, 0) for those that are missing.
 // Fewer than k candidates mean that all logits above -inf are candidates: the first -inf of the run follow.
+// `mine` is the number of the wave's candidates.
 template <typename T, int THREADS, typename Emit>
 __device__ __forceinline__ void emit_top(TopState<THREADS>& top, const T* __restrict__ z, const RowRun& run, int k,
-                                         float s, Emit&& emit) {
+                                         int mine, float s, Emit&& emit) {
+    using Top = TopState<THREADS>;
+    if ((threadIdx.x & 63) == 0) top.counts[threadIdx.x / 64] = mine;
     __syncthreads();
-    const int count = top.count;
-    if (count > CANDIDATES || s != s) {  // a NaN among a thread's logits leaves its maximum open
+    int counts[Top::WAVES], count = 0;
+    bool exact = s != s;  // a NaN among a thread's logits leaves its maximum open
+#pragma unroll
+    for (int w = 0; w < Top::WAVES; ++w) {
+        counts[w] = __builtin_amdgcn_readfirstlane(top.counts[w]);
+        count += counts[w];
+        exact = exact || counts[w] > Top::EACH;
+    }
+    if (exact) {
         const unsigned long long* best = exact_top(top, z, run, k);
         if (static_cast<int>(threadIdx.x) < k) emit(static_cast<int>(threadIdx.x), best[threadIdx.x]);
         return;
     }
+#pragma unroll 1
     for (int i = threadIdx.x; i < count; i += THREADS) {
-        const unsigned long long key = top.candidates[i];
+        int wave = 0, at = i;
+#pragma unroll
+        for (int w = 0; w + 1 < Top::WAVES; ++w)
+            if (wave == w && at >= counts[w]) {
+                at -= counts[w];
+                wave = w + 1;
+            }
+        const unsigned long long key = top.candidates[wave][at];
         int rank = 0;
-        for (int j = 0; j < count; ++j) rank += top.candidates[j] > key;
+#pragma unroll
+        for (int w = 0; w < Top::WAVES; ++w)
+#pragma unroll 4
+            for (int j = 0; j < counts[w]; ++j) rank += top.candidates[w][j] > key;
         if (rank < k) emit(rank, key);
     }
     if (count >= k || threadIdx.x >= 64) return;
     int next = count;
+#pragma unroll 1
     for (int base = run.begin; base < run.end && next < k; base += 64) {
         const int at = base + static_cast<int>(threadIdx.x);
         const bool ruled = at < run.end && static_cast<float>(z[at]) == -INFINITY;
@@ -356,74 +432,91 @@ __device__ __forceinline__ void emit_top(TopState<THREADS>& top, const T* __rest
     for (int rank = next + static_cast<int>(threadIdx.x); rank < k; rank += 64) emit(rank, 0);
 }
 
-// One tile into the thread's statistics and, with TOP, the list of candidates: those above `below`.
+// What a thread carries through the tiles of a run.
+struct RowState {
+    RowStats mine;
+    float below;  // candidates lie above this
+    int count;    // of the wave's candidates
+};
+
+// One tile into the thread's statistics and, with TOP, the wave's list of candidates.
 template <bool ENTROPY, bool TOP, typename T, int THREADS>
-__device__ __forceinline__ void take_tile(const RowTile<T, THREADS>& tile, RowStats& mine, float scale, int base, int end,
-                                          TopState<THREADS>* top, int top_k, float& below, int number) {
+__device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& state, float scale, int base,
+                                          TopState<THREADS>* top, int top_k, int number) {
     using Tile = RowTile<T, THREADS>;
-    constexpr int COUNT = TILE_PACKS * Tile::N;
-    float x[COUNT];
+    float pack_max[TILE_PACKS];
+#pragma unroll
+    for (int p = 0; p < TILE_PACKS; ++p) pack_max[p] = largest(tile.packs[p]);
+    static_assert(TILE_PACKS == 4, "the packs' maxima");
+    const float tile_max = fmaxf(max3(pack_max[0], pack_max[1], pack_max[2]), pack_max[3]);
+    const float to = fmaxf(state.mine.m, tile_max);
+    if constexpr (TOP) {
+#pragma unroll
+        for (int p = 0; p < TILE_PACKS; ++p) tile.packs[p].stay_packed();
+        // The threshold after the first tile, then raised at the tiles 1, 4, 16, ...: each time the candidates
+        // to come are at most those of the tiles so far, three times over.
+        if (number == 0) {
+            const float kth = kth_of_maxima(top->maxima[0], tile_max, top_k);
+            state.below = kth == -INFINITY ? kth : just_below(kth);
+        }
+        using Top = TopState<THREADS>;
+        unsigned long long* list = top->candidates[threadIdx.x / 64];
+        const unsigned long long before = (1ull << (threadIdx.x & 63)) - 1;
+#pragma unroll
+        for (int p = 0; p < TILE_PACKS; ++p) {
+            if (!__any(pack_max[p] > state.below)) continue;
+#pragma unroll
+            for (int e = 0; e < Tile::N; ++e) {
+                const float x = tile.packs[p].at(e);
+                const unsigned long long who = __ballot(x > state.below);
+                if (!who) continue;
+                const int slot = state.count + __popcll(who & before);
+                if (x > state.below && slot < Top::EACH) list[slot] = key_of(x, Tile::index(base, p, e));
+                state.count += __popcll(who);
+            }
+        }
+        if (number > 0 && (number & (number - 1)) == 0 && (__ffs(number) & 1)) {
+            const float kth = kth_of_maxima(top->maxima[((__ffs(number) >> 1) + 1) & 1], to > LOWEST ? to : -INFINITY, top_k);
+            state.below = fmaxf(state.below, kth);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < TILE_PACKS; ++p) tile.packs[p].stay_packed();
+    state.mine.rescale(to, scale);
 #pragma unroll
     for (int p = 0; p < TILE_PACKS; ++p)
 #pragma unroll
-        for (int e = 0; e < Tile::N; ++e) x[p * Tile::N + e] = tile.packs[p].at(e);
-    const float tile_max = largest(x);
-    const float to = fmaxf(mine.m, tile_max);
-    if constexpr (TOP) {
-        // The threshold after the first tile, then raised at the tiles 1, 4, 16, ...: each time the candidates
-        // to come are at most those of the tiles so far, three times over.
-        const bool first = number == 0;
-        if (first) {
-            const float kth = kth_of_maxima(top->maxima[0], tile_max, top_k);
-            below = kth == -INFINITY ? kth : just_below(kth);
+        for (int e = 0; e < Tile::N; ++e) {
+            const float d = tile.packs[p].at(e) - state.mine.m;
+            const float part = exp2_of(d * scale);
+            state.mine.s += part;
+            if constexpr (ENTROPY) state.mine.t += part * fmaxf(d, DIFFERENCE_FLOOR);
         }
-        if (tile_max > below) {
-#pragma unroll
-            for (int i = 0; i < COUNT; ++i)
-                if (x[i] > below) {
-                    const int slot = atomicAdd(&top->count, 1);
-                    if (slot < CANDIDATES)
-                        top->candidates[slot] = key_of(x[i], Tile::index(base, i / Tile::N, i % Tile::N));
-                }
-        }
-        if (!first && (number & (number - 1)) == 0 && (__ffs(number) & 1)) {
-            const float kth = kth_of_maxima(top->maxima[(__ffs(number) >> 1) + 1 & 1], to > LOWEST ? to : -INFINITY, top_k);
-            below = fmaxf(below, kth);
-        }
-    }
-    mine.rescale(to, scale);
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-        const float d = x[i] - mine.m;
-        const float e = exp2_of(d * scale);
-        mine.s += e;
-        if constexpr (ENTROPY) mine.t += e * fmaxf(d, DIFFERENCE_FLOOR);
-    }
 }
 
-// The statistics of a run, the same in every thread.
-template <bool ENTROPY, bool TOP, typename T, int THREADS>
+// The statistics of a run, the same in every thread, and the number of the wave's candidates. `meanwhile` runs
+// while the first tile's loads are in flight.
+template <bool ENTROPY, bool TOP, typename T, int THREADS, typename Meanwhile>
 __device__ __forceinline__ RowStats take_run(const T* __restrict__ z, const RowRun& run, float scale, TopState<THREADS>* top,
-                                             int top_k) {
+                                             int top_k, int& count, Meanwhile&& meanwhile) {
     using Tile = RowTile<T, THREADS>;
     __shared__ RowStats waves[THREADS / 64];
     __shared__ float wave_m[THREADS / 64];
-    if constexpr (TOP) {
-        if (threadIdx.x == 0) top->count = 0;  // before the barrier of the first threshold
-    }
-    RowStats mine = RowStats::none();
-    float below = -INFINITY;
+    RowState state{RowStats::none(), -INFINITY, 0};
+    Tile tile;
+    tile.load(z, run.begin, run.end);
+    meanwhile();
     int base = run.begin, number = 0;
-    for (; base + Tile::SIZE <= run.end; base += Tile::SIZE, ++number) {
-        Tile tile;
-        tile.load(z, base);
-        take_tile<ENTROPY, TOP>(tile, mine, scale, base, run.end, top, top_k, below, number);
+#pragma unroll 1
+    for (; base + Tile::SIZE < run.end; base += Tile::SIZE, ++number) {
+        Tile next;
+        next.load(z, base + Tile::SIZE, run.end);
+        take_tile<ENTROPY, TOP>(tile, state, scale, base, top, top_k, number);
+        tile = next;
     }
-    if (base < run.end) {
-        Tile tile;
-        tile.load_cut(z, base, run.end);
-        take_tile<ENTROPY, TOP>(tile, mine, scale, base, run.end, top, top_k, below, number);
-    }
+    take_tile<ENTROPY, TOP>(tile, state, scale, base, top, top_k, number);
+    count = state.count;
+    RowStats mine = state.mine;
     float m = wave_max(mine.m);
     if constexpr (THREADS > 64) {
         if ((threadIdx.x & 63) == 0) wave_m[threadIdx.x / 64] = m;
@@ -464,22 +557,28 @@ __global__ __launch_bounds__(THREADS) void log_probs_kernel(const T* __restrict_
     __shared__ TopState<TOP ? THREADS : 64> top;
     const RowRun run = run_of(split, f.vocab);
     const T* __restrict__ z = logits + run.row * f.stride;
+    const long long at = run.row * split.chunks + run.chunk;
+    GivenToken given{};
+    int count = 0;
+    const auto meanwhile = [&] {
+        if (split.chunks == 1 && threadIdx.x == 0) given = GivenToken(f, z, run.row);
+    };
     if constexpr (TOP) {
-        const RowStats row = take_run<true, true, T, THREADS>(z, run, LOG2E, &top, f.top);
+        const RowStats row = take_run<true, true, T, THREADS>(z, run, LOG2E, &top, f.top, count, meanwhile);
         if (split.chunks == 1) {
-            if (threadIdx.x == 0) finish_log_probs(f, z, run.row, row);
-            emit_top(top, z, run, f.top, row.s, [&](int rank, unsigned long long key) { write_top(f, run.row, rank, key, row); });
+            if (threadIdx.x == 0) finish_log_probs(f, run.row, given, row);
+            emit_top(top, z, run, f.top, count, row.s, [&](int rank, unsigned long long key) { write_top(f, run.row, rank, key, row); });
         } else {
-            const long long at = run.row * split.chunks + run.chunk;
             if (threadIdx.x == 0) partials.stats[at] = row;
-            emit_top(top, z, run, f.top, row.s,
+            emit_top(top, z, run, f.top, count, row.s,
                      [&](int rank, unsigned long long key) { partials.keys[at * f.top + rank] = key; });
         }
     } else {
-        const RowStats row = take_run<true, false, T, THREADS>(z, run, LOG2E, nullptr, 0);
+        const RowStats row =
+            take_run<true, false, T, THREADS>(z, run, LOG2E, static_cast<TopState<THREADS>*>(nullptr), 0, count, meanwhile);
         if (threadIdx.x != 0) return;
-        if (split.chunks == 1) finish_log_probs(f, z, run.row, row);
-        else partials.stats[run.row * split.chunks + run.chunk] = row;
+        if (split.chunks == 1) finish_log_probs(f, run.row, given, row);
+        else partials.stats[at] = row;
     }
 }
 
@@ -488,8 +587,13 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const T* __restrict__ 
                                                           RowPartials partials) {
     const RowRun run = run_of(split, f.vocab);
     const T* __restrict__ z = logits + run.row * f.stride;
-    const RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature, nullptr, 0);
-    if (split.chunks == 1) finish_distill(f, z, run.row, row);
+    int count;
+    TeacherRow<THREADS> teacher;
+    const RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature,
+                                                            static_cast<TopState<THREADS>*>(nullptr), 0, count, [&] {
+                                                                if (split.chunks == 1) teacher.read(f, z, run.row);
+                                                            });
+    if (split.chunks == 1) teacher.finish(f, run.row, row);
     else if (threadIdx.x == 0) partials.stats[run.row * split.chunks + run.chunk] = row;
 }
 
@@ -534,17 +638,21 @@ __global__ __launch_bounds__(JOIN_THREADS) void log_probs_join_kernel(const T* _
     __shared__ unsigned long long maxima[JOIN_THREADS], kept[SPLIT_MAX * TOP_MAX];
     __shared__ int count;
     const long long r = blockIdx.x;
-    const RowStats row = join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E);
-    if (threadIdx.x == 0) {
-        finish_log_probs(f, logits + r * f.stride, r, row);
-        count = 0;
-    }
-    if (f.top == 0) return;
     const unsigned long long* __restrict__ keys = partials.keys + r * split.chunks * f.top;
     const int total = split.chunks * f.top;
     unsigned long long mine = 0;
     for (int i = threadIdx.x; i < total; i += JOIN_THREADS) mine = max(mine, keys[i]);
-    const unsigned long long least = max(kth_of_keys(maxima, mine, f.top), 1ull);
+    GivenToken given{};
+    if (threadIdx.x == 0) given = GivenToken(f, logits + r * f.stride, r);
+    const RowStats row = join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E);
+    if (threadIdx.x == 0) {
+        finish_log_probs(f, r, given, row);
+        count = 0;
+    }
+    if (f.top == 0) return;
+    // Keys that the k-th largest of the threads' own do not reach are none of the k largest.
+    const unsigned long long least = max(total > JOIN_THREADS ? kth_of_keys(maxima, mine, f.top) : 0ull, 1ull);
+    if (total <= JOIN_THREADS) __syncthreads();
     for (int i = threadIdx.x; i < total; i += JOIN_THREADS)
         if (keys[i] >= least) kept[atomicAdd(&count, 1)] = keys[i];
     __syncthreads();
@@ -560,8 +668,9 @@ template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(const T* __restrict__ logits, DistillForward f, RowSplit split,
                                                           RowPartials partials) {
     const long long r = blockIdx.x;
-    finish_distill(f, logits + r * f.stride, r,
-                   join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E / f.temperature));
+    TeacherRow<64> teacher;
+    teacher.read(f, logits + r * f.stride, r);
+    teacher.finish(f, r, join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E / f.temperature));
 }
 
 // ---- the gradients --------------------------------------------------------------------------
@@ -594,14 +703,13 @@ __device__ __forceinline__ void form_span(const T* z, T* out, int first, int voc
     for (int p = 0; p < GRAD_PACKS; ++p) {
         const int at = base + p * GRAD_THREADS * N;
         if (at + N <= vocab) {
-            Pack<T, N> result;
+            float result[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const float v = value(in[p].at(e), at + e);
-                if constexpr (ADD) result.set(e, old[p].at(e) + v);
-                else result.set(e, v);
+                result[e] = value(in[p].at(e), at + e);
+                if constexpr (ADD) result[e] += old[p].at(e);
             }
-            store_pack(out + at, result);
+            store_pack(out + at, Pack<T, N>::of(result));
         } else {
             for (int j = at; j < vocab; ++j) {
                 const float v = value(static_cast<float>(z[j]), j);

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace mfh {
 
@@ -21,13 +22,46 @@ auto with_type(int type, F&& f) {
     return f(float{});
 }
 
-// N elements that one load or store moves. The address need only be aligned to one element: global memory
-// takes 16-byte accesses at any address.
+// N elements that one load or store moves, half types two to a word. The address need only be aligned to one
+// element: global memory takes 16-byte accesses at any address.
 template <typename T, int N>
 struct Pack {
-    T v[N];
-    __device__ __forceinline__ float at(int i) const { return static_cast<float>(v[i]); }
-    __device__ __forceinline__ void set(int i, float x) { v[i] = static_cast<T>(x); }
+    static constexpr bool PAIRS = sizeof(T) == 2 && N > 1;
+    static constexpr int WORDS = PAIRS ? N / 2 : N;
+    using Word = std::conditional_t<PAIRS, unsigned, T>;
+    Word w[WORDS];
+
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (!PAIRS) {
+            return static_cast<float>(w[i]);
+        } else if constexpr (std::is_same_v<T, __bf16>) {
+            return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        } else {
+            return static_cast<float>(__builtin_bit_cast(T, static_cast<unsigned short>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+        }
+    }
+    // The floats rounded to the type.
+    static __device__ __forceinline__ Pack of(const float (&x)[N]) {
+        Pack pack;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (PAIRS) {
+                typedef T Pair __attribute__((ext_vector_type(2)));
+                pack.w[i] = __builtin_bit_cast(unsigned, Pair{static_cast<T>(x[2 * i]), static_cast<T>(x[2 * i + 1])});
+            } else {
+                pack.w[i] = static_cast<T>(x[i]);
+            }
+        }
+        return pack;
+    }
+    // Between two passes over held packs: keeps the compiler from holding the first pass's floats of half types
+    // for the second, at twice the registers.
+    __device__ __forceinline__ void stay_packed() {
+        if constexpr (PAIRS) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
+        }
+    }
 };
 
 template <typename T, int N>
@@ -35,6 +69,15 @@ __device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
     Pack<T, N> pack;
     __builtin_memcpy(&pack, p, sizeof(pack));
     return pack;
+}
+
+// The pack at p of which `count` elements (fewer than N, or none) are there; `rest` beyond them.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_part(const T* p, int count, float rest) {
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = i < count ? static_cast<float>(p[i]) : rest;
+    return Pack<T, N>::of(x);
 }
 
 template <typename T, int N>
