@@ -179,16 +179,19 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
     float sum[VW] = {}, mean[VW], squares[VW] = {}, a[VW], beta[VW];
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         const int row = t.row + h * t.step;
         if (t.active && row < s.positions) held[h] = load_pack<T, VW>(x + base + row * s.channels);
     }
     t.by_column(f.gamma + place.channel, a);
     t.by_column(f.beta + place.channel, beta);
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h)
+    for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         if (t.active && t.row + h * t.step < s.positions)
 #pragma unroll
             for (int i = 0; i < VW; ++i) sum[i] += held[h].at(i);
+    }
     stay_packed(held);
     group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, sum, mean);
     const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
@@ -196,13 +199,15 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
     for (int i = 0; i < VW; ++i) mean[i] *= inv_count;
     if (static_cast<int>(threadIdx.x) < k.groups) f.mean[n * s.groups + place.group + threadIdx.x] = sums[threadIdx.x] * inv_count;
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h)
+    for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         if (t.active && t.row + h * t.step < s.positions)
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 const float d = held[h].at(i) - mean[i];
                 squares[i] += d * d;
             }
+    }
     float variance[VW];
     stay_packed(held);
     group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, squares, variance);
@@ -213,6 +218,7 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
     const float floor = f.act == ACT_RELU ? 0.0f : -INFINITY;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         const int row = t.row + h * t.step;
         if (t.active && row < s.positions) {
             float out[VW];
@@ -249,6 +255,7 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
     float mean[VW], inv[VW], gamma[VW], beta[VW], sum[VW] = {}, product[VW] = {};
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         const int row = t.row + h * t.step;
         if (t.active && row < s.positions) {
             held[h] = load_pack<T, VW>(x + base + row * s.channels);
@@ -264,7 +271,8 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
         return Backward<SILU>(held[h].at(i), grad[h].at(i), mean[i], inv[i], gamma[i], beta[i], floor);
     };
 #pragma unroll
-    for (int h = 0; h < HOLD; ++h)
+    for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         if (t.active && t.row + h * t.step < s.positions)
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
@@ -272,6 +280,7 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
                 sum[i] += e.du;
                 product[i] += e.du * e.hat;
             }
+    }
     stay_packed(held);
     stay_packed(grad);
     Sums::put(k, first, sum);
@@ -317,6 +326,7 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
     t.by_group(sums[1], mean_p);
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
+        if (h * t.step >= s.positions) break;
         const int row = t.row + h * t.step;
         if (t.active && row < s.positions) {
             T* to = dx + base + row * s.channels;

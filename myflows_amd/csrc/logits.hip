@@ -100,10 +100,10 @@ __device__ __forceinline__ void finish_log_probs(const LogProbsForward& f, long 
 }
 
 __device__ __forceinline__ void write_top(const LogProbsForward& f, long long r, int k, unsigned long long key,
-                                          const RowStats& row) {
+                                          const RowEnd& end) {
     const long long at = r * f.top + k;
     f.top_ids[at] = key ? key_index(key) : -1;
-    f.top_log_probs[at] = key ? RowEnd(row).log_prob(key_value(key)) : NOT_A_NUMBER;
+    f.top_log_probs[at] = key ? end.log_prob(key_value(key)) : NOT_A_NUMBER;
 }
 
 // The teacher's record of one row, by all threads of a workgroup: `read` loads it with the logits at its ids and
@@ -226,7 +226,7 @@ struct TeacherRow {
 // end each candidate's rank is counted. A list that overflows (all logits equal, or rising logits) is made
 // again by exact_top, which needs no threshold.
 constexpr int TILE_PACKS = 4;
-constexpr int CANDIDATES = 1024;  // of a workgroup, shared evenly by its waves
+constexpr int WAVE_CANDIDATES = 512;  // of a wave's list: a wave that holds a short run whole does not overflow
 
 struct RowRun {
     long long row;
@@ -239,13 +239,13 @@ struct RowPartials {
     unsigned long long* keys;
 };
 
-template <int THREADS>
+template <int WAVES>
 struct TopState {
-    static constexpr int WAVES = THREADS / 64, EACH = CANDIDATES / WAVES;
-    unsigned long long candidates[WAVES][EACH];
+    unsigned long long candidates[WAVES][WAVE_CANDIDATES];
     unsigned long long best[2][TOP_MAX];
     unsigned long long wave_best[WAVES];
-    float maxima[2][THREADS];
+    int ranks[WAVES * 64];
+    float kth[2][WAVES];
     int counts[WAVES];
 };
 
@@ -258,17 +258,25 @@ struct RowTile {
     static __device__ __forceinline__ int index(int base, int p, int e) {
         return base + (p * THREADS + static_cast<int>(threadIdx.x)) * N + e;
     }
-    // The tile at base; -inf past a run's end that cuts it.
+    // The tile at base; -inf past a run's end that cuts it. One pack at most lies across the end.
     __device__ __forceinline__ void load(const T* __restrict__ z, int base, int end) {
         if (base + SIZE <= end) {
 #pragma unroll
             for (int p = 0; p < TILE_PACKS; ++p) packs[p] = load_pack<T, N>(z + index(base, p, 0));
             return;
         }
+        const Pack<T, N> none = Pack<T, N>::all(-INFINITY);
 #pragma unroll
         for (int p = 0; p < TILE_PACKS; ++p) {
             const int at = index(base, p, 0);
-            packs[p] = at + N <= end ? load_pack<T, N>(z + at) : load_part<T, N>(z + at, end - at, -INFINITY);
+            packs[p] = at + N <= end ? load_pack<T, N>(z + at) : none;
+        }
+        const int whole = end / N * N, across = (whole - base) / N, p = across / THREADS;  // N divides base
+        if (across - p * THREADS == static_cast<int>(threadIdx.x) && whole < end) {
+            const Pack<T, N> part = load_part<T, N>(z + whole, end - whole, -INFINITY);
+#pragma unroll
+            for (int i = 0; i < TILE_PACKS; ++i)
+                if (i == p) packs[i] = part;
         }
     }
 };
@@ -291,31 +299,25 @@ __device__ __forceinline__ float largest(const Pack<T, N>& pack) {
     return fmaxf(a, b);
 }
 
-// A float that at least k of the threads' maxima reach (the k-th largest of them, its low 16 bits cleared
-// downwards), -inf where fewer than k lie above that. The same in every thread.
-template <int THREADS>
-__device__ __forceinline__ float kth_of_maxima(float (&maxima)[THREADS], float mine, int k) {
-    constexpr int EACH = THREADS / 64;
-    maxima[threadIdx.x] = mine;
-    __syncthreads();
-    unsigned order[EACH];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const unsigned bits = __float_as_uint(maxima[(threadIdx.x & 63) * EACH + i] + 0.0f);
-        order[i] = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
-    }
-    unsigned found = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 16; --bit) {
-        const unsigned probe = found | (1u << bit);
-        int reached = 0;
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) reached += __popcll(__ballot(order[i] >= probe));
-        if (reached >= k) found = probe;
-        if (reached == k) break;
-    }
-    if (found <= 0x007fffffu) return -INFINITY;  // -inf itself, or nothing
-    return __uint_as_float(found & 0x80000000u ? found & 0x7fffffffu : ~found);
+// The value of lane ^ DISTANCE.
+template <int DISTANCE>
+__device__ __forceinline__ float lane_across(float v) {
+    if constexpr (DISTANCE == 1) return lane_moved<0xB1>(v);
+    else if constexpr (DISTANCE == 2) return lane_moved<0x4E>(v);
+    else if constexpr (DISTANCE == 4) return lane_moved<0x1B>(lane_moved<0x141>(v));  // 7 - i, then 3 - i
+    else if constexpr (DISTANCE == 8) return lane_moved<0x128>(v);  // a row of 16 lanes turned by 8
+    else return __shfl_xor(v, DISTANCE);
+}
+
+// One wave's values sorted in falling order over its lanes (a bitonic network).
+template <int SIZE = 2, int DISTANCE = 1>
+__device__ __forceinline__ float wave_sorted(float v) {
+    const int lane = threadIdx.x & 63;
+    const float other = lane_across<DISTANCE>(v);
+    v = ((lane & DISTANCE) == 0) == ((lane & SIZE) == 0) ? fmaxf(v, other) : fminf(v, other);
+    if constexpr (DISTANCE > 1) return wave_sorted<SIZE, DISTANCE / 2>(v);
+    else if constexpr (SIZE < 64) return wave_sorted<2 * SIZE, SIZE>(v);
+    else return v;
 }
 
 // The next float below (of a float above -inf).
@@ -325,35 +327,43 @@ __device__ __forceinline__ float just_below(float v) {
 }
 
 // The k largest keys of a run in falling order (0 where there are fewer), by k rounds a tile of the largest key
-// below the last, for the tiles that hold a key above the k-th best so far. Every round reads the tile again.
+// below the last, for the tiles that hold a key above the k-th best so far.
 template <typename T, int THREADS>
-__device__ __forceinline__ const unsigned long long* exact_top(TopState<THREADS>& top, const T* __restrict__ z,
+__device__ __forceinline__ const unsigned long long* exact_top(TopState<THREADS / 64>& top, const T* __restrict__ z,
                                                                const RowRun& run, int k) {
-    constexpr int SIZE = THREADS * 16;
+    using Tile = RowTile<T, THREADS>;
     const int tid = threadIdx.x;
     int side = 0;
     __syncthreads();
     if (tid < k) top.best[0][tid] = 0;
     __syncthreads();
 #pragma unroll 1
-    for (int base = run.begin; base < run.end; base += SIZE) {
-        const int end = min(run.end, base + SIZE);
-        // The largest key of this thread's part of the tile below `last`.
-        const auto largest_below = [&](unsigned long long last) {
-            unsigned long long mine = 0;
-#pragma unroll 1
-            for (int at = base + tid; at < end; at += THREADS) {
-                const float x = static_cast<float>(z[at]);
-                const unsigned long long key = x == x ? key_of(x, at) : 0;
-                if (key < last && key > mine) mine = key;
-            }
-            return mine;
-        };
-        if (!__syncthreads_or(largest_below(~0ull) > top.best[side][k - 1])) continue;
+    for (int base = run.begin; base < run.end; base += Tile::SIZE) {
+        Tile tile;
+        tile.load(z, base, run.end);
+        const unsigned long long least = top.best[side][k - 1];
         unsigned long long last = ~0ull;
+        bool above = true;
 #pragma unroll 1
         for (int i = 0; i < k && last; ++i) {
-            unsigned long long mine = largest_below(last);
+            unsigned long long mine = 0;
+            int from = base;
+#pragma unroll
+            for (int p = 0; p < TILE_PACKS; ++p) {
+                tile.packs[p].stay_packed();
+                asm volatile("" : "+s"(from));  // the keys are formed anew: they would take 64 registers
+#pragma unroll
+                for (int e = 0; e < Tile::N; ++e) {
+                    const float x = tile.packs[p].at(e);
+                    const int at = Tile::index(from, p, e);
+                    const unsigned long long key = key_of(x, at);
+                    if (x == x && at < run.end && key < last && key > mine) mine = key;
+                }
+            }
+            if (i == 0) {
+                above = __syncthreads_or(mine > least);
+                if (!above) break;
+            }
             if (tid < k) {
                 const unsigned long long key = top.best[side][tid];
                 if (key < last && key > mine) mine = key;
@@ -373,51 +383,93 @@ __device__ __forceinline__ const unsigned long long* exact_top(TopState<THREADS>
             if (tid == 0) top.best[side ^ 1][i] = last;
             if (last == 0 && tid > i && tid < k) top.best[side ^ 1][tid] = 0;
         }
-        side ^= 1;
+        if (above) side ^= 1;
         __syncthreads();
     }
     return top.best[side];
 }
 
-// Takes every candidate to its rank: emit(rank, key) for the k largest, emit(rank, 0) for those that are missing.
-// Fewer than k candidates mean that all logits above -inf are candidates: the first -inf of the run follow.
-// `mine` is the number of the wave's candidates.
+// The ranks of `count` distinct keys, by all waves: emit(rank, key) for those below k. Each wave counts, for every
+// key, the larger ones of its own list (of `listed` keys); 256 keys at a time, four a lane. ranks is scratch.
+template <int WAVES, typename KeyAt, typename Emit>
+__device__ __forceinline__ void emit_ranks(KeyAt&& key_at, int count, int k, const unsigned long long* list, int listed,
+                                           int* ranks, Emit&& emit) {
+    static_assert(WAVES == 1 || WAVES == 4, "a lane's four keys go to one wave or to four");
+    const int tid = threadIdx.x, lane = tid & 63;
+#pragma unroll 1
+    for (int base = 0; base < count; base += 256) {
+        unsigned long long keys[4];
+        int larger[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) keys[i] = base + i * 64 + lane < count ? key_at(base + i * 64 + lane) : ~0ull;
+        const int blocks = (min(count - base, 256) + 63) / 64;
+        if constexpr (WAVES > 1) {
+            ranks[tid] = 0;
+            __syncthreads();
+        }
+        if (blocks <= 2) {
+#pragma unroll 4
+            for (int j = 0; j < listed; ++j) {
+                const unsigned long long other = list[j];
+                larger[0] += other > keys[0];
+                larger[1] += other > keys[1];
+            }
+        } else {
+#pragma unroll 2
+            for (int j = 0; j < listed; ++j) {
+                const unsigned long long other = list[j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) larger[i] += other > keys[i];
+            }
+        }
+        if constexpr (WAVES > 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < blocks) atomicAdd(&ranks[i * 64 + lane], larger[i]);
+            __syncthreads();
+            if (base + tid < count && ranks[tid] < k) emit(ranks[tid], key_at(base + tid));
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (keys[i] != ~0ull && larger[i] < k) emit(larger[i], keys[i]);
+        }
+    }
+}
+
+// Takes the run's k largest keys to emit(rank, key), and emit(rank, 0) for those that are missing. Fewer than k
+// candidates mean that all logits above -inf are candidates: the first -inf of the run follow. `mine` is the
+// number of the wave's candidates.
 template <typename T, int THREADS, typename Emit>
-__device__ __forceinline__ void emit_top(TopState<THREADS>& top, const T* __restrict__ z, const RowRun& run, int k,
+__device__ __forceinline__ void emit_top(TopState<THREADS / 64>& top, const T* __restrict__ z, const RowRun& run, int k,
                                          int mine, float s, Emit&& emit) {
-    using Top = TopState<THREADS>;
+    constexpr int WAVES = THREADS / 64;
     if ((threadIdx.x & 63) == 0) top.counts[threadIdx.x / 64] = mine;
     __syncthreads();
-    int counts[Top::WAVES], count = 0;
+    int counts[WAVES], count = 0;
     bool exact = s != s;  // a NaN among a thread's logits leaves its maximum open
 #pragma unroll
-    for (int w = 0; w < Top::WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         counts[w] = __builtin_amdgcn_readfirstlane(top.counts[w]);
         count += counts[w];
-        exact = exact || counts[w] > Top::EACH;
+        exact = exact || counts[w] > WAVE_CANDIDATES;
     }
     if (exact) {
-        const unsigned long long* best = exact_top(top, z, run, k);
+        const unsigned long long* best = exact_top<T, THREADS>(top, z, run, k);
         if (static_cast<int>(threadIdx.x) < k) emit(static_cast<int>(threadIdx.x), best[threadIdx.x]);
         return;
     }
-#pragma unroll 1
-    for (int i = threadIdx.x; i < count; i += THREADS) {
-        int wave = 0, at = i;
+    const auto key_at = [&](int i) {
+        int wave = 0;
 #pragma unroll
-        for (int w = 0; w + 1 < Top::WAVES; ++w)
-            if (wave == w && at >= counts[w]) {
-                at -= counts[w];
+        for (int w = 0; w + 1 < WAVES; ++w)
+            if (wave == w && i >= counts[w]) {
+                i -= counts[w];
                 wave = w + 1;
             }
-        const unsigned long long key = top.candidates[wave][at];
-        int rank = 0;
-#pragma unroll
-        for (int w = 0; w < Top::WAVES; ++w)
-#pragma unroll 4
-            for (int j = 0; j < counts[w]; ++j) rank += top.candidates[w][j] > key;
-        if (rank < k) emit(rank, key);
-    }
+        return top.candidates[wave][i];
+    };
+    emit_ranks<WAVES>(key_at, count, k, top.candidates[threadIdx.x / 64], mine, top.ranks, emit);
     if (count >= k || threadIdx.x >= 64) return;
     int next = count;
 #pragma unroll 1
@@ -435,31 +487,93 @@ __device__ __forceinline__ void emit_top(TopState<THREADS>& top, const T* __rest
 // What a thread carries through the tiles of a run.
 struct RowState {
     RowStats mine;
-    float below;  // candidates lie above this
-    int count;    // of the wave's candidates
+    float place_max[4];  // one wave: the largest at each place of a pack
+    float below;         // candidates lie above this
+    int count;           // of the wave's candidates
+    int side;            // of the shared thresholds
+    int sets, each;      // k logits reach the each-th largest of the 64 maxima of `sets` sets
+    bool lanes;          // one wave: of the lanes' maxima over all places, the only set
 };
 
-// One tile into the thread's statistics and, with TOP, the wave's list of candidates.
-template <bool ENTROPY, bool TOP, typename T, int THREADS>
-__device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& state, float scale, int base,
-                                          TopState<THREADS>* top, int top_k, int number) {
-    using Tile = RowTile<T, THREADS>;
-    float pack_max[TILE_PACKS];
+// The sets of a run's logits that a threshold is formed of: what a wave holds, or, in a workgroup of one wave,
+// what its threads hold at one place of their packs. The last is left out where too few of its lanes hold any.
+template <int WAVES>
+__device__ __forceinline__ void choose_sets(RowState& state, int logits, int k, int lane_logits) {
+    const int full = 64 * lane_logits;
+    int sets = min(4, (logits + full - 1) / full);
+    const int last = min(64, (logits - (sets - 1) * full + lane_logits - 1) / lane_logits);
+    if (sets > 1 && last < (k + sets - 1) / sets) --sets;
+    state.sets = sets;
+    state.each = (k + sets - 1) / sets;
+    // One set of all lanes lets a third more through for 20 alternatives, and many times more for 64.
+    state.lanes = WAVES == 1 && k <= 24 && logits >= full;
+    if (state.lanes) state.each = k;
+}
+
+// Raises the threshold to what the each-th largest of the 64 maxima of each set reaches: at least k logits do.
+// Drops the candidates below it.
+template <int WAVES>
+__device__ __forceinline__ void raise_threshold(RowState& state, TopState<WAVES>& top, float to) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    float kth;
+    if constexpr (WAVES > 1) {
+        const float sorted = wave_sorted(to > LOWEST ? to : -INFINITY);
+        const float own = lane_of(sorted, state.each - 1);
+        if (lane == 0) top.kth[state.side][wave] = own;
+        __syncthreads();
+        kth = top.kth[state.side][0];
 #pragma unroll
-    for (int p = 0; p < TILE_PACKS; ++p) pack_max[p] = largest(tile.packs[p]);
-    static_assert(TILE_PACKS == 4, "the packs' maxima");
-    const float tile_max = fmaxf(max3(pack_max[0], pack_max[1], pack_max[2]), pack_max[3]);
-    const float to = fmaxf(state.mine.m, tile_max);
+        for (int w = 1; w < WAVES; ++w)
+            if (w < state.sets) kth = fminf(kth, top.kth[state.side][w]);
+        state.side ^= 1;  // what is written next was read before the last barrier
+    } else if (state.lanes) {
+        kth = lane_of(wave_sorted(to > LOWEST ? to : -INFINITY), state.each - 1);
+    } else {
+        kth = INFINITY;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            if (p < state.sets) kth = fminf(kth, lane_of(wave_sorted(state.place_max[p]), state.each - 1));
+    }
+    if (!(kth > state.below)) return;
+    state.below = just_below(kth);
+    if (state.count > WAVE_CANDIDATES) return;  // the list is lost
+    unsigned long long* list = top.candidates[wave];
+    int kept = 0;
+#pragma unroll 1
+    for (int i = 0; i < state.count; i += 64) {
+        const unsigned long long key = i + lane < state.count ? list[i + lane] : 0;
+        const bool keep = key && key_value(key) > state.below;
+        const unsigned long long who = __ballot(keep);
+        if (keep) list[kept + __popcll(who & ((1ull << lane) - 1))] = key;  // at or before where it was read
+        kept += __popcll(who);
+    }
+    state.count = kept;
+}
+
+// One tile into the thread's statistics and, with TOP, the wave's list of candidates. Places of packs that lie
+// past the run's end are left out.
+template <bool ENTROPY, bool TOP, typename T, int THREADS>
+__device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& state, float scale, int base, int end,
+                                          TopState<THREADS / 64>* top, int number) {
+    using Tile = RowTile<T, THREADS>;
+    const auto there = [&](int p) { return p == 0 || base + p * THREADS * Tile::N < end; };
+    float pack_max[TILE_PACKS], to = state.mine.m;
+#pragma unroll
+    for (int p = 0; p < TILE_PACKS; ++p) {
+        pack_max[p] = -INFINITY;
+        if (there(p)) pack_max[p] = largest(tile.packs[p]);
+        to = fmaxf(to, pack_max[p]);
+    }
     if constexpr (TOP) {
 #pragma unroll
-        for (int p = 0; p < TILE_PACKS; ++p) tile.packs[p].stay_packed();
-        // The threshold after the first tile, then raised at the tiles 1, 4, 16, ...: each time the candidates
-        // to come are at most those of the tiles so far, three times over.
-        if (number == 0) {
-            const float kth = kth_of_maxima(top->maxima[0], tile_max, top_k);
-            state.below = kth == -INFINITY ? kth : just_below(kth);
+        for (int p = 0; p < TILE_PACKS; ++p) {
+            tile.packs[p].stay_packed();
+            if constexpr (THREADS == 64) state.place_max[p] = fmaxf(state.place_max[p], pack_max[p]);
         }
-        using Top = TopState<THREADS>;
+        // At the tiles 0, 2, 8, 32, ...: what a threshold lets through until the next is at most three times what
+        // it was formed from.
+        if (number == 0 || ((number & (number - 1)) == 0 && (__ffs(number) & 1) == 0))
+            raise_threshold<THREADS / 64>(state, *top, to);
         unsigned long long* list = top->candidates[threadIdx.x / 64];
         const unsigned long long before = (1ull << (threadIdx.x & 63)) - 1;
 #pragma unroll
@@ -471,20 +585,17 @@ __device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& s
                 const unsigned long long who = __ballot(x > state.below);
                 if (!who) continue;
                 const int slot = state.count + __popcll(who & before);
-                if (x > state.below && slot < Top::EACH) list[slot] = key_of(x, Tile::index(base, p, e));
+                if (x > state.below && slot < WAVE_CANDIDATES) list[slot] = key_of(x, Tile::index(base, p, e));
                 state.count += __popcll(who);
             }
-        }
-        if (number > 0 && (number & (number - 1)) == 0 && (__ffs(number) & 1)) {
-            const float kth = kth_of_maxima(top->maxima[((__ffs(number) >> 1) + 1) & 1], to > LOWEST ? to : -INFINITY, top_k);
-            state.below = fmaxf(state.below, kth);
         }
     }
 #pragma unroll
     for (int p = 0; p < TILE_PACKS; ++p) tile.packs[p].stay_packed();
     state.mine.rescale(to, scale);
 #pragma unroll
-    for (int p = 0; p < TILE_PACKS; ++p)
+    for (int p = 0; p < TILE_PACKS; ++p) {
+        if (!there(p)) continue;
 #pragma unroll
         for (int e = 0; e < Tile::N; ++e) {
             const float d = tile.packs[p].at(e) - state.mine.m;
@@ -492,29 +603,33 @@ __device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& s
             state.mine.s += part;
             if constexpr (ENTROPY) state.mine.t += part * fmaxf(d, DIFFERENCE_FLOOR);
         }
+    }
 }
 
 // The statistics of a run, the same in every thread, and the number of the wave's candidates. `meanwhile` runs
 // while the first tile's loads are in flight.
 template <bool ENTROPY, bool TOP, typename T, int THREADS, typename Meanwhile>
-__device__ __forceinline__ RowStats take_run(const T* __restrict__ z, const RowRun& run, float scale, TopState<THREADS>* top,
-                                             int top_k, int& count, Meanwhile&& meanwhile) {
+__device__ __forceinline__ RowStats take_run(const T* __restrict__ z, const RowRun& run, float scale,
+                                             TopState<THREADS / 64>* top, int top_k, int& count, Meanwhile&& meanwhile) {
     using Tile = RowTile<T, THREADS>;
     __shared__ RowStats waves[THREADS / 64];
     __shared__ float wave_m[THREADS / 64];
-    RowState state{RowStats::none(), -INFINITY, 0};
+    RowState state{RowStats::none(), {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, -INFINITY, 0, 0, 1, 1, false};
+    if constexpr (TOP) choose_sets<THREADS / 64>(state, run.end - run.begin, top_k, Tile::N);
     Tile tile;
     tile.load(z, run.begin, run.end);
     meanwhile();
-    int base = run.begin, number = 0;
+    int base = run.begin;
 #pragma unroll 1
-    for (; base + Tile::SIZE < run.end; base += Tile::SIZE, ++number) {
+    for (int number = 0;; ++number) {
         Tile next;
-        next.load(z, base + Tile::SIZE, run.end);
-        take_tile<ENTROPY, TOP>(tile, state, scale, base, top, top_k, number);
+        const bool last = base + Tile::SIZE >= run.end;
+        if (!last) next.load(z, base + Tile::SIZE, run.end);
+        take_tile<ENTROPY, TOP>(tile, state, scale, base, run.end, top, number);
+        if (last) break;
         tile = next;
+        base += Tile::SIZE;
     }
-    take_tile<ENTROPY, TOP>(tile, state, scale, base, top, top_k, number);
     count = state.count;
     RowStats mine = state.mine;
     float m = wave_max(mine.m);
@@ -552,9 +667,8 @@ __device__ __forceinline__ RowRun run_of(const RowSplit& split, int vocab) {
 }
 
 template <typename T, int THREADS, bool TOP>
-__global__ __launch_bounds__(THREADS) void log_probs_kernel(const T* __restrict__ logits, LogProbsForward f, RowSplit split,
+__global__ __launch_bounds__(THREADS, 8) void log_probs_kernel(const T* __restrict__ logits, LogProbsForward f, RowSplit split,
                                                             RowPartials partials) {
-    __shared__ TopState<TOP ? THREADS : 64> top;
     const RowRun run = run_of(split, f.vocab);
     const T* __restrict__ z = logits + run.row * f.stride;
     const long long at = run.row * split.chunks + run.chunk;
@@ -564,18 +678,20 @@ __global__ __launch_bounds__(THREADS) void log_probs_kernel(const T* __restrict_
         if (split.chunks == 1 && threadIdx.x == 0) given = GivenToken(f, z, run.row);
     };
     if constexpr (TOP) {
+        __shared__ TopState<THREADS / 64> top;
         const RowStats row = take_run<true, true, T, THREADS>(z, run, LOG2E, &top, f.top, count, meanwhile);
-        if (split.chunks == 1) {
-            if (threadIdx.x == 0) finish_log_probs(f, run.row, given, row);
-            emit_top(top, z, run, f.top, count, row.s, [&](int rank, unsigned long long key) { write_top(f, run.row, rank, key, row); });
-        } else {
-            if (threadIdx.x == 0) partials.stats[at] = row;
-            emit_top(top, z, run, f.top, count, row.s,
-                     [&](int rank, unsigned long long key) { partials.keys[at * f.top + rank] = key; });
+        if (threadIdx.x == 0) {
+            if (split.chunks == 1) finish_log_probs(f, run.row, given, row);
+            else partials.stats[at] = row;
         }
+        const RowEnd end(row);
+        emit_top<T, THREADS>(top, z, run, f.top, count, row.s, [&](int rank, unsigned long long key) {
+            if (split.chunks == 1) write_top(f, run.row, rank, key, end);
+            else partials.keys[at * f.top + rank] = key;
+        });
     } else {
         const RowStats row =
-            take_run<true, false, T, THREADS>(z, run, LOG2E, static_cast<TopState<THREADS>*>(nullptr), 0, count, meanwhile);
+            take_run<true, false, T, THREADS>(z, run, LOG2E, nullptr, 0, count, meanwhile);
         if (threadIdx.x != 0) return;
         if (split.chunks == 1) finish_log_probs(f, run.row, given, row);
         else partials.stats[at] = row;
@@ -590,7 +706,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const T* __restrict__ 
     int count;
     TeacherRow<THREADS> teacher;
     const RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature,
-                                                            static_cast<TopState<THREADS>*>(nullptr), 0, count, [&] {
+                                                            nullptr, 0, count, [&] {
                                                                 if (split.chunks == 1) teacher.read(f, z, run.row);
                                                             });
     if (split.chunks == 1) teacher.finish(f, run.row, row);
@@ -610,58 +726,47 @@ __device__ __forceinline__ RowStats join_runs(const RowStats* __restrict__ stats
 constexpr int JOIN_THREADS = 256;
 constexpr int SPLIT_MAX = 64;
 
-// The largest 64-bit key that k of the threads' keys reach (0 when fewer than k are above 0).
-__device__ __forceinline__ unsigned long long kth_of_keys(unsigned long long (&maxima)[JOIN_THREADS],
-                                                          unsigned long long mine, int k) {
-    constexpr int EACH = JOIN_THREADS / 64;
-    maxima[threadIdx.x] = mine;
-    __syncthreads();
-    unsigned long long key[EACH];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) key[i] = maxima[(threadIdx.x & 63) * EACH + i];
-    unsigned long long found = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-        const unsigned long long probe = found | (1ull << bit);
-        int reached = 0;
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) reached += __popcll(__ballot(key[i] >= probe));
-        if (reached >= k) found = probe;
-        if (reached == k) break;
-    }
-    return found;
-}
-
-// Joins a row's runs: one workgroup a row.
+// Joins a row's runs: one workgroup a row. Each run's keys come in falling order. At least k keys reach the
+// smallest of the runs' keys at place ceil(k / runs), and k those of any run its k-th: keys below the larger of
+// the two bounds are none of the k largest.
 template <typename T>
 __global__ __launch_bounds__(JOIN_THREADS) void log_probs_join_kernel(const T* __restrict__ logits, LogProbsForward f,
                                                                       RowSplit split, RowPartials partials) {
-    __shared__ unsigned long long maxima[JOIN_THREADS], kept[SPLIT_MAX * TOP_MAX];
-    __shared__ int count;
+    __shared__ unsigned long long kept[SPLIT_MAX * TOP_MAX], bounds[2][SPLIT_MAX];
+    __shared__ int ranks[JOIN_THREADS], count;
     const long long r = blockIdx.x;
-    const unsigned long long* __restrict__ keys = partials.keys + r * split.chunks * f.top;
-    const int total = split.chunks * f.top;
-    unsigned long long mine = 0;
-    for (int i = threadIdx.x; i < total; i += JOIN_THREADS) mine = max(mine, keys[i]);
+    const int tid = threadIdx.x, k = f.top;
+    const unsigned long long* __restrict__ keys = partials.keys + r * split.chunks * k;
+    if (k && tid < split.chunks) {
+        bounds[0][tid] = keys[tid * k + (k + split.chunks - 1) / split.chunks - 1];
+        bounds[1][tid] = keys[tid * k + k - 1];
+    }
     GivenToken given{};
-    if (threadIdx.x == 0) given = GivenToken(f, logits + r * f.stride, r);
+    if (tid == 0) given = GivenToken(f, logits + r * f.stride, r);
     const RowStats row = join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E);
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         finish_log_probs(f, r, given, row);
         count = 0;
     }
-    if (f.top == 0) return;
-    // Keys that the k-th largest of the threads' own do not reach are none of the k largest.
-    const unsigned long long least = max(total > JOIN_THREADS ? kth_of_keys(maxima, mine, f.top) : 0ull, 1ull);
-    if (total <= JOIN_THREADS) __syncthreads();
-    for (int i = threadIdx.x; i < total; i += JOIN_THREADS)
-        if (keys[i] >= least) kept[atomicAdd(&count, 1)] = keys[i];
+    if (k == 0) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < count; i += JOIN_THREADS) {
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += kept[j] > kept[i];
-        if (rank < f.top) write_top(f, r, rank, kept[i], row);
+    unsigned long long all = ~0ull, any = 0;
+    for (int i = 0; i < split.chunks; ++i) {
+        all = min(all, bounds[0][i]);
+        any = max(any, bounds[1][i]);
     }
-    for (int k = count + threadIdx.x; k < f.top; k += JOIN_THREADS) write_top(f, r, k, 0, row);
+    const unsigned long long least = max(max(all, any), 1ull);
+    for (int i = tid; i < split.chunks * k; i += JOIN_THREADS) {
+        const unsigned long long key = keys[i];
+        if (key >= least) kept[atomicAdd(&count, 1)] = key;
+    }
+    __syncthreads();
+    const RowEnd end(row);
+    constexpr int WAVES = JOIN_THREADS / 64;
+    const int found = count, part = (found + WAVES - 1) / WAVES, from = min(found, tid / 64 * part);
+    emit_ranks<WAVES>([&](int i) { return kept[i]; }, found, k, kept + from, min(part, found - from), ranks,
+               [&](int rank, unsigned long long key) { write_top(f, r, rank, key, end); });
+    for (int i = found + tid; i < k; i += JOIN_THREADS) write_top(f, r, i, 0, end);
 }
 
 template <typename T>
@@ -831,11 +936,18 @@ constexpr int SMALL_ROW_BYTES = 2 * 64 * TILE_PACKS * 16, WAVE_THREADS = 64;
 
 bool small_row(int vocab, int type) { return vocab * static_cast<std::int64_t>(type_bytes(type)) <= SMALL_ROW_BYTES; }
 
-// Runs of a row: as many as bring the workgroups to SPLIT_GROUPS (eight a CU of the 256), of at least one tile.
-// The number is fixed by the sizes, not by the device, so that results do not depend on it.
-constexpr int SPLIT_GROUPS = 2048;
+// Runs of a row. Rows are split where the time that whole rows leave CUs idle is more than a second launch takes:
+// of 256 CUs that read ROW_RATE bytes a microsecond each (5/8 of that with one workgroup), whole rows take the most
+// that one CU has of them, split ones their share and JOIN_TIME. Measured split / whole: 777 rows of 64 KB 18.7 /
+// 17.5 us, 1024 of them 18.1 / 17.4, one 4.3 / 5.3. Then as many runs as bring the workgroups to SPLIT_GROUPS, of
+// at least one tile. All of this follows from the sizes alone, so that results do not depend on the device.
+constexpr int SPLIT_GROUPS = 2048, ROW_RATE = 20000, JOIN_TIME = 5, SPLIT_CUS = 256;
 RowSplit row_split(std::int64_t rows, int vocab, int type) {
     if (rows == 0 || small_row(vocab, type)) return {1, vocab};
+    const std::int64_t bytes = static_cast<std::int64_t>(vocab) * type_bytes(type);
+    const std::int64_t whole = rows <= SPLIT_CUS ? bytes * 8 / 5 : (rows + SPLIT_CUS - 1) / SPLIT_CUS * bytes;
+    const std::int64_t shared = rows * bytes / SPLIT_CUS;
+    if (whole - shared <= JOIN_TIME * ROW_RATE) return {1, vocab};
     const int unit = ROW_THREADS * 16 / type_bytes(type);  // a pack a thread
     const std::int64_t wanted = std::min<std::int64_t>(SPLIT_MAX, std::max<std::int64_t>(1, SPLIT_GROUPS / rows));
     const std::int64_t packs = (vocab + unit - 1) / unit;

@@ -54,6 +54,12 @@ struct Pack {
         }
         return pack;
     }
+    static __device__ __forceinline__ Pack all(float x) {
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = x;
+        return of(v);
+    }
     // Between two passes over held packs: keeps the compiler from holding the first pass's floats of half types
     // for the second, at twice the registers.
     __device__ __forceinline__ void stay_packed() {

@@ -84,8 +84,7 @@ def group_norm_forward(x, gamma, beta, groups, *, eps=1e-5, activation=None):
         raise ValueError("eps must not be negative")
     gamma, beta = _per_channel(gamma, channels, "gamma"), _per_channel(beta, channels, "beta")
     y = torch.empty_like(x)
-    mean = torch.empty((n, groups), dtype=torch.float32, device=x.device)
-    inv_std = torch.empty((n, groups), dtype=torch.float32, device=x.device)
+    mean, inv_std = gamma.new_empty((n, groups)), gamma.new_empty((n, groups))
     code = native.TYPE_CODES[x.dtype]
     workspace, held = native.byte_workspace(_workspace(sizes, code, False))
     native._call("mfh_group_norm_forward", x.data_ptr(), code, *sizes, gamma.data_ptr(), beta.data_ptr(), act, eps,

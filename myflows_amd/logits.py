@@ -16,58 +16,114 @@ mean squared error.
 from __future__ import annotations
 
 from functools import lru_cache
-from typing import NamedTuple
 
 import torch
 
-from . import fused, native
+from . import native
 from .graph import GradientOp
 
+_TYPE_CODES = native.TYPE_CODES
 TOP_MAX = 64            # alternatives of a row
 DISTILL_HELD_MAX = 256  # teacher ids of a row
 ROWS_LIMIT = 1 << 22
 VOCAB_LIMIT = 1 << 24
 
 
-class LogProbs(NamedTuple):
-    """What ``log_probs_forward`` returns, and ``log_probs_backward`` takes back."""
-    log_prob: torch.Tensor | None       # (rows,), None without tokens
-    entropy: torch.Tensor               # (rows,)
-    log_sum: torch.Tensor               # (rows,): ln sum e^z
-    top_log_probs: torch.Tensor | None  # (rows, top), None for top 0
-    top_ids: torch.Tensor | None        # (rows, top) int32
-    stats: torch.Tensor                 # (2, rows): the largest logit m and sum e^(z - m)
+class LogProbs:
+    """What ``log_probs_forward`` returns, and ``log_probs_backward`` takes back.
+
+    log_prob (rows,), None without tokens; entropy (rows,); log_sum (rows,), ln sum e^z; top_log_probs
+    (rows, top) and top_ids (rows, top) int32, None for top 0; stats (2, rows), the largest logit m and
+    sum e^(z - m). Iterates over them in this order."""
+
+    __slots__ = ("_floats", "_given", "top_log_probs", "top_ids")
+
+    def __init__(self, floats, given, top_log_probs, top_ids):
+        self._floats, self._given = floats, given  # (5, rows): stats, entropy, log_sum, log_prob
+        self.top_log_probs, self.top_ids = top_log_probs, top_ids
+
+    @property
+    def log_prob(self):
+        return self._floats[4] if self._given else None
+
+    @property
+    def entropy(self):
+        return self._floats[2]
+
+    @property
+    def log_sum(self):
+        return self._floats[3]
+
+    @property
+    def stats(self):
+        return self._floats[:2]
+
+    def __iter__(self):
+        return iter((self.log_prob, self.entropy, self.log_sum, self.top_log_probs, self.top_ids, self.stats))
 
 
-class DistillLoss(NamedTuple):
-    """What ``distill_loss_forward`` returns, and ``distill_loss_backward`` takes back."""
-    loss: torch.Tensor      # (): the weighted mean of row_loss over the rows that count
-    row_loss: torch.Tensor  # (rows,)
-    weights: torch.Tensor   # (rows,): the weights that count
-    stats: torch.Tensor     # (2, rows): the largest logit m and sum e^((z - m) / temperature)
-    targets: torch.Tensor   # (rows, held): the teacher's probability of each id
-    scale: torch.Tensor     # (2,): the loss and 1 / sum of the weights
+class DistillLoss:
+    """What ``distill_loss_forward`` returns, and ``distill_loss_backward`` takes back.
+
+    loss (), the weighted mean of row_loss over the rows that count; row_loss (rows,); weights (rows,), those
+    that count; stats (2, rows), the largest logit m and sum e^((z - m) / temperature); targets (rows, held),
+    the teacher's probability of each id; scale (2,), the loss and 1 / sum of the weights."""
+
+    __slots__ = ("_floats", "_rows", "_held")
+
+    def __init__(self, floats, rows, held):
+        self._floats, self._rows, self._held = floats, rows, held  # scale, row_loss, weights, stats, targets
+
+    def _part(self, first, count):
+        return self._floats[first:first + count]
+
+    @property
+    def loss(self):
+        return self._floats[0]
+
+    @property
+    def scale(self):
+        return self._part(0, 2)
+
+    @property
+    def row_loss(self):
+        return self._part(2, self._rows)
+
+    @property
+    def weights(self):
+        return self._part(2 + self._rows, self._rows)
+
+    @property
+    def stats(self):
+        return self._part(2 + 2 * self._rows, 2 * self._rows).view(2, self._rows)
+
+    @property
+    def targets(self):
+        return self._part(2 + 4 * self._rows, self._rows * self._held).view(self._rows, self._held)
 
 
 def _logits(value):
     """(tensor, type code, rows, vocab, row stride) of a 2-D tensor of logits."""
-    if not (isinstance(value, torch.Tensor) and value.is_cuda and value.dtype in native.TYPE_CODES):
+    code = _TYPE_CODES.get(value.dtype) if isinstance(value, torch.Tensor) and value.is_cuda else None
+    if code is None:
         raise TypeError("logits must be a float32, bfloat16 or float16 torch tensor on the GPU")
     if value.ndim != 2:
         raise ValueError("logits must be 2-D (rows, vocabulary)")
     rows, vocab = value.shape
     if not 0 < vocab <= VOCAB_LIMIT or rows > ROWS_LIMIT:
         raise ValueError(f"logits take at most {ROWS_LIMIT} rows of 1 to {VOCAB_LIMIT} elements")
-    if (vocab > 1 and value.stride(1) != 1) or (rows > 1 and value.stride(0) < vocab):
+    row_stride, stride = value.stride()
+    if (vocab > 1 and stride != 1) or (rows > 1 and row_stride < vocab):
         value = value.contiguous()
-    return value, native.TYPE_CODES[value.dtype], rows, vocab, value.stride(0) if rows > 1 else vocab
+        row_stride = vocab
+    return value, code, rows, vocab, row_stride if rows > 1 else vocab
 
 
 def _whole(value, shape, name):
     """(tensor, whether it is int64) of GPU whole numbers of a shape."""
     if not (isinstance(value, torch.Tensor) and value.is_cuda and value.dtype in (torch.int32, torch.int64)):
         raise TypeError(f"{name} must be an int32 or int64 torch tensor on the GPU")
-    if tuple(value.shape) != shape:
+    if value.shape != shape:
         raise ValueError(f"{name} must have shape {shape}")
     return value.contiguous(), int(value.dtype is torch.int64)
 
@@ -76,7 +132,7 @@ def _row_floats(value, rows, name):
     """(tensor, stride) of one float32 a row; any stride, 0 (a broadcast scalar) included."""
     if not (isinstance(value, torch.Tensor) and value.is_cuda and value.dtype is torch.float32):
         raise TypeError(f"{name} must be a float32 torch tensor on the GPU")
-    if tuple(value.shape) != (rows,):
+    if value.shape != (rows,):
         raise ValueError(f"{name} must have shape {(rows,)}")
     return value, value.stride(0)
 
@@ -86,9 +142,10 @@ def _gradient(out, add, like):
     if out is None:
         if add:
             raise ValueError("add needs an out tensor")
-        out = torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    elif not (isinstance(out, torch.Tensor) and out.is_cuda and out.dtype is like.dtype and out.shape == like.shape
-              and (out.shape[1] <= 1 or out.stride(1) == 1) and (out.shape[0] <= 1 or out.stride(0) >= out.shape[1])):
+        out = torch.empty_like(like, memory_format=torch.contiguous_format)
+        return out, out.shape[1]
+    if not (isinstance(out, torch.Tensor) and out.is_cuda and out.dtype is like.dtype and out.shape == like.shape
+            and (out.shape[1] <= 1 or out.stride(1) == 1) and (out.shape[0] <= 1 or out.stride(0) >= out.shape[1])):
         raise ValueError("out must be a GPU tensor of the logits' type and shape with contiguous rows")
     return out, out.stride(0) if out.shape[0] > 1 else out.shape[1]
 
@@ -118,22 +175,20 @@ def log_probs_forward(logits, tokens=None, *, top=0):
     wide = 0
     if tokens is not None:
         tokens, wide = _whole(tokens, (rows,), "tokens")
-    device = logits.device
-    floats = torch.empty((5, rows), dtype=torch.float32, device=device)
-    log_prob, entropy, log_sum = floats[0] if tokens is not None else None, floats[1], floats[2]
-    stats = floats[3:]
-    top_log_probs = torch.empty((rows, top), dtype=torch.float32, device=device) if top else None
-    top_ids = torch.empty((rows, top), dtype=torch.int32, device=device) if top else None
+    floats = logits.new_empty((5, rows), dtype=torch.float32)
+    top_log_probs = logits.new_empty((rows, top), dtype=torch.float32) if top else None
+    top_ids = logits.new_empty((rows, top), dtype=torch.int32) if top else None
     workspace, held = native.byte_workspace(_log_probs_workspace(rows, vocab, code, top))
+    stats, row = floats.data_ptr(), 4 * rows
     native._call("mfh_log_probs", logits.data_ptr(), code, rows, vocab, stride, native._addr(tokens), wide,
-                 native._addr(log_prob), entropy.data_ptr(), log_sum.data_ptr(), stats.data_ptr(), top,
+                 0 if tokens is None else stats + 4 * row, stats + 2 * row, stats + 3 * row, stats, top,
                  native._addr(top_log_probs), native._addr(top_ids), workspace, held, native._stream())
-    return LogProbs(log_prob, entropy, log_sum, top_log_probs, top_ids, stats)
+    return LogProbs(floats, tokens is not None, top_log_probs, top_ids)
 
 
 def _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, factor, scale, out, add):
     logits, code, rows, vocab, stride = _logits(logits)
-    if tuple(saved.stats.shape) != (2, rows):
+    if not isinstance(saved, LogProbs) or saved._floats.shape[1] != rows:
         raise ValueError("saved must be the LogProbs of these logits")
     wide = lp_step = entropy_step = 0
     if log_prob_grad is not None:
@@ -144,9 +199,9 @@ def _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, fact
     if entropy_grad is not None:
         entropy_grad, entropy_step = _row_floats(entropy_grad, rows, "entropy_grad")
     out, out_stride = _gradient(out, add, logits)
+    stats = saved._floats.data_ptr()
     native._call("mfh_log_probs_backward", logits.data_ptr(), code, rows, vocab, stride,
-                 0 if log_prob_grad is None else tokens.data_ptr(), wide, saved.stats.data_ptr(),
-                 saved.entropy.data_ptr(), native._addr(log_prob_grad), lp_step, native._addr(entropy_grad),
+                 0 if log_prob_grad is None else tokens.data_ptr(), wide, stats, stats + 8 * rows, native._addr(log_prob_grad), lp_step, native._addr(entropy_grad),
                  entropy_step, native._addr(factor), scale, out.data_ptr(), out_stride, int(add), native._stream())
     return out
 
@@ -185,17 +240,14 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
         raise ValueError(f"teacher_logits must have shape {shape}")
     if row_weights is not None:
         row_weights = _row_floats(row_weights, rows, "row_weights")[0].contiguous()
-    device = logits.device
-    floats = torch.empty((4, rows), dtype=torch.float32, device=device)
-    row_loss, weights, stats = floats[0], floats[1], floats[2:]
-    targets = torch.empty(shape, dtype=torch.float32, device=device)
-    scale = torch.empty((2,), dtype=torch.float32, device=device)
+    floats = logits.new_empty((2 + rows * (4 + shape[1]),), dtype=torch.float32)
     workspace, held = native.byte_workspace(_distill_workspace(rows, vocab, code))
+    scale, row = floats.data_ptr(), 4 * rows
+    row_loss = scale + 8
     native._call("mfh_distill_loss", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
-                 teacher_logits.data_ptr(), shape[1], native._addr(row_weights), temperature, row_loss.data_ptr(),
-                 weights.data_ptr(), stats.data_ptr(), targets.data_ptr(), scale.data_ptr(), workspace, held,
-                 native._stream())
-    return DistillLoss(scale[0], row_loss, weights, stats, targets, scale)
+                 teacher_logits.data_ptr(), shape[1], native._addr(row_weights), temperature, row_loss, row_loss + row,
+                 row_loss + 2 * row, row_loss + 4 * row, scale, workspace, held, native._stream())
+    return DistillLoss(floats, rows, shape[1])
 
 
 def distill_loss_backward(logits, teacher_ids, saved, seed, *, temperature=1.0, out=None, add=False):
@@ -203,16 +255,17 @@ def distill_loss_backward(logits, teacher_ids, saved, seed, *, temperature=1.0, 
     the DistillLoss of the same arguments and seed one float on the GPU."""
     logits, code, rows, vocab, stride = _logits(logits)
     temperature = _temperature(temperature)
-    if tuple(saved.stats.shape) != (2, rows):
+    if not isinstance(saved, DistillLoss) or saved._rows != rows:
         raise ValueError("saved must be the DistillLoss of these logits")
-    teacher_ids, wide = _whole(teacher_ids, tuple(saved.targets.shape), "teacher_ids")
+    teacher_ids, wide = _whole(teacher_ids, (rows, saved._held), "teacher_ids")
     seed = native._device_f32(seed, "seed")
     if seed.numel() != 1:
         raise ValueError("seed must hold one value")
     out, out_stride = _gradient(out, add, logits)
+    scale, row = saved._floats.data_ptr(), 4 * rows
+    row_loss = scale + 8
     native._call("mfh_distill_loss_backward", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
-                 teacher_ids.shape[1], saved.targets.data_ptr(), saved.stats.data_ptr(), saved.weights.data_ptr(),
-                 saved.scale.data_ptr(), seed.data_ptr(), temperature, out.data_ptr(), out_stride, int(add),
+                 saved._held, row_loss + 4 * row, row_loss + 2 * row, row_loss + row, scale, seed.data_ptr(), temperature, out.data_ptr(), out_stride, int(add),
                  native._stream())
     return out
 
