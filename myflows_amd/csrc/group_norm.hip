@@ -717,13 +717,14 @@ int launch_group_norm_forward(const GroupNormShape& s, int type, const void* x, 
     float* squares = plan.held ? nullptr : means + s.n * plan.runs * s.groups * plan.parts;
     with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
         using T = decltype(zero);
-        constexpr int VW = decltype(pack)::value, HOLD = group_norm_hold(sizeof(T), VW, false);
+        constexpr int VW = decltype(pack)::value;
+        constexpr int HOLD = group_norm_hold(sizeof(T), VW, false, 256), HOLD_MANY = group_norm_hold(sizeof(T), VW, false, 1024);
         constexpr bool SILU = decltype(silu)::value;
         const T* in = static_cast<const T*>(x);
         if (plan.held && plan.threads == 256)
             launch(held_forward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, static_cast<T*>(y), s, block, f);
         else if (plan.held)
-            launch(held_forward_kernel<T, VW, SILU, 1024, HOLD>, groups, 1024, 0, stream, in, static_cast<T*>(y), s, block, f);
+            launch(held_forward_kernel<T, VW, SILU, 1024, HOLD_MANY>, groups, 1024, 0, stream, in, static_cast<T*>(y), s, block, f);
         else
             launch(run_stats_kernel<T, VW>, groups, SPLIT_THREADS, 0, stream, in, s, block, runs, means, squares);
     });
@@ -752,14 +753,15 @@ int launch_group_norm_backward(const GroupNormShape& s, int type, const void* x,
         float* run_columns = columns + columns_floats(s);
         with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
             using T = decltype(zero);
-            constexpr int VW = decltype(pack)::value, HOLD = group_norm_hold(sizeof(T), VW, true);
+            constexpr int VW = decltype(pack)::value;
+            constexpr int HOLD = group_norm_hold(sizeof(T), VW, true, 256), HOLD_MANY = group_norm_hold(sizeof(T), VW, true, 1024);
             constexpr bool SILU = decltype(silu)::value;
             const T *in = static_cast<const T*>(x), *grad = static_cast<const T*>(dy);
             if (plan.held && plan.threads == 256)
                 launch(held_backward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, grad, static_cast<T*>(dx), s,
                        block, b, parameters ? columns : nullptr);
             else if (plan.held)
-                launch(held_backward_kernel<T, VW, SILU, 1024, HOLD>, groups, 1024, 0, stream, in, grad, static_cast<T*>(dx), s,
+                launch(held_backward_kernel<T, VW, SILU, 1024, HOLD_MANY>, groups, 1024, 0, stream, in, grad, static_cast<T*>(dx), s,
                        block, b, parameters ? columns : nullptr);
             else
                 launch(run_gradients_kernel<T, VW, SILU>, groups, SPLIT_THREADS, 0, stream, in, grad, s, block, runs,

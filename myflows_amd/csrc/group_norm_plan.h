@@ -33,10 +33,12 @@ struct GroupNormPlan {
 constexpr int GROUP_NORM_BLOCK_GROUPS = 256;  // at most, so that a thread a group suffices
 constexpr int GROUP_NORM_SPLIT_THREADS = 256, GROUP_NORM_SPLIT_AHEAD = 4;  // rows that a thread reads ahead
 
-// Packs that a thread holds of x (and, backward, of dy): as many as leave 1024 threads their 128 registers
-// without spills beside the statistics of a pack's channels.
-constexpr int group_norm_hold(int type_size, int vw, bool backward) {
-    if (vw * type_size < 16) return backward ? 16 : 24;
+// Packs that a thread holds of x (and, backward, of dy). 256 threads take up to 8 in turn: 26 single elements each
+// took 9.2 and 13.1 us forward and backward where four times the threads with 7 each took 7.9 and 9.2 (33 x 405 x
+// 90 float16). 1024 threads hold as many as leave them their 128 registers without spills.
+constexpr int group_norm_hold(int type_size, int vw, bool backward, int threads) {
+    if (threads <= 256) return 8;
+    if (vw * type_size < 16) return 32;
     return type_size == 2 && backward ? 5 : 8;
 }
 
@@ -64,7 +66,7 @@ inline bool group_norm_holds(const GroupNormShape& s, int type_size, bool backwa
                              GroupNormPlan* plan) {
     const int width = groups * (s.channels / s.groups), vw = group_norm_pack(type_size, width);
     if (width / vw > threads || groups > GROUP_NORM_BLOCK_GROUPS) return false;
-    const int rows = (threads >> log2_up(width / vw)) * group_norm_hold(type_size, vw, backward);
+    const int rows = (threads >> log2_up(width / vw)) * group_norm_hold(type_size, vw, backward, threads);
     if (rows < s.positions) return false;
     group_norm_block(s, groups, vw, plan);
     plan->held = true, plan->threads = threads;

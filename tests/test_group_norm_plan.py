@@ -25,7 +25,7 @@ const char* fault(const GroupNormShape& s, int size, bool backward) {
         return "parts";
     }
     if (p.held) {
-        if (static_cast<long long>(step) * group_norm_hold(size, p.vw, backward) < s.positions) return "held rows";
+        if (static_cast<long long>(step) * group_norm_hold(size, p.vw, backward, p.threads) < s.positions) return "held rows";
     } else {
         if (p.threads != GROUP_NORM_SPLIT_THREADS || p.rows < 1 || p.runs < 1) return "runs";
         if (static_cast<long long>(p.runs) * p.rows < s.positions || static_cast<long long>(p.runs - 1) * p.rows >= s.positions)
