@@ -517,7 +517,10 @@ MFH_API int mfh_adam_step(const mfh_adam_tensor* tensors, int count, float grad_
 /* Element types of the calls below that take more than float: 0 float32, 1 bfloat16, 2 float16. `logits`
  * holds `rows` rows of `vocab` contiguous elements, row_stride elements apart (offsets between rows are 64
  * bits; at most 2^22 rows of at most 2^24 logits). Tokens and ids are int32, or int64 with their flag; a
- * negative one is none. No counterpart in the reference, whose only loss is the mean squared error. */
+ * negative one is none. `counters` are MFH_LOGIT_COUNTERS 32-bit zeros on the device, in which a call counts its
+ * workgroups and which it leaves zero: calls that may run at the same time need their own.
+ * No counterpart in the reference, whose only loss is the mean squared error. */
+#define MFH_LOGIT_COUNTERS 1025
 
 /* Bytes of workspace of mfh_log_probs (0: none), -1 when the sizes are out of range. */
 MFH_API int64_t mfh_log_probs_workspace(int64_t rows, int vocab, int type, int top);
@@ -532,7 +535,7 @@ MFH_API int64_t mfh_log_probs_workspace(int64_t rows, int vocab, int type, int t
 MFH_API int mfh_log_probs(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
                           int tokens_int64, uint64_t log_prob, uint64_t entropy, uint64_t log_sum, uint64_t stats, int top,
                           uint64_t top_log_probs, uint64_t top_ids, uint64_t workspace, int64_t workspace_bytes,
-                          uint64_t stream);
+                          uint64_t counters, uint64_t stream);
 
 /* grad[r][j] (grad_stride elements a row, of the logits' type) = g ([j = token] - p) - h p (ln p + entropy), or
  * grad += that when add != 0, with g = scale * factor[0] * log_prob_grad[r * log_prob_grad_stride] (0 where
@@ -557,7 +560,7 @@ MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
 MFH_API int mfh_distill_loss(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,
                              int ids_int64, uint64_t teacher, int held, uint64_t row_weights, float temperature,
                              uint64_t row_loss, uint64_t weights, uint64_t stats, uint64_t targets, uint64_t loss,
-                             uint64_t workspace, int64_t workspace_bytes, uint64_t stream);
+                             uint64_t workspace, int64_t workspace_bytes, uint64_t counters, uint64_t stream);
 
 /* grad[r][j] = seed[0] w loss[1] temperature (q[j] - sum over k of p[k] [ids[k] = j]), or grad += that. */
 MFH_API int mfh_distill_loss_backward(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,

@@ -1178,11 +1178,11 @@ MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int
                           std::uint64_t tokens, int tokens_int64, std::uint64_t log_prob, std::uint64_t entropy,
                           std::uint64_t log_sum, std::uint64_t stats, int top, std::uint64_t top_log_probs,
                           std::uint64_t top_ids, std::uint64_t workspace, std::int64_t workspace_bytes,
-                          std::uint64_t stream) {
+                          std::uint64_t counters, std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(top >= 0 && top <= TOP_MAX && top <= vocab, "number of alternatives out of range");
-    MFH_REQUIRE(rows == 0 || (logits && entropy && log_sum && stats && (!log_prob || tokens) &&
+    MFH_REQUIRE(rows == 0 || (logits && entropy && log_sum && stats && counters && (!log_prob || tokens) &&
                               (top == 0 || (top_log_probs && top_ids))),
                 "log probabilities received a null buffer");
     const std::int64_t bytes = log_probs_workspace(rows, vocab, type, top);
@@ -1193,7 +1193,7 @@ MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int
     f.log_prob = as_ptr<float>(log_prob), f.entropy = as_ptr<float>(entropy), f.log_sum = as_ptr<float>(log_sum);
     f.stats = as_ptr<float>(stats);
     f.top_log_probs = as_ptr<float>(top_log_probs), f.top_ids = as_ptr<int>(top_ids);
-    f.workspace = as_ptr<void>(workspace);
+    f.workspace = as_ptr<void>(workspace), f.counters = as_ptr<unsigned>(counters);
     return launch_log_probs(as_ptr<const void>(logits), type, f, as_stream(stream));
 }
 
@@ -1227,12 +1227,12 @@ MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, 
                              std::uint64_t ids, int ids_int64, std::uint64_t teacher, int held,
                              std::uint64_t row_weights, float temperature, std::uint64_t row_loss, std::uint64_t weights,
                              std::uint64_t stats, std::uint64_t targets, std::uint64_t loss, std::uint64_t workspace,
-                             std::int64_t workspace_bytes, std::uint64_t stream) {
+                             std::int64_t workspace_bytes, std::uint64_t counters, std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(held > 0 && held <= DISTILL_HELD_MAX, "number of teacher logits a row out of range");
     MFH_REQUIRE(temperature > 0.0f && temperature <= FLT_MAX, "the temperature must be positive and finite");
-    MFH_REQUIRE(loss && (rows == 0 || (logits && ids && teacher && row_loss && weights && stats && targets)),
+    MFH_REQUIRE(loss && (rows == 0 || (logits && ids && teacher && row_loss && weights && stats && targets && counters)),
                 "distillation loss received a null buffer");
     const std::int64_t bytes = distill_workspace(rows, vocab, type);
     MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "distillation loss workspace too small");
@@ -1243,6 +1243,7 @@ MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, 
     f.temperature = temperature;
     f.row_loss = as_ptr<float>(row_loss), f.weights = as_ptr<float>(weights), f.stats = as_ptr<float>(stats);
     f.targets = as_ptr<float>(targets), f.loss = as_ptr<float>(loss), f.workspace = as_ptr<void>(workspace);
+    f.counters = as_ptr<unsigned>(counters);
     return launch_distill(as_ptr<const void>(logits), type, f, as_stream(stream));
 }
 

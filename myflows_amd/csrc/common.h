@@ -467,6 +467,8 @@ constexpr int TOP_MAX = 64;           // alternatives of a row
 constexpr int DISTILL_HELD_MAX = 256;  // teacher ids of a row
 constexpr std::int64_t LOGIT_ROWS_LIMIT = 1 << 22;  // rows of a call
 constexpr int LOGIT_VOCAB_LIMIT = 1 << 24;          // logits of a row
+constexpr int LOGIT_SPLIT_ROWS = 1024;              // rows that may be split over several workgroups
+constexpr int LOGIT_COUNTERS = LOGIT_SPLIT_ROWS + 1;  // zeros that a call counts its workgroups in, and leaves zero
 
 struct LogProbsForward {
     std::int64_t rows, stride;
@@ -480,6 +482,7 @@ struct LogProbsForward {
     float* top_log_probs;  // rows x top, with top_ids
     int* top_ids;
     void* workspace;
+    unsigned* counters;  // LOGIT_COUNTERS
 };
 std::int64_t log_probs_workspace(std::int64_t rows, int vocab, int type, int top);  // bytes
 int launch_log_probs(const void* logits, int type, const LogProbsForward& f, hipStream_t stream);
@@ -515,6 +518,7 @@ struct DistillForward {
     float* targets;  // rows x held: the teacher's probability of each id, summed over its occurrences
     float* loss;     // sum w row_loss / sum w, 1 / sum w
     void* workspace;
+    unsigned* counters;
 };
 std::int64_t distill_workspace(std::int64_t rows, int vocab, int type);  // bytes
 int launch_distill(const void* logits, int type, const DistillForward& f, hipStream_t stream);

@@ -11,6 +11,7 @@
 // log_prob -inf, entropy 0, gradient 0. A NaN or +inf makes its row NaN. All sums are float32.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
 #include "typed.h"
@@ -75,6 +76,23 @@ struct RowEnd {
     __device__ __forceinline__ explicit RowEnd(const RowStats& row) : m(row.m), s(row.s), ln_s(logf(row.s)), empty(row.s == 0.0f) {}
     __device__ __forceinline__ float log_prob(float z) const { return empty ? -INFINITY : (z - m) - ln_s; }
 };
+
+// Values that workgroups hand to one another within a launch. A fence over the whole GPU writes back and drops an
+// XCD's cache, which took 200 us for a thousand workgroups; instead these few values are written through to the
+// memory that all XCDs share, and read from there, as relaxed atomics of that scope.
+template <typename V>
+__device__ __forceinline__ void hand_over(V* to, V value) {
+    __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V>
+__device__ __forceinline__ V handed_over(const V* from) {
+    return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void hand_over(RowStats* to, const RowStats& value) {
+    hand_over(&to->m, value.m);
+    hand_over(&to->s, value.s);
+    hand_over(&to->t, value.t);
+}
 
 // A row's token and its logit, read ahead of the row's end.
 struct GivenToken {
@@ -207,8 +225,8 @@ struct TeacherRow {
         }
         loss = joint(loss, [](float a, float b) { return a + b; });
         if (threadIdx.x != 0) return;
-        f.row_loss[r] = weight == 0.0f ? 0.0f : poisoned ? NOT_A_NUMBER : f.temperature * f.temperature * loss;
-        f.weights[r] = weight;
+        hand_over(f.row_loss + r, weight == 0.0f ? 0.0f : poisoned ? NOT_A_NUMBER : f.temperature * f.temperature * loss);
+        hand_over(f.weights + r, weight);
         f.stats[r] = row.m;
         f.stats[f.rows + r] = poisoned ? NOT_A_NUMBER : row.s;
     }
@@ -233,7 +251,7 @@ struct RowRun {
     int chunk, begin, end;
 };
 
-// Where a run's results go when a row is split: statistics and k keys a run, joined by a second launch.
+// Where a run's results go when a row is split: statistics and k keys a run.
 struct RowPartials {
     RowStats* stats;
     unsigned long long* keys;
@@ -666,116 +684,171 @@ __device__ __forceinline__ RowRun run_of(const RowSplit& split, int vocab) {
     return {row, chunk, chunk * split.length, min(vocab, (chunk + 1) * split.length)};
 }
 
-template <typename T, int THREADS, bool TOP>
-__global__ __launch_bounds__(THREADS, 8) void log_probs_kernel(const T* __restrict__ logits, LogProbsForward f, RowSplit split,
-                                                            RowPartials partials) {
-    const RowRun run = run_of(split, f.vocab);
-    const T* __restrict__ z = logits + run.row * f.stride;
-    const long long at = run.row * split.chunks + run.chunk;
-    GivenToken given{};
-    int count = 0;
-    const auto meanwhile = [&] {
-        if (split.chunks == 1 && threadIdx.x == 0) given = GivenToken(f, z, run.row);
-    };
-    if constexpr (TOP) {
-        __shared__ TopState<THREADS / 64> top;
-        const RowStats row = take_run<true, true, T, THREADS>(z, run, LOG2E, &top, f.top, count, meanwhile);
-        if (threadIdx.x == 0) {
-            if (split.chunks == 1) finish_log_probs(f, run.row, given, row);
-            else partials.stats[at] = row;
-        }
-        const RowEnd end(row);
-        emit_top<T, THREADS>(top, z, run, f.top, count, row.s, [&](int rank, unsigned long long key) {
-            if (split.chunks == 1) write_top(f, run.row, rank, key, end);
-            else partials.keys[at * f.top + rank] = key;
-        });
-    } else {
-        const RowStats row =
-            take_run<true, false, T, THREADS>(z, run, LOG2E, nullptr, 0, count, meanwhile);
-        if (threadIdx.x != 0) return;
-        if (split.chunks == 1) finish_log_probs(f, run.row, given, row);
-        else partials.stats[at] = row;
+// Whether this workgroup is the last of `total` to get here; what the others handed over before is then there to
+// read. Every wave waits until its own writes are done before the workgroup is counted. The last one leaves the
+// counter at 0 for the next call. Nobody waits for another workgroup.
+__device__ __forceinline__ bool last_to_come(unsigned* counter, unsigned total) {
+    __shared__ bool last;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = atomicAdd(counter, 1u) + 1 == total;
+        if (last) hand_over(counter, 0u);
     }
+    __syncthreads();
+    return last;
 }
 
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void distill_kernel(const T* __restrict__ logits, DistillForward f, RowSplit split,
-                                                          RowPartials partials) {
-    const RowRun run = run_of(split, f.vocab);
-    const T* __restrict__ z = logits + run.row * f.stride;
-    int count;
-    TeacherRow<THREADS> teacher;
-    const RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature,
-                                                            nullptr, 0, count, [&] {
-                                                                if (split.chunks == 1) teacher.read(f, z, run.row);
-                                                            });
-    if (split.chunks == 1) teacher.finish(f, run.row, row);
-    else if (threadIdx.x == 0) partials.stats[run.row * split.chunks + run.chunk] = row;
-}
+constexpr int SPLIT_MAX = 64;
 
-// The runs of a row (at most 64) joined by one wave, the same in every lane.
-__device__ __forceinline__ RowStats join_runs(const RowStats* __restrict__ stats, int chunks, float scale) {
+// The runs of a row (at most 64) joined by each wave, the same in every lane.
+__device__ __forceinline__ RowStats join_runs(const RowStats* stats, int chunks, float scale) {
     const int lane = threadIdx.x & 63;
-    RowStats mine = lane < chunks ? stats[lane] : RowStats::none();
+    RowStats mine = RowStats::none();
+    if (lane < chunks) mine = {handed_over(&stats[lane].m), handed_over(&stats[lane].s), handed_over(&stats[lane].t)};
     mine.rescale(wave_max(mine.m), scale);
     mine.s = wave_sum(mine.s);
     mine.t = wave_sum(mine.t);
     return mine;
 }
 
-constexpr int JOIN_THREADS = 256;
-constexpr int SPLIT_MAX = 64;
+struct JoinState {
+    unsigned long long kept[SPLIT_MAX * TOP_MAX], bounds[2][SPLIT_MAX];
+    int ranks[ROW_THREADS], count;
+};
 
-// Joins a row's runs: one workgroup a row. Each run's keys come in falling order. At least k keys reach the
-// smallest of the runs' keys at place ceil(k / runs), and k those of any run its k-th: keys below the larger of
-// the two bounds are none of the k largest.
-template <typename T>
-__global__ __launch_bounds__(JOIN_THREADS) void log_probs_join_kernel(const T* __restrict__ logits, LogProbsForward f,
-                                                                      RowSplit split, RowPartials partials) {
-    __shared__ unsigned long long kept[SPLIT_MAX * TOP_MAX], bounds[2][SPLIT_MAX];
-    __shared__ int ranks[JOIN_THREADS], count;
-    const long long r = blockIdx.x;
-    const int tid = threadIdx.x, k = f.top;
-    const unsigned long long* __restrict__ keys = partials.keys + r * split.chunks * k;
-    if (k && tid < split.chunks) {
-        bounds[0][tid] = keys[tid * k + (k + split.chunks - 1) / split.chunks - 1];
-        bounds[1][tid] = keys[tid * k + k - 1];
+// The k largest keys of a row's runs, each run's in falling order. At least k keys reach the smallest of the runs'
+// keys at place ceil(k / runs), and k those of any run its k-th: keys below the larger of the two bounds are none
+// of the k largest.
+template <typename Emit>
+__device__ __forceinline__ void join_top(JoinState& join, const unsigned long long* keys, int chunks, int k,
+                                         Emit&& emit) {
+    constexpr int WAVES = ROW_THREADS / 64;
+    const int tid = threadIdx.x;
+    __syncthreads();  // what the run's own alternatives left in LDS is read
+    if (tid < chunks) {
+        join.bounds[0][tid] = handed_over(keys + tid * k + (k + chunks - 1) / chunks - 1);
+        join.bounds[1][tid] = handed_over(keys + tid * k + k - 1);
     }
-    GivenToken given{};
-    if (tid == 0) given = GivenToken(f, logits + r * f.stride, r);
-    const RowStats row = join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E);
-    if (tid == 0) {
-        finish_log_probs(f, r, given, row);
-        count = 0;
-    }
-    if (k == 0) return;
+    if (tid == 0) join.count = 0;
     __syncthreads();
     unsigned long long all = ~0ull, any = 0;
-    for (int i = 0; i < split.chunks; ++i) {
-        all = min(all, bounds[0][i]);
-        any = max(any, bounds[1][i]);
+    for (int i = 0; i < chunks; ++i) {
+        all = min(all, join.bounds[0][i]);
+        any = max(any, join.bounds[1][i]);
     }
     const unsigned long long least = max(max(all, any), 1ull);
-    for (int i = tid; i < split.chunks * k; i += JOIN_THREADS) {
-        const unsigned long long key = keys[i];
-        if (key >= least) kept[atomicAdd(&count, 1)] = key;
+    for (int i = tid; i < chunks * k; i += ROW_THREADS) {
+        const unsigned long long key = handed_over(keys + i);
+        if (key >= least) join.kept[atomicAdd(&join.count, 1)] = key;
     }
     __syncthreads();
-    const RowEnd end(row);
-    constexpr int WAVES = JOIN_THREADS / 64;
-    const int found = count, part = (found + WAVES - 1) / WAVES, from = min(found, tid / 64 * part);
-    emit_ranks<WAVES>([&](int i) { return kept[i]; }, found, k, kept + from, min(part, found - from), ranks,
-               [&](int rank, unsigned long long key) { write_top(f, r, rank, key, end); });
-    for (int i = found + tid; i < k; i += JOIN_THREADS) write_top(f, r, i, 0, end);
+    const int found = join.count, part = (found + WAVES - 1) / WAVES, from = min(found, tid / 64 * part);
+    emit_ranks<WAVES>([&](int i) { return join.kept[i]; }, found, k, join.kept + from, min(part, found - from), join.ranks, emit);
+    for (int i = found + tid; i < k; i += ROW_THREADS) emit(i, 0);
 }
 
-template <typename T>
-__global__ __launch_bounds__(64) void distill_join_kernel(const T* __restrict__ logits, DistillForward f, RowSplit split,
+// With SPLIT a workgroup takes a run of a row and the last one of a row joins its runs.
+template <typename T, int THREADS, bool TOP, bool SPLIT>
+__global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void log_probs_kernel(const T* __restrict__ logits, LogProbsForward f,
+                                                                           RowSplit split, RowPartials partials) {
+    union Shared {
+        TopState<THREADS / 64> top;
+        JoinState join;
+    };
+    const RowRun run = run_of(split, f.vocab);
+    const T* __restrict__ z = logits + run.row * f.stride;
+    const long long at = run.row * split.chunks + run.chunk;
+    GivenToken given{};
+    int count = 0;
+    const auto meanwhile = [&] {
+        if (threadIdx.x == 0) given = GivenToken(f, z, run.row);
+    };
+    RowStats row;
+    if constexpr (TOP) {
+        __shared__ std::conditional_t<SPLIT, Shared, TopState<THREADS / 64>> shared;
+        auto& top = *reinterpret_cast<TopState<THREADS / 64>*>(&shared);
+        row = take_run<true, true, T, THREADS>(z, run, LOG2E, &top, f.top, count, meanwhile);
+        if constexpr (!SPLIT) {
+            const RowEnd end(row);
+            emit_top<T, THREADS>(top, z, run, f.top, count, row.s,
+                                 [&](int rank, unsigned long long key) { write_top(f, run.row, rank, key, end); });
+        } else {
+            emit_top<T, THREADS>(top, z, run, f.top, count, row.s,
+                                 [&](int rank, unsigned long long key) { hand_over(partials.keys + at * f.top + rank, key); });
+        }
+        if constexpr (SPLIT) {
+            if (threadIdx.x == 0) hand_over(partials.stats + at, row);
+            if (!last_to_come(f.counters + run.row, split.chunks)) return;
+            row = join_runs(partials.stats + run.row * split.chunks, split.chunks, LOG2E);
+            const RowEnd end(row);
+            join_top(reinterpret_cast<Shared*>(&shared)->join, partials.keys + run.row * split.chunks * f.top, split.chunks, f.top,
+                     [&](int rank, unsigned long long key) { write_top(f, run.row, rank, key, end); });
+        }
+    } else {
+        row = take_run<true, false, T, THREADS>(z, run, LOG2E, nullptr, 0, count, meanwhile);
+        if constexpr (SPLIT) {
+            if (threadIdx.x == 0) hand_over(partials.stats + at, row);
+            if (!last_to_come(f.counters + run.row, split.chunks)) return;
+            row = join_runs(partials.stats + run.row * split.chunks, split.chunks, LOG2E);
+        }
+    }
+    if (threadIdx.x == 0) finish_log_probs(f, run.row, given, row);
+}
+
+// out[0] = scale * sum w v / sum w and out[1] = 1 / sum w (both 0 when nothing counts), in FP64 by one workgroup:
+// thread t adds rows t, t + threads, ... in order, a fixed tree the threads' sums. weight_of(r) is 0 for a row
+// that does not count; it adds nothing, whatever its value is.
+template <int THREADS, typename ValueOf, typename WeightOf>
+__device__ __forceinline__ void mean_of_rows(ValueOf&& value_of, WeightOf&& weight_of, long long rows, float scale,
+                                             float* __restrict__ out) {
+    __shared__ double sum[THREADS], weight[THREADS];
+    double a = 0.0, b = 0.0;
+    for (long long r = threadIdx.x; r < rows; r += THREADS) {
+        const float w = weight_of(r);
+        if (w == 0.0f) continue;
+        a += static_cast<double>(w) * static_cast<double>(value_of(r));
+        b += static_cast<double>(w);
+    }
+    sum[threadIdx.x] = a;
+    weight[threadIdx.x] = b;
+    __syncthreads();
+    for (int half = THREADS / 2; half > 0; half /= 2) {
+        if (static_cast<int>(threadIdx.x) < half) {
+            sum[threadIdx.x] += sum[threadIdx.x + half];
+            weight[threadIdx.x] += weight[threadIdx.x + half];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x != 0) return;
+    out[0] = weight[0] == 0.0 ? 0.0f : static_cast<float>(scale * sum[0] / weight[0]);
+    out[1] = weight[0] == 0.0 ? 0.0f : static_cast<float>(1.0 / weight[0]);
+}
+
+// The loss of few rows comes from the last workgroup of all, that of many from a launch of its own.
+constexpr int MEAN_ROWS = 128;
+
+template <typename T, int THREADS, bool SPLIT>
+__global__ __launch_bounds__(THREADS) void distill_kernel(const T* __restrict__ logits, DistillForward f, RowSplit split,
                                                           RowPartials partials) {
-    const long long r = blockIdx.x;
-    TeacherRow<64> teacher;
-    teacher.read(f, logits + r * f.stride, r);
-    teacher.finish(f, r, join_runs(partials.stats + r * split.chunks, split.chunks, LOG2E / f.temperature));
+    const RowRun run = run_of(split, f.vocab);
+    const T* __restrict__ z = logits + run.row * f.stride;
+    int count;
+    TeacherRow<THREADS> teacher;
+    RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature, nullptr, 0, count, [&] {
+        if constexpr (!SPLIT) teacher.read(f, z, run.row);
+    });
+    if constexpr (SPLIT) {
+        if (threadIdx.x == 0) hand_over(partials.stats + run.row * split.chunks + run.chunk, row);
+        if (!last_to_come(f.counters + run.row, split.chunks)) return;
+        teacher.read(f, z, run.row);
+        row = join_runs(partials.stats + run.row * split.chunks, split.chunks, LOG2E / f.temperature);
+    }
+    teacher.finish(f, run.row, row);
+    if (f.rows > MEAN_ROWS || !last_to_come(f.counters + LOGIT_SPLIT_ROWS, static_cast<unsigned>(f.rows))) return;
+    mean_of_rows<THREADS>([&](long long r) { return handed_over(f.row_loss + r); },
+                          [&](long long r) { return handed_over(f.weights + r); }, f.rows, 1.0f, f.loss);
 }
 
 // ---- the gradients --------------------------------------------------------------------------
@@ -897,51 +970,28 @@ __global__ __launch_bounds__(GRAD_THREADS) void distill_backward_kernel(const T*
     if (id >= 0) out[id] = static_cast<T>(held + coef * (share(at_id) - target));
 }
 
-// out[0] = scale * sum w v / sum w and out[1] = 1 / sum w (both 0 when nothing counts), in FP64: thread t
-// adds rows t, t + threads, ... in order, a fixed tree the threads' sums. w is the row's weight, or whether
-// its token is given, or 1; a row of weight 0 adds nothing, whatever its value is.
+// w is the row's weight, or whether its token is given, or 1.
 __global__ __launch_bounds__(MEAN_THREADS) void row_mean_kernel(const float* __restrict__ values,
                                                                 const float* __restrict__ weights,
                                                                 const void* __restrict__ tokens, int tokens_wide,
                                                                 long long rows, float scale, float* __restrict__ out) {
-    __shared__ double sum[MEAN_THREADS], weight[MEAN_THREADS];
-    double a = 0.0, b = 0.0;
-    for (long long r = threadIdx.x; r < rows; r += MEAN_THREADS) {
-        const float w = weights ? weights[r] : tokens && whole_at(tokens, tokens_wide, r) < 0 ? 0.0f : 1.0f;
-        if (w == 0.0f) continue;
-        a += static_cast<double>(w) * static_cast<double>(values[r]);
-        b += static_cast<double>(w);
-    }
-    sum[threadIdx.x] = a;
-    weight[threadIdx.x] = b;
-    __syncthreads();
-    for (int half = MEAN_THREADS / 2; half > 0; half /= 2) {
-        if (static_cast<int>(threadIdx.x) < half) {
-            sum[threadIdx.x] += sum[threadIdx.x + half];
-            weight[threadIdx.x] += weight[threadIdx.x + half];
-        }
-        __syncthreads();
-    }
-    if (threadIdx.x != 0) return;
-    out[0] = weight[0] == 0.0 ? 0.0f : static_cast<float>(scale * sum[0] / weight[0]);
-    out[1] = weight[0] == 0.0 ? 0.0f : static_cast<float>(1.0 / weight[0]);
+    mean_of_rows<MEAN_THREADS>(
+        [&](long long r) { return values[r]; },
+        [&](long long r) { return weights ? weights[r] : tokens && whole_at(tokens, tokens_wide, r) < 0 ? 0.0f : 1.0f; },
+        rows, scale, out);
 }
-
-}  // namespace
-
-namespace {
 
 // Threads of a row's workgroup: a wave while a row is at most two tiles of it (no barriers), else four.
 constexpr int SMALL_ROW_BYTES = 2 * 64 * TILE_PACKS * 16, WAVE_THREADS = 64;
 
 bool small_row(int vocab, int type) { return vocab * static_cast<std::int64_t>(type_bytes(type)) <= SMALL_ROW_BYTES; }
 
-// Runs of a row. Rows are split where the time that whole rows leave CUs idle is more than a second launch takes:
+// Runs of a row. Rows are split where the time that whole rows leave CUs idle is more than joining them takes:
 // of 256 CUs that read ROW_RATE bytes a microsecond each (5/8 of that with one workgroup), whole rows take the most
 // that one CU has of them, split ones their share and JOIN_TIME. Measured split / whole: 777 rows of 64 KB 18.7 /
 // 17.5 us, 1024 of them 18.1 / 17.4, one 4.3 / 5.3. Then as many runs as bring the workgroups to SPLIT_GROUPS, of
 // at least one tile. All of this follows from the sizes alone, so that results do not depend on the device.
-constexpr int SPLIT_GROUPS = 2048, ROW_RATE = 20000, JOIN_TIME = 5, SPLIT_CUS = 256;
+constexpr int SPLIT_GROUPS = 1024, ROW_RATE = 20000, JOIN_TIME = 5, SPLIT_CUS = 256;
 RowSplit row_split(std::int64_t rows, int vocab, int type) {
     if (rows == 0 || small_row(vocab, type)) return {1, vocab};
     const std::int64_t bytes = static_cast<std::int64_t>(vocab) * type_bytes(type);
@@ -952,8 +1002,9 @@ RowSplit row_split(std::int64_t rows, int vocab, int type) {
     const std::int64_t wanted = std::min<std::int64_t>(SPLIT_MAX, std::max<std::int64_t>(1, SPLIT_GROUPS / rows));
     const std::int64_t packs = (vocab + unit - 1) / unit;
     const int length = static_cast<int>(std::max<std::int64_t>(TILE_PACKS, (packs + wanted - 1) / wanted)) * unit;
-    return {static_cast<int>((vocab + length - 1) / length), length};
+    return {static_cast<int>((vocab + length - 1) / length), length};  // several runs of at most LOGIT_SPLIT_ROWS rows
 }
+static_assert(SPLIT_GROUPS / 2 <= LOGIT_SPLIT_ROWS, "a counter a row that is split");
 
 RowPartials partials_in(void* workspace, std::int64_t runs, std::int64_t top) {
     auto* keys = static_cast<unsigned long long*>(workspace);
@@ -984,19 +1035,14 @@ int launch_log_probs(const void* logits, int type, const LogProbsForward& f, hip
         const T* z = static_cast<const T*>(logits);
         const auto run = [&](auto kernel, int threads) { launch(kernel, groups, threads, 0, stream, z, f, split, partials); };
         const bool small = small_row(f.vocab, type);
-        if (f.top && small) run(log_probs_kernel<T, WAVE_THREADS, true>, WAVE_THREADS);
-        else if (f.top) run(log_probs_kernel<T, ROW_THREADS, true>, ROW_THREADS);
-        else if (small) run(log_probs_kernel<T, WAVE_THREADS, false>, WAVE_THREADS);
-        else run(log_probs_kernel<T, ROW_THREADS, false>, ROW_THREADS);
+        if (f.top && small) run(log_probs_kernel<T, WAVE_THREADS, true, false>, WAVE_THREADS);
+        else if (f.top && split.chunks > 1) run(log_probs_kernel<T, ROW_THREADS, true, true>, ROW_THREADS);
+        else if (f.top) run(log_probs_kernel<T, ROW_THREADS, true, false>, ROW_THREADS);
+        else if (small) run(log_probs_kernel<T, WAVE_THREADS, false, false>, WAVE_THREADS);
+        else if (split.chunks > 1) run(log_probs_kernel<T, ROW_THREADS, false, true>, ROW_THREADS);
+        else run(log_probs_kernel<T, ROW_THREADS, false, false>, ROW_THREADS);
     });
-    MFH_TRY(MFH_CHECK_LAUNCH("log_probs", stream));
-    if (split.chunks == 1) return OK;
-    with_type(type, [&](auto zero) {
-        using T = decltype(zero);
-        launch(log_probs_join_kernel<T>, static_cast<unsigned>(f.rows), f.top ? JOIN_THREADS : 64, 0, stream,
-               static_cast<const T*>(logits), f, split, partials);
-    });
-    return MFH_CHECK_LAUNCH("log_probs_join", stream);
+    return MFH_CHECK_LAUNCH("log_probs", stream);
 }
 
 int launch_log_probs_backward(const void* logits, void* grad, int type, const LogProbsBackward& b, hipStream_t stream) {
@@ -1022,20 +1068,13 @@ int launch_distill(const void* logits, int type, const DistillForward& f, hipStr
         with_type(type, [&](auto zero) {
             using T = decltype(zero);
             const T* z = static_cast<const T*>(logits);
-            if (small_row(f.vocab, type))
-                launch(distill_kernel<T, WAVE_THREADS>, groups, WAVE_THREADS, 0, stream, z, f, split, partials);
-            else
-                launch(distill_kernel<T, ROW_THREADS>, groups, ROW_THREADS, 0, stream, z, f, split, partials);
+            const auto run = [&](auto kernel, int threads) { launch(kernel, groups, threads, 0, stream, z, f, split, partials); };
+            if (small_row(f.vocab, type)) run(distill_kernel<T, WAVE_THREADS, false>, WAVE_THREADS);
+            else if (split.chunks > 1) run(distill_kernel<T, ROW_THREADS, true>, ROW_THREADS);
+            else run(distill_kernel<T, ROW_THREADS, false>, ROW_THREADS);
         });
         MFH_TRY(MFH_CHECK_LAUNCH("distill", stream));
-        if (split.chunks > 1) {
-            with_type(type, [&](auto zero) {
-                using T = decltype(zero);
-                launch(distill_join_kernel<T>, static_cast<unsigned>(f.rows), 64, 0, stream, static_cast<const T*>(logits),
-                       f, split, partials);
-            });
-            MFH_TRY(MFH_CHECK_LAUNCH("distill_join", stream));
-        }
+        if (f.rows <= MEAN_ROWS) return OK;
     }
     return launch_row_mean(f.row_loss, f.weights, nullptr, 0, f.rows, 1.0f, f.loss, stream);
 }

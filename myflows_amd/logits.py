@@ -182,7 +182,8 @@ def log_probs_forward(logits, tokens=None, *, top=0):
     stats, row = floats.data_ptr(), 4 * rows
     native._call("mfh_log_probs", logits.data_ptr(), code, rows, vocab, stride, native._addr(tokens), wide,
                  0 if tokens is None else stats + 4 * row, stats + 2 * row, stats + 3 * row, stats, top,
-                 native._addr(top_log_probs), native._addr(top_ids), workspace, held, native._stream())
+                 native._addr(top_log_probs), native._addr(top_ids), workspace, held, native.stream_counters(),
+                 native._stream())
     return LogProbs(floats, tokens is not None, top_log_probs, top_ids)
 
 
@@ -246,7 +247,8 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
     row_loss = scale + 8
     native._call("mfh_distill_loss", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
                  teacher_logits.data_ptr(), shape[1], native._addr(row_weights), temperature, row_loss, row_loss + row,
-                 row_loss + 2 * row, row_loss + 4 * row, scale, workspace, held, native._stream())
+                 row_loss + 2 * row, row_loss + 4 * row, scale, workspace, held, native.stream_counters(),
+                 native._stream())
     return DistillLoss(floats, rows, shape[1])
 
 

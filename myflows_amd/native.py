@@ -137,10 +137,10 @@ _SIGNATURES = {
     "mfh_mse_loss_backward": ("i", "ppppqip"),
     "mfh_column_sums": ("i", "ppqqp"),
     "mfh_log_probs_workspace": ("q", "qiii"),
-    "mfh_log_probs": ("i", "piqiq" + "pi" + "pppp" + "ipp" + "pqp"),
+    "mfh_log_probs": ("i", "piqiq" + "pi" + "pppp" + "ipp" + "pqpp"),
     "mfh_log_probs_backward": ("i", "piqiq" + "pi" + "pp" + "pqpq" + "pf" + "pqi" + "p"),
     "mfh_distill_workspace": ("q", "qii"),
-    "mfh_distill_loss": ("i", "piqiq" + "pipi" + "pf" + "ppppp" + "pqp"),
+    "mfh_distill_loss": ("i", "piqiq" + "pipi" + "pf" + "ppppp" + "pqpp"),
     "mfh_distill_loss_backward": ("i", "piqiq" + "pii" + "ppppp" + "f" + "pqi" + "p"),
     "mfh_row_mean": ("i", "ppiqfpp"),
     "mfh_group_norm_workspace": ("q", "qiiiii"),
@@ -621,6 +621,20 @@ def stream_workspaces():
 
 def _holds_pending_split(block):
     return any(entry[1] is block for entry in _PENDING_SPLITS.values())
+
+
+_STREAM_COUNTERS = {}
+LOGIT_COUNTERS = 1025  # MFH_LOGIT_COUNTERS of include/mfhip.h
+
+
+def stream_counters():
+    """The address of the zeros in which calls on the current stream count their workgroups. Each call leaves
+    them zero, and calls on one stream run one after the other, so they are cleared once, on that stream."""
+    key = (_current_device(), _stream())
+    held = _STREAM_COUNTERS.get(key)
+    if held is None:
+        held = _STREAM_COUNTERS[key] = fill_(torch.empty(LOGIT_COUNTERS, dtype=torch.float32, device="cuda"), 0.0)
+    return held.data_ptr()
 
 
 def workspace_bytes(symbol, *sizes):
