@@ -29,7 +29,7 @@ namespace {
 
 // A plan's block as the kernels take it (GroupNormPlan's fields).
 struct Block {
-    int per, groups, parts, width, blocks, lanes_log2;
+    int per, groups, parts, width, blocks, lanes;
     FastDiv per_div;
 };
 constexpr int BLOCK_GROUPS_MAX = GROUP_NORM_BLOCK_GROUPS;
@@ -71,21 +71,28 @@ template <int THREADS, int VW>
 struct ColumnSums {
     static constexpr int FLOATS = THREADS * VW;
 
-    // Parts that a column has in LDS, and the floats from one part to the next.
-    static __device__ __forceinline__ int parts(const Block& k) { return THREADS >> max(k.lanes_log2, 6); }
-    static __device__ __forceinline__ int pitch(const Block& k) { return VW << k.lanes_log2; }
+    // Whether a wave's rows are joined across its lanes; parts that a column then has in LDS, and the floats from
+    // one part to the next.
+    static __device__ __forceinline__ bool joined(const Block& k) { return k.lanes <= 32; }
+    static __device__ __forceinline__ int parts(const Block& k) { return joined(k) ? THREADS / 64 : THREADS / k.lanes; }
+    static __device__ __forceinline__ int pitch(const Block& k) { return VW * k.lanes; }
 
     static __device__ __forceinline__ void put(const Block& k, float (&lds)[FLOATS], const float (&mine)[VW]) {
-        const int lanes = 1 << k.lanes_log2;
         float v[VW];
 #pragma unroll
         for (int i = 0; i < VW; ++i) v[i] = mine[i];
-        for (int o = lanes; o < 64; o <<= 1)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) v[i] += __shfl_xor(v[i], o);
         const int tid = threadIdx.x;
-        if (lanes < 64 && (tid & 63) >= lanes) return;
-        float* to = lds + (tid >> max(k.lanes_log2, 6)) * pitch(k) + (tid & (lanes - 1)) * VW;
+        int part = tid / k.lanes, lane = tid - part * k.lanes;
+        if (joined(k)) {
+            for (int o = k.lanes; o < 64; o <<= 1)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) v[i] += __shfl_xor(v[i], o);
+            part = tid / 64;
+            if ((tid & 63) >= k.lanes) return;
+        } else if (part >= parts(k)) {
+            return;
+        }
+        float* to = lds + part * pitch(k) + lane * VW;
 #pragma unroll
         for (int i = 0; i < VW; ++i) to[i] = v[i];
     }
@@ -127,11 +134,11 @@ struct Thread {
     int group[VW];  // of the block's groups
 
     __device__ __forceinline__ Thread(const Block& k, int width) {
-        const int tid = threadIdx.x, lanes = 1 << k.lanes_log2;
-        column = (tid & (lanes - 1)) * VW;
-        row = tid >> k.lanes_log2;
-        step = THREADS >> k.lanes_log2;
-        active = column < width;
+        const int tid = threadIdx.x;
+        row = tid / k.lanes;
+        column = (tid - row * k.lanes) * VW;
+        step = THREADS / k.lanes;
+        active = column < width && row < step;
 #pragma unroll
         for (int i = 0; i < VW; ++i) group[i] = active && k.parts == 1 ? k.per_div.div(column + i) : 0;
     }
@@ -429,13 +436,25 @@ __global__ __launch_bounds__(SPLIT_THREADS) void run_stats_kernel(const T* __res
     if (static_cast<int>(threadIdx.x) < k.groups) squares[to + threadIdx.x] = sums[threadIdx.x];
 }
 
-// The runs and parts of each (sample, group) joined: one wave each.
-__global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict__ means, const float* __restrict__ squares,
-                                                         GroupNormShape s, Block k, Runs runs, GroupNormForward f) {
-    const long long at = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 64;
-    if (at >= s.n * s.groups) return;  // the whole wave
-    const int lane = threadIdx.x & 63, g = static_cast<int>(at % s.groups), pieces = runs.count * k.parts;
-    const long long n = at / s.groups;
+__device__ __forceinline__ float group_sum(float v) {
+    __shared__ float part[SPLIT_THREADS / 64];
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int w = 1; w < SPLIT_THREADS / 64; ++w) v += part[w];
+    return v;
+}
+
+// The runs and parts of each (sample, group) joined: one workgroup each.
+__global__ __launch_bounds__(SPLIT_THREADS) void join_stats_kernel(const float* __restrict__ means,
+                                                                   const float* __restrict__ squares, GroupNormShape s,
+                                                                   Block k, Runs runs, GroupNormForward f) {
+    const unsigned sample = blockIdx.x / static_cast<unsigned>(s.groups);
+    const int g = static_cast<int>(blockIdx.x - sample * s.groups), pieces = runs.count * k.parts;
+    const long long n = sample;
     const auto piece = [&](int i, float& count) {
         const int run = i / k.parts, part = i - run * k.parts;
         const int rows = min(s.positions - run * runs.rows, runs.rows);
@@ -444,24 +463,24 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict
         return ((n * runs.count + run) * s.groups + g) * k.parts + part;
     };
     float sum = 0.0f;
-    for (int i = lane; i < pieces; i += 64) {
+    for (int i = threadIdx.x; i < pieces; i += SPLIT_THREADS) {
         float count;
         const long long from = piece(i, count);
         sum += count * means[from];
     }
     const float inv_count = 1.0f / (static_cast<float>(s.positions) * static_cast<float>(k.per));
-    const float mean = wave_sum(sum) * inv_count;
+    const float mean = group_sum(sum) * inv_count;
     float about = 0.0f;
-    for (int i = lane; i < pieces; i += 64) {
+    for (int i = threadIdx.x; i < pieces; i += SPLIT_THREADS) {
         float count;
         const long long from = piece(i, count);
         const float d = means[from] - mean;
         about += squares[from] + count * (d * d);
     }
-    about = wave_sum(about);
-    if (lane != 0) return;
-    f.mean[at] = mean;
-    f.inv_std[at] = 1.0f / sqrtf(about * inv_count + f.eps);
+    about = group_sum(about);
+    if (threadIdx.x != 0) return;
+    f.mean[blockIdx.x] = mean;
+    f.inv_std[blockIdx.x] = 1.0f / sqrtf(about * inv_count + f.eps);
 }
 
 template <typename T, int VW, bool SILU>
@@ -666,7 +685,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void apply_backward_kernel(const T* 
 
 // ---- launches --------------------------------------------------------------------------------
 Block block_of(const GroupNormPlan& plan) {
-    return {plan.per, plan.groups, plan.parts, plan.width, plan.blocks, plan.lanes_log2, FastDiv(plan.per)};
+    return {plan.per, plan.groups, plan.parts, plan.width, plan.blocks, plan.lanes, FastDiv(plan.per)};
 }
 
 constexpr std::int64_t THREADS_LIMIT = (1LL << 32) - 1;  // threads of a launch
@@ -730,7 +749,7 @@ int launch_group_norm_forward(const GroupNormShape& s, int type, const void* x, 
     });
     MFH_TRY(MFH_CHECK_LAUNCH("group_norm_forward", stream));
     if (plan.held) return OK;
-    launch(join_stats_kernel, blocks_for(s.n * s.groups, 4), 256, 0, stream, means, squares, s, block, runs, f);
+    launch(join_stats_kernel, static_cast<unsigned>(s.n * s.groups), SPLIT_THREADS, 0, stream, means, squares, s, block, runs, f);
     MFH_TRY(MFH_CHECK_LAUNCH("group_norm_join", stream));
     with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
         using T = decltype(zero);

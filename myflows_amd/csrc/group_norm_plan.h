@@ -14,8 +14,9 @@ struct GroupNormShape {
 };
 
 // A block is what one workgroup takes of a row: `groups` whole groups, or, where a group is wider than a
-// workgroup, one of `parts` pieces of a group. Threads lie over it in `lanes` (a power of two) side by side, a
-// pack of `vw` channels each (those beyond the block idle), threads / lanes rows at a time.
+// workgroup, one of `parts` pieces of a group. Threads lie over it in `lanes` side by side, a pack of `vw`
+// channels each (those beyond the block idle), threads / lanes rows at a time (those beyond idle). Lanes are a
+// power of two up to 32, so that the rows of a wave join across its lanes; from 33 packs on as many as there are.
 struct GroupNormPlan {
     bool held;       // a workgroup holds its block over all positions
     int threads;
@@ -25,7 +26,7 @@ struct GroupNormPlan {
     int parts;       // blocks of a group
     int width;       // channels of a block (the last part of a group may hold fewer)
     int blocks;      // blocks of a sample
-    int lanes_log2;
+    int lanes;
     int runs, rows;  // split: runs of a sample's positions, and positions of a run
     std::int64_t grid() const { return blocks * static_cast<std::int64_t>(held ? 1 : runs); }  // workgroups of a sample
 };
@@ -49,16 +50,17 @@ inline int group_norm_pack(int type_size, int channels) {
     return type_size == 2 && channels % 2 == 0 ? 2 : 1;
 }
 
-inline int log2_up(int value) {
-    int log2 = 0;
-    while ((1 << log2) < value) ++log2;
-    return log2;
+inline int group_norm_lanes(int packs) {
+    if (packs > 32) return packs;
+    int lanes = 1;
+    while (lanes < packs) lanes *= 2;
+    return lanes;
 }
 
 inline void group_norm_block(const GroupNormShape& s, int groups, int vw, GroupNormPlan* plan) {
     plan->vw = vw, plan->per = s.channels / s.groups, plan->groups = groups, plan->parts = 1;
     plan->width = groups * plan->per, plan->blocks = s.groups / groups;
-    plan->lanes_log2 = log2_up(plan->width / vw);
+    plan->lanes = group_norm_lanes(plan->width / vw);
 }
 
 // Whether `threads` threads hold a block of `groups` groups over all positions.
@@ -66,8 +68,11 @@ inline bool group_norm_holds(const GroupNormShape& s, int type_size, bool backwa
                              GroupNormPlan* plan) {
     const int width = groups * (s.channels / s.groups), vw = group_norm_pack(type_size, width);
     if (width / vw > threads || groups > GROUP_NORM_BLOCK_GROUPS) return false;
-    const int rows = (threads >> log2_up(width / vw)) * group_norm_hold(type_size, vw, backward, threads);
-    if (rows < s.positions) return false;
+    // Where the blocks leave half of the CUs idle, up to 16 narrow packs a thread: 64 blocks of 32 each took 28 us
+    // backward (2 x 4096 x 320 float16), by runs of positions over all CUs 19.
+    int hold = group_norm_hold(type_size, vw, backward, threads);
+    if (s.n * (s.groups / groups) < 128) hold = std::min(hold, 16);
+    if (threads / group_norm_lanes(width / vw) * hold < s.positions) return false;
     group_norm_block(s, groups, vw, plan);
     plan->held = true, plan->threads = threads;
     return true;
@@ -76,7 +81,7 @@ inline bool group_norm_holds(const GroupNormShape& s, int type_size, bool backwa
 inline GroupNormPlan group_norm_plan(const GroupNormShape& s, int type_size, bool backward) {
     constexpr int FILL = 256;        // workgroups that fill the CUs
     constexpr int LINE_BYTES = 128;  // a cache line
-    constexpr int RUN_GROUPS = 2048; // workgroups of a split pass: eight a CU
+    constexpr int RUN_GROUPS = 1024; // workgroups of a split pass: four a CU
     GroupNormPlan plan{};
     const int per = s.channels / s.groups;
     // Held: whole groups side by side until a block's row fills a cache line and the block two packs a thread of
@@ -105,9 +110,9 @@ inline GroupNormPlan group_norm_plan(const GroupNormShape& s, int type_size, boo
         plan.width = plan.threads * vw;
         plan.parts = (per + plan.width - 1) / plan.width;
         plan.blocks = s.groups * plan.parts;
-        plan.lanes_log2 = log2_up(plan.threads);
+        plan.lanes = plan.threads;
     }
-    const int step = (plan.threads >> plan.lanes_log2) * GROUP_NORM_SPLIT_AHEAD;
+    const int step = plan.threads / plan.lanes * 2 * GROUP_NORM_SPLIT_AHEAD;  // a thread reads ahead twice at least
     const std::int64_t most = (s.positions + static_cast<std::int64_t>(step) - 1) / step;
     const std::int64_t wanted = std::max<std::int64_t>(1, RUN_GROUPS / (s.n * plan.blocks));
     const std::int64_t count = std::min(most, wanted);

@@ -991,7 +991,7 @@ bool small_row(int vocab, int type) { return vocab * static_cast<std::int64_t>(t
 // that one CU has of them, split ones their share and JOIN_TIME. Measured split / whole: 777 rows of 64 KB 18.7 /
 // 17.5 us, 1024 of them 18.1 / 17.4, one 4.3 / 5.3. Then as many runs as bring the workgroups to SPLIT_GROUPS, of
 // at least one tile. All of this follows from the sizes alone, so that results do not depend on the device.
-constexpr int SPLIT_GROUPS = 1024, ROW_RATE = 20000, JOIN_TIME = 5, SPLIT_CUS = 256;
+constexpr int SPLIT_GROUPS = 1024, ROW_RATE = 20000, JOIN_TIME = 2, SPLIT_CUS = 256;
 RowSplit row_split(std::int64_t rows, int vocab, int type) {
     if (rows == 0 || small_row(vocab, type)) return {1, vocab};
     const std::int64_t bytes = static_cast<std::int64_t>(vocab) * type_bytes(type);

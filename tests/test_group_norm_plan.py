@@ -14,8 +14,9 @@ using namespace mfh;
 
 const char* fault(const GroupNormShape& s, int size, bool backward) {
     const GroupNormPlan p = group_norm_plan(s, size, backward);
-    const int lanes = 1 << p.lanes_log2, step = p.threads >> p.lanes_log2;
+    const int lanes = p.lanes, step = lanes > 0 ? p.threads / lanes : 0;
     if (p.vw < 1 || p.vw * size > 16 || s.channels % p.vw || p.width % p.vw) return "pack";
+    if (lanes <= 32 && (lanes & (lanes - 1))) return "lanes that join across a wave";
     if (lanes > p.threads || lanes * p.vw < p.width || step < 1) return "lanes";
     if (p.groups < 1 || p.groups > p.threads || p.groups > GROUP_NORM_BLOCK_GROUPS) return "groups";
     if (p.parts == 1) {
