@@ -518,7 +518,8 @@ MFH_API int mfh_adam_step(const mfh_adam_tensor* tensors, int count, float grad_
  * holds `rows` rows of `vocab` contiguous elements, row_stride elements apart (offsets between rows are 64
  * bits; at most 2^22 rows of at most 2^24 logits). Tokens and ids are int32, or int64 with their flag; a
  * negative one is none. `counters` are MFH_LOGIT_COUNTERS 32-bit zeros on the device, in which a call counts its
- * workgroups and which it leaves zero: calls that may run at the same time need their own.
+ * workgroups and which it leaves zero: calls that may run at the same time need their own. (mfh_log_probs takes
+ * none where it takes no workspace.)
  * No counterpart in the reference, whose only loss is the mean squared error. */
 #define MFH_LOGIT_COUNTERS 1025
 

@@ -1182,11 +1182,11 @@ MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(top >= 0 && top <= TOP_MAX && top <= vocab, "number of alternatives out of range");
-    MFH_REQUIRE(rows == 0 || (logits && entropy && log_sum && stats && counters && (!log_prob || tokens) &&
+    MFH_REQUIRE(rows == 0 || (logits && entropy && log_sum && stats && (!log_prob || tokens) &&
                               (top == 0 || (top_log_probs && top_ids))),
                 "log probabilities received a null buffer");
     const std::int64_t bytes = log_probs_workspace(rows, vocab, type, top);
-    MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "log probabilities workspace too small");
+    MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes && counters), "log probabilities workspace too small");
     LogProbsForward f{};
     f.rows = rows, f.stride = row_stride, f.vocab = vocab, f.top = top;
     f.tokens = as_ptr<const void>(tokens), f.tokens_wide = tokens_int64 != 0;

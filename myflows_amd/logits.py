@@ -182,8 +182,8 @@ def log_probs_forward(logits, tokens=None, *, top=0):
     stats, row = floats.data_ptr(), 4 * rows
     native._call("mfh_log_probs", logits.data_ptr(), code, rows, vocab, stride, native._addr(tokens), wide,
                  0 if tokens is None else stats + 4 * row, stats + 2 * row, stats + 3 * row, stats, top,
-                 native._addr(top_log_probs), native._addr(top_ids), workspace, held, native.stream_counters(),
-                 native._stream())
+                 native._addr(top_log_probs), native._addr(top_ids), workspace, held,
+                 native.stream_counters() if held else 0, native._stream())
     return LogProbs(floats, tokens is not None, top_log_probs, top_ids)
 
 
