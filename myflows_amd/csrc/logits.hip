@@ -611,6 +611,7 @@ __device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& s
 #pragma unroll
     for (int p = 0; p < TILE_PACKS; ++p) tile.packs[p].stay_packed();
     state.mine.rescale(to, scale);
+    float s = 0.0f, t = 0.0f;  // of the tile: a chain of additions is a tile's logits and the tiles, not all logits
 #pragma unroll
     for (int p = 0; p < TILE_PACKS; ++p) {
         if (!there(p)) continue;
@@ -618,10 +619,12 @@ __device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& s
         for (int e = 0; e < Tile::N; ++e) {
             const float d = tile.packs[p].at(e) - state.mine.m;
             const float part = exp2_of(d * scale);
-            state.mine.s += part;
-            if constexpr (ENTROPY) state.mine.t += part * fmaxf(d, DIFFERENCE_FLOOR);
+            s += part;
+            if constexpr (ENTROPY) t += part * fmaxf(d, DIFFERENCE_FLOOR);
         }
     }
+    state.mine.s += s;
+    state.mine.t += t;
 }
 
 // The statistics of a run, the same in every thread, and the number of the wave's candidates. `meanwhile` runs

@@ -192,6 +192,26 @@ def test_a_sample_does_not_depend_on_its_batch(positions):
 
 
 @gpu
+def test_samples_beyond_32_bit_offsets():
+    """Three samples of 2^30 elements: the last one's results are its own, alone, on the same plan."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.empty((3, 2 ** 20, 1024), dtype=torch.bfloat16, device="cuda")
+    x[2] = torch.randn((2 ** 20, 1024), generator=g, device="cuda", dtype=torch.bfloat16)
+    x[:2] = 1.0
+    gamma, beta = torch.rand(1024, generator=g, device="cuda"), torch.rand(1024, generator=g, device="cuda")
+    y, mean, inv = ops.group_norm_forward(x, gamma, beta, 8, activation="silu")
+    alone = ops.group_norm_forward(x[2:], gamma, beta, 8, activation="silu")
+    assert bool(((mean[2] - alone[1][0]).abs() <= 2.0 ** -20).all()) and bool(((inv[2] / alone[2][0] - 1).abs() <= 2.0 ** -18).all())
+    assert bool(((y[2].float() - alone[0][0].float()).abs() <= 2.0 ** -6 * alone[0][0].float().abs() + 2.0 ** -8).all())
+    del alone
+    dx = torch.empty_like(x)
+    ops.group_norm_backward(x, x, gamma, beta, mean, inv, activation="silu", x_grad=dx, accumulate=(False,) * 3)
+    want = torch.empty_like(x[2:])
+    ops.group_norm_backward(x[2:], x[2:], gamma, beta, mean[2:], inv[2:], activation="silu", x_grad=want, accumulate=(False,) * 3)
+    assert bool(((dx[2].float() - want[0].float()).abs() <= 2.0 ** -6 * want[0].float().abs() + 2.0 ** -8).all())
+
+
+@gpu
 def test_single_gradients_and_unaligned_views():
     x, dy, gamma, beta = _data(4, 300, 64, "float16", 6)
     shifted = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape).copy_(x)

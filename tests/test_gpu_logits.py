@@ -460,6 +460,27 @@ def test_rows_beyond_32_bit_offsets():
 
 
 @gpu
+def test_gradients_in_the_logits_place_and_strided_inputs():
+    z, gen = _z(5, 3000, "float32", 25)
+    ids, teacher = _record(5, 3000, 40, gen, duplicates=True)
+    d = ops.distill_loss_forward(z, ids, teacher)
+    one = torch.ones((), device="cuda")
+    want = ops.distill_loss_backward(z, ids, d, one)
+    taken = z.clone()
+    ops.distill_loss_backward(taken, ids, d, one, out=taken)  # logits at the ids are read before any write
+    assert torch.equal(taken, want)
+    # logits whose rows are not contiguous, and whole numbers and gradients that are columns of wider tensors
+    turned = z.t().contiguous().t()
+    tokens = torch.randint(0, 3000, (5, 3), generator=gen).cuda()[:, 1]
+    g = torch.randn((5, 2), generator=gen).cuda()[:, 0]
+    first, second = ops.log_probs_forward(z, tokens.contiguous(), top=9), ops.log_probs_forward(turned, tokens, top=9)
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+    a = ops.log_probs_backward(z, tokens.contiguous(), first, log_prob_grad=g.contiguous())
+    assert torch.equal(ops.log_probs_backward(turned, tokens, first, log_prob_grad=g), a)
+
+
+@gpu
 def test_no_rows():
     z = torch.empty((0, 10), device="cuda")
     tokens = torch.empty((0,), dtype=torch.int64, device="cuda")
