@@ -17,7 +17,8 @@
  *     "<file>:<line>: <reason>".
  *
  * Kernels index buffers with int32 offsets; entry points reject problems whose buffers exceed
- * 2^31 - 1 elements.
+ * 2^31 - 1 elements. (The rows of logits and the samples of the group norm lie at 64-bit offsets: there a row
+ * or a sample is bounded instead.)
  *
  * GEMM engine codes (engine arguments), with the reference's arithmetic: 1 = the FP32 MFMA engine
  * with its automatic tile and split-K plan; 16 + n * 32 + (slices - 1) = the reference's named tile n

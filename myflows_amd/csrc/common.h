@@ -1,7 +1,8 @@
 // Host-side plumbing shared by the translation units of libmfhip: status codes, the thread-local
 // error text, launch checks, and the internal interfaces through which the C ABI (api.hip) reaches
-// the kernels of conv.hip, gemm.hip, matmul.hip, norm.hip and pointwise.hip. Every kernel indexes
-// its buffers with int32 offsets; the entry points reject larger problems before launching anything.
+// the kernels of conv.hip, gemm.hip, matmul.hip, norm.hip, pointwise.hip, head.hip, logits.hip and
+// group_norm.hip. Kernels index their buffers with int32 offsets (within a row or a sample in the last two);
+// the entry points reject larger problems before launching anything.
 #pragma once
 
 #include <hip/hip_runtime.h>
