@@ -153,7 +153,7 @@ struct TeacherRow {
     }
 
     template <typename T>
-    __device__ __forceinline__ void read(const DistillForward& f, const T* __restrict__ row, long long r) {
+    __device__ __forceinline__ void read(const DistillForward& f, const T* __restrict__ row, long long r, bool write) {
         __shared__ int ids[DISTILL_HELD_MAX];
         __shared__ float probs[DISTILL_HELD_MAX];
         const int tid = threadIdx.x;
@@ -203,6 +203,7 @@ struct TeacherRow {
                 probs[k] = p[i];
             }
         }
+        if (!write) return;
         __syncthreads();
         // An id that the record holds twice has the sum of its probabilities as its target.
 #pragma unroll
@@ -722,19 +723,41 @@ struct JoinState {
     int ranks[ROW_THREADS], count;
 };
 
+// The first keys of a row's runs, KEPT a thread, on their way while the runs' statistics are joined.
+struct JoinKeys {
+    static constexpr int KEPT = 2;
+    unsigned long long keys[KEPT];
+    __device__ __forceinline__ JoinKeys(const unsigned long long* from, int total) {
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i) {
+            const int at = static_cast<int>(threadIdx.x) + i * ROW_THREADS;
+            keys[i] = at < total ? handed_over(from + at) : 0;
+        }
+    }
+};
+
 // The k largest keys of a row's runs, each run's in falling order. At least k keys reach the smallest of the runs'
 // keys at place ceil(k / runs), and k those of any run its k-th: keys below the larger of the two bounds are none
 // of the k largest.
 template <typename Emit>
-__device__ __forceinline__ void join_top(JoinState& join, const unsigned long long* keys, int chunks, int k,
-                                         Emit&& emit) {
+__device__ __forceinline__ void join_top(JoinState& join, const JoinKeys& first, const unsigned long long* keys, int chunks,
+                                         int k, Emit&& emit) {
     constexpr int WAVES = ROW_THREADS / 64;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, total = chunks * k, place = (k + chunks - 1) / chunks - 1;
+    const auto bound = [&](int at, unsigned long long key) {
+        const int chunk = at / k, rank = at - chunk * k;
+        if (rank == place) join.bounds[0][chunk] = key;
+        if (rank == k - 1) join.bounds[1][chunk] = key;
+    };
+    // Calls with every key of this thread.
+    const auto each = [&](auto&& take) {
+#pragma unroll
+        for (int i = 0; i < JoinKeys::KEPT; ++i)
+            if (tid + i * ROW_THREADS < total) take(tid + i * ROW_THREADS, first.keys[i]);
+        for (int at = tid + JoinKeys::KEPT * ROW_THREADS; at < total; at += ROW_THREADS) take(at, handed_over(keys + at));
+    };
     __syncthreads();  // what the run's own alternatives left in LDS is read
-    if (tid < chunks) {
-        join.bounds[0][tid] = handed_over(keys + tid * k + (k + chunks - 1) / chunks - 1);
-        join.bounds[1][tid] = handed_over(keys + tid * k + k - 1);
-    }
+    each(bound);
     if (tid == 0) join.count = 0;
     __syncthreads();
     unsigned long long all = ~0ull, any = 0;
@@ -743,10 +766,9 @@ __device__ __forceinline__ void join_top(JoinState& join, const unsigned long lo
         any = max(any, join.bounds[1][i]);
     }
     const unsigned long long least = max(max(all, any), 1ull);
-    for (int i = tid; i < chunks * k; i += ROW_THREADS) {
-        const unsigned long long key = handed_over(keys + i);
+    each([&](int, unsigned long long key) {
         if (key >= least) join.kept[atomicAdd(&join.count, 1)] = key;
-    }
+    });
     __syncthreads();
     const int found = join.count, part = (found + WAVES - 1) / WAVES, from = min(found, tid / 64 * part);
     emit_ranks<WAVES>([&](int i) { return join.kept[i]; }, found, k, join.kept + from, min(part, found - from), join.ranks, emit);
@@ -785,9 +807,11 @@ __global__ __launch_bounds__(THREADS, SPLIT ? 4 : 8) void log_probs_kernel(const
         if constexpr (SPLIT) {
             if (threadIdx.x == 0) hand_over(partials.stats + at, row);
             if (!last_to_come(f.counters + run.row, split.chunks)) return;
+            const unsigned long long* keys = partials.keys + run.row * split.chunks * f.top;
+            const JoinKeys first(keys, split.chunks * f.top);
             row = join_runs(partials.stats + run.row * split.chunks, split.chunks, LOG2E);
             const RowEnd end(row);
-            join_top(reinterpret_cast<Shared*>(&shared)->join, partials.keys + run.row * split.chunks * f.top, split.chunks, f.top,
+            join_top(reinterpret_cast<Shared*>(&shared)->join, first, keys, split.chunks, f.top,
                      [&](int rank, unsigned long long key) { write_top(f, run.row, rank, key, end); });
         }
     } else {
@@ -840,13 +864,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const T* __restrict__ 
     const T* __restrict__ z = logits + run.row * f.stride;
     int count;
     TeacherRow<THREADS> teacher;
-    RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature, nullptr, 0, count, [&] {
-        if constexpr (!SPLIT) teacher.read(f, z, run.row);
-    });
+    // Every run of a row reads the teacher's record while its first tile is on the way (any may be the last).
+    RowStats row = take_run<false, false, T, THREADS>(z, run, LOG2E / f.temperature, nullptr, 0, count,
+                                                      [&] { teacher.read(f, z, run.row, run.chunk == 0); });
     if constexpr (SPLIT) {
         if (threadIdx.x == 0) hand_over(partials.stats + run.row * split.chunks + run.chunk, row);
         if (!last_to_come(f.counters + run.row, split.chunks)) return;
-        teacher.read(f, z, run.row);
         row = join_runs(partials.stats + run.row * split.chunks, split.chunks, LOG2E / f.temperature);
     }
     teacher.finish(f, run.row, row);
