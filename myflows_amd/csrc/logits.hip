@@ -1016,10 +1016,13 @@ bool small_row(int vocab, int type) { return vocab * static_cast<std::int64_t>(t
 
 // Runs of a row. Rows are split where the time that whole rows leave CUs idle is more than joining them takes:
 // of 256 CUs that read ROW_RATE bytes a microsecond each (5/8 of that with one workgroup), whole rows take the most
-// that one CU has of them, split ones their share and JOIN_TIME. Measured split / whole: 777 rows of 64 KB 18.7 /
-// 17.5 us, 1024 of them 18.1 / 17.4, one 4.3 / 5.3. Then as many runs as bring the workgroups to SPLIT_GROUPS, of
-// at least one tile. All of this follows from the sizes alone, so that results do not depend on the device.
-constexpr int SPLIT_GROUPS = 1024, ROW_RATE = 20000, JOIN_TIME = 2, SPLIT_CUS = 256;
+// that one CU has of them, split ones their share and JOIN_TIME. Measured without / with 20 alternatives, float32,
+// whole -> split: one row of 16384 3.8 / 8.8 -> 3.5 / 8.2 us and of 131072 17.7 / 31.2 -> 4.1 / 10.9, 250 of 16384
+// 4.4 / 11.2 -> 5.9 / 11.9 and of 131072 26.2 / 44.9 -> 23.8 / 29.6. Over 260 sizes from 1 to 500 rows of 12 to
+// 512 KB the rule's choice is 1% slower than the better one, always whole 18%, always split 7%. Then as many runs as
+// bring the workgroups to SPLIT_GROUPS, of at least one tile. All of this follows from the sizes alone, so that
+// results do not depend on the device.
+constexpr int SPLIT_GROUPS = 1024, ROW_RATE = 20000, JOIN_TIME = 3, SPLIT_CUS = 256;
 RowSplit row_split(std::int64_t rows, int vocab, int type) {
     if (rows == 0 || small_row(vocab, type)) return {1, vocab};
     const std::int64_t bytes = static_cast<std::int64_t>(vocab) * type_bytes(type);

@@ -279,7 +279,8 @@ def _on_gpu(value, op):
 
 class CrossEntropyLoss(GradientOp):
     """The mean of -log_prob of the labels (rows,) over the rows whose label is not negative (0 without
-    any). ``log_probs`` holds the last forward's LogProbs, entropies included."""
+    any). A label beyond the vocabulary makes the loss NaN. ``log_probs`` holds the last forward's LogProbs,
+    entropies included."""
 
     def __init__(self, logits, labels, name="CrossEntropyLoss"):
         super().__init__(logits, labels, name=name)
