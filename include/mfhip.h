@@ -69,6 +69,11 @@ MFH_API void mfh_set_debug_sync(int enabled);
  * on a second stream, such as the dW products of a backward pass beside its dX products. */
 MFH_API int mfh_stream_wait(uint64_t waiting, uint64_t signalling);
 
+/* *id names the stream capture (of a HIP graph) that `stream` takes part in, or is 0 while it takes part in
+ * none; two captures never share one. For callers whose scratch memory belongs to one capture. No counterpart
+ * in the reference. */
+MFH_API int mfh_capture_id(uint64_t stream, uint64_t* id);
+
 /* ---- recorded programs ---------------------------------------------------------------------- */
 
 /* Start recording, on the calling thread, every kernel launch and stream ordering the library

@@ -364,6 +364,17 @@ MFH_API int mfh_stream_wait(std::uint64_t waiting, std::uint64_t signalling) {
     return order_after(as_stream(waiting), as_stream(signalling));
 }
 
+MFH_API int mfh_capture_id(std::uint64_t stream, std::uint64_t* id) {
+    MFH_TRY(require_ready());
+    MFH_REQUIRE(id, "mfh_capture_id needs somewhere to put the id");
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    const hipError_t rc = hipStreamGetCaptureInfo(as_stream(stream), &status, &capture);
+    if (rc != hipSuccess) return MFH_FAIL(ERR_HIP, std::string("capture info: ") + hipGetErrorString(rc));
+    *id = status == hipStreamCaptureStatusActive ? capture + 1 : 0;
+    return OK;
+}
+
 MFH_API int mfh_program_begin(void) {
     MFH_TRY(require_ready());
     MFH_REQUIRE(recording() == nullptr, "a program is already being recorded on this thread");

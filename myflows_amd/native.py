@@ -88,6 +88,7 @@ _SIGNATURES = {
     "mfh_info": ("s", ""),
     "mfh_set_debug_sync": ("-", "i"),
     "mfh_stream_wait": ("i", "pp"),
+    "mfh_capture_id": ("i", "pU"),
     "mfh_program_begin": ("i", ""),
     "mfh_program_end": ("i", "UL"),
     "mfh_program_run": ("i", "p"),
@@ -234,6 +235,7 @@ try:
 except AttributeError:  # another torch build: the public accessors
     _raw_stream = lambda device: torch.cuda.current_stream(device).cuda_stream  # noqa: E731
     _current_device = torch.cuda.current_device
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 def current_device_index():
@@ -627,13 +629,46 @@ _STREAM_COUNTERS = {}
 LOGIT_COUNTERS = 1025  # MFH_LOGIT_COUNTERS of include/mfhip.h
 
 
+_CAPTURE_BLOCKS = {}  # by (device, stream): the last capture's id, its counters, its workspaces
+
+
+class _CaptureBlocks:
+    __slots__ = ("id", "counters", "workspaces")
+
+    def __init__(self, capture):
+        self.id, self.counters, self.workspaces = capture, None, []
+
+
+def _capture_blocks(key):
+    """The blocks of the stream capture under way on the stream of `key`. A captured graph runs on whatever
+    stream replays it, beside other graphs and eager calls of this stream, so it has counters and workspaces of
+    its own, in its memory pool. They are held until the next capture here, so that nothing else of this
+    capture is given them."""
+    capture = ctypes.c_uint64(0)
+    _call("mfh_capture_id", key[1], ctypes.byref(capture))
+    blocks = _CAPTURE_BLOCKS.get(key)
+    if blocks is None or blocks.id != capture.value:
+        blocks = _CAPTURE_BLOCKS[key] = _CaptureBlocks(capture.value)
+    return blocks
+
+
+def _zero_counters():
+    return fill_(torch.empty(LOGIT_COUNTERS, dtype=torch.float32, device="cuda"), 0.0)
+
+
 def stream_counters():
     """The address of the zeros in which calls on the current stream count their workgroups. Each call leaves
-    them zero, and calls on one stream run one after the other, so they are cleared once, on that stream."""
+    them zero, and calls on one stream run one after the other, so they are cleared once, on that stream (in a
+    capture once a replay, ahead of its first use)."""
     key = (_current_device(), _stream())
+    if _capturing():
+        blocks = _capture_blocks(key)
+        if blocks.counters is None:
+            blocks.counters = _zero_counters()
+        return blocks.counters.data_ptr()
     held = _STREAM_COUNTERS.get(key)
     if held is None:
-        held = _STREAM_COUNTERS[key] = fill_(torch.empty(LOGIT_COUNTERS, dtype=torch.float32, device="cuda"), 0.0)
+        held = _STREAM_COUNTERS[key] = _zero_counters()
     return held.data_ptr()
 
 
@@ -646,9 +681,14 @@ def workspace_bytes(symbol, *sizes):
 
 
 def byte_workspace(count):
-    """(address, bytes) of a stream workspace of `count` bytes; (0, 0) for none."""
+    """(address, bytes) of a stream workspace of `count` bytes (in a capture, one of its own); (0, 0) for none."""
     if not count:
         return 0, 0
+    if _capturing():
+        held = _capture_blocks((_current_device(), _stream())).workspaces
+        if not held or held[-1].numel() < count:
+            held.append(torch.empty(count, dtype=torch.uint8, device="cuda"))
+        return held[-1].data_ptr(), count
     return stream_workspace((count + 7) // 8, torch.float64).data_ptr(), count
 
 

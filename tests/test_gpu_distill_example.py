@@ -96,3 +96,53 @@ def test_the_operators_in_a_captured_graph():
         torch.cuda.synchronize()
         for a, b in zip(captured, want):
             assert torch.equal(a, b)
+
+
+def test_captured_graphs_share_no_scratch_memory():
+    """Two graphs of calls that join workgroups, captured one after the other: the second is replayed first, then
+    both side by side on two streams. One of them forks to a second stream within its capture."""
+    g = torch.Generator().manual_seed(6)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    rows = [torch.randn((4, 120000), generator=g).cuda() for _ in range(4)]
+    ids, teacher = torch.randint(0, 120000, (4, 8), generator=g).cuda(), torch.randn((4, 8), generator=g).cuda()
+
+    def run(z):
+        r = logits.log_probs_forward(z, top=20)
+        d = logits.distill_loss_forward(z, ids, teacher)
+        return [r.entropy, r.log_sum, r.top_log_probs, r.top_ids, d.scale, d.row_loss]
+
+    want = [run(z) for z in rows]
+    torch.cuda.synchronize()
+    graphs, captured = [], []
+    for i in range(2):
+        graph, outputs = torch.cuda.CUDAGraph(), []
+        with torch.cuda.graph(graph):
+            outputs.append(run(rows[2 * i]))
+            if i == 1:
+                sides[0].wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(sides[0]):
+                    outputs.append(run(rows[2 * i + 1]))
+                torch.cuda.current_stream().wait_stream(sides[0])
+            else:
+                outputs.append(run(rows[2 * i + 1]))
+        graphs.append(graph)
+        captured.append(outputs)
+
+    def check(which):
+        for i in which:
+            for j in range(2):
+                for a, b in zip(captured[i][j], want[2 * i + j]):
+                    assert torch.equal(a, b)
+                    a.zero_()
+        torch.cuda.synchronize()
+
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    check([1])
+    for _ in range(5):
+        for side, graph in zip(sides, graphs):
+            with torch.cuda.stream(side):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        check([0, 1])
