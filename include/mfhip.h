@@ -561,7 +561,8 @@ MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
 /* The distillation loss of a student's logits against a teacher's record of `held` (1..256) ids and float32
  * logits a row: with p = softmax(teacher / temperature) over the ids >= 0 and q = softmax(logits / temperature),
  *   row_loss = temperature^2 sum p (ln p - ln q[id]),  loss[0] = sum w row_loss / sum w,  loss[1] = 1 / sum w
- * over the rows that count: w = row_weights[r] (optional, else 1), 0 without an id. A row that does not count
+ * over the rows that count: w = row_weights[r] (optional, else 1), 0 without an id (or with teacher logits of -inf
+ * alone). A row that does not count
  * has row_loss 0 whatever its logits hold; without any, loss is 0. An id >= vocab makes a counting row NaN.
  * For the backward: weights (rows), stats (2 x rows) and targets (rows x held, p summed over equal ids). */
 MFH_API int mfh_distill_loss(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,

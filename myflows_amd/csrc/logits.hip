@@ -237,8 +237,9 @@ struct TeacherRow {
 // A workgroup takes a run of a row's logits tile by tile, in 16-byte packs, the next tile's loads in flight:
 // each thread keeps the running statistics of its own logits, and the threads' are joined once, at the end of
 // the run. One read of the logits, one exp a logit. Bound by HBM for float32; a bfloat16 or float16 logit
-// costs about as many vector instructions as the time that its two bytes take allows: 2048 x 131072 bfloat16
-// with 20 alternatives 114 us (4.7 TB/s), 1000 x 50021 float32 without any 34 (5.8), 2048 x 32768 bfloat16 27.
+// costs about as many vector instructions as the time that its two bytes take allows (float16 compared in pairs
+// and converted within the subtraction: 2048 x 32768 with 20 alternatives 38.9 us, 41.4 with conversions of its
+// own): 2048 x 131072 bfloat16 with 20 alternatives 114 us (4.7 TB/s), 1000 x 50021 float32 without any 34 (5.8), 2048 x 32768 bfloat16 27.
 //
 // The top alternatives come out of the same read. The k-th largest of the threads' own maxima is at most the
 // row's k-th largest logit, so only logits above that threshold can be alternatives: about k of a tile's
@@ -307,9 +308,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
+__device__ __forceinline__ unsigned max_of_pairs(unsigned a, unsigned b) {
+    unsigned r;
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
+// The largest of a pack; a NaN is left out, or makes it one. float16 pairs are compared as they are, two at a time.
 template <typename T, int N>
 __device__ __forceinline__ float largest(const Pack<T, N>& pack) {
     static_assert(N % 4 == 0, "two chains of pairs");
+    if constexpr (std::is_same_v<T, _Float16>) {
+        static_assert(N == 8, "four words");
+        const unsigned both = max_of_pairs(max_of_pairs(pack.w[0], pack.w[1]), max_of_pairs(pack.w[2], pack.w[3]));
+        const Pack<T, 2> pair{both};
+        return fmaxf(pair.at(0), pair.at(1));
+    }
     float a = fmaxf(pack.at(0), pack.at(1)), b = fmaxf(pack.at(2), pack.at(3));
 #pragma unroll
     for (int i = 4; i < N; i += 4) {
@@ -317,6 +331,18 @@ __device__ __forceinline__ float largest(const Pack<T, N>& pack) {
         b = max3(b, pack.at(i + 2), pack.at(i + 3));
     }
     return fmaxf(a, b);
+}
+
+// Element i of a pack minus m, rounded once. The mixed multiply-add converts a float16 operand by itself.
+template <typename T, int N>
+__device__ __forceinline__ float less(const Pack<T, N>& pack, int i, float m) {
+    if constexpr (std::is_same_v<T, _Float16>) {
+        float r;
+        if (i & 1) asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pack.w[i / 2]), "v"(m));
+        else asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pack.w[i / 2]), "v"(m));
+        return r;
+    }
+    return pack.at(i) - m;
 }
 
 // The value of lane ^ DISTANCE.
@@ -619,7 +645,7 @@ __device__ __forceinline__ void take_tile(RowTile<T, THREADS>& tile, RowState& s
         if (!there(p)) continue;
 #pragma unroll
         for (int e = 0; e < Tile::N; ++e) {
-            const float d = tile.packs[p].at(e) - state.mine.m;
+            const float d = less(tile.packs[p], e, state.mine.m);
             const float part = exp2_of(d * scale);
             s += part;
             if constexpr (ENTROPY) t += part * fmaxf(d, DIFFERENCE_FLOOR);

@@ -227,8 +227,8 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
     p = softmax(teacher_logits / T) over the ids that are held and the student's q = softmax(logits / T),
     row_loss = T^2 sum p (ln p - ln q[id]) and loss is its mean by row_weights (1 each without them).
 
-    A row without an id or with weight 0 does not count: its loss and gradient are 0, whatever its logits
-    hold, and without any row that counts the loss is 0. An id beyond the vocabulary makes a counting row
+    A row without an id, with teacher logits of -inf alone or with weight 0 does not count: its loss and
+    gradient are 0, whatever its logits hold, and without any row that counts the loss is 0. An id beyond the vocabulary makes a counting row
     NaN."""
     logits, code, rows, vocab, stride = _logits(logits)
     temperature = _temperature(temperature)
