@@ -239,7 +239,8 @@ struct TeacherRow {
 // the run. One read of the logits, one exp a logit. Bound by HBM for float32; a bfloat16 or float16 logit
 // costs about as many vector instructions as the time that its two bytes take allows (float16 compared in pairs
 // and converted within the subtraction: 2048 x 32768 with 20 alternatives 38.9 us, 41.4 with conversions of its
-// own): 2048 x 131072 bfloat16 with 20 alternatives 114 us (4.7 TB/s), 1000 x 50021 float32 without any 34 (5.8), 2048 x 32768 bfloat16 27.
+// own). 2048 x 131072 bfloat16 with 20 alternatives 115 us (4.7 TB/s), 1000 x 50021 float32 without any 34 (5.8),
+// 2048 x 32768 bfloat16 27.
 //
 // The top alternatives come out of the same read. The k-th largest of the threads' own maxima is at most the
 // row's k-th largest logit, so only logits above that threshold can be alternatives: about k of a tile's

@@ -202,8 +202,9 @@ def _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, fact
     out, out_stride = _gradient(out, add, logits)
     stats = saved._floats.data_ptr()
     native._call("mfh_log_probs_backward", logits.data_ptr(), code, rows, vocab, stride,
-                 0 if log_prob_grad is None else tokens.data_ptr(), wide, stats, stats + 8 * rows, native._addr(log_prob_grad), lp_step, native._addr(entropy_grad),
-                 entropy_step, native._addr(factor), scale, out.data_ptr(), out_stride, int(add), native._stream())
+                 0 if log_prob_grad is None else tokens.data_ptr(), wide, stats, stats + 8 * rows,
+                 native._addr(log_prob_grad), lp_step, native._addr(entropy_grad), entropy_step,
+                 native._addr(factor), scale, out.data_ptr(), out_stride, int(add), native._stream())
     return out
 
 
@@ -267,8 +268,8 @@ def distill_loss_backward(logits, teacher_ids, saved, seed, *, temperature=1.0, 
     scale, row = saved._floats.data_ptr(), 4 * rows
     row_loss = scale + 8
     native._call("mfh_distill_loss_backward", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
-                 saved._held, row_loss + 4 * row, row_loss + 2 * row, row_loss + row, scale, seed.data_ptr(), temperature, out.data_ptr(), out_stride, int(add),
-                 native._stream())
+                 saved._held, row_loss + 4 * row, row_loss + 2 * row, row_loss + row, scale, seed.data_ptr(), temperature,
+                 out.data_ptr(), out_stride, int(add), native._stream())
     return out
 
 
