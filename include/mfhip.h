@@ -523,7 +523,8 @@ MFH_API int mfh_adam_step(const mfh_adam_tensor* tensors, int count, float grad_
 /* Element types of the calls below that take more than float: 0 float32, 1 bfloat16, 2 float16. `logits`
  * holds `rows` rows of `vocab` contiguous elements, row_stride elements apart (offsets between rows are 64
  * bits; at most 2^22 rows of at most 2^24 logits). Tokens and ids are int32, or int64 with their flag; a
- * negative one is none. `counters` are MFH_LOGIT_COUNTERS 32-bit zeros on the device, in which a call counts its
+ * negative one is none. What holds one value a row lies its stride in elements apart (0: one value for all rows), a
+ * row of ids or of teacher logits side by side and its rows their stride apart. `counters` are MFH_LOGIT_COUNTERS 32-bit zeros on the device, in which a call counts its
  * workgroups and which it leaves zero: calls that may run at the same time need their own. (mfh_log_probs takes
  * none where it takes no workspace.)
  * No counterpart in the reference, whose only loss is the mean squared error. */
@@ -540,20 +541,20 @@ MFH_API int64_t mfh_log_probs_workspace(int64_t rows, int vocab, int type, int t
  * A logit of -inf has probability 0. A row of nothing else: log_sum, log_prob and the alternatives -inf,
  * entropy 0. A NaN or +inf makes its row NaN; a NaN is no alternative (ids that are then missing are -1). */
 MFH_API int mfh_log_probs(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
-                          int tokens_int64, uint64_t log_prob, uint64_t entropy, uint64_t log_sum, uint64_t stats, int top,
-                          uint64_t top_log_probs, uint64_t top_ids, uint64_t workspace, int64_t workspace_bytes,
-                          uint64_t counters, uint64_t stream);
+                          int tokens_int64, int64_t tokens_stride, uint64_t log_prob, uint64_t entropy, uint64_t log_sum,
+                          uint64_t stats, int top, uint64_t top_log_probs, uint64_t top_ids, uint64_t workspace,
+                          int64_t workspace_bytes, uint64_t counters, uint64_t stream);
 
 /* grad[r][j] (grad_stride elements a row, of the logits' type) = g ([j = token] - p) - h p (ln p + entropy), or
  * grad += that when add != 0, with g = scale * factor[0] * log_prob_grad[r * log_prob_grad_stride] (0 where
  * token < 0) and h = factor[0] * entropy_grad[r * entropy_grad_stride]. factor (one float on the device, 1
- * when 0), log_prob_grad and entropy_grad are optional; strides may be 0. stats and entropy are those of
+ * when 0), log_prob_grad and entropy_grad are optional. stats and entropy are those of
  * mfh_log_probs. A row whose g and h are 0 gets 0 whatever its logits hold. */
 MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
-                                   int tokens_int64, uint64_t stats, uint64_t entropy, uint64_t log_prob_grad,
-                                   int64_t log_prob_grad_stride, uint64_t entropy_grad, int64_t entropy_grad_stride,
-                                   uint64_t factor, float scale, uint64_t grad, int64_t grad_stride, int add,
-                                   uint64_t stream);
+                                   int tokens_int64, int64_t tokens_stride, uint64_t stats, uint64_t entropy,
+                                   uint64_t log_prob_grad, int64_t log_prob_grad_stride, uint64_t entropy_grad,
+                                   int64_t entropy_grad_stride, uint64_t factor, float scale, uint64_t grad,
+                                   int64_t grad_stride, int add, uint64_t stream);
 
 /* Bytes of workspace of mfh_distill_loss (0: none), -1 when the sizes are out of range. */
 MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
@@ -566,20 +567,21 @@ MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
  * has row_loss 0 whatever its logits hold; without any, loss is 0. An id >= vocab makes a counting row NaN.
  * For the backward: weights (rows), stats (2 x rows) and targets (rows x held, p summed over equal ids). */
 MFH_API int mfh_distill_loss(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,
-                             int ids_int64, uint64_t teacher, int held, uint64_t row_weights, float temperature,
-                             uint64_t row_loss, uint64_t weights, uint64_t stats, uint64_t targets, uint64_t loss,
-                             uint64_t workspace, int64_t workspace_bytes, uint64_t counters, uint64_t stream);
+                             int ids_int64, int64_t ids_stride, uint64_t teacher, int64_t teacher_stride, int held,
+                             uint64_t row_weights, int64_t row_weights_stride, float temperature, uint64_t row_loss,
+                             uint64_t weights, uint64_t stats, uint64_t targets, uint64_t loss, uint64_t workspace,
+                             int64_t workspace_bytes, uint64_t counters, uint64_t stream);
 
 /* grad[r][j] = seed[0] w loss[1] temperature (q[j] - sum over k of p[k] [ids[k] = j]), or grad += that. */
 MFH_API int mfh_distill_loss_backward(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t ids,
-                                      int ids_int64, int held, uint64_t targets, uint64_t stats, uint64_t weights,
-                                      uint64_t loss, uint64_t seed, float temperature, uint64_t grad, int64_t grad_stride,
-                                      int add, uint64_t stream);
+                                      int ids_int64, int64_t ids_stride, int held, uint64_t targets, uint64_t stats,
+                                      uint64_t weights, uint64_t loss, uint64_t seed, float temperature, uint64_t grad,
+                                      int64_t grad_stride, int add, uint64_t stream);
 
 /* out[0] = scale * mean of the values whose token is >= 0 (of all, when tokens is 0), out[1] = 1 / their
  * number (both 0 without any): FP64 sums in a fixed order. */
-MFH_API int mfh_row_mean(uint64_t values, uint64_t tokens, int tokens_int64, int64_t rows, float scale, uint64_t out,
-                         uint64_t stream);
+MFH_API int mfh_row_mean(uint64_t values, uint64_t tokens, int tokens_int64, int64_t tokens_stride, int64_t rows,
+                         float scale, uint64_t out, uint64_t stream);
 
 /* ---- group norm ------------------------------------------------------------------------------ */
 

@@ -1186,10 +1186,10 @@ MFH_API std::int64_t mfh_log_probs_workspace(std::int64_t rows, int vocab, int t
 }
 
 MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
-                          std::uint64_t tokens, int tokens_int64, std::uint64_t log_prob, std::uint64_t entropy,
-                          std::uint64_t log_sum, std::uint64_t stats, int top, std::uint64_t top_log_probs,
-                          std::uint64_t top_ids, std::uint64_t workspace, std::int64_t workspace_bytes,
-                          std::uint64_t counters, std::uint64_t stream) {
+                          std::uint64_t tokens, int tokens_int64, std::int64_t tokens_stride, std::uint64_t log_prob,
+                          std::uint64_t entropy, std::uint64_t log_sum, std::uint64_t stats, int top,
+                          std::uint64_t top_log_probs, std::uint64_t top_ids, std::uint64_t workspace,
+                          std::int64_t workspace_bytes, std::uint64_t counters, std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(top >= 0 && top <= TOP_MAX && top <= vocab, "number of alternatives out of range");
@@ -1200,7 +1200,7 @@ MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int
     MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes && counters), "log probabilities workspace too small");
     LogProbsForward f{};
     f.rows = rows, f.stride = row_stride, f.vocab = vocab, f.top = top;
-    f.tokens = as_ptr<const void>(tokens), f.tokens_wide = tokens_int64 != 0;
+    f.tokens = as_ptr<const void>(tokens), f.tokens_wide = tokens_int64 != 0, f.tokens_step = tokens_stride;
     f.log_prob = as_ptr<float>(log_prob), f.entropy = as_ptr<float>(entropy), f.log_sum = as_ptr<float>(log_sum);
     f.stats = as_ptr<float>(stats);
     f.top_log_probs = as_ptr<float>(top_log_probs), f.top_ids = as_ptr<int>(top_ids);
@@ -1209,8 +1209,8 @@ MFH_API int mfh_log_probs(std::uint64_t logits, int type, std::int64_t rows, int
 }
 
 MFH_API int mfh_log_probs_backward(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
-                                   std::uint64_t tokens, int tokens_int64, std::uint64_t stats, std::uint64_t entropy,
-                                   std::uint64_t log_prob_grad, std::int64_t log_prob_grad_stride,
+                                   std::uint64_t tokens, int tokens_int64, std::int64_t tokens_stride, std::uint64_t stats,
+                                   std::uint64_t entropy, std::uint64_t log_prob_grad, std::int64_t log_prob_grad_stride,
                                    std::uint64_t entropy_grad, std::int64_t entropy_grad_stride, std::uint64_t factor,
                                    float scale, std::uint64_t grad, std::int64_t grad_stride, int add,
                                    std::uint64_t stream) {
@@ -1221,7 +1221,7 @@ MFH_API int mfh_log_probs_backward(std::uint64_t logits, int type, std::int64_t 
                 "log probabilities backward received a null buffer");
     LogProbsBackward b{};
     b.rows = rows, b.stride = row_stride, b.grad_stride = grad_stride, b.vocab = vocab;
-    b.tokens = as_ptr<const void>(tokens), b.tokens_wide = tokens_int64 != 0;
+    b.tokens = as_ptr<const void>(tokens), b.tokens_wide = tokens_int64 != 0, b.tokens_step = tokens_stride;
     b.stats = as_ptr<const float>(stats), b.entropy = as_ptr<const float>(entropy);
     b.log_prob_grad = as_ptr<const float>(log_prob_grad), b.log_prob_step = log_prob_grad_stride;
     b.entropy_grad = as_ptr<const float>(entropy_grad), b.entropy_step = entropy_grad_stride;
@@ -1235,10 +1235,12 @@ MFH_API std::int64_t mfh_distill_workspace(std::int64_t rows, int vocab, int typ
 }
 
 MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
-                             std::uint64_t ids, int ids_int64, std::uint64_t teacher, int held,
-                             std::uint64_t row_weights, float temperature, std::uint64_t row_loss, std::uint64_t weights,
-                             std::uint64_t stats, std::uint64_t targets, std::uint64_t loss, std::uint64_t workspace,
-                             std::int64_t workspace_bytes, std::uint64_t counters, std::uint64_t stream) {
+                             std::uint64_t ids, int ids_int64, std::int64_t ids_stride, std::uint64_t teacher,
+                             std::int64_t teacher_stride, int held, std::uint64_t row_weights,
+                             std::int64_t row_weights_stride, float temperature, std::uint64_t row_loss,
+                             std::uint64_t weights, std::uint64_t stats, std::uint64_t targets, std::uint64_t loss,
+                             std::uint64_t workspace, std::int64_t workspace_bytes, std::uint64_t counters,
+                             std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(held > 0 && held <= DISTILL_HELD_MAX, "number of teacher logits a row out of range");
@@ -1249,8 +1251,9 @@ MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, 
     MFH_REQUIRE(bytes == 0 || (workspace && workspace_bytes >= bytes), "distillation loss workspace too small");
     DistillForward f{};
     f.rows = rows, f.stride = row_stride, f.vocab = vocab, f.held = held;
-    f.ids = as_ptr<const void>(ids), f.ids_wide = ids_int64 != 0;
-    f.teacher = as_ptr<const float>(teacher), f.row_weights = as_ptr<const float>(row_weights);
+    f.ids = as_ptr<const void>(ids), f.ids_wide = ids_int64 != 0, f.ids_step = ids_stride;
+    f.teacher = as_ptr<const float>(teacher), f.teacher_step = teacher_stride;
+    f.row_weights = as_ptr<const float>(row_weights), f.weights_step = row_weights_stride;
     f.temperature = temperature;
     f.row_loss = as_ptr<float>(row_loss), f.weights = as_ptr<float>(weights), f.stats = as_ptr<float>(stats);
     f.targets = as_ptr<float>(targets), f.loss = as_ptr<float>(loss), f.workspace = as_ptr<void>(workspace);
@@ -1259,10 +1262,10 @@ MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, 
 }
 
 MFH_API int mfh_distill_loss_backward(std::uint64_t logits, int type, std::int64_t rows, int vocab,
-                                      std::int64_t row_stride, std::uint64_t ids, int ids_int64, int held,
-                                      std::uint64_t targets, std::uint64_t stats, std::uint64_t weights,
-                                      std::uint64_t loss, std::uint64_t seed, float temperature, std::uint64_t grad,
-                                      std::int64_t grad_stride, int add, std::uint64_t stream) {
+                                      std::int64_t row_stride, std::uint64_t ids, int ids_int64,
+                                      std::int64_t ids_stride, int held, std::uint64_t targets, std::uint64_t stats,
+                                      std::uint64_t weights, std::uint64_t loss, std::uint64_t seed, float temperature,
+                                      std::uint64_t grad, std::int64_t grad_stride, int add, std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(grad_stride >= vocab, "rows of the gradient must not overlap");
@@ -1272,20 +1275,20 @@ MFH_API int mfh_distill_loss_backward(std::uint64_t logits, int type, std::int64
                 "distillation loss backward received a null buffer");
     DistillBackward b{};
     b.rows = rows, b.stride = row_stride, b.grad_stride = grad_stride, b.vocab = vocab, b.held = held;
-    b.ids = as_ptr<const void>(ids), b.ids_wide = ids_int64 != 0;
+    b.ids = as_ptr<const void>(ids), b.ids_wide = ids_int64 != 0, b.ids_step = ids_stride;
     b.targets = as_ptr<const float>(targets), b.stats = as_ptr<const float>(stats);
     b.weights = as_ptr<const float>(weights), b.loss = as_ptr<const float>(loss), b.seed = as_ptr<const float>(seed);
     b.temperature = temperature, b.add = add != 0;
     return launch_distill_backward(as_ptr<const void>(logits), as_ptr<void>(grad), type, b, as_stream(stream));
 }
 
-MFH_API int mfh_row_mean(std::uint64_t values, std::uint64_t tokens, int tokens_int64, std::int64_t rows, float scale,
-                         std::uint64_t out, std::uint64_t stream) {
+MFH_API int mfh_row_mean(std::uint64_t values, std::uint64_t tokens, int tokens_int64, std::int64_t tokens_stride,
+                         std::int64_t rows, float scale, std::uint64_t out, std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_REQUIRE(rows >= 0, "rows out of range");
     MFH_REQUIRE(out && (rows == 0 || values), "row mean received a null buffer");
-    return launch_row_mean(as_ptr<const float>(values), nullptr, as_ptr<const void>(tokens), tokens_int64 != 0, rows,
-                           scale, as_ptr<float>(out), as_stream(stream));
+    return launch_row_mean(as_ptr<const float>(values), nullptr, as_ptr<const void>(tokens), tokens_int64 != 0, tokens_stride,
+                           rows, scale, as_ptr<float>(out), as_stream(stream));
 }
 
 // ---- group norm -------------------------------------------------------------------------------

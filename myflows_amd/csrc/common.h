@@ -474,8 +474,9 @@ constexpr int LOGIT_COUNTERS = LOGIT_SPLIT_ROWS + 1;  // zeros that a call count
 struct LogProbsForward {
     std::int64_t rows, stride;
     int vocab, top;
-    const void* tokens;  // optional, with log_prob
+    const void* tokens;  // optional, with log_prob; element r at r * tokens_step
     int tokens_wide;
+    std::int64_t tokens_step;
     float* log_prob;
     float* entropy;
     float* log_sum;
@@ -491,8 +492,9 @@ int launch_log_probs(const void* logits, int type, const LogProbsForward& f, hip
 struct LogProbsBackward {
     std::int64_t rows, stride, grad_stride;
     int vocab;
-    const void* tokens;
+    const void* tokens;  // as LogProbsForward's
     int tokens_wide;
+    std::int64_t tokens_step;
     const float* stats;
     const float* entropy;
     const float* log_prob_grad;  // optional; element r at r * log_prob_step
@@ -508,10 +510,13 @@ int launch_log_probs_backward(const void* logits, void* grad, int type, const Lo
 struct DistillForward {
     std::int64_t rows, stride;
     int vocab, held;
-    const void* ids;  // rows x held
+    const void* ids;  // rows x held, a row's side by side, row r at r * ids_step
     int ids_wide;
-    const float* teacher;      // rows x held logits
-    const float* row_weights;  // optional
+    std::int64_t ids_step;
+    const float* teacher;  // rows x held logits, likewise
+    std::int64_t teacher_step;
+    const float* row_weights;  // optional; element r at r * weights_step
+    std::int64_t weights_step;
     float temperature;
     float* row_loss;
     float* weights;  // the weights that count
@@ -527,8 +532,9 @@ int launch_distill(const void* logits, int type, const DistillForward& f, hipStr
 struct DistillBackward {
     std::int64_t rows, stride, grad_stride;
     int vocab, held;
-    const void* ids;
+    const void* ids;  // as DistillForward's
     int ids_wide;
+    std::int64_t ids_step;
     const float* targets;
     const float* stats;
     const float* weights;
@@ -540,9 +546,9 @@ struct DistillBackward {
 int launch_distill_backward(const void* logits, void* grad, int type, const DistillBackward& b, hipStream_t stream);
 
 // out[0] = scale * (weighted mean of values), out[1] = 1 / sum of the weights; both 0 when nothing counts.
-// A row's weight is weights[r], else whether tokens[r] >= 0, else 1.
-int launch_row_mean(const float* values, const float* weights, const void* tokens, int tokens_wide, std::int64_t rows,
-                    float scale, float* out, hipStream_t stream);
+// A row's weight is weights[r], else whether tokens[r * tokens_step] >= 0, else 1.
+int launch_row_mean(const float* values, const float* weights, const void* tokens, int tokens_wide, std::int64_t tokens_step,
+                    std::int64_t rows, float scale, float* out, hipStream_t stream);
 
 // ---- group_norm.hip ---------------------------------------------------------------------------
 // Group norm over the (positions, channels / groups) of each (sample, group) of a channels-last tensor

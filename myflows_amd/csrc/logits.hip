@@ -102,7 +102,7 @@ struct GivenToken {
     template <typename T>
     __device__ __forceinline__ GivenToken(const LogProbsForward& f, const T* __restrict__ row, long long r) : token(-1), z(0.0f) {
         if (!f.log_prob) return;
-        token = whole_at(f.tokens, f.tokens_wide, r);
+        token = whole_at(f.tokens, f.tokens_wide, r * f.tokens_step);
         if (token >= 0 && token < f.vocab) z = static_cast<float>(row[token]);
     }
 };
@@ -167,9 +167,9 @@ struct TeacherRow {
             z[i] = 0.0f;
             id[i] = -1;
             if (k >= f.held) continue;
-            const long long given = whole_at(f.ids, f.ids_wide, r * f.held + k);
+            const long long given = whole_at(f.ids, f.ids_wide, r * f.ids_step + k);
             if (given < 0) continue;
-            u[i] = f.teacher[r * f.held + k] * inv_t;
+            u[i] = f.teacher[r * f.teacher_step + k] * inv_t;
             if (given >= f.vocab) {
                 bad = 1.0f;
                 continue;
@@ -190,7 +190,7 @@ struct TeacherRow {
             sum += p[i];
         }
         sum = joint(sum, [](float a, float b) { return a + b; });
-        weight = sum == 0.0f ? 0.0f : f.row_weights ? f.row_weights[r] : 1.0f;
+        weight = sum == 0.0f ? 0.0f : f.row_weights ? f.row_weights[r * f.weights_step] : 1.0f;
         poisoned = weight != 0.0f && bad != 0.0f;
         const float ln_sum = logf(sum);
 #pragma unroll
@@ -961,7 +961,7 @@ __global__ __launch_bounds__(GRAD_THREADS) void log_probs_backward_kernel(const 
     const T* z = logits + r * b.stride;
     T* out = grad + r * b.grad_stride;
     const float m = b.stats[r], s = b.stats[b.rows + r], inv = s == 0.0f ? 0.0f : 1.0f / s;
-    const long long t = b.log_prob_grad ? whole_at(b.tokens, b.tokens_wide, r) : -1;
+    const long long t = b.log_prob_grad ? whole_at(b.tokens, b.tokens_wide, r * b.tokens_step) : -1;
     const float factor = b.factor ? b.factor[0] : 1.0f;
     float g = t < 0 || s == 0.0f ? 0.0f : b.scale * factor * b.log_prob_grad[r * b.log_prob_step];
     if (t >= b.vocab) g = NOT_A_NUMBER;
@@ -1011,7 +1011,7 @@ __global__ __launch_bounds__(GRAD_THREADS) void distill_backward_kernel(const T*
     long long id = -1;
     float target = 0.0f, at_id = 0.0f, held = 0.0f;
     if (static_cast<int>(threadIdx.x) < b.held) {
-        id = whole_at(b.ids, b.ids_wide, r * b.held + threadIdx.x);
+        id = whole_at(b.ids, b.ids_wide, r * b.ids_step + threadIdx.x);
         if (id >= first && id < b.vocab && id < first + GradSpan<T>::SIZE) {
             target = b.targets[r * b.held + threadIdx.x];
             at_id = static_cast<float>(z[id]);
@@ -1029,10 +1029,10 @@ __global__ __launch_bounds__(GRAD_THREADS) void distill_backward_kernel(const T*
 __global__ __launch_bounds__(MEAN_THREADS) void row_mean_kernel(const float* __restrict__ values,
                                                                 const float* __restrict__ weights,
                                                                 const void* __restrict__ tokens, int tokens_wide,
-                                                                long long rows, float scale, float* __restrict__ out) {
+                                                                long long tokens_step, long long rows, float scale, float* __restrict__ out) {
     mean_of_rows<MEAN_THREADS>(
         [&](long long r) { return values[r]; },
-        [&](long long r) { return weights ? weights[r] : tokens && whole_at(tokens, tokens_wide, r) < 0 ? 0.0f : 1.0f; },
+        [&](long long r) { return weights ? weights[r] : tokens && whole_at(tokens, tokens_wide, r * tokens_step) < 0 ? 0.0f : 1.0f; },
         rows, scale, out);
 }
 
@@ -1134,7 +1134,7 @@ int launch_distill(const void* logits, int type, const DistillForward& f, hipStr
         MFH_TRY(MFH_CHECK_LAUNCH("distill", stream));
         if (f.rows <= MEAN_ROWS) return OK;
     }
-    return launch_row_mean(f.row_loss, f.weights, nullptr, 0, f.rows, 1.0f, f.loss, stream);
+    return launch_row_mean(f.row_loss, f.weights, nullptr, 0, 0, f.rows, 1.0f, f.loss, stream);
 }
 
 int launch_distill_backward(const void* logits, void* grad, int type, const DistillBackward& b, hipStream_t stream) {
@@ -1152,9 +1152,9 @@ int launch_distill_backward(const void* logits, void* grad, int type, const Dist
     return MFH_CHECK_LAUNCH("distill_backward", stream);
 }
 
-int launch_row_mean(const float* values, const float* weights, const void* tokens, int tokens_wide, std::int64_t rows,
-                    float scale, float* out, hipStream_t stream) {
-    launch(row_mean_kernel, 1, MEAN_THREADS, 0, stream, values, weights, tokens, tokens_wide, rows, scale, out);
+int launch_row_mean(const float* values, const float* weights, const void* tokens, int tokens_wide, std::int64_t tokens_step,
+                    std::int64_t rows, float scale, float* out, hipStream_t stream) {
+    launch(row_mean_kernel, 1, MEAN_THREADS, 0, stream, values, weights, tokens, tokens_wide, tokens_step, rows, scale, out);
     return MFH_CHECK_LAUNCH("row_mean", stream);
 }
 

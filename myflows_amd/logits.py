@@ -8,9 +8,9 @@
 
 Logits are 2-D GPU tensors of float32, bfloat16 or float16 whose rows are contiguous; the rows may lie
 apart (a slice of a padded product is read in place). Everything else is float32, tokens and ids are
-int32 or int64, and a negative token or id is none. All arithmetic is float32, and a gradient is rounded
-once to the logits' type. There is no host path. The reference has no counterpart: its only loss is the
-mean squared error.
+int32 or int64, and a negative token or id is none; they are read in place too, at their own strides. All
+arithmetic is float32, and a gradient is rounded once to the logits' type. There is no host path. The
+reference has no counterpart: its only loss is the mean squared error.
 """
 
 from __future__ import annotations
@@ -120,12 +120,19 @@ def _logits(value):
 
 
 def _whole(value, shape, name):
-    """(tensor, whether it is int64) of GPU whole numbers of a shape."""
+    """(tensor, whether it is int64, row stride) of GPU whole numbers of a shape, read in place: one a row at any
+    stride, or rows side by side at any row stride (others are copied)."""
     if not (isinstance(value, torch.Tensor) and value.is_cuda and value.dtype in (torch.int32, torch.int64)):
         raise TypeError(f"{name} must be an int32 or int64 torch tensor on the GPU")
     if value.shape != shape:
         raise ValueError(f"{name} must have shape {shape}")
-    return value.contiguous(), int(value.dtype is torch.int64)
+    value = _side_by_side(value)
+    return value, int(value.dtype is torch.int64), value.stride(0)
+
+
+def _side_by_side(value):
+    """A 2-D tensor's rows side by side: itself, or a copy."""
+    return value.contiguous() if value.ndim == 2 and value.shape[1] > 1 and value.stride(1) != 1 else value
 
 
 def _row_floats(value, rows, name):
@@ -172,16 +179,16 @@ def log_probs_forward(logits, tokens=None, *, top=0):
     top = int(top)
     if not 0 <= top <= min(TOP_MAX, vocab):
         raise ValueError(f"top must lie between 0 and {min(TOP_MAX, vocab)} (at most {TOP_MAX} and the vocabulary)")
-    wide = 0
+    wide = tokens_stride = 0
     if tokens is not None:
-        tokens, wide = _whole(tokens, (rows,), "tokens")
+        tokens, wide, tokens_stride = _whole(tokens, (rows,), "tokens")
     floats = logits.new_empty((5, rows), dtype=torch.float32)
     top_log_probs = logits.new_empty((rows, top), dtype=torch.float32) if top else None
     top_ids = logits.new_empty((rows, top), dtype=torch.int32) if top else None
     workspace, held = native.byte_workspace(_log_probs_workspace(rows, vocab, code, top))
     stats, row = floats.data_ptr(), 4 * rows
     native._call("mfh_log_probs", logits.data_ptr(), code, rows, vocab, stride, native._addr(tokens), wide,
-                 0 if tokens is None else stats + 4 * row, stats + 2 * row, stats + 3 * row, stats, top,
+                 tokens_stride, 0 if tokens is None else stats + 4 * row, stats + 2 * row, stats + 3 * row, stats, top,
                  native._addr(top_log_probs), native._addr(top_ids), workspace, held,
                  native.stream_counters() if held else 0, native._stream())
     return LogProbs(floats, tokens is not None, top_log_probs, top_ids)
@@ -191,18 +198,18 @@ def _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, fact
     logits, code, rows, vocab, stride = _logits(logits)
     if not isinstance(saved, LogProbs) or saved._floats.shape[1] != rows:
         raise ValueError("saved must be the LogProbs of these logits")
-    wide = lp_step = entropy_step = 0
+    wide = tokens_stride = lp_step = entropy_step = 0
     if log_prob_grad is not None:
         if tokens is None:
             raise ValueError("a gradient of the log probabilities needs their tokens")
-        tokens, wide = _whole(tokens, (rows,), "tokens")
+        tokens, wide, tokens_stride = _whole(tokens, (rows,), "tokens")
         log_prob_grad, lp_step = _row_floats(log_prob_grad, rows, "log_prob_grad")
     if entropy_grad is not None:
         entropy_grad, entropy_step = _row_floats(entropy_grad, rows, "entropy_grad")
     out, out_stride = _gradient(out, add, logits)
     stats = saved._floats.data_ptr()
     native._call("mfh_log_probs_backward", logits.data_ptr(), code, rows, vocab, stride,
-                 0 if log_prob_grad is None else tokens.data_ptr(), wide, stats, stats + 8 * rows,
+                 0 if log_prob_grad is None else tokens.data_ptr(), wide, tokens_stride, stats, stats + 8 * rows,
                  native._addr(log_prob_grad), lp_step, native._addr(entropy_grad), entropy_step,
                  native._addr(factor), scale, out.data_ptr(), out_stride, int(add), native._stream())
     return out
@@ -236,20 +243,23 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
     if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.ndim != 2 or not 0 < teacher_ids.shape[1] <= DISTILL_HELD_MAX:
         raise ValueError(f"teacher_ids must be a (rows, held) tensor with held between 1 and {DISTILL_HELD_MAX}")
     shape = (rows, teacher_ids.shape[1])
-    teacher_ids, wide = _whole(teacher_ids, shape, "teacher_ids")
-    teacher_logits = native._device_f32(teacher_logits, "teacher_logits")
-    if tuple(teacher_logits.shape) != shape:
+    teacher_ids, wide, ids_stride = _whole(teacher_ids, shape, "teacher_ids")
+    if not (isinstance(teacher_logits, torch.Tensor) and teacher_logits.is_cuda and teacher_logits.dtype is torch.float32):
+        raise TypeError("teacher_logits must be a float32 torch tensor on the GPU")
+    if teacher_logits.shape != shape:
         raise ValueError(f"teacher_logits must have shape {shape}")
+    teacher_logits = _side_by_side(teacher_logits)
+    weights_stride = 0
     if row_weights is not None:
-        row_weights = _row_floats(row_weights, rows, "row_weights")[0].contiguous()
+        row_weights, weights_stride = _row_floats(row_weights, rows, "row_weights")
     floats = logits.new_empty((2 + rows * (4 + shape[1]),), dtype=torch.float32)
     workspace, held = native.byte_workspace(_distill_workspace(rows, vocab, code))
     scale, row = floats.data_ptr(), 4 * rows
     row_loss = scale + 8
     native._call("mfh_distill_loss", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
-                 teacher_logits.data_ptr(), shape[1], native._addr(row_weights), temperature, row_loss, row_loss + row,
-                 row_loss + 2 * row, row_loss + 4 * row, scale, workspace, held, native.stream_counters(),
-                 native._stream())
+                 ids_stride, teacher_logits.data_ptr(), teacher_logits.stride(0), shape[1], native._addr(row_weights),
+                 weights_stride, temperature, row_loss, row_loss + row, row_loss + 2 * row, row_loss + 4 * row, scale,
+                 workspace, held, native.stream_counters(), native._stream())
     return DistillLoss(floats, rows, shape[1])
 
 
@@ -260,7 +270,7 @@ def distill_loss_backward(logits, teacher_ids, saved, seed, *, temperature=1.0, 
     temperature = _temperature(temperature)
     if not isinstance(saved, DistillLoss) or saved._rows != rows:
         raise ValueError("saved must be the DistillLoss of these logits")
-    teacher_ids, wide = _whole(teacher_ids, (rows, saved._held), "teacher_ids")
+    teacher_ids, wide, ids_stride = _whole(teacher_ids, (rows, saved._held), "teacher_ids")
     seed = native._device_f32(seed, "seed")
     if seed.numel() != 1:
         raise ValueError("seed must hold one value")
@@ -268,7 +278,7 @@ def distill_loss_backward(logits, teacher_ids, saved, seed, *, temperature=1.0, 
     scale, row = saved._floats.data_ptr(), 4 * rows
     row_loss = scale + 8
     native._call("mfh_distill_loss_backward", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
-                 saved._held, row_loss + 4 * row, row_loss + 2 * row, row_loss + row, scale, seed.data_ptr(), temperature,
+                 ids_stride, saved._held, row_loss + 4 * row, row_loss + 2 * row, row_loss + row, scale, seed.data_ptr(), temperature,
                  out.data_ptr(), out_stride, int(add), native._stream())
     return out
 
@@ -290,10 +300,10 @@ class CrossEntropyLoss(GradientOp):
     def forward(self, logits, labels):
         _on_gpu(logits, "CrossEntropyLoss")
         self.log_probs = log_probs_forward(logits, labels)
-        labels, wide = _whole(labels, (logits.shape[0],), "labels")
+        labels, wide, stride = _whole(labels, (logits.shape[0],), "labels")
         self._scale = torch.empty((2,), dtype=torch.float32, device=logits.device)
-        native._call("mfh_row_mean", self.log_probs.log_prob.data_ptr(), labels.data_ptr(), wide, logits.shape[0], -1.0,
-                     self._scale.data_ptr(), native._stream())
+        native._call("mfh_row_mean", self.log_probs.log_prob.data_ptr(), labels.data_ptr(), wide, stride, logits.shape[0],
+                     -1.0, self._scale.data_ptr(), native._stream())
         self.value = self._scale[0]
 
     def backward(self):

@@ -138,12 +138,12 @@ _SIGNATURES = {
     "mfh_mse_loss_backward": ("i", "ppppqip"),
     "mfh_column_sums": ("i", "ppqqp"),
     "mfh_log_probs_workspace": ("q", "qiii"),
-    "mfh_log_probs": ("i", "piqiq" + "pi" + "pppp" + "ipp" + "pqpp"),
-    "mfh_log_probs_backward": ("i", "piqiq" + "pi" + "pp" + "pqpq" + "pf" + "pqi" + "p"),
+    "mfh_log_probs": ("i", "piqiq" + "piq" + "pppp" + "ipp" + "pqpp"),
+    "mfh_log_probs_backward": ("i", "piqiq" + "piq" + "pp" + "pqpq" + "pf" + "pqi" + "p"),
     "mfh_distill_workspace": ("q", "qii"),
-    "mfh_distill_loss": ("i", "piqiq" + "pipi" + "pf" + "ppppp" + "pqpp"),
-    "mfh_distill_loss_backward": ("i", "piqiq" + "pii" + "ppppp" + "f" + "pqi" + "p"),
-    "mfh_row_mean": ("i", "ppiqfpp"),
+    "mfh_distill_loss": ("i", "piqiq" + "piqpqi" + "pqf" + "ppppp" + "pqpp"),
+    "mfh_distill_loss_backward": ("i", "piqiq" + "piqi" + "ppppp" + "f" + "pqi" + "p"),
+    "mfh_row_mean": ("i", "ppiqqfpp"),
     "mfh_group_norm_workspace": ("q", "qiiiii"),
     "mfh_group_norm_forward": ("i", "piqiii" + "ppif" + "ppp" + "pqp"),
     "mfh_group_norm_backward": ("i", "ppiqiii" + "pppp" + "i" + "ppp" + "iii" + "pqp"),
