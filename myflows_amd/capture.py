@@ -115,8 +115,9 @@ class RecordedStep(_ReplayedStep):
     every tensor it allocates in a private memory pool: the blocks of the pass's temporaries stay
     reserved for the replays, which write them in the recorded order; the stream workspaces it uses
     are held by the step. Every GPU write of the pass
-    is a library launch (the backward's seed too), so the program is the whole pass. The same rules
-    as for ``CapturedStep`` hold: fixed shapes and leaf flags, inputs refreshed in place, outputs and
+    is a library launch (the backward's seed too), so the program is the whole pass; a pass with work of torch's
+    own (an ``Add`` outside a fused unit, a copy of a tensor that is not contiguous) raises RuntimeError instead of
+    being recorded. The same rules as for ``CapturedStep`` hold: fixed shapes and leaf flags, inputs refreshed in place, outputs and
     gradients overwritten by each replay, the optimiser update eager."""
 
     def __init__(self, optimizer, warmup=2):

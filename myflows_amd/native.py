@@ -25,6 +25,8 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
+from torch.utils._pytree import tree_leaves
 
 from . import build as _build
 
@@ -256,14 +258,48 @@ def fill_(tensor, value):
     return tensor
 
 
+class _LibraryWritesOnly(TorchDispatchMode):
+    """Refuses what torch itself would write on the GPU while a program is being recorded: the program holds the
+    library's launches alone, so a replay would read what such a write left, or what lies there since. Memory
+    without a value, views, and the zero gradient of a leaf that no operator reached (nothing adds to it) pass."""
+
+    _MEMORY = frozenset((torch.ops.aten.empty.memory_format, torch.ops.aten.empty_like.default,
+                         torch.ops.aten.empty_strided.default, torch.ops.aten.new_empty.default,
+                         torch.ops.aten.new_empty_strided.default, torch.ops.aten.zeros_like.default))
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        result = func(*args, **(kwargs or {}))
+        if func in self._MEMORY:
+            return result
+        on_gpu = lambda tree: [t for t in tree_leaves(tree) if isinstance(t, torch.Tensor) and t.is_cuda]  # noqa: E731
+        given = on_gpu((args, kwargs))
+        if func._schema.is_mutable:
+            writes = bool(given)
+        else:
+            held = {t.untyped_storage().data_ptr() for t in given}
+            writes = any(t.numel() and t.untyped_storage().data_ptr() not in held for t in on_gpu(result))
+        if writes:
+            raise RuntimeError(f"torch's {func} writes on the GPU while a pass is being recorded: a replay would not "
+                               "repeat it (an operator without a library kernel, or a copy of a tensor that is not contiguous)")
+        return result
+
+
+_recorded = threading.local()
+
+
 def program_begin():
     """Record every launch and stream ordering the library issues on this thread from now on into a
-    program (mfh_program_begin); program_end returns it."""
+    program (mfh_program_begin); program_end returns it. A GPU write of torch's own raises meanwhile."""
     _call("mfh_program_begin")
+    _recorded.guard = _LibraryWritesOnly()
+    _recorded.guard.__enter__()
 
 
 def program_end():
     """(handle, kernel launches) of the program recorded since program_begin."""
+    guard, _recorded.guard = getattr(_recorded, "guard", None), None
+    if guard is not None:
+        guard.__exit__(None, None, None)
     handle, launches = ctypes.c_uint64(0), ctypes.c_int64(0)
     _call("mfh_program_end", ctypes.byref(handle), ctypes.byref(launches))
     return handle.value, launches.value

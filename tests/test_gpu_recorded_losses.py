@@ -75,3 +75,28 @@ def test_a_recorded_distillation_reads_slices_of_a_record():
 
     _steps_agree(lambda out: mf.DistillationLoss(out, _constant(ids[:, :6]), _constant(teacher[:, :6]),
                                                  _constant(weights[:, 1]), temperature=1.5), refresh)
+
+
+def _sum_of_losses(out):
+    ids = torch.randint(0, CLASSES, (ROWS, 6), generator=torch.Generator().manual_seed(4)).cuda()
+    teacher = torch.randn((ROWS, 6), generator=torch.Generator().manual_seed(5)).cuda()
+    return mf.Add(mf.CrossEntropyLoss(out, _constant(ids[:, 0])), mf.DistillationLoss(out, _constant(ids), _constant(teacher)))
+
+
+def _turned_record(out):
+    ids = torch.randint(0, CLASSES, (6, ROWS), generator=torch.Generator().manual_seed(4)).cuda()
+    teacher = torch.randn((6, ROWS), generator=torch.Generator().manual_seed(5)).cuda()
+    return mf.DistillationLoss(out, _constant(ids.t()), _constant(teacher.t()))
+
+
+@pytest.mark.parametrize("make_loss", (_sum_of_losses, _turned_record))
+def test_work_of_another_library_is_refused_while_a_pass_is_recorded(make_loss):
+    """Torch's own launches (an Add, a copy of a tensor whose rows are not contiguous) are no steps of the program: a
+    replay would read what they left, or what has been written there since. The pass runs eagerly as ever."""
+    print("refused in a recorded pass", make_loss.__name__, flush=True)
+    _, _, loss, optimizer = _network(make_loss)
+    with pytest.raises(RuntimeError, match="recorded"):
+        mf.RecordedStep(optimizer)
+    optimizer.one_step()
+    assert bool(torch.isfinite(loss.value)) and bool(torch.ones(3, device="cuda").add(1.0).eq(2.0).all())
+    mf.RecordedStep(_network(lambda out: mf.CrossEntropyLoss(out, _constant(torch.zeros(ROWS, dtype=torch.int64, device="cuda"))))[3]).close()
