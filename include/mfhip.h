@@ -549,7 +549,8 @@ MFH_API int mfh_log_probs(uint64_t logits, int type, int64_t rows, int vocab, in
  * grad += that when add != 0, with g = scale * factor[0] * log_prob_grad[r * log_prob_grad_stride] (0 where
  * token < 0) and h = factor[0] * entropy_grad[r * entropy_grad_stride]. factor (one float on the device, 1
  * when 0), log_prob_grad and entropy_grad are optional. stats and entropy are those of
- * mfh_log_probs. A row whose g and h are 0 gets 0 whatever its logits hold. */
+ * mfh_log_probs. A row whose g and h are 0 gets 0 whatever its logits hold; a token >= vocab makes it NaN where
+ * g is not 0. */
 MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
                                    int tokens_int64, int64_t tokens_stride, uint64_t stats, uint64_t entropy,
                                    uint64_t log_prob_grad, int64_t log_prob_grad_stride, uint64_t entropy_grad,

@@ -963,8 +963,9 @@ __global__ __launch_bounds__(GRAD_THREADS) void log_probs_backward_kernel(const 
     const float m = b.stats[r], s = b.stats[b.rows + r], inv = s == 0.0f ? 0.0f : 1.0f / s;
     const long long t = b.log_prob_grad ? whole_at(b.tokens, b.tokens_wide, r * b.tokens_step) : -1;
     const float factor = b.factor ? b.factor[0] : 1.0f;
-    float g = t < 0 || s == 0.0f ? 0.0f : b.scale * factor * b.log_prob_grad[r * b.log_prob_step];
-    if (t >= b.vocab) g = NOT_A_NUMBER;
+    float g = t < 0 ? 0.0f : b.scale * factor * b.log_prob_grad[r * b.log_prob_step];
+    if (t >= b.vocab && g != 0.0f) g = NOT_A_NUMBER;  // as its log probability
+    else if (s == 0.0f) g = 0.0f;
     const float h = b.entropy_grad && s != 0.0f ? factor * b.entropy_grad[r * b.entropy_step] : 0.0f;
     if (g == 0.0f && h == 0.0f) {
         form_span<ADD>(z, out, first, b.vocab, [](float, int) { return 0.0f; }, [] {});

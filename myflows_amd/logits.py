@@ -218,7 +218,8 @@ def _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, fact
 def log_probs_backward(logits, tokens, saved, *, log_prob_grad=None, entropy_grad=None, out=None, add=False):
     """The gradient of sum(log_prob_grad * log_prob) + sum(entropy_grad * entropy) by the logits, written to
     (or, with add, added to) out. ``saved`` is the LogProbs of the same logits; the gradients (rows,) may have
-    any stride (an expanded scalar). A row whose gradients are 0 gets 0, whatever its logits hold."""
+    any stride (an expanded scalar). A row whose gradients are 0 gets 0, whatever its logits hold and its token is; a
+    token beyond the vocabulary makes its row NaN where its log_prob_grad is not 0."""
     return _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, None, 1.0, out, add)
 
 

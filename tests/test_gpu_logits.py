@@ -240,6 +240,31 @@ def test_log_probs_gradient_matches_differences():
     assert float((slope - (grad * v).double().sum(dim=1)).abs().max()) <= 2.0 ** -12 / 6 + 40 * 2.0 ** -21 * 64
 
 
+@gpu
+@pytest.mark.parametrize("vocab", (9, 5000))
+def test_a_row_without_gradient_gets_zeros_whatever_its_token(vocab):
+    """A padding row whose token lies beyond the vocabulary: its log probability is NaN, its gradient only where the
+    row's gradient is not 0."""
+    z, gen = _z(7, vocab, "float32", 31)
+    z[4:6] = NEG
+    tokens = torch.tensor([vocab, vocab + 2 ** 32, vocab, 1, vocab, vocab, -1], device="cuda")
+    g = torch.tensor([0.0, -0.0, 1.0, 2.0, 0.0, 1.0, 3.0], device="cuda")
+    r = ops.log_probs_forward(z, tokens)
+    assert torch.isnan(r.log_prob).tolist() == [True, True, True, False, True, True, False]
+    grad = ops.log_probs_backward(z, tokens, r, log_prob_grad=g)
+    assert torch.isnan(grad).all(dim=1).tolist() == [False, False, True, False, False, True, False]
+    assert not grad[[0, 1, 4, 6]].any() and bool(grad[3].any())
+    # with a gradient of the entropy, the row has that one alone
+    h = torch.tensor([0.5, 0.0, 0.0, 0.0, 0.5, 0.0, 0.0], device="cuda")
+    both = ops.log_probs_backward(z, tokens, r, log_prob_grad=g, entropy_grad=h)
+    alone = ops.log_probs_backward(z, None, r, entropy_grad=h)
+    assert torch.equal(both[:2], alone[:2]) and bool(both[0].any()) and not both[[1, 4, 6]].any()
+    # added to what is there: nothing
+    out = torch.ones_like(z)
+    ops.log_probs_backward(z, tokens, r, log_prob_grad=g, out=out, add=True)
+    assert bool((out[[0, 1, 4, 6]] == 1.0).all())
+
+
 # ---- distillation -----------------------------------------------------------------------------
 def _record(rows, vocab, held, gen, ragged=True, duplicates=False):
     ids = torch.stack([torch.randperm(vocab, generator=gen)[:held] if vocab >= held else
