@@ -6,6 +6,8 @@
 // and, with du = dy act'(u) and the averages over the group,
 //   dgamma[c] = sum du xhat,  dbeta[c] = sum du,
 //   dx = inv_std (gamma du - average(gamma du) - xhat average(gamma du xhat)).
+// u is formed as a (x - mean) + beta, a = gamma inv_std, in every pass alike (affine): the backward's ReLU lets
+// through exactly what the forward's did.
 // Sums are float32; the variance is a sum of squares about a mean, never a difference of large sums. Every
 // sum is formed in one fixed order.
 //
@@ -55,6 +57,11 @@ template <bool SILU>
 __device__ __forceinline__ float activate(float u, float floor) {
     if constexpr (SILU) return u * sigmoid_of(u);
     return u < floor ? floor : u;
+}
+// u, rounded the same way in every pass.
+__device__ __forceinline__ float affine(float less_mean, float a, float beta) { return fmaf(less_mean, a, beta); }
+__device__ __forceinline__ float inv_std_of(float squares, float inv_count, float eps) {
+    return 1.0f / sqrtf(fmaf(squares, inv_count, eps));
 }
 // dy act'(u)
 template <bool SILU>
@@ -221,9 +228,9 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
     stay_packed(held);
     group_sums<THREADS, VW>(k, place.width, lds, sums, t.group, squares, variance);
     if (static_cast<int>(threadIdx.x) < k.groups)
-        f.inv_std[n * s.groups + place.group + threadIdx.x] = 1.0f / sqrtf(sums[threadIdx.x] * inv_count + f.eps);
+        f.inv_std[n * s.groups + place.group + threadIdx.x] = inv_std_of(sums[threadIdx.x], inv_count, f.eps);
 #pragma unroll
-    for (int i = 0; i < VW; ++i) a[i] *= 1.0f / sqrtf(variance[i] * inv_count + f.eps);
+    for (int i = 0; i < VW; ++i) a[i] *= inv_std_of(variance[i], inv_count, f.eps);
     const float floor = f.act == ACT_RELU ? 0.0f : -INFINITY;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
@@ -232,19 +239,24 @@ __global__ __launch_bounds__(THREADS) void held_forward_kernel(const T* __restri
         if (t.active && row < s.positions) {
             float out[VW];
 #pragma unroll
-            for (int i = 0; i < VW; ++i) out[i] = activate<SILU>((held[h].at(i) - mean[i]) * a[i] + beta[i], floor);
+            for (int i = 0; i < VW; ++i) out[i] = activate<SILU>(affine(held[h].at(i) - mean[i], a[i], beta[i]), floor);
             store_pack(y + base + row * s.channels, Pack<T, VW>::of(out));
         }
     }
 }
 
-// What the backward forms of an element: xhat and du.
+// What the backward forms of an element: xhat and du, with a = gamma inv as in the forward.
 template <bool SILU>
 struct Backward {
     float hat, du;
-    __device__ __forceinline__ Backward(float x, float dy, float mean, float inv, float gamma, float beta, float floor) {
-        hat = (x - mean) * inv;
-        du = through<SILU>(hat * gamma + beta, dy, floor);
+    __device__ __forceinline__ Backward(float x, float dy, float mean, float inv, float a, float beta, float floor) {
+        const float d = x - mean;
+        hat = d * inv;
+        du = through<SILU>(affine(d, a, beta), dy, floor);
+    }
+    // dx from the group's averages of gamma du and gamma du xhat.
+    __device__ __forceinline__ float dx(float inv, float a, float average, float average_hat) const {
+        return du * a - inv * (average + hat * average_hat);
     }
 };
 
@@ -261,7 +273,7 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
     const Thread<THREADS, VW> t(k, place.width);
     const long long base = n * s.positions * s.channels + place.channel + t.column;
     Pack<T, VW> held[HOLD], grad[HOLD];
-    float mean[VW], inv[VW], gamma[VW], beta[VW], sum[VW] = {}, product[VW] = {};
+    float mean[VW], inv[VW], a[VW], beta[VW], sum[VW] = {}, product[VW] = {};
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
         if (h * t.step >= s.positions) break;
@@ -273,11 +285,13 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
     }
     t.by_group(b.mean + n * s.groups + place.group, mean);
     t.by_group(b.inv_std + n * s.groups + place.group, inv);
-    t.by_column(b.gamma + place.channel, gamma);
+    t.by_column(b.gamma + place.channel, a);
     t.by_column(b.beta + place.channel, beta);
+#pragma unroll
+    for (int i = 0; i < VW; ++i) a[i] *= inv[i];
     const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
     const auto form = [&](int h, int i) {
-        return Backward<SILU>(held[h].at(i), grad[h].at(i), mean[i], inv[i], gamma[i], beta[i], floor);
+        return Backward<SILU>(held[h].at(i), grad[h].at(i), mean[i], inv[i], a[i], beta[i], floor);
     };
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
@@ -343,7 +357,7 @@ __global__ __launch_bounds__(THREADS) void held_backward_kernel(const T* __restr
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
                 const Backward<SILU> e = form(h, i);
-                out[i] = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
+                out[i] = e.dx(inv[i], a[i], mean_d[i], mean_p[i]);
             }
             if (b.add_x) add_pack(out, to);
             store_pack(to, Pack<T, VW>::of(out));
@@ -482,7 +496,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void join_stats_kernel(const float* 
     about = group_sum(about);
     if (threadIdx.x != 0) return;
     f.mean[blockIdx.x] = mean;
-    f.inv_std[blockIdx.x] = 1.0f / sqrtf(about * inv_count + f.eps);
+    f.inv_std[blockIdx.x] = inv_std_of(about, inv_count, f.eps);
 }
 
 template <typename T, int VW, bool SILU>
@@ -504,7 +518,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void apply_forward_kernel(const T* _
     const auto write = [&](int row, const Pack<T, VW>& in) {
         float out[VW];
 #pragma unroll
-        for (int i = 0; i < VW; ++i) out[i] = activate<SILU>((in.at(i) - mean[i]) * a[i] + beta[i], floor);
+        for (int i = 0; i < VW; ++i) out[i] = activate<SILU>(affine(in.at(i) - mean[i], a[i], beta[i]), floor);
         store_pack(y + base + row * s.channels, Pack<T, VW>::of(out));
     };
     int row = r.begin + t.row;
@@ -528,16 +542,18 @@ __global__ __launch_bounds__(SPLIT_THREADS) void run_gradients_kernel(const T* _
     const RunAt r = run_at(runs, k, s.positions, false);
     const Thread<SPLIT_THREADS, VW> t(k, r.place.width);
     const long long base = r.n * s.positions * s.channels + r.place.channel + t.column;
-    float mean[VW], inv[VW], gamma[VW], beta[VW], sum[VW] = {}, product[VW] = {};
+    float mean[VW], inv[VW], a[VW], beta[VW], sum[VW] = {}, product[VW] = {};
     t.by_group(b.mean + r.n * s.groups + r.place.group, mean);
     t.by_group(b.inv_std + r.n * s.groups + r.place.group, inv);
-    t.by_column(b.gamma + r.place.channel, gamma);
+    t.by_column(b.gamma + r.place.channel, a);
     t.by_column(b.beta + r.place.channel, beta);
+#pragma unroll
+    for (int i = 0; i < VW; ++i) a[i] *= inv[i];
     const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
     const auto take = [&](const Pack<T, VW>& in, const Pack<T, VW>& grad) {
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], gamma[i], beta[i], floor);
+            const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], a[i], beta[i], floor);
             sum[i] += e.du;
             product[i] += e.du * e.hat;
         }
@@ -651,11 +667,13 @@ __global__ __launch_bounds__(SPLIT_THREADS) void apply_backward_kernel(const T* 
     __syncthreads();
     if (!t.active) return;
     const long long base = r.n * s.positions * s.channels + r.place.channel + t.column;
-    float mean[VW], inv[VW], gamma[VW], beta[VW], mean_d[VW], mean_p[VW];
+    float mean[VW], inv[VW], a[VW], beta[VW], mean_d[VW], mean_p[VW];
     t.by_group(b.mean + r.n * s.groups + r.place.group, mean);
     t.by_group(b.inv_std + r.n * s.groups + r.place.group, inv);
-    t.by_column(b.gamma + r.place.channel, gamma);
+    t.by_column(b.gamma + r.place.channel, a);
     t.by_column(b.beta + r.place.channel, beta);
+#pragma unroll
+    for (int i = 0; i < VW; ++i) a[i] *= inv[i];
     t.by_group(sums[0], mean_d);
     t.by_group(sums[1], mean_p);
     const float floor = b.act == ACT_RELU ? 0.0f : -INFINITY;
@@ -664,8 +682,8 @@ __global__ __launch_bounds__(SPLIT_THREADS) void apply_backward_kernel(const T* 
         float out[VW];
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], gamma[i], beta[i], floor);
-            out[i] = inv[i] * (e.du * gamma[i] - mean_d[i] - e.hat * mean_p[i]);
+            const Backward<SILU> e(in.at(i), grad.at(i), mean[i], inv[i], a[i], beta[i], floor);
+            out[i] = e.dx(inv[i], a[i], mean_d[i], mean_p[i]);
         }
         if (b.add_x) add_pack(out, to);
         store_pack(to, Pack<T, VW>::of(out));

@@ -272,6 +272,29 @@ def test_group_norm_layer_in_a_graph():
 
 
 @gpu
+@pytest.mark.parametrize("n,positions,channels,groups", [
+    (4096, 1, 64, 4), (300, 16, 32, 2), (16, 405, 90, 6), (2, 9000, 64, 8), (3, 20000, 33, 3), (2, 5, 40000, 2)])
+def test_the_relu_gate_of_the_gradient_is_that_of_the_output(n, positions, channels, groups):
+    """The gradient passes exactly where y > 0. beta cancels gamma xhat of one position a channel up to its
+    rounding, so that many u lie within a rounding of 0; dy = 1 and dbeta count what passes."""
+    x, _, gamma, _ = _data(n, positions, channels, "float32", 13)
+    x = x.round(decimals=1)  # many equal values
+    _, mean, inv = ops.group_norm_forward(x, gamma, torch.zeros_like(gamma), groups)
+    per = channels // groups
+    spread = lambda v: v[0].repeat_interleave(per)  # noqa: E731
+    beta = -gamma * ((x[0, 0] - spread(mean)) * spread(inv))
+    x[:] = x[:1, :1]  # of every sample and position; the statistics are those that the forward takes
+    x += torch.arange(positions, device="cuda").reshape(1, -1, 1) % 3 * 0.25
+    y, mean, inv = ops.group_norm_forward(x, gamma, beta, groups, activation="relu")
+    beta = -gamma * ((x[0, 0] - spread(mean)) * spread(inv))
+    y, mean, inv = ops.group_norm_forward(x, gamma, beta, groups, activation="relu")
+    grads = torch.empty_like(gamma), torch.empty_like(gamma)
+    ops.group_norm_backward(x, torch.ones_like(x), gamma, beta, mean, inv, activation="relu", gamma_grad=grads[0],
+                            beta_grad=grads[1], accumulate=(False,) * 3)
+    assert torch.equal(grads[1], (y > 0).sum(dim=(0, 1)).float())  # whole numbers below 2^24: exact
+
+
+@gpu
 def test_no_samples_and_refusals():
     gamma, beta = torch.ones(6, device="cuda"), torch.zeros(6, device="cuda")
     empty = torch.empty((0, 4, 6), device="cuda")
