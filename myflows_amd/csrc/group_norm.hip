@@ -591,7 +591,7 @@ __global__ __launch_bounds__(SPLIT_THREADS) void run_gradients_kernel(const T* _
 
 // out[outer][j] = the sum over `inner` rows of from[outer][row][j], j < columns: 16 runs of rows a column, each in
 // order, then in run order.
-constexpr int COLUMN_SPAN = 64, COLUMN_RUNS = 16;
+constexpr int COLUMN_SPAN = GROUP_NORM_COLUMN_SPAN, COLUMN_RUNS = GROUP_NORM_COLUMN_RUNS;
 __device__ __forceinline__ float sum_of_rows(const float* __restrict__ from, long long rows, long long columns, long long j,
                                              float (&lds)[COLUMN_RUNS][COLUMN_SPAN]) {
     const int c = threadIdx.x % COLUMN_SPAN, g = threadIdx.x / COLUMN_SPAN;
@@ -708,10 +708,14 @@ Block block_of(const GroupNormPlan& plan) {
     return {plan.per, plan.groups, plan.parts, plan.width, plan.blocks, plan.lanes, FastDiv(plan.per)};
 }
 
-constexpr std::int64_t THREADS_LIMIT = (1LL << 32) - 1;  // threads of a launch
-
-int require_grid(const GroupNormShape& s, const GroupNormPlan& plan) {
-    MFH_REQUIRE(s.n * plan.grid() * plan.threads <= THREADS_LIMIT, "too many samples for one group norm");
+// Calls f(first sample, the slice's shape) for each slice of the samples that a launch takes.
+template <typename F>
+int for_slices(const GroupNormShape& s, std::int64_t slice, F&& f) {
+    for (std::int64_t first = 0; first < s.n; first += slice) {
+        GroupNormShape part = s;
+        part.n = std::min(slice, s.n - first);
+        MFH_TRY(f(first, part));
+    }
     return OK;
 }
 
@@ -748,83 +752,96 @@ std::int64_t group_norm_workspace(const GroupNormShape& s, int type, bool backwa
 int launch_group_norm_forward(const GroupNormShape& s, int type, const void* x, void* y, const GroupNormForward& f,
                               hipStream_t stream) {
     const GroupNormPlan plan = group_norm_plan(s, type_bytes(type), false);
-    MFH_TRY(require_grid(s, plan));
     const Block block = block_of(plan);
     const Runs runs{plan.runs, plan.rows};
-    const unsigned groups = static_cast<unsigned>(s.n * plan.grid());
-    float* means = static_cast<float*>(f.workspace);
-    float* squares = plan.held ? nullptr : means + s.n * plan.runs * s.groups * plan.parts;
-    with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
-        using T = decltype(zero);
-        constexpr int VW = decltype(pack)::value;
-        constexpr int HOLD = group_norm_hold(sizeof(T), VW, false, 256), HOLD_MANY = group_norm_hold(sizeof(T), VW, false, 1024);
-        constexpr bool SILU = decltype(silu)::value;
-        const T* in = static_cast<const T*>(x);
-        if (plan.held && plan.threads == 256)
-            launch(held_forward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, static_cast<T*>(y), s, block, f);
-        else if (plan.held)
-            launch(held_forward_kernel<T, VW, SILU, 1024, HOLD_MANY>, groups, 1024, 0, stream, in, static_cast<T*>(y), s, block, f);
-        else
-            launch(run_stats_kernel<T, VW>, groups, SPLIT_THREADS, 0, stream, in, s, block, runs, means, squares);
+    const std::int64_t sample = static_cast<std::int64_t>(s.positions) * s.channels;
+    const std::int64_t pieces = static_cast<std::int64_t>(plan.runs) * s.groups * plan.parts;  // of a sample, where split
+    return for_slices(s, group_norm_slice(s, plan, false), [&](std::int64_t first, const GroupNormShape& part) -> int {
+        const unsigned groups = static_cast<unsigned>(part.n * plan.grid());
+        GroupNormForward own = f;
+        own.mean += first * s.groups;
+        own.inv_std += first * s.groups;
+        float* means = plan.held ? nullptr : static_cast<float*>(f.workspace) + first * pieces;
+        float* squares = plan.held ? nullptr : means + s.n * pieces;
+        with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
+            using T = decltype(zero);
+            constexpr int VW = decltype(pack)::value;
+            constexpr int HOLD = group_norm_hold(sizeof(T), VW, false, 256), HOLD_MANY = group_norm_hold(sizeof(T), VW, false, 1024);
+            constexpr bool SILU = decltype(silu)::value;
+            const T* in = static_cast<const T*>(x) + first * sample;
+            T* out = static_cast<T*>(y) + first * sample;
+            if (plan.held && plan.threads == 256)
+                launch(held_forward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, out, part, block, own);
+            else if (plan.held)
+                launch(held_forward_kernel<T, VW, SILU, 1024, HOLD_MANY>, groups, 1024, 0, stream, in, out, part, block, own);
+            else
+                launch(run_stats_kernel<T, VW>, groups, SPLIT_THREADS, 0, stream, in, part, block, runs, means, squares);
+        });
+        MFH_TRY(MFH_CHECK_LAUNCH("group_norm_forward", stream));
+        if (plan.held) return OK;
+        launch(join_stats_kernel, static_cast<unsigned>(part.n * s.groups), SPLIT_THREADS, 0, stream, means, squares, part,
+               block, runs, own);
+        MFH_TRY(MFH_CHECK_LAUNCH("group_norm_join", stream));
+        with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
+            using T = decltype(zero);
+            launch(apply_forward_kernel<T, decltype(pack)::value, decltype(silu)::value>, groups, SPLIT_THREADS, 0, stream,
+                   static_cast<const T*>(x) + first * sample, static_cast<T*>(y) + first * sample, part, block, runs, own);
+        });
+        return MFH_CHECK_LAUNCH("group_norm_apply", stream);
     });
-    MFH_TRY(MFH_CHECK_LAUNCH("group_norm_forward", stream));
-    if (plan.held) return OK;
-    launch(join_stats_kernel, static_cast<unsigned>(s.n * s.groups), SPLIT_THREADS, 0, stream, means, squares, s, block, runs, f);
-    MFH_TRY(MFH_CHECK_LAUNCH("group_norm_join", stream));
-    with_kernel(type, plan.vw, f.act, [&](auto zero, auto pack, auto silu) {
-        using T = decltype(zero);
-        launch(apply_forward_kernel<T, decltype(pack)::value, decltype(silu)::value>, groups, SPLIT_THREADS, 0, stream,
-               static_cast<const T*>(x), static_cast<T*>(y), s, block, runs, f);
-    });
-    return MFH_CHECK_LAUNCH("group_norm_apply", stream);
 }
 
 int launch_group_norm_backward(const GroupNormShape& s, int type, const void* x, const void* dy, void* dx,
                                const GroupNormBackward& b, hipStream_t stream) {
     const bool parameters = b.gamma_grad || b.beta_grad;
-    float* columns = static_cast<float*>(b.workspace);
+    float* every = static_cast<float*>(b.workspace);
     if (s.n > 0) {
         const GroupNormPlan plan = group_norm_plan(s, type_bytes(type), true);
-        MFH_TRY(require_grid(s, plan));
         const Block block = block_of(plan);
         const Runs runs{plan.runs, plan.rows};
-        const unsigned groups = static_cast<unsigned>(s.n * plan.grid());
-        float* run_columns = columns + columns_floats(s);
-        with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
-            using T = decltype(zero);
-            constexpr int VW = decltype(pack)::value;
-            constexpr int HOLD = group_norm_hold(sizeof(T), VW, true, 256), HOLD_MANY = group_norm_hold(sizeof(T), VW, true, 1024);
-            constexpr bool SILU = decltype(silu)::value;
-            const T *in = static_cast<const T*>(x), *grad = static_cast<const T*>(dy);
-            if (plan.held && plan.threads == 256)
-                launch(held_backward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, grad, static_cast<T*>(dx), s,
-                       block, b, parameters ? columns : nullptr);
-            else if (plan.held)
-                launch(held_backward_kernel<T, VW, SILU, 1024, HOLD_MANY>, groups, 1024, 0, stream, in, grad, static_cast<T*>(dx), s,
-                       block, b, parameters ? columns : nullptr);
-            else
-                launch(run_gradients_kernel<T, VW, SILU>, groups, SPLIT_THREADS, 0, stream, in, grad, s, block, runs,
-                       b, run_columns);
-        });
-        MFH_TRY(MFH_CHECK_LAUNCH("group_norm_backward", stream));
-        if (!plan.held) {
+        const std::int64_t sample = static_cast<std::int64_t>(s.positions) * s.channels;
+        MFH_TRY(for_slices(s, group_norm_slice(s, plan, true), [&](std::int64_t first, const GroupNormShape& part) -> int {
+            const unsigned groups = static_cast<unsigned>(part.n * plan.grid());
+            GroupNormBackward own = b;
+            own.mean += first * s.groups;
+            own.inv_std += first * s.groups;
+            float* columns = every + 2 * first * s.channels;
+            float* run_columns = every + columns_floats(s) + 2 * first * plan.runs * s.channels;
+            with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
+                using T = decltype(zero);
+                constexpr int VW = decltype(pack)::value;
+                constexpr int HOLD = group_norm_hold(sizeof(T), VW, true, 256), HOLD_MANY = group_norm_hold(sizeof(T), VW, true, 1024);
+                constexpr bool SILU = decltype(silu)::value;
+                const T *in = static_cast<const T*>(x) + first * sample, *grad = static_cast<const T*>(dy) + first * sample;
+                T* out = dx ? static_cast<T*>(dx) + first * sample : nullptr;
+                if (plan.held && plan.threads == 256)
+                    launch(held_backward_kernel<T, VW, SILU, 256, HOLD>, groups, 256, 0, stream, in, grad, out, part, block, own,
+                           parameters ? columns : nullptr);
+                else if (plan.held)
+                    launch(held_backward_kernel<T, VW, SILU, 1024, HOLD_MANY>, groups, 1024, 0, stream, in, grad, out, part,
+                           block, own, parameters ? columns : nullptr);
+                else
+                    launch(run_gradients_kernel<T, VW, SILU>, groups, SPLIT_THREADS, 0, stream, in, grad, part, block, runs,
+                           own, run_columns);
+            });
+            MFH_TRY(MFH_CHECK_LAUNCH("group_norm_backward", stream));
+            if (plan.held) return OK;
             const int tiles = static_cast<int>(blocks_for(2LL * s.channels, COLUMN_SPAN));
-            launch(join_columns_kernel, static_cast<unsigned>(s.n * tiles), COLUMN_SPAN * COLUMN_RUNS, 0, stream, run_columns,
+            launch(join_columns_kernel, static_cast<unsigned>(part.n * tiles), COLUMN_SPAN * COLUMN_RUNS, 0, stream, run_columns,
                    plan.runs, 2 * s.channels, tiles, columns);
             MFH_TRY(MFH_CHECK_LAUNCH("group_norm_join_columns", stream));
-            if (dx) {
-                with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
-                    using T = decltype(zero);
-                    launch(apply_backward_kernel<T, decltype(pack)::value, decltype(silu)::value>, groups, SPLIT_THREADS, 0,
-                           stream, static_cast<const T*>(x), static_cast<const T*>(dy), static_cast<T*>(dx), s, block,
-                           runs, b, columns);
-                });
-                MFH_TRY(MFH_CHECK_LAUNCH("group_norm_apply_backward", stream));
-            }
-        }
+            if (!dx) return OK;
+            with_kernel(type, plan.vw, b.act, [&](auto zero, auto pack, auto silu) {
+                using T = decltype(zero);
+                launch(apply_backward_kernel<T, decltype(pack)::value, decltype(silu)::value>, groups, SPLIT_THREADS, 0, stream,
+                       static_cast<const T*>(x) + first * sample, static_cast<const T*>(dy) + first * sample,
+                       static_cast<T*>(dx) + first * sample, part, block, runs, own, columns);
+            });
+            return MFH_CHECK_LAUNCH("group_norm_apply_backward", stream);
+        }));
     }
     if (!parameters) return OK;
-    launch(parameter_grads_kernel, blocks_for(2LL * s.channels, COLUMN_SPAN), COLUMN_SPAN * COLUMN_RUNS, 0, stream, columns, s, b);
+    launch(parameter_grads_kernel, blocks_for(2LL * s.channels, COLUMN_SPAN), COLUMN_SPAN * COLUMN_RUNS, 0, stream, every, s, b);
     return MFH_CHECK_LAUNCH("group_norm_parameter_grads", stream);
 }
 

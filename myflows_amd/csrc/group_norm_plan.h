@@ -33,6 +33,8 @@ struct GroupNormPlan {
 
 constexpr int GROUP_NORM_BLOCK_GROUPS = 256;  // at most, so that a thread a group suffices
 constexpr int GROUP_NORM_SPLIT_THREADS = 256, GROUP_NORM_SPLIT_AHEAD = 4;  // rows that a thread reads ahead
+constexpr int GROUP_NORM_COLUMN_SPAN = 64, GROUP_NORM_COLUMN_RUNS = 16;  // columns and runs of rows of a summing workgroup
+constexpr std::int64_t GROUP_NORM_LAUNCH_THREADS = (1LL << 32) - 1;      // threads of a launch, at most
 
 // Packs that a thread holds of x (and, backward, of dy). 256 threads take up to 8 in turn: 26 single elements each
 // took 9.2 and 13.1 us forward and backward where four times the threads with 7 each took 7.9 and 9.2 (33 x 405 x
@@ -119,6 +121,19 @@ inline GroupNormPlan group_norm_plan(const GroupNormShape& s, int type_size, boo
     plan.rows = static_cast<int>((s.positions + count - 1) / count);
     plan.runs = static_cast<int>((s.positions + static_cast<std::int64_t>(plan.rows) - 1) / plan.rows);
     return plan;
+}
+
+// Samples that one launch of any of a call's kernels takes: a call with more of them goes in slices of this many.
+// A sample takes at most 65536 workgroups of 1024 threads.
+inline std::int64_t group_norm_slice(const GroupNormShape& s, const GroupNormPlan& plan, bool backward) {
+    std::int64_t threads = plan.grid() * plan.threads;
+    if (!plan.held) {
+        const std::int64_t tiles = (2LL * s.channels + GROUP_NORM_COLUMN_SPAN - 1) / GROUP_NORM_COLUMN_SPAN;
+        const std::int64_t join = backward ? tiles * GROUP_NORM_COLUMN_SPAN * GROUP_NORM_COLUMN_RUNS
+                                           : static_cast<std::int64_t>(s.groups) * GROUP_NORM_SPLIT_THREADS;
+        threads = std::max(threads, join);
+    }
+    return GROUP_NORM_LAUNCH_THREADS / threads;
 }
 
 }  // namespace mfh

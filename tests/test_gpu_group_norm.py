@@ -211,6 +211,55 @@ def test_samples_beyond_32_bit_offsets():
     assert bool(((dx[2].float() - want[0].float()).abs() <= 2.0 ** -6 * want[0].float().abs() + 2.0 ** -8).all())
 
 
+def _same_as_alone(x, dy, gamma, beta, groups, parts):
+    """A call's results for these samples against calls on them alone (the same plan, so the same bits); dbeta of a
+    gradient of ones against the number of values, dgamma against the sum of xhat in 64 bits."""
+    n, positions, channels = x.shape
+    y, mean, inv = ops.group_norm_forward(x, gamma, beta, groups)
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(beta)
+    ops.group_norm_backward(x, dy, gamma, beta, mean, inv, x_grad=dx, gamma_grad=dgamma, beta_grad=dbeta, accumulate=(False,) * 3)
+    for part in parts:
+        alone = ops.group_norm_forward(x[part], gamma, beta, groups)
+        for a, b in zip((y, mean, inv), alone):
+            assert torch.equal(a[part], b)
+        want = torch.empty_like(x[part])
+        ops.group_norm_backward(x[part], dy[part], gamma, beta, *alone[1:], x_grad=want, accumulate=(False,) * 3)
+        assert torch.equal(dx[part], want)
+    ops.group_norm_backward(x, torch.ones_like(x), gamma, beta, mean, inv, gamma_grad=dgamma, beta_grad=dbeta, accumulate=(False,) * 3)
+    assert bool((dbeta == n * positions).all())  # whole numbers that float32 holds
+    spread = lambda v: v.repeat_interleave(channels // groups, dim=1).double()  # noqa: E731
+    total, size = 0.0, 0.0
+    for first in range(0, n, 2 ** 24 // channels):
+        rows = slice(first, first + 2 ** 24 // channels)
+        hat = (x[rows].double() - spread(mean[rows])[:, None]) * spread(inv[rows])[:, None]
+        total, size = total + hat.sum(dim=(0, 1)), size + hat.abs().sum(dim=(0, 1))
+    # A column's 16 runs of samples are added in order, then the runs: n / 16 + 20 additions; xhat takes two roundings.
+    assert bool(((dgamma - total).abs() <= (n / 16 + 40) * U * size).all())
+
+
+@gpu
+def test_wide_groups_of_more_samples_than_a_launch_takes():
+    """n C = 2100 x 65536: the join of the column sums takes 2^21 threads a sample, so the samples go in two slices."""
+    print("wide groups, sliced", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(21)
+    x = torch.randn((2100, 1, 65536), generator=g, device="cuda").half()
+    dy = torch.randn((2100, 1, 65536), generator=g, device="cuda").half()
+    gamma, beta = torch.rand(65536, generator=g, device="cuda"), torch.rand(65536, generator=g, device="cuda")
+    _same_as_alone(x, dy, gamma, beta, 1, (slice(0, 3), slice(2045, 2050), slice(2090, 2100)))
+
+
+@gpu
+def test_more_samples_than_a_launch_takes():
+    """2^24 + 8 samples of one position and two channels: a workgroup each would be 2^32 threads and more."""
+    print("many samples, sliced", flush=True)
+    n = 2 ** 24 + 8
+    g = torch.Generator(device="cuda").manual_seed(22)
+    x = torch.randn((n, 1, 2), generator=g, device="cuda").half()
+    dy = torch.randn((n, 1, 2), generator=g, device="cuda").half()
+    gamma, beta = torch.rand(2, generator=g, device="cuda"), torch.rand(2, generator=g, device="cuda")
+    _same_as_alone(x, dy, gamma, beta, 1, (slice(0, 1000), slice(n - 1009, n)))
+
+
 @gpu
 def test_single_gradients_and_unaligned_views():
     x, dy, gamma, beta = _data(4, 300, 64, "float16", 6)

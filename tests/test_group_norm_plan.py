@@ -72,3 +72,51 @@ def test_every_plan_covers_its_sample(tmp_path):
     assert result.returncode == 0, result.stdout
     plans, held = map(int, result.stdout.split())
     assert 0 < held < plans
+
+
+LIMITS = r"""
+#include <cstdio>
+#include "group_norm_plan.h"
+using namespace mfh;
+
+int main() {
+    const int pers[] = {1, 2, 3, 8, 15, 64, 255, 1000, 2048, 4096, 8192, 8193, 16384, 40000, 65535, 65536};
+    const int groups[] = {1, 2, 3, 8, 32, 256, 257, 1024, 8192, 65536};
+    const int positions[] = {1, 2, 20, 405, 4096, 40000, 1000000, 1073741824};
+    const long long samples[] = {1, 7, 300, 2049, 4096, 20000, 65536, 1048576, 16777216, 16777224, 268435456};
+    const long long most = 4294967295LL;  // threads of a launch
+    long sliced = 0;
+    for (int size : {2, 4})
+        for (bool backward : {false, true})
+            for (long long n : samples)
+                for (int per : pers)
+                    for (int g : groups)
+                        for (int at : positions) {
+                            const long long channels = static_cast<long long>(per) * g;
+                            if (channels > 65536 || channels * at > 2147483647LL || n * channels > (1LL << 28)) continue;
+                            const GroupNormShape s{n, at, static_cast<int>(channels), g};
+                            const GroupNormPlan p = group_norm_plan(s, size, backward);
+                            const long long slice = group_norm_slice(s, p, backward), count = slice < n ? slice : n;
+                            // Every launch of a call, as csrc/group_norm.hip issues them.
+                            const long long pass = count * p.blocks * (p.held ? 1 : p.runs) * p.threads;
+                            const long long stats = p.held || backward ? 0 : count * g * 256;
+                            const long long columns = p.held || !backward ? 0 : count * ((2 * channels + 63) / 64) * 1024;
+                            sliced += slice < n;
+                            if (slice >= 1 && pass <= most && stats <= most && columns <= most) continue;
+                            std::printf("n %lld positions %d channels %lld groups %d size %d backward %d: slices of %lld, %lld "
+                                        "%lld %lld threads\n", n, at, channels, g, size, backward, slice, pass, stats, columns);
+                            return 1;
+                        }
+    std::printf("%ld\n", sliced);
+    return 0;
+}
+"""
+
+
+def test_every_launch_of_every_accepted_size_is_one_that_can_be_issued(tmp_path):
+    source = tmp_path / "limits.cpp"
+    source.write_text(LIMITS)
+    subprocess.run(["g++", "-std=c++17", "-O2", "-I", str(CSRC), str(source), "-o", str(tmp_path / "limits")], check=True)
+    result = subprocess.run([str(tmp_path / "limits")], capture_output=True, text=True, timeout=100)
+    assert result.returncode == 0, result.stdout
+    assert int(result.stdout) > 0  # sizes beyond one launch are among them
