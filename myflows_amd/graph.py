@@ -50,7 +50,7 @@ class Node:
 
     def clear_grad(self):
         """Zero gradient of the value's shape (None before the first forward)."""
-        self.grad = None if self.value is None else torch.zeros_like(self.value)
+        self.grad = None if self.value is None else torch.zeros_like(self.value, memory_format=torch.contiguous_format)
 
     def accumulate_grad(self, contribution, *, owned=False):
         """Add a gradient contribution. The first one becomes the gradient: as is when the caller
@@ -71,10 +71,10 @@ class Node:
 
     def grad_buffer(self):
         """(tensor, add): where to write this node's gradient, and whether to add to what is
-        there (True) or overwrite a fresh, uninitialised buffer (False)."""
+        there (True) or overwrite a fresh, uninitialised buffer (False); contiguous, whatever the value's strides."""
         if self.grad is not None:
             return self.grad, True
-        self.grad = torch.empty_like(self.value)
+        self.grad = torch.empty_like(self.value, memory_format=torch.contiguous_format)
         return self.grad, False
 
 

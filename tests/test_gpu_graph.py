@@ -356,3 +356,28 @@ def test_recorded_step_at_the_bench_shape_replays_the_eager_step_bit_for_bit():
     and replayed: the same loss and parameters as the eager step after each of three Adam steps."""
     print("recorded step bs64", flush=True)
     _recorded_against_eager(64, base_width=64, shape=(120, 160), steps=3)
+
+
+@pytest.mark.parametrize("make", ("cross entropy", "group norm", "mse"))
+def test_a_turned_leaf_gets_its_gradient(make):
+    """A leaf whose value is a transposed view: its gradient is that of a contiguous copy."""
+    g = torch.Generator().manual_seed(14)
+    turned = torch.randn((24, 36), generator=g).cuda().t()
+    labels = torch.randint(0, 24, (36,), generator=g).cuda()
+    want = torch.randn((36, 24), generator=g).cuda()
+    grads = []
+    for value in (turned, turned.contiguous()):
+        x = mf.Variable(value, requires_grad=True)
+        if make == "cross entropy":
+            loss = mf.CrossEntropyLoss(x, mf.Variable(labels, requires_grad=False))
+        elif make == "group norm":
+            norm = mf.GroupNorm_Op(x, mf.Variable(torch.ones(24, device="cuda"), requires_grad=False),
+                                   mf.Variable(torch.zeros(24, device="cuda"), requires_grad=False), 4, positions=6)
+            loss = mf.MSELoss(norm, mf.Variable(want, requires_grad=False))
+        else:
+            loss = mf.MSELoss(x, mf.Variable(want, requires_grad=False))
+        graph = mf.Graph(loss)
+        graph.forward()
+        graph.backward()
+        grads.append(x.grad)
+    assert torch.equal(*grads)
