@@ -44,12 +44,6 @@ struct RowStats {
         s *= f;
         m = to;
     }
-    __device__ __forceinline__ void add(float z, float scale) {
-        const float d = z - m;
-        const float e = exp2_of(d * scale);
-        s += e;
-        t += e * fmaxf(d, DIFFERENCE_FLOOR);
-    }
 };
 
 // Keys order logits by (value, lower index first) as unsigned 64-bit numbers; -0 counts as 0. NaN is
