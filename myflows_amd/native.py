@@ -665,7 +665,7 @@ _STREAM_COUNTERS = {}
 LOGIT_COUNTERS = 1025  # MFH_LOGIT_COUNTERS of include/mfhip.h
 
 
-_CAPTURE_BLOCKS = {}  # by (device, stream): the last capture's id, its counters, its workspaces
+_CAPTURE_BLOCKS = {}  # by (device, stream): a capture's id, counters and workspaces, until an eager call asks for its own
 
 
 class _CaptureBlocks:
@@ -678,14 +678,26 @@ class _CaptureBlocks:
 def _capture_blocks(key):
     """The blocks of the stream capture under way on the stream of `key`. A captured graph runs on whatever
     stream replays it, beside other graphs and eager calls of this stream, so it has counters and workspaces of
-    its own, in its memory pool. They are held until the next capture here, so that nothing else of this
-    capture is given them."""
+    its own, in its memory pool. They are held while the capture goes on, so that nothing else of it is given
+    them; then the pool, and with it the graph, alone decides how long their memory is kept."""
     capture = ctypes.c_uint64(0)
     _call("mfh_capture_id", key[1], ctypes.byref(capture))
     blocks = _CAPTURE_BLOCKS.get(key)
     if blocks is None or blocks.id != capture.value:
         blocks = _CAPTURE_BLOCKS[key] = _CaptureBlocks(capture.value)
     return blocks
+
+
+def _drop_ended_captures():
+    """Give up the blocks of the captures that have ended."""
+    capture = ctypes.c_uint64(0)
+    for key, blocks in list(_CAPTURE_BLOCKS.items()):
+        try:
+            _call("mfh_capture_id", key[1], ctypes.byref(capture))
+        except NativeHipError:  # the stream is no longer there
+            capture.value = 0
+        if capture.value != blocks.id:
+            _CAPTURE_BLOCKS.pop(key, None)
 
 
 def _zero_counters():
@@ -702,6 +714,8 @@ def stream_counters():
         if blocks.counters is None:
             blocks.counters = _zero_counters()
         return blocks.counters.data_ptr()
+    if _CAPTURE_BLOCKS:
+        _drop_ended_captures()
     held = _STREAM_COUNTERS.get(key)
     if held is None:
         held = _STREAM_COUNTERS[key] = _zero_counters()
@@ -725,6 +739,8 @@ def byte_workspace(count):
         if not held or held[-1].numel() < count:
             held.append(torch.empty(count, dtype=torch.uint8, device="cuda"))
         return held[-1].data_ptr(), count
+    if _CAPTURE_BLOCKS:
+        _drop_ended_captures()
     return stream_workspace((count + 7) // 8, torch.float64).data_ptr(), count
 
 

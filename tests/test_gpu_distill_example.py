@@ -146,3 +146,31 @@ def test_captured_graphs_share_no_scratch_memory():
                 graph.replay()
         torch.cuda.synchronize()
         check([0, 1])
+
+
+def test_a_capture_keeps_no_memory_beyond_its_graph():
+    """The scratch memory of a capture is given up by the first eager call after it that takes some itself. The graph
+    keeps it for its replays (no later tensor gets it), and without the graph it is free."""
+    g = torch.Generator().manual_seed(7)
+    z = torch.randn((2, 120000), generator=g).cuda()
+    ids, teacher = torch.randint(0, 120000, (2, 8), generator=g).cuda(), torch.randn((2, 8), generator=g).cuda()
+
+    def run():
+        r = logits.log_probs_forward(z, top=64)
+        return [r.entropy, r.log_sum, r.top_log_probs, r.top_ids, logits.distill_loss_forward(z, ids, teacher).scale]
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+        during = len(mf.native._CAPTURE_BLOCKS)
+        assert during >= 1
+    want = run()
+    assert not mf.native._CAPTURE_BLOCKS
+    later = [torch.full((n,), 7, dtype=torch.uint8, device="cuda") for n in (512, 2048, 4100, 8192, 16384, 65536, 2 ** 20) * 8]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, want):
+            assert torch.equal(a, b)
+    assert all(bool((t == 7).all()) for t in later)
