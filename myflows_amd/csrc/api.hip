@@ -370,7 +370,10 @@ MFH_API int mfh_capture_id(std::uint64_t stream, std::uint64_t* id) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     unsigned long long capture = 0;
     const hipError_t rc = hipStreamGetCaptureInfo(as_stream(stream), &status, &capture);
-    if (rc != hipSuccess) return MFH_FAIL(ERR_HIP, std::string("capture info: ") + hipGetErrorString(rc));
+    if (rc != hipSuccess) {
+        (void)hipGetLastError();  // the next launch's check must not find it
+        return MFH_FAIL(ERR_HIP, std::string("capture info: ") + hipGetErrorString(rc));
+    }
     *id = status == hipStreamCaptureStatusActive ? capture + 1 : 0;
     return OK;
 }
