@@ -561,7 +561,7 @@ MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int 
 MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
 
 /* The distillation loss of a student's logits against a teacher's record of `held` (1..256) ids and float32
- * logits a row: with p = softmax(teacher / temperature) over the ids >= 0 and q = softmax(logits / temperature),
+ * logits a row, at a temperature between 2^-63 and 2^63: with p = softmax(teacher / temperature) over the ids >= 0 and q = softmax(logits / temperature),
  *   row_loss = temperature^2 sum p (ln p - ln q[id]),  loss[0] = sum w row_loss / sum w,  loss[1] = 1 / sum w
  * over the rows that count: w = row_weights[r] (optional, else 1), 0 without an id (or with teacher logits of -inf
  * alone). A row that does not count

@@ -1,7 +1,6 @@
 // The C ABI of libmfhip (declared in include/mfhip.h): initialisation, error reporting, argument
 // validation, and the launch sequences behind each entry point. Invalid calls return status 2 with
 // a message naming the reason, before anything is launched.
-#include <cfloat>
 #include <chrono>
 #include <cstdio>
 #include <cstdlib>
@@ -1247,7 +1246,7 @@ MFH_API int mfh_distill_loss(std::uint64_t logits, int type, std::int64_t rows, 
     MFH_TRY(require_ready());
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(held > 0 && held <= DISTILL_HELD_MAX, "number of teacher logits a row out of range");
-    MFH_REQUIRE(temperature > 0.0f && temperature <= FLT_MAX, "the temperature must be positive and finite");
+    MFH_REQUIRE(temperature >= 1.0f / TEMPERATURE_LIMIT && temperature <= TEMPERATURE_LIMIT, "temperature out of range");
     MFH_REQUIRE(loss && (rows == 0 || (logits && ids && teacher && row_loss && weights && stats && targets && counters)),
                 "distillation loss received a null buffer");
     const std::int64_t bytes = distill_workspace(rows, vocab, type);
@@ -1273,7 +1272,7 @@ MFH_API int mfh_distill_loss_backward(std::uint64_t logits, int type, std::int64
     MFH_TRY(require_rows(type, rows, vocab, row_stride));
     MFH_REQUIRE(grad_stride >= vocab, "rows of the gradient must not overlap");
     MFH_REQUIRE(held > 0 && held <= DISTILL_HELD_MAX, "number of teacher logits a row out of range");
-    MFH_REQUIRE(temperature > 0.0f && temperature <= FLT_MAX, "the temperature must be positive and finite");
+    MFH_REQUIRE(temperature >= 1.0f / TEMPERATURE_LIMIT && temperature <= TEMPERATURE_LIMIT, "temperature out of range");
     MFH_REQUIRE(rows == 0 || (logits && ids && targets && stats && weights && loss && seed && grad),
                 "distillation loss backward received a null buffer");
     DistillBackward b{};

@@ -466,6 +466,7 @@ int launch_column_sums(const float* src, float* out, std::int64_t rows, std::int
 // their `wide` flag. A negative token or id is none.
 constexpr int TOP_MAX = 64;           // alternatives of a row
 constexpr int DISTILL_HELD_MAX = 256;  // teacher ids of a row
+constexpr float TEMPERATURE_LIMIT = 0x1p63f;  // and its inverse: T^2 and 1 / T^2 are normal floats
 constexpr std::int64_t LOGIT_ROWS_LIMIT = 1 << 22;  // rows of a call
 constexpr int LOGIT_VOCAB_LIMIT = 1 << 24;          // logits of a row
 constexpr int LOGIT_SPLIT_ROWS = 1024;              // rows that may be split over several workgroups

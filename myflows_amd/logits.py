@@ -225,8 +225,8 @@ def log_probs_backward(logits, tokens, saved, *, log_prob_grad=None, entropy_gra
 
 def _temperature(value):
     value = float(value)
-    if not 0.0 < value < float("inf"):
-        raise ValueError("the temperature must be positive and finite")
+    if not 2.0 ** -63 <= value <= 2.0 ** 63:  # its square and the square's inverse are normal floats
+        raise ValueError("the temperature must lie between 2^-63 and 2^63")
     return value
 
 

@@ -566,6 +566,21 @@ def test_refusals():
     assert b"out of range" in lib.mfh_last_error()
 
 
+@gpu
+def test_temperatures_whose_square_is_no_normal_float_are_refused():
+    """T^2 scales the loss and 1 / T the logits: beyond these the results were NaN."""
+    z, ids, teacher = torch.randn((2, 9), device="cuda"), torch.zeros((2, 1), dtype=torch.int32, device="cuda"), torch.ones((2, 1), device="cuda")
+    for t in (1e-39, 1e-30, 2.0 ** -64, 2.0 ** 64, 1e30, 1e300):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.distill_loss_forward(z, ids, teacher, temperature=t)
+        with pytest.raises(ValueError, match="temperature"):
+            mf.DistillationLoss(mf.Variable(z), mf.Variable(ids), mf.Variable(teacher), temperature=t)
+    for t in (2.0 ** -63, 2.0 ** 63):
+        r = ops.distill_loss_forward(z, ids, teacher, temperature=t)
+        assert not torch.isnan(r.row_loss).any()
+        assert bool(torch.isfinite(ops.distill_loss_backward(z, ids, r, torch.ones((), device="cuda"), temperature=t)).all())
+
+
 def test_host_tensors_are_refused():
     z = torch.zeros((2, 3))
     with pytest.raises(TypeError):
