@@ -100,3 +100,39 @@ def test_work_of_another_library_is_refused_while_a_pass_is_recorded(make_loss):
     optimizer.one_step()
     assert bool(torch.isfinite(loss.value)) and bool(torch.ones(3, device="cuda").add(1.0).eq(2.0).all())
     mf.RecordedStep(_network(lambda out: mf.CrossEntropyLoss(out, _constant(torch.zeros(ROWS, dtype=torch.int64, device="cuda"))))[3]).close()
+
+
+@pytest.mark.parametrize("replayed", (mf.RecordedStep, mf.CapturedStep))
+def test_a_classifier_of_images_trains_on_labels_through_replays(replayed):
+    """ResNet18 with a cross entropy: the eager steps' loss and parameters, bit for bit, with new images and labels
+    before each step."""
+    print("resnet cross entropy", replayed.__name__, flush=True)
+    table = torch.zeros((4, 3), dtype=torch.int64, device="cuda")
+
+    def build():
+        model = mf.ResNet18(output_dim=10, base_width=16, initializer=mf.make_initializer(seed=0), conv_backend="hip_native")
+        x = _constant(torch.ones((4, 3, 48, 64), device="cuda"))
+        loss = mf.CrossEntropyLoss(model(x), _constant(table[:, 1]))
+        return model, x, loss, mf.Adam(mf.Graph(loss, optimize=True), learning_rate=1e-3)
+
+    mf.set_device("cuda")
+    eager_model, eager_x, eager_loss, eager = build()
+    model, x, loss, optimizer = build()
+    step = replayed(optimizer, warmup=1)
+    for _ in range(1 + (replayed is mf.RecordedStep)):  # the passes so far moved the running statistics
+        eager.graph.forward()
+        eager.graph.backward()
+    for i in range(3):
+        g = torch.Generator().manual_seed(60 + i)
+        images = torch.randn((4, 3, 48, 64), generator=g).cuda()
+        eager_x.value.copy_(images)
+        x.value.copy_(images)
+        table.copy_(torch.randint(-1, 10, (4, 3), generator=g))
+        eager.one_step()
+        step.one_step()
+        torch.cuda.synchronize()
+        assert torch.equal(loss.value, eager_loss.value), f"loss of step {i}"
+        eager.update()
+        step.update()
+        for a, b in zip(model.params, eager_model.params):
+            assert torch.equal(a.value, b.value), f"a parameter after step {i}"
