@@ -23,6 +23,7 @@ from . import native
 from .graph import GradientOp
 
 _TYPE_CODES = native.TYPE_CODES
+_WHOLE = {torch.int32: 0, torch.int64: 1}  # whether whole numbers are int64
 TOP_MAX = 64            # alternatives of a row
 DISTILL_HELD_MAX = 256  # teacher ids of a row
 ROWS_LIMIT = 1 << 22
@@ -122,17 +123,15 @@ def _logits(value):
 def _whole(value, shape, name):
     """(tensor, whether it is int64, row stride) of GPU whole numbers of a shape, read in place: one a row at any
     stride, or rows side by side at any row stride (others are copied)."""
-    if not (isinstance(value, torch.Tensor) and value.is_cuda and value.dtype in (torch.int32, torch.int64)):
+    wide = _WHOLE.get(value.dtype) if isinstance(value, torch.Tensor) and value.is_cuda else None
+    if wide is None:
         raise TypeError(f"{name} must be an int32 or int64 torch tensor on the GPU")
     if value.shape != shape:
         raise ValueError(f"{name} must have shape {shape}")
-    value = _side_by_side(value)
-    return value, int(value.dtype is torch.int64), value.stride(0)
-
-
-def _side_by_side(value):
-    """A 2-D tensor's rows side by side: itself, or a copy."""
-    return value.contiguous() if value.ndim == 2 and value.shape[1] > 1 and value.stride(1) != 1 else value
+    strides = value.stride()
+    if strides[-1] != 1 and len(shape) == 2 and shape[1] > 1:
+        return value.contiguous(), wide, shape[1]
+    return value, wide, strides[0]
 
 
 def _row_floats(value, rows, name):
@@ -237,8 +236,8 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
     row_loss = T^2 sum p (ln p - ln q[id]) and loss is its mean by row_weights (1 each without them).
 
     A row without an id, with teacher logits of -inf alone or with weight 0 does not count: its loss and
-    gradient are 0, whatever its logits hold, and without any row that counts the loss is 0. An id beyond the vocabulary makes a counting row
-    NaN."""
+    gradient are 0, whatever its logits hold, and without any row that counts the loss is 0. An id beyond the
+    vocabulary makes a counting row NaN. The temperature lies between 2^-63 and 2^63."""
     logits, code, rows, vocab, stride = _logits(logits)
     temperature = _temperature(temperature)
     if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.ndim != 2 or not 0 < teacher_ids.shape[1] <= DISTILL_HELD_MAX:
@@ -249,7 +248,9 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
         raise TypeError("teacher_logits must be a float32 torch tensor on the GPU")
     if teacher_logits.shape != shape:
         raise ValueError(f"teacher_logits must have shape {shape}")
-    teacher_logits = _side_by_side(teacher_logits)
+    teacher_stride, stride_within = teacher_logits.stride()
+    if stride_within != 1 and shape[1] > 1:
+        teacher_logits, teacher_stride = teacher_logits.contiguous(), shape[1]
     weights_stride = 0
     if row_weights is not None:
         row_weights, weights_stride = _row_floats(row_weights, rows, "row_weights")
@@ -258,7 +259,7 @@ def distill_loss_forward(logits, teacher_ids, teacher_logits, *, temperature=1.0
     scale, row = floats.data_ptr(), 4 * rows
     row_loss = scale + 8
     native._call("mfh_distill_loss", logits.data_ptr(), code, rows, vocab, stride, teacher_ids.data_ptr(), wide,
-                 ids_stride, teacher_logits.data_ptr(), teacher_logits.stride(0), shape[1], native._addr(row_weights),
+                 ids_stride, teacher_logits.data_ptr(), teacher_stride, shape[1], native._addr(row_weights),
                  weights_stride, temperature, row_loss, row_loss + row, row_loss + 2 * row, row_loss + 4 * row, scale,
                  workspace, held, native.stream_counters(), native._stream())
     return DistillLoss(floats, rows, shape[1])

@@ -199,7 +199,9 @@ def _raise_for(status, lib):
 def _call(symbol, *args):
     """Call a status-returning entry point on the current stream; raise on failure."""
     lib = _library()
-    _raise_for(getattr(lib, symbol)(*args), lib)
+    status = getattr(lib, symbol)(*args)
+    if status:
+        _raise_for(status, lib)
 
 
 def _addr(tensor):
