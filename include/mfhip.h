@@ -523,10 +523,10 @@ MFH_API int mfh_adam_step(const mfh_adam_tensor* tensors, int count, float grad_
 /* Element types of the calls below that take more than float: 0 float32, 1 bfloat16, 2 float16. `logits`
  * holds `rows` rows of `vocab` contiguous elements, row_stride elements apart (offsets between rows are 64
  * bits; at most 2^22 rows of at most 2^24 logits). Tokens and ids are int32, or int64 with their flag; a
- * negative one is none. What holds one value a row lies its stride in elements apart (0: one value for all rows), a
- * row of ids or of teacher logits side by side and its rows their stride apart. `counters` are MFH_LOGIT_COUNTERS 32-bit zeros on the device, in which a call counts its
- * workgroups and which it leaves zero: calls that may run at the same time need their own. (mfh_log_probs takes
- * none where it takes no workspace.)
+ * negative one is none. What holds one value a row lies its stride in elements apart (0: one value for all
+ * rows); a row of ids or of teacher logits lies side by side, the rows their stride apart. `counters` are
+ * MFH_LOGIT_COUNTERS 32-bit zeros on the device, in which a call counts its workgroups and which it leaves zero:
+ * calls that may run at the same time need their own. (mfh_log_probs takes none where it takes no workspace.)
  * No counterpart in the reference, whose only loss is the mean squared error. */
 #define MFH_LOGIT_COUNTERS 1025
 
@@ -561,7 +561,8 @@ MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int 
 MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
 
 /* The distillation loss of a student's logits against a teacher's record of `held` (1..256) ids and float32
- * logits a row, at a temperature between 2^-63 and 2^63: with p = softmax(teacher / temperature) over the ids >= 0 and q = softmax(logits / temperature),
+ * logits a row, at a temperature between 2^-63 and 2^63: with p = softmax(teacher / temperature) over the ids >= 0
+ * and q = softmax(logits / temperature),
  *   row_loss = temperature^2 sum p (ln p - ln q[id]),  loss[0] = sum w row_loss / sum w,  loss[1] = 1 / sum w
  * over the rows that count: w = row_weights[r] (optional, else 1), 0 without an id (or with teacher logits of -inf
  * alone). A row that does not count

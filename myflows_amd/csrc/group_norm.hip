@@ -14,7 +14,7 @@
 // Two routes, both bound by HBM (or, in small calls, by latency):
 //   * held: a workgroup reads its groups of a sample into registers, once, forms the sums and writes the
 //     result from there. One launch forward; backward a second one adds the samples' dgamma and dbeta.
-//     64 x 1131 x 64 float32 in 32 groups 12.2 us forward (3.0 TB/s), 13.8 backward (4.0): 256 workgroups, one a
+//     64 x 1131 x 64 float32 in 32 groups 12.8 us forward (2.9 TB/s), 13.8 backward (4.0): 256 workgroups, one a
 //     CU, whose loads, sums and stores follow one another; the split route took 22.5 and 30;
 //   * split: groups that no workgroup holds are summed by runs of positions over many workgroups, the runs
 //     joined, and a last launch reads the activations again. It starts with those read last, which a cache

@@ -73,7 +73,9 @@ struct RowEnd {
 
 // Values that workgroups hand to one another within a launch. A fence over the whole GPU writes back and drops an
 // XCD's cache, which took 200 us for a thousand workgroups; instead these few values are written through to the
-// memory that all XCDs share, and read from there, as relaxed atomics of that scope.
+// memory that all XCDs share, and read from there, as relaxed atomics of that scope. That a written-through value has
+// reached that memory once s_waitcnt has counted its store is how gfx950 works; the language's memory model, which knows
+// fences only, does not promise it.
 template <typename V>
 __device__ __forceinline__ void hand_over(V* to, V value) {
     __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -546,7 +548,10 @@ __device__ __forceinline__ void choose_sets(RowState& state, int logits, int k, 
     if (sets > 1 && last < (k + sets - 1) / sets) --sets;
     state.sets = sets;
     state.each = (k + sets - 1) / sets;
-    // One set of all lanes lets a third more through for 20 alternatives, and many times more for 64.
+    // One set of all lanes lets a third more through for 20 alternatives, and many times more for 64. One set against
+    // places, 4096 rows of 1000 float32 logits: 5 alternatives 7.6 / 12.0 us, 24 9.6 / 12.8, 32 10.1 / 13.4, 48 12.0 / 14.3,
+    // 64 83 / 17.4 (the lists overflow); of 2000 float16 ones 24 11.5 / 15.2, 48 14.8 / 17.2, 64 151 / 20.8. So the rule
+    // stays well clear of where one set fails; between 24 and 48 it gives up 2 to 4 us.
     state.lanes = WAVES == 1 && k <= 24 && logits >= full;
     if (state.lanes) state.each = k;
 }
@@ -875,7 +880,10 @@ __device__ __forceinline__ void mean_of_rows(ValueOf&& value_of, WeightOf&& weig
     out[1] = weight[0] == 0.0 ? 0.0f : static_cast<float>(1.0 / weight[0]);
 }
 
-// The loss of few rows comes from the last workgroup of all, that of many from a launch of its own.
+// The loss of few rows comes from the last workgroup of all, that of many from a launch of its own. Last workgroup
+// against launch: 16 rows of 1000 float32 logits 6.6 / 7.5 us, 64 7.0 / 7.6, 128 8.2 / 7.7, 256 10.5 / 8.1, 1024 27 / 8.2
+// (its 64 threads read the rows' values one round trip after another); of 32768 bfloat16 logits, by 256 threads, 64 rows
+// 8.8 / 9.6, 256 12.5 / 11.2.
 constexpr int MEAN_ROWS = 128;
 
 template <typename T, int THREADS, bool SPLIT>
@@ -902,7 +910,8 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(const T* __restrict__ 
 // ---- the gradients --------------------------------------------------------------------------
 // A workgroup forms GRAD_PACKS packs a thread of one row's gradient: every logit is read once and every
 // gradient written once, p formed again from the row's m and s. Bound by HBM: 1000 x 50021 float32 61 us (6.6
-// TB/s, part of it from the cache), 2048 x 65536 bfloat16 against 64 teacher logits a row 75 (7.2).
+// TB/s, part of it from the cache), 2048 x 65536 bfloat16 against 64 teacher logits a row 75 behind the
+// forward, which leaves part of them in the cache (7.2), and 102 alone.
 constexpr int GRAD_THREADS = 256, GRAD_PACKS = 4;
 
 template <typename T>
@@ -1042,8 +1051,11 @@ bool small_row(int vocab, int type) { return vocab * static_cast<std::int64_t>(t
 // whole -> split: one row of 16384 3.8 / 8.8 -> 3.5 / 8.2 us and of 131072 17.7 / 31.2 -> 4.1 / 10.9, 250 of 16384
 // 4.4 / 11.2 -> 5.9 / 11.9 and of 131072 26.2 / 44.9 -> 23.8 / 29.6. Over 260 sizes from 1 to 500 rows of 12 to
 // 512 KB the rule's choice is 1% slower than the better one, always whole 18%, always split 7%. Then as many runs as
-// bring the workgroups to SPLIT_GROUPS, of at least one tile. All of this follows from the sizes alone, so that
-// results do not depend on the device.
+// bring the workgroups to SPLIT_GROUPS, of at least one tile; from 513 rows on that is one, whatever the estimate says.
+// Whole against two runs a row there, without / with 20 alternatives: 513 x 32771 float16 11.7 / 18.7 -> 12.8 / 26.5 us,
+// 777 x 32771 16.3 / 24.4 -> 17.0 / 33.1, 700 x 131072 bfloat16 37.6 / 50.3 -> 39.5 / 57.9; the best gain was 36.8 -> 32.9
+// (520 x 131072 without alternatives). All of this follows from the sizes alone, so that results do not depend on the
+// device.
 constexpr int SPLIT_GROUPS = 1024, ROW_RATE = 20000, JOIN_TIME = 3, SPLIT_CUS = 256;
 RowSplit row_split(std::int64_t rows, int vocab, int type) {
     if (rows == 0 || small_row(vocab, type)) return {1, vocab};

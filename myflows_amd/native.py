@@ -282,7 +282,8 @@ class _LibraryWritesOnly(TorchDispatchMode):
             writes = any(t.numel() and t.untyped_storage().data_ptr() not in held for t in on_gpu(result))
         if writes:
             raise RuntimeError(f"torch's {func} writes on the GPU while a pass is being recorded: a replay would not "
-                               "repeat it (an operator without a library kernel, or a copy of a tensor that is not contiguous)")
+                               "repeat it (an operator without a library kernel, or a copy of a tensor that is not "
+                               "contiguous)")
         return result
 
 

@@ -99,7 +99,8 @@ def test_work_of_another_library_is_refused_while_a_pass_is_recorded(make_loss):
         mf.RecordedStep(optimizer)
     optimizer.one_step()
     assert bool(torch.isfinite(loss.value)) and bool(torch.ones(3, device="cuda").add(1.0).eq(2.0).all())
-    mf.RecordedStep(_network(lambda out: mf.CrossEntropyLoss(out, _constant(torch.zeros(ROWS, dtype=torch.int64, device="cuda"))))[3]).close()
+    labels = _constant(torch.zeros(ROWS, dtype=torch.int64, device="cuda"))
+    mf.RecordedStep(_network(lambda out: mf.CrossEntropyLoss(out, labels))[3]).close()
 
 
 @pytest.mark.parametrize("replayed", (mf.RecordedStep, mf.CapturedStep))
