@@ -608,6 +608,27 @@ MFH_API int mfh_group_norm_backward(uint64_t x, uint64_t dy, int type, int64_t n
                                     uint64_t x_grad, uint64_t gamma_grad, uint64_t beta_grad, int add_x, int add_gamma,
                                     int add_beta, uint64_t workspace, int64_t workspace_bytes, uint64_t stream);
 
+/* ---- embedding ------------------------------------------------------------------------------- */
+
+/* out[p] = scale * table[ids[p]] for `count` tokens (at most 2^30) and a table of `vocab` rows (at most 2^24) of
+ * `dim` contiguous elements (at most 2^20) of an element type, rows their stride apart; token p lies at
+ * p * ids_stride of int32, or int64 with its flag. A negative token has a row of zeros, one >= vocab a row of NaN.
+ * No counterpart in the reference, whose layers take floats. */
+MFH_API int mfh_embedding(uint64_t table, int type, int64_t vocab, int dim, int64_t table_stride, uint64_t ids,
+                          int ids_int64, int64_t ids_stride, int64_t count, float scale, uint64_t out, int64_t out_stride,
+                          uint64_t stream);
+
+/* Bytes of workspace of mfh_embedding_backward, -1 when the sizes are out of range. */
+MFH_API int64_t mfh_embedding_workspace(int64_t count, int64_t vocab, int dim, int type);
+
+/* table_grad[v] (written, or added to with add) = scale * the sum of the rows grad[p] with ids[p] = v, in rising
+ * order of p and float32, rounded once; grad is of `type`, table_grad (vocab x dim) of the same or float32. Tokens
+ * outside of the table count nowhere. Every row is written; with add, rows that no token names stay as they are. */
+MFH_API int mfh_embedding_backward(uint64_t grad, int type, int64_t count, int dim, int64_t grad_stride, uint64_t ids,
+                                   int ids_int64, int64_t ids_stride, int64_t vocab, float scale, uint64_t table_grad,
+                                   int table_grad_type, int64_t table_grad_stride, int add, uint64_t workspace,
+                                   int64_t workspace_bytes, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

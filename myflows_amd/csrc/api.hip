@@ -110,6 +110,14 @@ int require_rows(int type, std::int64_t rows, int vocab, std::int64_t row_stride
     return OK;
 }
 
+int require_embedding(int type, std::int64_t count, std::int64_t vocab, int dim) {
+    MFH_REQUIRE(type_valid(type), "unknown element type");
+    MFH_REQUIRE(count >= 0 && count <= EMBEDDING_COUNT_LIMIT, "number of tokens out of range");
+    MFH_REQUIRE(vocab > 0 && vocab <= EMBEDDING_VOCAB_LIMIT, "vocabulary out of range");
+    MFH_REQUIRE(dim > 0 && dim <= EMBEDDING_DIM_LIMIT, "length of an embedding out of range");
+    return OK;
+}
+
 int require_group_norm(const GroupNormShape& s, int type, int activation) {
     MFH_REQUIRE(type_valid(type), "unknown element type");
     MFH_REQUIRE(s.n >= 0 && s.positions > 0 && s.channels > 0 && s.groups > 0, "group norm sizes must be positive");
@@ -1338,6 +1346,48 @@ MFH_API int mfh_group_norm_backward(std::uint64_t x, std::uint64_t dy, int type,
     b.workspace = as_ptr<void>(workspace);
     return launch_group_norm_backward(s, type, as_ptr<const void>(x), as_ptr<const void>(dy),
                                       n == 0 ? nullptr : as_ptr<void>(x_grad), b, as_stream(stream));
+}
+
+// ---- embedding ----------------------------------------------------------------------------------
+MFH_API int mfh_embedding(std::uint64_t table, int type, std::int64_t vocab, int dim, std::int64_t table_stride,
+                          std::uint64_t ids, int ids_int64, std::int64_t ids_stride, std::int64_t count, float scale,
+                          std::uint64_t out, std::int64_t out_stride, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_embedding(type, count, vocab, dim));
+    MFH_REQUIRE(table_stride >= dim && out_stride >= dim, "rows must not overlap");
+    MFH_REQUIRE(count == 0 || (table && ids && out), "embedding received a null buffer");
+    EmbeddingLookup f{};
+    f.count = count, f.table_stride = table_stride, f.out_stride = out_stride;
+    f.vocab = static_cast<int>(vocab), f.dim = dim;
+    f.ids = as_ptr<const void>(ids), f.ids_wide = ids_int64 != 0, f.ids_step = ids_stride, f.scale = scale;
+    return launch_embedding(as_ptr<const void>(table), as_ptr<void>(out), type, f, as_stream(stream));
+}
+
+MFH_API std::int64_t mfh_embedding_workspace(std::int64_t count, std::int64_t vocab, int dim, int type) {
+    if (require_embedding(type, count, vocab, dim) != OK) return -1;
+    EmbeddingGradient g{};
+    g.count = count, g.vocab = static_cast<int>(vocab), g.dim = dim;
+    return embedding_workspace(g, type);
+}
+
+MFH_API int mfh_embedding_backward(std::uint64_t grad, int type, std::int64_t count, int dim, std::int64_t grad_stride,
+                                   std::uint64_t ids, int ids_int64, std::int64_t ids_stride, std::int64_t vocab,
+                                   float scale, std::uint64_t table_grad, int table_grad_type,
+                                   std::int64_t table_grad_stride, int add, std::uint64_t workspace,
+                                   std::int64_t workspace_bytes, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_embedding(type, count, vocab, dim));
+    MFH_REQUIRE(table_grad_type == type || table_grad_type == TYPE_F32, "the table's gradient is of the rows' type or float32");
+    MFH_REQUIRE(grad_stride >= dim && table_grad_stride >= dim, "rows must not overlap");
+    MFH_REQUIRE(table_grad && (count == 0 || (grad && ids)), "embedding backward received a null buffer");
+    EmbeddingGradient g{};
+    g.count = count, g.grad_stride = grad_stride, g.out_stride = table_grad_stride;
+    g.vocab = static_cast<int>(vocab), g.dim = dim;
+    g.ids = as_ptr<const void>(ids), g.ids_wide = ids_int64 != 0, g.ids_step = ids_stride;
+    g.scale = scale, g.add = add != 0;
+    MFH_REQUIRE(workspace && workspace_bytes >= embedding_workspace(g, type), "embedding backward workspace too small");
+    return launch_embedding_backward(as_ptr<const void>(grad), type, as_ptr<void>(table_grad), table_grad_type, g,
+                                     as_ptr<void>(workspace), as_stream(stream));
 }
 
 }  // extern "C"

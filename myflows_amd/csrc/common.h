@@ -1,7 +1,7 @@
 // Host-side plumbing shared by the translation units of libmfhip: status codes, the thread-local
 // error text, launch checks, and the internal interfaces through which the C ABI (api.hip) reaches
-// the kernels of conv.hip, gemm.hip, matmul.hip, norm.hip, pointwise.hip, head.hip, logits.hip and
-// group_norm.hip. Kernels index their buffers with int32 offsets (within a row or a sample in the last two);
+// the kernels of conv.hip, gemm.hip, matmul.hip, norm.hip, pointwise.hip, head.hip, logits.hip,
+// group_norm.hip and embedding.hip. Kernels index their buffers with int32 offsets (within a row or a sample in the last three);
 // the entry points reject larger problems before launching anything.
 #pragma once
 
@@ -584,5 +584,36 @@ struct GroupNormBackward {
 };
 int launch_group_norm_backward(const GroupNormShape& s, int type, const void* x, const void* dy, void* dx,
                                const GroupNormBackward& b, hipStream_t stream);
+
+// ---- embedding.hip ----------------------------------------------------------------------------
+constexpr std::int64_t EMBEDDING_COUNT_LIMIT = 1 << 30;  // tokens of a call
+constexpr int EMBEDDING_VOCAB_LIMIT = 1 << 24;
+constexpr int EMBEDDING_DIM_LIMIT = 1 << 20;
+
+// y[p] = scale * table[id[p]] for `count` tokens; token p at p * ids_step of int32, or int64 with ids_wide.
+struct EmbeddingLookup {
+    std::int64_t count, table_stride, out_stride;
+    int vocab, dim;
+    const void* ids;
+    int ids_wide;
+    std::int64_t ids_step;
+    float scale;
+};
+int launch_embedding(const void* table, void* out, int type, const EmbeddingLookup& f, hipStream_t stream);
+
+// The table's gradient from the rows' gradients (count x dim, grad_stride apart).
+struct EmbeddingGradient {
+    std::int64_t count, grad_stride, out_stride;
+    int vocab, dim;
+    const void* ids;
+    int ids_wide;
+    std::int64_t ids_step;
+    float scale;
+    bool add;
+};
+std::int64_t embedding_workspace(const EmbeddingGradient& g, int type);  // bytes
+// out_type is type, or float32.
+int launch_embedding_backward(const void* grad, int type, void* out, int out_type, const EmbeddingGradient& g,
+                              void* workspace, hipStream_t stream);
 
 }  // namespace mfh

@@ -149,6 +149,9 @@ _SIGNATURES = {
     "mfh_group_norm_workspace": ("q", "qiiiii"),
     "mfh_group_norm_forward": ("i", "piqiii" + "ppif" + "ppp" + "pqp"),
     "mfh_group_norm_backward": ("i", "ppiqiii" + "pppp" + "i" + "ppp" + "iii" + "pqp"),
+    "mfh_embedding": ("i", "piqiq" + "piqq" + "fpqp"),
+    "mfh_embedding_workspace": ("q", "qqii"),
+    "mfh_embedding_backward": ("i", "piqiq" + "piqqf" + "piqi" + "pqp"),
 }
 EXPORTS = tuple(_SIGNATURES)
 
@@ -348,6 +351,14 @@ def _device_f32(value, name):
     if not (isinstance(value, torch.Tensor) and value.dtype is _F32 and value.is_cuda):
         raise TypeError(f"{name} must be a float32 torch tensor on the GPU")
     return value if value.is_contiguous() else value.contiguous()
+
+
+def _on_current_device(*tensors):
+    """The calls run on the current device's stream: tensors of another device are refused."""
+    device = _current_device()
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != device:
+            raise ValueError(f"a tensor lies on cuda:{tensor.get_device()}, the current device is cuda:{device}")
 
 
 def _within_int32(**counts):
