@@ -8,6 +8,7 @@
 // bits every time.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
 #include "typed.h"
@@ -23,7 +24,8 @@ constexpr float NOT_A_NUMBER = __builtin_nanf("");
 // ---- lookup -----------------------------------------------------------------------------------
 // Bound by HBM (each row looked up is read and written once) or, for few rows, by the two dependent loads of an
 // id and its row. A workgroup takes a few neighbouring rows, whose packs its threads share whatever the rows'
-// length is; four packs a thread are in flight.
+// length is; four packs a thread are in flight. 65536 rows of 2048 bfloat16: 73 us (7 TB/s, rows of frequent tokens
+// from the caches).
 constexpr int LOOKUP_PACKS = 4;
 
 template <typename T>
@@ -75,54 +77,82 @@ __global__ __launch_bounds__(THREADS) void lookup_kernel(const T* __restrict__ t
 }
 
 // ---- positions by token -----------------------------------------------------------------------
-// order: the positions whose token lies in the table, by (token, position); starts[v]: where token v's begin, and
-// starts[vocab] their number. One launch: a workgroup owns `slice` neighbouring tokens and reads all ids twice
-// (from the caches: the ids are few beside the gradients' rows). Each of its waves takes a sixteenth of the
-// positions: first it counts its own of each token, then, from the sums over the tokens and waves before, it
-// places them in their order. Lanes with the same token find one another by ballots.
+// Token v's slot is (v mod classes) * slice + v / classes, with a power of two of classes: neighbouring tokens,
+// the frequent ones of a vocabulary, lie in different classes. order: the positions whose token lies in the table,
+// by (slot, position); slots: their slots; starts[s]: where slot s's begin, and starts[classes * slice] their number.
+// One launch: a workgroup owns a class and reads all ids (from the caches: the ids are few beside the gradients'
+// rows). Each of its waves takes a sixteenth of the positions, counts its own of each token and lists them in
+// LDS; from the sums over the tokens and waves before it, it then places those it listed in their order, lanes with
+// the same token finding one another by ballots, a token at a time. A wave whose list overflows (a token of every
+// fourth position, say) reads its ids again instead. Bound by the instructions of the walk: 65536 ids of 65536
+// tokens, 1 / k of them the k-th, 21 us (44 with two walks, 370 with neighbouring tokens in one class).
+struct Sorted {
+    int* order;
+    int* slots;
+    int* starts;
+    int classes_log, slice;
+};
+
+__host__ __device__ __forceinline__ int slot_of(const Sorted& s, int token) {
+    return (token & ((1 << s.classes_log) - 1)) * s.slice + (token >> s.classes_log);
+}
+
 // What one lane of a wave wrote to LDS is there for the others' next read: the wave's accesses run in order.
 __device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-template <typename F>
-__device__ __forceinline__ void walk_ids(const EmbeddingGradient& g, int begin, int end, F&& each) {
+// each(whether the token is of the class, its place there, position) for the positions begin .. end - 1, a wave's
+// width at a time; adds this lane's positions of lower classes to `below`.
+template <typename Whole, typename F>
+__device__ __forceinline__ void walk_ids(const EmbeddingGradient& g, const Sorted& s, int begin, int end, int& below, F&& each) {
     constexpr int AHEAD = 8;
-    for (int at = begin + (threadIdx.x & 63); at - static_cast<int>(threadIdx.x & 63) < end; at += 64 * AHEAD) {
-        int id[AHEAD];
+    const int mask = (1 << s.classes_log) - 1, own = blockIdx.x, lane = threadIdx.x & 63;
+    const Whole* ids = static_cast<const Whole*>(g.ids) + (begin + lane) * g.ids_step;
+    for (int base = begin; base < end; base += 64 * AHEAD, ids += 64 * AHEAD * g.ids_step) {
+        Whole id[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) id[k] = base + 64 * k + lane < end ? ids[64 * k * g.ids_step] : -1;
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            const int p = at + 64 * k;
-            const long long v = p < end ? whole_at(g.ids, g.ids_wide, p * g.ids_step) : -1;
-            id[k] = v < 0 || v >= g.vocab ? -1 : static_cast<int>(v);
+            using Unsigned = std::make_unsigned_t<Whole>;
+            const bool there = static_cast<Unsigned>(id[k]) < static_cast<Unsigned>(g.vocab);
+            const int token = static_cast<int>(id[k]), of = token & mask;
+            below += there && of < own;
+            each(there && of == own, token >> s.classes_log, base + 64 * k + lane);
         }
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) each(id[k], at + 64 * k);
     }
 }
 
-__global__ __launch_bounds__(SORT_THREADS) void sort_kernel(EmbeddingGradient g, int slice, int wave_ids, int* __restrict__ order,
-                                                            int* __restrict__ starts) {
+// The lanes below this one that a ballot holds.
+__device__ __forceinline__ int lanes_before(unsigned long long ballot) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(ballot >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(ballot), 0u));
+}
+
+constexpr int LISTED = 512;  // positions of a wave's list
+
+template <typename Whole>
+__global__ __launch_bounds__(SORT_THREADS) void sort_kernel(EmbeddingGradient g, Sorted s, int wave_ids) {
     extern __shared__ int counters[];  // SORT_WAVES x slice
+    __shared__ int positions[SORT_WAVES][LISTED];
+    __shared__ unsigned short tokens[SORT_WAVES][LISTED];
     __shared__ int below_of[SORT_WAVES], sums[SORT_WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, tid = threadIdx.x;
-    const int first = static_cast<int>(blockIdx.x) * slice, tokens = min(slice, g.vocab - first);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, tid = threadIdx.x, slice = s.slice;
     const int begin = static_cast<int>(min(static_cast<std::int64_t>(wave) * wave_ids, g.count));
     const int end = static_cast<int>(min(static_cast<std::int64_t>(wave + 1) * wave_ids, g.count));
     int* const mine = counters + wave * slice;
     for (int i = lane; i < slice; i += 64) mine[i] = 0;
     wave_order();
-    int below = 0;
-    walk_ids(g, begin, end, [&](int id, int) {
-        below += __popcll(__ballot(id >= 0 && id < first));
-        const int local = id - first;
-        const bool here = local >= 0 && local < tokens && id >= 0;
-        for (unsigned long long left = __ballot(here); left;) {
-            const int token = __builtin_amdgcn_readlane(local, __builtin_ctzll(left));
-            const unsigned long long same = __ballot(here && local == token);
-            if (lane == 0) mine[token] += __popcll(same);
-            wave_order();
-            left &= ~same;
+    int below = 0, unused = 0, listed = 0;
+    walk_ids<Whole>(g, s, begin, end, below, [&](bool here, int local, int position) {
+        const unsigned long long all = __ballot(here);
+        if (!all) return;
+        const int at = listed + lanes_before(all);
+        if (here) {
+            atomicAdd(&mine[local], 1);
+            if (at < LISTED) positions[wave][at] = position, tokens[wave][at] = static_cast<unsigned short>(local);
         }
+        listed += __popcll(all);
     });
+    for (int o = 32; o > 0; o /= 2) below += __shfl_xor(below, o);
     if (lane == 0) below_of[wave] = below;
     __syncthreads();
     // The sums over the tokens before, one token a thread.
@@ -139,54 +169,68 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(EmbeddingGradient g,
     __syncthreads();
     for (int w = 0; w < SORT_WAVES; ++w) before += below_of[w] + (w < wave ? sums[w] : 0);
     int at = before + scan - total;
-    if (tid < tokens) starts[first + tid] = at;
-    if (tid == tokens - 1 && first + tokens == g.vocab) starts[g.vocab] = at + total;
-    if (tid < slice)
+    const int first = static_cast<int>(blockIdx.x) * slice;
+    if (tid < slice) {
+        s.starts[first + tid] = at;
+        if (tid == slice - 1 && blockIdx.x == gridDim.x - 1) s.starts[first + slice] = at + total;
         for (int w = 0; w < SORT_WAVES; ++w) {
             const int held = counters[w * slice + tid];
             counters[w * slice + tid] = at;
             at += held;
         }
+    }
     __syncthreads();
-    walk_ids(g, begin, end, [&](int id, int position) {
-        const int local = id - first;
-        const bool here = local >= 0 && local < tokens && id >= 0;
+    const auto place = [&](bool here, int local, int position) {
         for (unsigned long long left = __ballot(here); left;) {
             const int token = __builtin_amdgcn_readlane(local, __builtin_ctzll(left));
             const unsigned long long same = __ballot(here && local == token);
             const int to = mine[token];
-            if (here && local == token)
-                order[to + __builtin_amdgcn_mbcnt_hi(static_cast<unsigned>(same >> 32),
-                                                     __builtin_amdgcn_mbcnt_lo(static_cast<unsigned>(same), 0u))] = position;
+            if (here && local == token) {
+                s.order[to + lanes_before(same)] = position;
+                s.slots[to + lanes_before(same)] = first + token;
+            }
             wave_order();
             if (lane == 0) mine[token] = to + __popcll(same);
             wave_order();
             left &= ~same;
         }
-    });
+    };
+    if (listed > LISTED) {
+        walk_ids<Whole>(g, s, begin, end, unused, place);
+        return;
+    }
+    wave_order();
+    for (int i = 0; i < listed; i += 64) {
+        const bool here = i + lane < listed;
+        const int at = here ? i + lane : 0;
+        place(here, tokens[wave][at], positions[wave][at]);
+    }
 }
 
 // ---- sums -------------------------------------------------------------------------------------
 // A token that comes more often than SumPlan::chunk times is summed in pieces: the sorted positions lie in chunks
 // of that many, and a chunk holds a piece of at most two such tokens, the one that it begins with and the one that
-// it ends with. part_kernel sums the pieces, row_kernel a token's pieces, or the rows of any other token. Bound by
-// HBM: each gradient row is read once, the table's gradient written once.
+// it ends with. sum_kernel's first workgroups sum the pieces, the others the rows of each other token; join_kernel
+// sums the pieces of a token, of which at most one begins in a chunk. Bound by HBM: each gradient row is read once,
+// the table's gradient written once. 65536 rows of 2048 bfloat16 into a table of 65536: 143 us and 9 (3.5 TB/s).
 struct SumPlan {
     int chunk;       // positions of a piece
     int lanes;       // lanes (a power of two) that share a row's packs
     int columns;     // groups of `lanes` packs in a row
     int part_width;  // floats of a piece's row: whole packs
+    unsigned part_blocks;
 };
 
 constexpr int IN_FLIGHT = 8;
 
-// Adds the rows row(i), i = begin .. end - 1, of which each load gives a pack at this lane's columns.
-template <typename P, int N, typename Row>
-__device__ __forceinline__ void add_rows(float (&sum)[N], int begin, int end, Row&& row) {
+// Adds the rows begin .. end - 1 of a lane's columns, IN_FLIGHT of them loaded at a time; load(i) gives row i's pack.
+template <typename P, int N, typename Load>
+__device__ __forceinline__ void add_rows(float (&sum)[N], int begin, int end, Load&& load) {
     for (int i = begin; i < end; i += IN_FLIGHT) {
         P pack[IN_FLIGHT];
 #pragma unroll
-        for (int k = 0; k < IN_FLIGHT; ++k) pack[k] = row(min(i + k, end - 1));
+        for (int k = 0; k < IN_FLIGHT; ++k)
+            if (i + k < end) pack[k] = load(i + k);
 #pragma unroll
         for (int k = 0; k < IN_FLIGHT; ++k) {
             if (i + k >= end) break;
@@ -196,88 +240,123 @@ __device__ __forceinline__ void add_rows(float (&sum)[N], int begin, int end, Ro
     }
 }
 
-template <typename T, int N>
+// Adds the gradient's rows at the sorted positions begin .. end - 1. Where a wave is one row's, it reads 64 of the
+// positions at once.
+template <bool WAVE, typename T, int N>
 __device__ __forceinline__ void add_positions(float (&sum)[N], const T* __restrict__ grad, const EmbeddingGradient& g,
                                               const int* __restrict__ order, int begin, int end, int column) {
     const T* at = grad + column;
-    if (column + N <= g.dim)
-        add_rows<Pack<T, N>>(sum, begin, end, [&](int i) { return load_pack<T, N>(at + order[i] * g.grad_stride); });
-    else
-        add_rows<Pack<T, N>>(sum, begin, end, [&](int i) { return load_part<T, N>(at + order[i] * g.grad_stride, g.dim - column, 0.0f); });
+    const int there = g.dim - column;
+    const auto load = [&](std::int64_t position) {
+        const T* row = at + position * g.grad_stride;
+        return there >= N ? load_pack<T, N>(row) : load_part<T, N>(row, there, 0.0f);
+    };
+    if constexpr (WAVE) {
+        for (int base = begin; base < end; base += 64) {
+            const int here = min(64, end - base);
+            const int held = order[base + min(static_cast<int>(threadIdx.x & 63), here - 1)];
+            add_rows<Pack<T, N>>(sum, 0, here, [&](int i) { return load(__builtin_amdgcn_readlane(held, i)); });
+        }
+    } else {
+        add_rows<Pack<T, N>>(sum, begin, end, [&](int i) { return load(order[i]); });
+    }
 }
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void part_kernel(const T* __restrict__ grad, EmbeddingGradient g, SumPlan plan,
-                                                       const int* __restrict__ order, const int* __restrict__ starts,
-                                                       float* __restrict__ parts) {
+template <typename Out, int N>
+__device__ __forceinline__ void write_sum(Out* __restrict__ out, const float (&sum)[N], const EmbeddingGradient& g, int token,
+                                          int column) {
+    Out* to = out + token * g.out_stride + column;
+    float v[N];
+    if (g.add) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = column + e < g.dim ? static_cast<float>(to[e]) + sum[e] * g.scale : 0.0f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = sum[e] * g.scale;
+    }
+    if (column + N <= g.dim) {
+        store_pack(to, Pack<Out, N>::of(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (column + e < g.dim) to[e] = static_cast<Out>(v[e]);
+    }
+}
+
+// A value that a wave's lanes share, or each lane's own.
+template <bool WAVE>
+__device__ __forceinline__ int shared_by(int value) {
+    return WAVE ? __builtin_amdgcn_readfirstlane(value) : value;
+}
+
+// each(task, the lane's column) for the tasks of the launch's blocks from first_block on: `rows` rows by
+// plan.columns, a wave's lanes sharing 64 / plan.lanes of them.
+template <bool WAVE, int N, typename F>
+__device__ __forceinline__ void walk_tasks(const SumPlan& plan, const EmbeddingGradient& g, unsigned first_block, unsigned blocks,
+                                           std::int64_t rows, F&& each) {
+    const int lanes = WAVE ? 64 : plan.lanes, groups = 64 / lanes, lane = threadIdx.x & 63;
+    const std::int64_t tasks = rows * plan.columns, step = static_cast<std::int64_t>(blocks) * (THREADS / 64) * groups;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    for (std::int64_t task = (static_cast<std::int64_t>(blockIdx.x - first_block) * (THREADS / 64) + wave) * groups +
+                             (WAVE ? 0 : lane / lanes);
+         task < tasks; task += step) {
+        const int row = shared_by<WAVE>(static_cast<int>(task / plan.columns));
+        const int column = (static_cast<int>(task - static_cast<std::int64_t>(row) * plan.columns) * lanes + (WAVE ? lane : lane % lanes)) * N;
+        if (WAVE || column < g.dim) each(row, min(column, g.dim - 1), column < g.dim);
+    }
+}
+
+template <bool WAVE, typename T, typename Out>
+__global__ __launch_bounds__(THREADS) void sum_kernel(const T* __restrict__ grad, Out* __restrict__ out, EmbeddingGradient g,
+                                                      SumPlan plan, Sorted s, float* __restrict__ parts) {
     constexpr int N = 16 / sizeof(T);
-    const int given = starts[g.vocab];
-    const int lane = threadIdx.x & 63, groups = 64 / plan.lanes;
-    const std::int64_t chunks = (static_cast<std::int64_t>(given) + plan.chunk - 1) / plan.chunk, tasks = chunks * plan.columns;
-    const std::int64_t waves = static_cast<std::int64_t>(gridDim.x) * (THREADS / 64) * groups;
-    for (std::int64_t task = (static_cast<std::int64_t>(blockIdx.x) * (THREADS / 64) + threadIdx.x / 64) * groups + lane / plan.lanes;
-         task < tasks; task += waves) {
-        const int chunk = static_cast<int>(task / plan.columns);
-        const int column = (static_cast<int>(task - static_cast<std::int64_t>(chunk) * plan.columns) * plan.lanes + lane % plan.lanes) * N;
-        if (column >= g.dim) continue;
-        const int begin = chunk * plan.chunk, end = min(begin + plan.chunk, given);
+    if (blockIdx.x < plan.part_blocks) {
+        const int given = shared_by<WAVE>(s.starts[s.slice << s.classes_log]);
+        const int chunks = (given + plan.chunk - 1) / plan.chunk;
+        walk_tasks<WAVE, N>(plan, g, 0, plan.part_blocks, chunks, [&](int chunk, int column, bool there) {
+            const int begin = chunk * plan.chunk, end = min(begin + plan.chunk, given);
 #pragma unroll 1
-        for (int last = 0; last < 2; ++last) {
-            const int token = static_cast<int>(whole_at(g.ids, g.ids_wide, order[last ? end - 1 : begin] * g.ids_step));
-            const int from = starts[token], to = starts[token + 1];
-            if (to - from <= plan.chunk || (last && from <= begin)) continue;
-            float sum[N] = {};
-            add_positions<T, N>(sum, grad, g, order, max(from, begin), min(to, end), column);
-            float* out = parts + (2 * static_cast<std::int64_t>(chunk) + last) * plan.part_width + column;
+            for (int last = 0; last < 2; ++last) {
+                const int slot = shared_by<WAVE>(s.slots[last ? end - 1 : begin]);
+                const int from = shared_by<WAVE>(s.starts[slot]), to = shared_by<WAVE>(s.starts[slot + 1]);
+                if (to - from <= plan.chunk || (last && from <= begin)) continue;
+                float sum[N] = {};
+                add_positions<WAVE, T, N>(sum, grad, g, s.order, max(from, begin), min(to, end), column);
+                if (!there) continue;
+                float* to_part = parts + (2 * static_cast<std::int64_t>(chunk) + last) * plan.part_width + column;
 #pragma unroll
-            for (int e = 0; e < N; ++e) out[e] = sum[e];
-        }
+                for (int e = 0; e < N; ++e) to_part[e] = sum[e];
+            }
+        });
+        return;
     }
+    walk_tasks<WAVE, N>(plan, g, plan.part_blocks, gridDim.x - plan.part_blocks, g.vocab, [&](int token, int column, bool there) {
+        const int slot = slot_of(s, token), from = shared_by<WAVE>(s.starts[slot]), to = shared_by<WAVE>(s.starts[slot + 1]);
+        if (to - from > plan.chunk || (from == to && g.add)) return;
+        float sum[N] = {};
+        add_positions<WAVE, T, N>(sum, grad, g, s.order, from, to, column);
+        if (there) write_sum(out, sum, g, token, column);
+    });
 }
 
-template <typename T, typename Out>
-__global__ __launch_bounds__(THREADS) void row_kernel(const T* __restrict__ grad, Out* __restrict__ out, EmbeddingGradient g,
-                                                      SumPlan plan, const int* __restrict__ order,
-                                                      const int* __restrict__ starts, const float* __restrict__ parts) {
-    constexpr int N = 16 / sizeof(T);
-    const int lane = threadIdx.x & 63, groups = 64 / plan.lanes;
-    const std::int64_t tasks = static_cast<std::int64_t>(g.vocab) * plan.columns;
-    const std::int64_t waves = static_cast<std::int64_t>(gridDim.x) * (THREADS / 64) * groups;
-    for (std::int64_t task = (static_cast<std::int64_t>(blockIdx.x) * (THREADS / 64) + threadIdx.x / 64) * groups + lane / plan.lanes;
-         task < tasks; task += waves) {
-        const int token = static_cast<int>(task / plan.columns);
-        const int column = (static_cast<int>(task - static_cast<std::int64_t>(token) * plan.columns) * plan.lanes + lane % plan.lanes) * N;
-        if (column >= g.dim) continue;
-        const int from = starts[token], to = starts[token + 1];
-        if (from == to && g.add) continue;
+template <int N, typename Out>
+__global__ __launch_bounds__(THREADS) void join_kernel(Out* __restrict__ out, EmbeddingGradient g, SumPlan plan, Sorted s,
+                                                       const float* __restrict__ parts) {
+    const int given = s.starts[s.slice << s.classes_log];
+    const int chunks = (given + plan.chunk - 1) / plan.chunk;
+    walk_tasks<false, N>(plan, g, 0, gridDim.x, chunks, [&](int chunk, int column, bool) {
+        const int begin = chunk * plan.chunk, slot = s.slots[min(begin + plan.chunk, given) - 1];
+        const int from = s.starts[slot], to = s.starts[slot + 1];
+        if (to - from <= plan.chunk || from < begin) return;
+        // The first piece ends its chunk, unless it begins there; every further one begins its chunk.
         float sum[N] = {};
-        if (to - from <= plan.chunk) {
-            add_positions<T, N>(sum, grad, g, order, from, to, column);
-        } else {
-            // The first piece ends its chunk, unless it begins there; every further one begins its chunk.
-            const int first = from / plan.chunk, last = (to - 1) / plan.chunk;
-            add_rows<Pack<float, N>>(sum, first, last + 1, [&](int c) {
-                const int slot = c == first && from != first * plan.chunk;
-                return load_pack<float, N>(parts + (2 * static_cast<std::int64_t>(c) + slot) * plan.part_width + column);
-            });
-        }
-        Out* to_row = out + token * g.out_stride + column;
-        float v[N];
-        if (g.add) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = column + e < g.dim ? static_cast<float>(to_row[e]) + sum[e] * g.scale : 0.0f;
-        } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = sum[e] * g.scale;
-        }
-        if (column + N <= g.dim) {
-            store_pack(to_row, Pack<Out, N>::of(v));
-        } else {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (column + e < g.dim) to_row[e] = static_cast<Out>(v[e]);
-        }
-    }
+        add_rows<Pack<float, N>>(sum, chunk, (to - 1) / plan.chunk + 1, [&](int c) {
+            const int ends = c == chunk && from != begin;
+            return load_pack<float, N>(parts + (2 * static_cast<std::int64_t>(c) + ends) * plan.part_width + column);
+        });
+        const int token_class = slot / s.slice;
+        write_sum(out, sum, g, ((slot - token_class * s.slice) << s.classes_log) + token_class, column);
+    });
 }
 
 // Pieces of 64 positions, longer ones for many positions: a piece and the join of all pieces of one token take
@@ -288,24 +367,43 @@ int chunk_of(std::int64_t count) {
     return chunk;
 }
 
+unsigned wave_blocks(std::int64_t rows, const SumPlan& plan) {
+    const std::int64_t groups = 64 / plan.lanes * (THREADS / 64);
+    return static_cast<unsigned>(std::min<std::int64_t>((rows * plan.columns + groups - 1) / groups, BLOCKS_MAX));
+}
+
+std::int64_t chunks_of(const EmbeddingGradient& g, const SumPlan& plan) {
+    return g.count <= plan.chunk ? 0 : (g.count + plan.chunk - 1) / plan.chunk;
+}
+
 SumPlan sum_plan(const EmbeddingGradient& g, int type) {
     const int n = 16 / type_bytes(type), packs = (g.dim + n - 1) / n;
-    SumPlan plan{chunk_of(g.count), 1, 1, packs * n};
+    SumPlan plan{chunk_of(g.count), 1, 1, packs * n, 0};
     while (plan.lanes < 64 && plan.lanes < packs) plan.lanes *= 2;
     plan.columns = (packs + plan.lanes - 1) / plan.lanes;
+    plan.part_blocks = wave_blocks(chunks_of(g, plan), plan);
     return plan;
 }
 
-unsigned wave_blocks(std::int64_t tasks, const SumPlan& plan) {
-    const std::int64_t groups = 64 / plan.lanes * (THREADS / 64);
-    return static_cast<unsigned>(std::min<std::int64_t>((tasks + groups - 1) / groups, BLOCKS_MAX));
+// A class of tokens for every workgroup that the GPU takes at once; more where a class would have over 1024.
+Sorted sorted_layout(const EmbeddingGradient& g) {
+    Sorted s{};
+    while ((1 << s.classes_log) < device_cu_count() && (1 << s.classes_log) < g.vocab) ++s.classes_log;
+    while (g.vocab > static_cast<std::int64_t>(SORT_THREADS) << s.classes_log) ++s.classes_log;
+    s.slice = (g.vocab + (1 << s.classes_log) - 1) >> s.classes_log;
+    return s;
 }
 
 std::int64_t aligned(std::int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-std::int64_t parts_of(const EmbeddingGradient& g, const SumPlan& plan) {
-    return g.count <= plan.chunk ? 0 : 2 * ((g.count + plan.chunk - 1) / plan.chunk);
-}
+// The bytes of order and slots, of starts, and of the pieces.
+struct Workspace {
+    std::int64_t positions, starts, parts;
+    Workspace(const EmbeddingGradient& g, const Sorted& s, const SumPlan& plan)
+        : positions(aligned(4 * g.count)), starts(aligned(4 * ((static_cast<std::int64_t>(s.slice) << s.classes_log) + 1))),
+          parts(4 * 2 * chunks_of(g, plan) * plan.part_width) {}
+    std::int64_t bytes() const { return 2 * positions + starts + parts; }
+};
 
 }  // namespace
 
@@ -325,39 +423,37 @@ int launch_embedding(const void* table, void* out, int type, const EmbeddingLook
 }
 
 std::int64_t embedding_workspace(const EmbeddingGradient& g, int type) {
-    const SumPlan plan = sum_plan(g, type);
-    return aligned(4 * g.count) + aligned(4 * (static_cast<std::int64_t>(g.vocab) + 1)) + 4 * parts_of(g, plan) * plan.part_width;
+    return Workspace(g, sorted_layout(g), sum_plan(g, type)).bytes();
 }
 
 int launch_embedding_backward(const void* grad, int type, void* out, int out_type, const EmbeddingGradient& g,
                               void* workspace, hipStream_t stream) {
     const SumPlan plan = sum_plan(g, type);
+    Sorted s = sorted_layout(g);
+    const Workspace held(g, s, plan);
     char* at = static_cast<char*>(workspace);
-    int* order = reinterpret_cast<int*>(at);
-    int* starts = reinterpret_cast<int*>(at + aligned(4 * g.count));
-    float* parts = reinterpret_cast<float*>(at + aligned(4 * g.count) + aligned(4 * (static_cast<std::int64_t>(g.vocab) + 1)));
-    // A slice of tokens for every workgroup that the GPU takes at once, at least one wave's width of them.
-    int slice = 64;
-    while (slice < SORT_THREADS && static_cast<std::int64_t>(slice) * device_cu_count() < g.vocab) slice *= 2;
-    const std::int64_t wave_ids = ((g.count + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
-    launch(sort_kernel, dim3(blocks_for(g.vocab, slice)), dim3(SORT_THREADS), sizeof(int) * SORT_WAVES * slice, stream, g, slice,
-           static_cast<int>(wave_ids), order, starts);
+    s.order = reinterpret_cast<int*>(at);
+    s.slots = reinterpret_cast<int*>(at + held.positions);
+    s.starts = reinterpret_cast<int*>(at + 2 * held.positions);
+    float* parts = reinterpret_cast<float*>(at + 2 * held.positions + held.starts);
+    const int wave_ids = static_cast<int>(((g.count + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64);
+    launch(g.ids_wide ? sort_kernel<long long> : sort_kernel<int>, dim3(1u << s.classes_log), dim3(SORT_THREADS),
+           sizeof(int) * SORT_WAVES * s.slice, stream, g, s, wave_ids);
     MFH_TRY(MFH_CHECK_LAUNCH("embedding sort", stream));
+    const auto sums = [&](auto element, auto* to) {
+        using T = decltype(element);
+        using Out = std::remove_pointer_t<decltype(to)>;
+        launch(plan.lanes == 64 ? sum_kernel<true, T, Out> : sum_kernel<false, T, Out>,
+               dim3(plan.part_blocks + wave_blocks(g.vocab, plan)), dim3(THREADS), 0, stream, static_cast<const T*>(grad), to, g,
+               plan, s, parts);
+        MFH_TRY(MFH_CHECK_LAUNCH("embedding sums", stream));
+        if (plan.part_blocks == 0) return static_cast<int>(OK);
+        launch(join_kernel<16 / sizeof(T), Out>, dim3(plan.part_blocks), dim3(THREADS), 0, stream, to, g, plan, s, parts);
+        return MFH_CHECK_LAUNCH("embedding join", stream);
+    };
     return with_type(type, [&](auto element) {
         using T = decltype(element);
-        const T* from = static_cast<const T*>(grad);
-        if (parts_of(g, plan)) {
-            launch(part_kernel<T>, dim3(wave_blocks(parts_of(g, plan) / 2 * plan.columns, plan)), dim3(THREADS), 0, stream, from, g,
-                   plan, order, starts, parts);
-            MFH_TRY(MFH_CHECK_LAUNCH("embedding parts", stream));
-        }
-        const dim3 grid(wave_blocks(static_cast<std::int64_t>(g.vocab) * plan.columns, plan));
-        if (out_type == type)
-            launch(row_kernel<T, T>, grid, dim3(THREADS), 0, stream, from, static_cast<T*>(out), g, plan, order, starts, parts);
-        else
-            launch(row_kernel<T, float>, grid, dim3(THREADS), 0, stream, from, static_cast<float*>(out), g, plan, order, starts,
-                   parts);
-        return MFH_CHECK_LAUNCH("embedding rows", stream);
+        return out_type == type ? sums(element, static_cast<T*>(out)) : sums(element, static_cast<float*>(out));
     });
 }
 
