@@ -557,6 +557,23 @@ MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int 
                                    int64_t entropy_grad_stride, uint64_t factor, float scale, uint64_t grad,
                                    int64_t grad_stride, int add, uint64_t stream);
 
+/* out[r][v] = the logits adjusted before a row is answered with. Each part is optional (a null pointer, or 0 of them):
+ *   tokens: `held` (at most 2^20 - 1) of a row's history, its prompt (the first prompt_lengths[r], none without) and
+ *     its answer. A token of the history: z / repetition where z > 0, else z * repetition. One that is n > 0 times
+ *     in the answer: less frequency * n, less presence. The three are one a row, or (with a null pointer) the
+ *     value given for all rows.
+ *   bias_ids, bias_values: `biases` (at most 1024) of a row; values of equal ids add up in their order.
+ *   allowed: bits, bit v % 32 of 32-bit word v / 32 of a row; a token without its bit gets -inf.
+ * Tokens and ids outside of the vocabulary count nowhere. Computed in float32 and rounded once to the logits' type.
+ * out is logits (with the same stride) or shares no memory with them. No counterpart in the reference. */
+MFH_API int mfh_adjust_logits(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
+                              int tokens_int64, int64_t tokens_stride, int held, uint64_t prompt_lengths, int prompt_int64,
+                              int64_t prompt_stride, uint64_t repetition, int64_t repetition_stride, float repetition_all,
+                              uint64_t presence, int64_t presence_stride, float presence_all, uint64_t frequency,
+                              int64_t frequency_stride, float frequency_all, uint64_t bias_ids, int bias_int64,
+                              int64_t bias_ids_stride, uint64_t bias_values, int64_t bias_values_stride, int biases,
+                              uint64_t allowed, int64_t allowed_stride, uint64_t out, int64_t out_stride, uint64_t stream);
+
 /* Bytes of workspace of mfh_distill_loss (0: none), -1 when the sizes are out of range. */
 MFH_API int64_t mfh_distill_workspace(int64_t rows, int vocab, int type);
 

@@ -1239,6 +1239,37 @@ MFH_API int mfh_log_probs_backward(std::uint64_t logits, int type, std::int64_t 
     return launch_log_probs_backward(as_ptr<const void>(logits), as_ptr<void>(grad), type, b, as_stream(stream));
 }
 
+MFH_API int mfh_adjust_logits(std::uint64_t logits, int type, std::int64_t rows, int vocab, std::int64_t row_stride,
+                              std::uint64_t tokens, int tokens_int64, std::int64_t tokens_stride, int held,
+                              std::uint64_t prompt_lengths, int prompt_int64, std::int64_t prompt_stride,
+                              std::uint64_t repetition, std::int64_t repetition_stride, float repetition_all,
+                              std::uint64_t presence, std::int64_t presence_stride, float presence_all,
+                              std::uint64_t frequency, std::int64_t frequency_stride, float frequency_all,
+                              std::uint64_t bias_ids, int bias_int64, std::int64_t bias_ids_stride,
+                              std::uint64_t bias_values, std::int64_t bias_values_stride, int biases,
+                              std::uint64_t allowed, std::int64_t allowed_stride, std::uint64_t out,
+                              std::int64_t out_stride, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_TRY(require_rows(type, rows, vocab, row_stride));
+    MFH_REQUIRE(out_stride >= vocab, "rows of the adjusted logits must not overlap");
+    MFH_REQUIRE(held >= 0 && held <= ADJUST_HELD_LIMIT, "number of tokens a row out of range");
+    MFH_REQUIRE(biases >= 0 && biases <= ADJUST_BIAS_MAX, "number of biases a row out of range");
+    MFH_REQUIRE(rows == 0 || (logits && out && (held == 0 || tokens) && (biases == 0 || (bias_ids && bias_values))),
+                "adjusted logits received a null buffer");
+    MFH_REQUIRE(out != logits || out_stride == row_stride, "in place, the adjusted logits lie as the logits do");
+    AdjustLogits a{};
+    a.rows = rows, a.stride = row_stride, a.out_stride = out_stride, a.vocab = vocab, a.held = held;
+    a.tokens = as_ptr<const void>(tokens), a.tokens_wide = tokens_int64 != 0, a.tokens_step = tokens_stride;
+    a.prompt_lengths = as_ptr<const void>(prompt_lengths), a.prompt_wide = prompt_int64 != 0, a.prompt_step = prompt_stride;
+    a.repetition = as_ptr<const float>(repetition), a.repetition_step = repetition_stride, a.repetition_all = repetition_all;
+    a.presence = as_ptr<const float>(presence), a.presence_step = presence_stride, a.presence_all = presence_all;
+    a.frequency = as_ptr<const float>(frequency), a.frequency_step = frequency_stride, a.frequency_all = frequency_all;
+    a.biases = biases, a.bias_ids = as_ptr<const void>(bias_ids), a.bias_wide = bias_int64 != 0, a.bias_step = bias_ids_stride;
+    a.bias_values = as_ptr<const float>(bias_values), a.bias_values_step = bias_values_stride;
+    a.allowed = as_ptr<const unsigned>(allowed), a.allowed_step = allowed_stride;
+    return launch_adjust(as_ptr<const void>(logits), as_ptr<void>(out), type, a, as_stream(stream));
+}
+
 MFH_API std::int64_t mfh_distill_workspace(std::int64_t rows, int vocab, int type) {
     if (require_rows(type, rows, vocab, vocab) != OK) return -1;
     return distill_workspace(rows, vocab, type);

@@ -1,7 +1,8 @@
 // Host-side plumbing shared by the translation units of libmfhip: status codes, the thread-local
 // error text, launch checks, and the internal interfaces through which the C ABI (api.hip) reaches
 // the kernels of conv.hip, gemm.hip, matmul.hip, norm.hip, pointwise.hip, head.hip, logits.hip,
-// group_norm.hip and embedding.hip. Kernels index their buffers with int32 offsets (within a row or a sample in the last three);
+// adjust.hip, group_norm.hip and embedding.hip. Kernels index their buffers with int32 offsets (within a row or a
+// sample in the last four);
 // the entry points reject larger problems before launching anything.
 #pragma once
 
@@ -550,6 +551,43 @@ int launch_distill_backward(const void* logits, void* grad, int type, const Dist
 // A row's weight is weights[r], else whether tokens[r * tokens_step] >= 0, else 1.
 int launch_row_mean(const float* values, const float* weights, const void* tokens, int tokens_wide, std::int64_t tokens_step,
                     std::int64_t rows, float scale, float* out, hipStream_t stream);
+
+// ---- adjust.hip -------------------------------------------------------------------------------
+constexpr int ADJUST_HELD_LIMIT = (1 << 20) - 1;  // tokens of a row's history
+constexpr int ADJUST_BIAS_MAX = 1024;             // biases of a row
+
+// What rows of logits are adjusted by; each part is optional (null, or 0 of them). Rows of tokens, biases and
+// mask words lie side by side, the rows their step apart; one value a row lies at r * its step.
+struct AdjustLogits {
+    std::int64_t rows, stride, out_stride;
+    int vocab;
+    int held;  // tokens of a row, prompt and answer; a negative one is none
+    const void* tokens;
+    int tokens_wide;
+    std::int64_t tokens_step;
+    const void* prompt_lengths;  // the first tokens of a row that are its prompt; none without
+    int prompt_wide;
+    std::int64_t prompt_step;
+    const float* repetition;  // one a row, else the value for all
+    std::int64_t repetition_step;
+    float repetition_all;
+    const float* presence;
+    std::int64_t presence_step;
+    float presence_all;
+    const float* frequency;
+    std::int64_t frequency_step;
+    float frequency_all;
+    int biases;
+    const void* bias_ids;
+    int bias_wide;
+    std::int64_t bias_step;
+    const float* bias_values;
+    std::int64_t bias_values_step;
+    const unsigned* allowed;  // bit v % 32 of word v / 32: whether token v may be given
+    std::int64_t allowed_step;
+};
+// out may be logits, or share no memory with them.
+int launch_adjust(const void* logits, void* out, int type, const AdjustLogits& a, hipStream_t stream);
 
 // ---- group_norm.hip ---------------------------------------------------------------------------
 // Group norm over the (positions, channels / groups) of each (sample, group) of a channels-last tensor

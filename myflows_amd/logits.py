@@ -2,6 +2,7 @@
 
 * ``log_probs_forward`` / ``log_probs_backward``: the log probabilities of given tokens, each row's
   entropy and its top alternatives, and the gradient of the log probabilities and entropies;
+* ``adjust_logits``: penalties for tokens given before, biases and a grammar's mask, ahead of an answer;
 * ``distill_loss_forward`` / ``distill_loss_backward``: the loss of a student against a teacher's
   recorded top logits (``log_probs_forward`` with ``top`` makes such a record), and its gradient;
 * ``CrossEntropyLoss`` and ``DistillationLoss``: both as losses of a ``Graph``.
@@ -15,6 +16,7 @@ reference has no counterpart: its only loss is the mean squared error.
 
 from __future__ import annotations
 
+import math
 from functools import lru_cache
 
 import torch
@@ -28,6 +30,8 @@ TOP_MAX = 64            # alternatives of a row
 DISTILL_HELD_MAX = 256  # teacher ids of a row
 ROWS_LIMIT = 1 << 22
 VOCAB_LIMIT = 1 << 24
+HELD_LIMIT = (1 << 20) - 1  # tokens of a row's history
+BIAS_MAX = 1024            # biases of a row
 
 
 class LogProbs:
@@ -220,6 +224,99 @@ def log_probs_backward(logits, tokens, saved, *, log_prob_grad=None, entropy_gra
     any stride (an expanded scalar). A row whose gradients are 0 gets 0, whatever its logits hold and its token is; a
     token beyond the vocabulary makes its row NaN where its log_prob_grad is not 0."""
     return _log_probs_gradient(logits, tokens, saved, log_prob_grad, entropy_grad, None, 1.0, out, add)
+
+
+def _penalty(value, rows, name, positive=False):
+    """(tensor or None, stride, value for all rows) of a penalty: a number, or one float32 a row."""
+    if isinstance(value, torch.Tensor):
+        return *_row_floats(value, rows, name), 0.0
+    value = float(value)
+    if not math.isfinite(value) or (positive and value <= 0.0):
+        raise ValueError(f"{name} must be finite{' and positive' if positive else ''}")
+    return None, 0, value
+
+
+def _rows_of(value, rows, name):
+    """A 2-D view of a tensor with a row for each of `rows`; a 1-D one is every row's."""
+    if isinstance(value, torch.Tensor) and value.ndim == 1:
+        value = value.expand(rows, -1)
+    if not isinstance(value, torch.Tensor) or value.ndim != 2 or value.shape[0] != rows:
+        raise ValueError(f"{name} must be a (rows, n) tensor, or an (n,) one for all rows")
+    return value
+
+
+def _span(value):
+    """The addresses from a 2-D tensor's first byte to behind its last one."""
+    last = sum((size - 1) * stride for size, stride in zip(value.shape, value.stride()))
+    return value.data_ptr(), value.data_ptr() + (last + 1) * value.element_size()
+
+
+def adjust_logits(logits, *, tokens=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0,
+                  bias_ids=None, bias_values=None, allowed=None, out=None):
+    """The logits as an answer is drawn from them, of their type; out may be the logits themselves.
+
+    ``tokens`` (rows, held) are a row's history: its prompt, the first ``prompt_lengths[row]`` of them (none
+    without), and its answer so far. A logit z of a token in the history becomes z / repetition where z > 0 and
+    z * repetition else; one that is n > 0 times in the answer then loses frequency * n and presence. Each
+    penalty is a number or one float32 a row. ``bias_values`` are added at ``bias_ids``, equal ids' values in
+    their order. Where ``allowed`` (int32 words; bit v % 32 of word v // 32 is token v's) has no bit, the logit
+    is -inf. Biases and masks are (rows, n), or (n,) for all rows. A negative token or id is none, one beyond the
+    vocabulary counts nowhere. Computed in float32 and rounded once."""
+    logits, code, rows, vocab, stride = _logits(logits)
+    wide = tokens_stride = held = 0
+    if tokens is not None:
+        if not isinstance(tokens, torch.Tensor) or tokens.ndim != 2 or tokens.shape[1] > HELD_LIMIT:
+            raise ValueError(f"tokens must be a (rows, held) tensor with at most {HELD_LIMIT} a row")
+        held = tokens.shape[1]
+        tokens, wide, tokens_stride = _whole(tokens, (rows, held), "tokens")
+    prompt_wide = prompt_stride = 0
+    if prompt_lengths is not None:
+        if tokens is None:
+            raise ValueError("prompt_lengths need their tokens")
+        prompt_lengths, prompt_wide, prompt_stride = _whole(prompt_lengths, (rows,), "prompt_lengths")
+    repetition, repetition_stride, repetition_all = _penalty(repetition, rows, "repetition", positive=True)
+    presence, presence_stride, presence_all = _penalty(presence, rows, "presence")
+    frequency, frequency_stride, frequency_all = _penalty(frequency, rows, "frequency")
+    if (bias_ids is None) != (bias_values is None):
+        raise ValueError("bias_ids and bias_values go together")
+    bias_wide = bias_ids_stride = bias_values_stride = biases = 0
+    if bias_ids is not None:
+        bias_ids, bias_values = _rows_of(bias_ids, rows, "bias_ids"), _rows_of(bias_values, rows, "bias_values")
+        biases = bias_ids.shape[1]
+        if biases > BIAS_MAX:
+            raise ValueError(f"a row takes at most {BIAS_MAX} biases")
+        bias_ids, bias_wide, bias_ids_stride = _whole(bias_ids, (rows, biases), "bias_ids")
+        if not (bias_values.is_cuda and bias_values.dtype is torch.float32):
+            raise TypeError("bias_values must be a float32 torch tensor on the GPU")
+        if bias_values.shape != bias_ids.shape:
+            raise ValueError("bias_values must have the shape of bias_ids")
+        if bias_values.stride(1) != 1 and biases > 1:
+            bias_values = bias_values.contiguous()
+        bias_values_stride = bias_values.stride(0)
+    allowed_stride = 0
+    if allowed is not None:
+        allowed = _rows_of(allowed, rows, "allowed")
+        if not (allowed.is_cuda and allowed.dtype is torch.int32):
+            raise TypeError("allowed must be an int32 torch tensor on the GPU")
+        if allowed.shape[1] < (vocab + 31) // 32:
+            raise ValueError(f"allowed must have {(vocab + 31) // 32} words a row")
+        if allowed.stride(1) != 1 and allowed.shape[1] > 1:
+            allowed = allowed.contiguous()
+        allowed_stride = allowed.stride(0)
+    out, out_stride = _gradient(out, False, logits)
+    if rows and (out.data_ptr() != logits.data_ptr() or out_stride != stride):
+        (first, end), (out_first, out_end) = _span(logits), _span(out)
+        if first < out_end and out_first < end:
+            raise ValueError("out must be the logits themselves or share no memory with them")
+    native._on_current_device(logits, tokens, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
+                              allowed, out)
+    native._call("mfh_adjust_logits", logits.data_ptr(), code, rows, vocab, stride, native._addr(tokens), wide,
+                 tokens_stride, held, native._addr(prompt_lengths), prompt_wide, prompt_stride, native._addr(repetition),
+                 repetition_stride, repetition_all, native._addr(presence), presence_stride, presence_all,
+                 native._addr(frequency), frequency_stride, frequency_all, native._addr(bias_ids), bias_wide,
+                 bias_ids_stride, native._addr(bias_values), bias_values_stride, biases, native._addr(allowed),
+                 allowed_stride, out.data_ptr(), out_stride, native._stream())
+    return out
 
 
 def _temperature(value):

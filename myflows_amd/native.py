@@ -142,6 +142,7 @@ _SIGNATURES = {
     "mfh_log_probs_workspace": ("q", "qiii"),
     "mfh_log_probs": ("i", "piqiq" + "piq" + "pppp" + "ipp" + "pqpp"),
     "mfh_log_probs_backward": ("i", "piqiq" + "piq" + "pp" + "pqpq" + "pf" + "pqi" + "p"),
+    "mfh_adjust_logits": ("i", "piqiq" + "piqi" + "piq" + "pqf" * 3 + "piqpqi" + "pq" + "pqp"),
     "mfh_distill_workspace": ("q", "qii"),
     "mfh_distill_loss": ("i", "piqiq" + "piqpqi" + "pqf" + "ppppp" + "pqpp"),
     "mfh_distill_loss_backward": ("i", "piqiq" + "piqi" + "ppppp" + "f" + "pqi" + "p"),
