@@ -245,10 +245,14 @@ def _rows_of(value, rows, name):
     return value
 
 
-def _span(value):
-    """The addresses from a 2-D tensor's first byte to behind its last one."""
-    last = sum((size - 1) * stride for size, stride in zip(value.shape, value.stride()))
-    return value.data_ptr(), value.data_ptr() + (last + 1) * value.element_size()
+def _disjoint(one, other, stride, other_stride):
+    """Whether two tensors of one shape and type, of contiguous rows at these strides, share no memory: one lies
+    behind the other, or their rows lie side by side."""
+    rows, length = one.shape
+    apart = (other.data_ptr() - one.data_ptr()) // one.element_size()
+    if apart >= (rows - 1) * stride + length or -apart >= (rows - 1) * other_stride + length:
+        return True
+    return stride == other_stride and length <= apart % stride <= stride - length
 
 
 def adjust_logits(logits, *, tokens=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0,
@@ -305,8 +309,7 @@ def adjust_logits(logits, *, tokens=None, prompt_lengths=None, repetition=1.0, p
         allowed_stride = allowed.stride(0)
     out, out_stride = _gradient(out, False, logits)
     if rows and (out.data_ptr() != logits.data_ptr() or out_stride != stride):
-        (first, end), (out_first, out_end) = _span(logits), _span(out)
-        if first < out_end and out_first < end:
+        if not _disjoint(logits, out, stride, out_stride):
             raise ValueError("out must be the logits themselves or share no memory with them")
     native._on_current_device(logits, tokens, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
                               allowed, out)

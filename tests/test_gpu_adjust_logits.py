@@ -247,3 +247,8 @@ def test_refusals():
         ops.adjust_logits(held[:200].view(4, 50), out=held[50:250].view(4, 50))
     with pytest.raises(ValueError, match="share no memory"):
         ops.adjust_logits(held[:400].view(4, 100)[:, :50], out=held[:200].view(4, 50))
+    side = torch.randn((4, 110), device="cuda")
+    got = ops.adjust_logits(side[:, 3:53], presence=1.0, tokens=tokens, out=side[:, 53:103])  # rows side by side
+    _check(got, side[:, 3:53], tokens, presence=1.0)
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.adjust_logits(side[:, 3:53], out=side[:, 52:102])
