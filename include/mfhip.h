@@ -646,6 +646,27 @@ MFH_API int mfh_embedding_backward(uint64_t grad, int type, int64_t count, int d
                                    int table_grad_type, int64_t table_grad_stride, int add, uint64_t workspace,
                                    int64_t workspace_bytes, uint64_t stream);
 
+/* ---- orthogonal matrices --------------------------------------------------------------------- */
+
+/* One matrix of mfh_orthogonalize: rows x cols elements (sides of at most 2^20, at most 2^31 - 1 elements), rows of
+ * contiguous elements their stride apart. out may be in; it overlaps no other matrix of the call. */
+typedef struct mfh_orthogonal_matrix {
+    uint64_t in, out;
+    int64_t in_stride, out_stride;
+    int32_t rows, cols;
+} mfh_orthogonal_matrix;
+
+/* Bytes of workspace of mfh_orthogonalize, -1 when a size is out of range. */
+MFH_API int64_t mfh_orthogonalize_workspace(const mfh_orthogonal_matrix* matrices, int count);
+
+/* out = the matrix M of an element type taken through `steps` (1..64) Newton-Schulz steps: with X = M / (|M| + eps)
+ * (the Frobenius norm) and the shorter side as rows, X = a X + (b G + c G G) X with G = X X^T, so that each singular
+ * value x becomes x (a + b x^2 + c x^4). Formed to the precision of float32 products and rounded once. The
+ * polynomial must keep the values from 0 to 1 below 3.5, and a + b x^2 + c x^4 below 15, at every step. The table is
+ * host memory, read during the call. No counterpart in the reference. */
+MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, int type, int steps, float a, float b, float c,
+                              float eps, uint64_t workspace, int64_t workspace_bytes, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,7 +6,7 @@ The public names mirror the reference package (``Variable``, ``Graph``, ``Conv2D
 (``conv_backend=`` for ResNet18); the kernels live in ``libmfhip.so`` (``native`` and ``fused``).
 """
 
-from . import embedding, fused, group_norm, logits, native
+from . import embedding, fused, group_norm, logits, native, orthogonal
 from .capture import CapturedStep, RecordedStep
 from .device import cuda_available, get_device, set_device
 from .embedding import Embedding, Embedding_Op
@@ -31,5 +31,5 @@ __all__ = [
     "MSELoss", "MaxPool2d", "MaxPool2d_Op", "NATIVE_BACKENDS", "Node", "Optimizer", "ParameterGroups",
     "RecordedStep", "ReLU", "ResNet18", "Variable",
     "apply_graph_optimizations", "cuda_available", "embedding", "fused", "get_device", "group_norm", "logits",
-    "make_initializer", "native", "set_device",
+    "make_initializer", "native", "orthogonal", "set_device",
 ]

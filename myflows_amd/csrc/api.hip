@@ -1421,4 +1421,41 @@ MFH_API int mfh_embedding_backward(std::uint64_t grad, int type, std::int64_t co
                                      as_ptr<void>(workspace), as_stream(stream));
 }
 
+// ---- orthogonal matrices --------------------------------------------------------------------------
+static_assert(sizeof(mfh_orthogonal_matrix) == sizeof(OrthogonalMatrix), "the C table is read as OrthogonalMatrix rows");
+
+static int require_orthogonal(const mfh_orthogonal_matrix* matrices, int count, std::vector<OrthogonalMatrix>& table) {
+    MFH_REQUIRE(count >= 0 && (count == 0 || matrices), "orthogonalisation received a null table");
+    for (int i = 0; i < count; ++i) {
+        const mfh_orthogonal_matrix& m = matrices[i];
+        MFH_REQUIRE(m.rows > 0 && m.cols > 0 && m.rows <= ORTHOGONAL_SIDE_LIMIT && m.cols <= ORTHOGONAL_SIDE_LIMIT &&
+                        fits_index(static_cast<std::int64_t>(m.rows) * m.cols),
+                    "sides of a matrix out of range");
+        MFH_REQUIRE(m.in_stride >= m.cols && m.out_stride >= m.cols, "rows of a matrix must not overlap");
+        table.push_back({as_ptr<const void>(m.in), as_ptr<void>(m.out), m.in_stride, m.out_stride, m.rows, m.cols});
+    }
+    return OK;
+}
+
+MFH_API std::int64_t mfh_orthogonalize_workspace(const mfh_orthogonal_matrix* matrices, int count) {
+    std::vector<OrthogonalMatrix> table;
+    if (require_orthogonal(matrices, count, table) != OK) return -1;
+    return orthogonal_workspace(table.data(), count);
+}
+
+MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, int type, int steps, float a, float b, float c,
+                              float eps, std::uint64_t workspace, std::int64_t workspace_bytes, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_REQUIRE(type_valid(type), "unknown element type");
+    MFH_REQUIRE(steps > 0 && steps <= ORTHOGONAL_STEPS_MAX, "number of steps out of range");
+    MFH_REQUIRE(eps >= 0.0f, "eps must not be negative");
+    std::vector<OrthogonalMatrix> table;
+    MFH_TRY(require_orthogonal(matrices, count, table));
+    for (const OrthogonalMatrix& m : table) MFH_REQUIRE(m.in && m.out, "orthogonalisation received a null buffer");
+    MFH_REQUIRE(count == 0 || (workspace && workspace_bytes >= orthogonal_workspace(table.data(), count)),
+                "orthogonalisation workspace too small");
+    return launch_orthogonal(table.data(), count, type, OrthogonalSteps{steps, a, b, c, eps}, as_ptr<void>(workspace),
+                             as_stream(stream));
+}
+
 }  // extern "C"

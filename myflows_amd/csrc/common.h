@@ -1,7 +1,7 @@
 // Host-side plumbing shared by the translation units of libmfhip: status codes, the thread-local
 // error text, launch checks, and the internal interfaces through which the C ABI (api.hip) reaches
 // the kernels of conv.hip, gemm.hip, matmul.hip, norm.hip, pointwise.hip, head.hip, logits.hip,
-// adjust.hip, group_norm.hip and embedding.hip. Kernels index their buffers with int32 offsets (within a row or a
+// adjust.hip, group_norm.hip, embedding.hip and orthogonal.hip. Kernels index their buffers with int32 offsets (within a row or a
 // sample in the last four);
 // the entry points reject larger problems before launching anything.
 #pragma once
@@ -653,5 +653,23 @@ std::int64_t embedding_workspace(const EmbeddingGradient& g, int type);  // byte
 // out_type is type, or float32.
 int launch_embedding_backward(const void* grad, int type, void* out, int out_type, const EmbeddingGradient& g,
                               void* workspace, hipStream_t stream);
+
+// ---- orthogonal.hip ---------------------------------------------------------------------------
+constexpr int ORTHOGONAL_SIDE_LIMIT = 1 << 20;
+constexpr int ORTHOGONAL_STEPS_MAX = 64;
+
+struct OrthogonalMatrix {  // out has the shape and type of in, and may be in
+    const void* in;
+    void* out;
+    std::int64_t in_stride, out_stride;
+    int rows, cols;
+};
+struct OrthogonalSteps {
+    int steps;
+    float a, b, c, eps;
+};
+std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count);  // bytes
+int launch_orthogonal(const OrthogonalMatrix* matrices, int count, int type, const OrthogonalSteps& o, void* workspace,
+                      hipStream_t stream);
 
 }  // namespace mfh

@@ -1,0 +1,438 @@
+// Matrices orthogonalised by Newton-Schulz products: with X = M / (|M| + eps) (|M| the Frobenius norm, X with the
+// shorter side s as rows and the longer l as columns), `steps` times
+//   G = X X^T,  B = b G + c G G,  X = a X + B X,
+// after which X's singular values lie near 1 (each went through x (a + b x^2 + c x^4)).
+//
+// Precision. The polynomial raises small singular values by up to a each step (485 times in five), and with them
+// whatever error the products have: in 16-bit products it would be a tenth of the result. So every matrix is held as
+// the sum of two float16 values, hi + lo, 22 bits, and a product is hi hi + hi lo + lo hi on the matrix cores, added in
+// float32 (the splitting of single-precision products that Ootomo and Yokota published in 2022): as near to the
+// definition as float32 products, at three times the cost of one float16 product instead of the sixteen that the
+// matrix cores' float32 rate is below it. X and B are at most a few: values are held 2^12 times as large,
+// which keeps hi out of float16's subnormals and lo's steps below 2^-36.
+//
+// Layout. A matrix lies in rows padded to whole tiles, zeros there; a row's 32 neighbouring values are 64 bytes of
+// hi and 64 of lo, so that one step of a product reads a cache line of each row. Every product is of the form A B^T
+// with rows of both read along k: X is kept as X and as X^T. Symmetric products form the tiles on and below the
+// diagonal and write them to both places.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <vector>
+
+#include "common.h"
+#include "typed.h"
+
+namespace mfh {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(1))) void GlobalBytes;
+typedef __attribute__((address_space(3))) void LocalBytes;
+
+constexpr int THREADS = 256;
+constexpr int K_STEP = 32;          // values of a row in one step: 128 bytes, hi and lo
+constexpr int ROW_STEP = 2 * K_STEP;  // halves
+constexpr int LARGE = 128, SMALL = 64;  // sides of a workgroup's tile
+constexpr int SCALE_LOG = 12;
+constexpr float SCALE = 1 << SCALE_LOG, UNSCALE = 1.0f / SCALE;
+constexpr int GROUP = 32;  // matrices of a launch: their descriptors travel in its arguments
+constexpr int XCD_COUNT = 8;
+
+// out = alpha A B^T + beta add, or the caller's matrix in its type.
+struct Product {
+    const _Float16* a;  // rows of A and of B, ksteps * ROW_STEP halves each
+    const _Float16* b;
+    const _Float16* add_t;  // optional, transposed (a symmetric one is its own)
+    _Float16* out;          // optional
+    _Float16* out_t;        // optional, transposed
+    void* final;
+    std::int64_t final_stride;
+    float alpha, beta;
+    int ksteps, m_tiles, n_tiles;  // tiles of its own side
+    int rows, cols;                // of the caller's matrix, the shorter side as rows
+    bool symmetric, small, tall;   // tall: the caller's matrix is the transposed result
+};
+
+struct ProductGroup {
+    Product p[GROUP];
+    int first_unit[GROUP + 1];
+    int count;
+};
+static_assert(sizeof(ProductGroup) <= 4096, "descriptors must fit the kernel arguments");
+
+// Copies ROWS rows of one step to LDS, 16 bytes a lane. A row's eight 16-byte parts are stored in the order
+// part ^ (row % 8), so that neighbouring rows' equal parts lie in other banks.
+template <int ROWS>
+__device__ __forceinline__ void stage_rows(const _Float16* __restrict__ rows, std::int64_t pitch, int step, _Float16* lds) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    constexpr int EACH = ROWS / 8 / (THREADS / 64);  // instructions of a wave, 8 rows each
+    const _Float16* from = rows + (wave * EACH * 8 + lane / 8) * pitch + step * ROW_STEP + ((lane & 7) ^ (lane / 8)) * 8;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        __builtin_amdgcn_global_load_lds((const GlobalBytes*)(from + i * 8 * pitch), (LocalBytes*)(lds + (wave * EACH + i) * 8 * ROW_STEP),
+                                         16, 0, 0);
+}
+
+// The lane's 8 values of a 32 x 16 operand at LDS row `row` (its own lane % 32 included): part p of hi, or of lo.
+__device__ __forceinline__ half8 operand(const _Float16* lds, int row, int part) {
+    return *reinterpret_cast<const half8*>(lds + row * ROW_STEP + (part ^ (row & 7)) * 8);
+}
+
+// Value and place of the split halves of 4 values, neighbours along i, in row j of a matrix of `pitch` halves a row.
+__device__ __forceinline__ void write_four(_Float16* to, std::int64_t row, std::int64_t pitch, int i, const float (&v)[4]) {
+    half4 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        hi[k] = static_cast<_Float16>(v[k]);
+        lo[k] = static_cast<_Float16>(v[k] - static_cast<float>(hi[k]));
+    }
+    _Float16* at = to + row * pitch + i / K_STEP * ROW_STEP + i % K_STEP;
+    *reinterpret_cast<half4*>(at) = hi;
+    *reinterpret_cast<half4*>(at + K_STEP) = lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_final(const Product& p, int i, int j, float v) {
+    if (i >= p.rows || j >= p.cols) return;
+    static_cast<T*>(p.final)[(p.tall ? j * p.final_stride + i : i * p.final_stride + j)] = static_cast<T>(v);
+}
+
+// One 32 x 32 piece of a tile: this lane's column j and rows i0 + 8 q + 4 (lane / 32) + 0 .. 3.
+template <typename T>
+__device__ __forceinline__ void write_piece(const Product& p, const float16v& sum, int i0, int j0, int side, bool mirrored) {
+    const int lane = threadIdx.x & 63, j = j0 + (lane & 31);
+    const std::int64_t pitch = static_cast<std::int64_t>(p.n_tiles) * side * 2, pitch_t = static_cast<std::int64_t>(p.m_tiles) * side * 2;
+    const float alpha = p.alpha * UNSCALE;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int i = i0 + 8 * q + 4 * (lane / 32);
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = sum[4 * q + k] * alpha;
+        if (p.add_t) {
+            const _Float16* at = p.add_t + j * pitch_t + i / K_STEP * ROW_STEP + i % K_STEP;
+            const half4 hi = *reinterpret_cast<const half4*>(at), lo = *reinterpret_cast<const half4*>(at + K_STEP);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += p.beta * (static_cast<float>(hi[k]) + static_cast<float>(lo[k]));
+        }
+        if (p.final) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) write_final<T>(p, i + k, j, v[k] * UNSCALE);
+            continue;
+        }
+        if (p.out_t) write_four(p.out_t, j, pitch_t, i, v);
+        if (!mirrored) continue;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const _Float16 hi = static_cast<_Float16>(v[k]);
+            _Float16* at = p.out + (i + k) * pitch + j / K_STEP * ROW_STEP + j % K_STEP;
+            at[0] = hi;
+            at[K_STEP] = static_cast<_Float16>(v[k] - static_cast<float>(hi));
+        }
+    }
+}
+
+// One SIDE x SIDE tile by four waves of SIDE / 2 x SIDE / 2, two steps in LDS: while a step is multiplied the next
+// one's rows are on their way.
+template <int SIDE, typename T>
+__device__ __forceinline__ void tile_product(const Product& p, int tile_i, int tile_j, _Float16* lds) {
+    constexpr int PIECES = SIDE / 64, STAGE = SIDE * ROW_STEP;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wave_i = wave / 2 * (SIDE / 2), wave_j = wave % 2 * (SIDE / 2);
+    const std::int64_t pitch = static_cast<std::int64_t>(p.ksteps) * ROW_STEP;
+    const _Float16* a = p.a + static_cast<std::int64_t>(tile_i) * SIDE * pitch;
+    const _Float16* b = p.b + static_cast<std::int64_t>(tile_j) * SIDE * pitch;
+    float16v sum[PIECES][PIECES] = {};
+    stage_rows<SIDE>(a, pitch, 0, lds);
+    stage_rows<SIDE>(b, pitch, 0, lds + STAGE);
+    for (int step = 0; step < p.ksteps; ++step) {
+        const _Float16* at = lds + (step & 1) * 2 * STAGE;
+        // This wave's rows of the step have arrived, and with the barrier everyone's; and everyone has read the step before.
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        __syncthreads();
+        half8 x[2][PIECES][2], y[2][PIECES][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int piece = 0; piece < PIECES; ++piece)
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    x[k][piece][part] = operand(at, wave_i + piece * 32 + (lane & 31), part * 4 + k * 2 + lane / 32);
+                    y[k][piece][part] = operand(at + STAGE, wave_j + piece * 32 + (lane & 31), part * 4 + k * 2 + lane / 32);
+                }
+        if (step + 1 < p.ksteps) {
+            _Float16* next = lds + ((step + 1) & 1) * 2 * STAGE;
+            stage_rows<SIDE>(a, pitch, step + 1, next);
+            stage_rows<SIDE>(b, pitch, step + 1, next + STAGE);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int term = 0; term < 3; ++term)
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                    for (int j = 0; j < PIECES; ++j)
+                        sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[k][i][term == 2], y[k][j][term == 1], sum[i][j], 0, 0, 0);
+    }
+    const bool mirrored = p.out && (!p.symmetric || tile_i != tile_j);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j)
+            write_piece<T>(p, sum[i][j], tile_i * SIDE + wave_i + i * 32, tile_j * SIDE + wave_j + j * 32, SIDE, mirrored);
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS, 2) void product_kernel(ProductGroup group) {
+    __shared__ __align__(1024) _Float16 lds[4 * LARGE * ROW_STEP];
+    // Neighbouring units go to the same die: workgroups are dealt to the dies in turn.
+    const int units = gridDim.x, die = blockIdx.x % XCD_COUNT, share = units / XCD_COUNT, more = units % XCD_COUNT;
+    const int unit = die * share + min(die, more) + blockIdx.x / XCD_COUNT;
+    int item = 0;
+    while (unit >= group.first_unit[item + 1]) ++item;
+    const Product& p = group.p[item];
+    const int t = unit - group.first_unit[item];
+    int i, j;
+    if (p.symmetric) {  // the tiles on and below the diagonal, row by row
+        i = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+        while (i * (i + 1) / 2 > t) --i;
+        while ((i + 1) * (i + 2) / 2 <= t) ++i;
+        j = t - i * (i + 1) / 2;
+    } else {  // columns of eight tiles, so that a die's tiles share rows of both operands
+        const int width = 8 * p.n_tiles, first = t / width * 8, rows = min(8, p.m_tiles - first), within = t % width;
+        i = first + within % rows, j = within / rows;
+    }
+    if (p.small) tile_product<SMALL, T>(p, i, j, lds);
+    else tile_product<LARGE, T>(p, i, j, lds);
+}
+
+// ---- before the products ----------------------------------------------------------------------
+struct Source {
+    const void* in;
+    std::int64_t stride;
+    _Float16* same;     // the split matrix as the caller has it, and transposed
+    _Float16* across;
+    double* squares;    // sums of squares, one a workgroup of squares_kernel
+    int rows, cols, padded_rows, padded_cols;
+    FastDiv columns;
+};
+
+struct SourceGroup {
+    Source s[GROUP];
+    int first_block[GROUP + 1];
+    int square_blocks[GROUP];
+    int count;
+    float eps;
+};
+static_assert(sizeof(SourceGroup) <= 4096, "descriptors must fit the kernel arguments");
+
+constexpr int SQUARES_EACH = 16384;  // elements of a workgroup, while they are at most SQUARES_BLOCKS
+constexpr int SQUARES_BLOCKS = 256;
+
+template <typename Group>
+__device__ __forceinline__ int item_of(const Group& group, int block) {
+    int item = 0;
+    while (block >= group.first_block[item + 1]) ++item;
+    return item;
+}
+
+__device__ __forceinline__ double wave_total(double v) {
+    for (int o = 32; o > 0; o /= 2) v += __shfl_xor(v, o);
+    return v;
+}
+
+// The squares are added in 64 bits: no float32 overflows them.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void squares_kernel(SourceGroup group) {
+    __shared__ double parts[THREADS / 64];
+    const int item = item_of(group, blockIdx.x), block = blockIdx.x - group.first_block[item], blocks = group.square_blocks[item];
+    const Source& s = group.s[item];
+    const T* in = static_cast<const T*>(s.in);
+    const long long count = static_cast<long long>(s.rows) * s.cols, each = (count + blocks - 1) / blocks;
+    const long long begin = block * each, end = min(begin + each, count);
+    double sum = 0.0;
+#pragma unroll 8
+    for (long long at = begin + threadIdx.x; at < end; at += THREADS) {
+        int column;
+        const int row = s.columns.divmod(static_cast<int>(at), column);
+        const double v = static_cast<float>(in[row * s.stride + column]);
+        sum += v * v;
+    }
+    sum = wave_total(sum);
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x / 64] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) s.squares[block] = parts[0] + parts[1] + parts[2] + parts[3];
+}
+
+// 64 x 64 values of a matrix, scaled, split and written in both orientations, with zeros in the padding.
+template <typename T>
+__global__ __launch_bounds__(THREADS) void split_kernel(SourceGroup group) {
+    __shared__ float tile[64][65];
+    __shared__ double factor;  // products in 64 bits: of the smallest norms it lies beyond float32
+    const int item = item_of(group, blockIdx.x), tid = threadIdx.x;
+    const Source& s = group.s[item];
+    if (tid < 64) {
+        double sum = 0.0;
+        for (int i = tid; i < group.square_blocks[item]; i += 64) sum += s.squares[i];
+        sum = wave_total(sum);
+        if (tid == 0) factor = static_cast<double>(SCALE) / (sqrt(sum) + static_cast<double>(group.eps));
+    }
+    __syncthreads();
+    const int block = blockIdx.x - group.first_block[item], across = s.padded_cols / 64;
+    const int row0 = block / across * 64, col0 = block % across * 64;
+    const T* in = static_cast<const T*>(s.in);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int row = k * 4 + tid / 64, col = tid & 63;
+        const bool there = row0 + row < s.rows && col0 + col < s.cols;
+        tile[row][col] = there ? static_cast<float>(static_cast<float>(in[(row0 + row) * s.stride + col0 + col]) * factor) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int row = (k * THREADS + tid) / 8, part = (k * THREADS + tid) % 8;
+        half8 hi[2], lo[2];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v[2] = {tile[row][part * 8 + e], tile[part * 8 + e][row]};
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                hi[o][e] = static_cast<_Float16>(v[o]);
+                lo[o][e] = static_cast<_Float16>(v[o] - static_cast<float>(hi[o][e]));
+            }
+        }
+        const int at = part * 8 / K_STEP * ROW_STEP + part * 8 % K_STEP;
+        _Float16* same = s.same + static_cast<std::int64_t>(row0 + row) * s.padded_cols * 2 + col0 * 2 + at;
+        _Float16* other = s.across + static_cast<std::int64_t>(col0 + row) * s.padded_rows * 2 + row0 * 2 + at;
+        *reinterpret_cast<half8*>(same) = hi[0];
+        *reinterpret_cast<half8*>(same + K_STEP) = lo[0];
+        *reinterpret_cast<half8*>(other) = hi[1];
+        *reinterpret_cast<half8*>(other + K_STEP) = lo[1];
+    }
+}
+
+// ---- the plan of one matrix -------------------------------------------------------------------
+// Large tiles need half the loads of small ones a product; small ones fill more of the GPU with a small matrix and
+// pad it less.
+int side_of(int shorter) { return shorter >= 256 ? LARGE : SMALL; }
+
+struct Plan {
+    int side, s, l;              // padded
+    std::int64_t x, square;      // bytes of X and of a square matrix
+    int square_blocks;
+    explicit Plan(const OrthogonalMatrix& m) {
+        const int shorter = std::min(m.rows, m.cols), longer = std::max(m.rows, m.cols);
+        side = side_of(shorter);
+        s = (shorter + side - 1) / side * side, l = (longer + side - 1) / side * side;
+        x = static_cast<std::int64_t>(s) * l * 4, square = static_cast<std::int64_t>(s) * s * 4;
+        const std::int64_t blocks = (static_cast<std::int64_t>(m.rows) * m.cols + SQUARES_EACH - 1) / SQUARES_EACH;
+        square_blocks = static_cast<int>(std::min<std::int64_t>(blocks, SQUARES_BLOCKS));
+    }
+    std::int64_t bytes() const { return 3 * x + 2 * square + SQUARES_BLOCKS * 8; }
+};
+
+struct Buffers {
+    _Float16 *x, *x_t[2], *g, *p;
+    double* squares;
+    Buffers(const Plan& plan, char* at) {
+        const auto take = [&](std::int64_t bytes) {
+            char* here = at;
+            at += bytes;
+            return reinterpret_cast<_Float16*>(here);
+        };
+        x = take(plan.x), x_t[0] = take(plan.x), x_t[1] = take(plan.x), g = take(plan.square), p = take(plan.square);
+        squares = reinterpret_cast<double*>(at);
+    }
+};
+
+template <typename T>
+int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps& o, char* workspace, hipStream_t stream) {
+    std::vector<Plan> plans;
+    std::vector<Buffers> buffers;
+    for (int i = 0; i < count; ++i) {
+        plans.emplace_back(matrices[i]);
+        buffers.emplace_back(plans[i], workspace);
+        workspace += plans[i].bytes();
+    }
+    SourceGroup sources{};
+    sources.count = count, sources.eps = o.eps;
+    for (int i = 0; i < count; ++i) {
+        const OrthogonalMatrix& m = matrices[i];
+        const bool tall = m.rows > m.cols;
+        Source& s = sources.s[i];
+        s.in = m.in, s.stride = m.in_stride, s.rows = m.rows, s.cols = m.cols, s.columns = FastDiv(m.cols);
+        s.same = tall ? buffers[i].x_t[0] : buffers[i].x, s.across = tall ? buffers[i].x : buffers[i].x_t[0];
+        s.padded_rows = tall ? plans[i].l : plans[i].s, s.padded_cols = tall ? plans[i].s : plans[i].l;
+        s.squares = buffers[i].squares;
+        sources.square_blocks[i] = plans[i].square_blocks;
+        sources.first_block[i + 1] = sources.first_block[i] + plans[i].square_blocks;
+    }
+    launch(squares_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
+    MFH_TRY(MFH_CHECK_LAUNCH("orthogonal squares", stream));
+    for (int i = 0; i < count; ++i)
+        sources.first_block[i + 1] = sources.first_block[i] + sources.s[i].padded_rows / 64 * (sources.s[i].padded_cols / 64);
+    launch(split_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
+    MFH_TRY(MFH_CHECK_LAUNCH("orthogonal split", stream));
+    const auto products = [&](auto&& describe) {
+        ProductGroup group{};
+        group.count = count;
+        for (int i = 0; i < count; ++i) {
+            Product& p = group.p[i];
+            const Plan& plan = plans[i];
+            const OrthogonalMatrix& m = matrices[i];
+            p.alpha = 1.0f, p.small = plan.side == SMALL, p.tall = m.rows > m.cols;
+            p.rows = std::min(m.rows, m.cols), p.cols = std::max(m.rows, m.cols);
+            describe(i, p);
+            p.m_tiles = plan.s / plan.side, p.n_tiles = p.symmetric ? p.m_tiles : plan.l / plan.side;
+            group.first_unit[i + 1] = group.first_unit[i] + (p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles);
+        }
+        launch(product_kernel<T>, dim3(group.first_unit[count]), dim3(THREADS), 0, stream, group);
+        return MFH_CHECK_LAUNCH("orthogonal product", stream);
+    };
+    for (int step = 0; step < o.steps; ++step) {
+        const int from = step & 1;
+        MFH_TRY(products([&](int i, Product& p) {
+            const Buffers& at = buffers[i];
+            p.symmetric = true, p.a = p.b = at.x, p.out = p.out_t = at.g, p.ksteps = plans[i].l / K_STEP;
+        }));
+        MFH_TRY(products([&](int i, Product& p) {
+            const Buffers& at = buffers[i];
+            p.symmetric = true, p.a = p.b = p.add_t = at.g, p.out = p.out_t = at.p, p.ksteps = plans[i].s / K_STEP;
+            p.alpha = o.c, p.beta = o.b;
+        }));
+        MFH_TRY(products([&](int i, Product& p) {
+            const Buffers& at = buffers[i];
+            p.a = at.p, p.b = p.add_t = at.x_t[from], p.ksteps = plans[i].s / K_STEP, p.beta = o.a;
+            if (step + 1 == o.steps) p.final = matrices[i].out, p.final_stride = matrices[i].out_stride;
+            else p.out = at.x, p.out_t = at.x_t[from ^ 1];
+        }));
+    }
+    return OK;
+}
+
+}  // namespace
+
+std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count) {
+    std::int64_t most = 0;
+    for (int i = 0; i < count; i += GROUP) {
+        std::int64_t bytes = 0;
+        for (int k = i; k < std::min(count, i + GROUP); ++k) bytes += Plan(matrices[k]).bytes();
+        most = std::max(most, bytes);
+    }
+    return most;
+}
+
+int launch_orthogonal(const OrthogonalMatrix* matrices, int count, int type, const OrthogonalSteps& o, void* workspace,
+                      hipStream_t stream) {
+    return with_type(type, [&](auto element) {
+        for (int i = 0; i < count; i += GROUP)
+            MFH_TRY(run_group<decltype(element)>(matrices + i, std::min(GROUP, count - i), o, static_cast<char*>(workspace), stream));
+        return static_cast<int>(OK);
+    });
+}
+
+}  // namespace mfh

@@ -76,11 +76,17 @@ class AdamTensor(ctypes.Structure):
                 ("bias_correction2", ctypes.c_float)]
 
 
+class OrthogonalMatrix(ctypes.Structure):
+    """One row of the mfh_orthogonalize table (include/mfhip.h)."""
+    _fields_ = [("input", ctypes.c_uint64), ("out", ctypes.c_uint64), ("in_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32)]
+
+
 # Argument codes: p device pointer / stream (uint64), i int32, q int64, f float, d double,
-# t pointer to an AdamTensor table, P pointer to int32 (host array), U pointer to uint64 (host array),
+# t pointer to an AdamTensor table, m pointer to an OrthogonalMatrix table, P pointer to int32 (host array), U pointer to uint64 (host array),
 # L pointer to int64.
 _CTYPE = {"p": ctypes.c_uint64, "i": ctypes.c_int, "q": ctypes.c_int64, "f": ctypes.c_float, "d": ctypes.c_double,
-          "t": ctypes.POINTER(AdamTensor), "P": ctypes.POINTER(ctypes.c_int), "s": ctypes.c_char_p, "-": None,
+          "t": ctypes.POINTER(AdamTensor), "m": ctypes.POINTER(OrthogonalMatrix), "P": ctypes.POINTER(ctypes.c_int), "s": ctypes.c_char_p, "-": None,
           "U": ctypes.POINTER(ctypes.c_uint64), "L": ctypes.POINTER(ctypes.c_int64)}
 _CONV = "i" * 13
 # symbol: (result code, argument codes); mirrors include/mfhip.h.
@@ -150,6 +156,8 @@ _SIGNATURES = {
     "mfh_group_norm_workspace": ("q", "qiiiii"),
     "mfh_group_norm_forward": ("i", "piqiii" + "ppif" + "ppp" + "pqp"),
     "mfh_group_norm_backward": ("i", "ppiqiii" + "pppp" + "i" + "ppp" + "iii" + "pqp"),
+    "mfh_orthogonalize_workspace": ("q", "mi"),
+    "mfh_orthogonalize": ("i", "mii" + "iffff" + "pqp"),
     "mfh_embedding": ("i", "piqiq" + "piqq" + "fpqp"),
     "mfh_embedding_workspace": ("q", "qqii"),
     "mfh_embedding_backward": ("i", "piqiq" + "piqqf" + "piqi" + "pqp"),

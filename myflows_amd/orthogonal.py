@@ -1,0 +1,115 @@
+"""Matrices orthogonalised by Newton-Schulz products, on libmfhip: the update that the ``Muon`` optimiser makes of a
+parameter's momentum.
+
+``orthogonalize`` and ``orthogonalize_many`` take float32, bfloat16 or float16 matrices; a tensor of more
+dimensions (a convolution's kernel) is one of its first dimension by the others. All matrices of a call go
+through their products together, one launch a product. There is no host path. The reference has no counterpart:
+its only optimisers with a state are elementwise.
+"""
+
+from __future__ import annotations
+
+import math
+from functools import lru_cache
+
+import torch
+
+from . import native
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # steep at 0, and within 0.7 .. 1.2 for what began above 0.002, in five steps
+STEPS = 5
+STEPS_MAX = 64
+SIDE_LIMIT = 1 << 20
+ELEMENTS_LIMIT = 2 ** 31 - 1
+
+
+def _matrix(value, name):
+    """A 2-D view (or copy) of contiguous rows of a GPU tensor of two or more dimensions."""
+    if not (isinstance(value, torch.Tensor) and value.is_cuda and value.dtype in native.TYPE_CODES):
+        raise TypeError(f"{name} must be a float32, bfloat16 or float16 torch tensor on the GPU")
+    if value.ndim < 2:
+        raise ValueError(f"{name} must have two dimensions or more")
+    if value.ndim > 2:
+        value = value.reshape(value.shape[0], math.prod(value.shape[1:]))
+    rows, cols = value.shape
+    if max(rows, cols) > SIDE_LIMIT or rows * cols > ELEMENTS_LIMIT:
+        raise ValueError(f"{name} may have sides of {SIDE_LIMIT} and {ELEMENTS_LIMIT} elements at most")
+    if rows and cols and ((cols > 1 and value.stride(1) != 1) or (rows > 1 and value.stride(0) < cols)):
+        value = value.contiguous()
+    return value
+
+
+@lru_cache(maxsize=64)
+def _checked_polynomial(coefficients, steps):
+    """The coefficients, once a sampling of 0 .. 1 shows that the steps keep every singular value below 3.5 and the
+    polynomial's factor below 15: the range that the kernels hold."""
+    a, b, c = coefficients
+    values = [i / 4096 for i in range(4097)]
+    for _ in range(steps):
+        factors = [a + b * x * x + c * x ** 4 for x in values]
+        values = [x * f for x, f in zip(values, factors)]
+        if not (max(map(abs, factors)) < 15.0 and max(map(abs, values)) < 3.5):
+            raise ValueError(f"the coefficients {coefficients} take singular values out of range in {steps} steps")
+    return coefficients
+
+
+def _polynomial(coefficients, steps):
+    steps = int(steps)
+    if not 1 <= steps <= STEPS_MAX:
+        raise ValueError(f"steps must lie between 1 and {STEPS_MAX}")
+    coefficients = tuple(float(v) for v in coefficients)
+    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+        raise ValueError("coefficients must be three finite numbers")
+    return _checked_polynomial(coefficients, steps), steps
+
+
+@lru_cache(maxsize=256)
+def _workspace(shapes):
+    table = (native.OrthogonalMatrix * len(shapes))(*((0, 0, cols, cols, rows, cols) for rows, cols in shapes))
+    return native.workspace_bytes("mfh_orthogonalize_workspace", table, len(shapes))
+
+
+def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7, out=None):
+    """Each matrix M taken through ``steps`` Newton-Schulz steps, as a list of tensors of their shapes and types.
+
+    With X = M / (|M| + eps), |M| the Frobenius norm, a step makes X = a X + (b G + c G G) X of X X^T = G (of the
+    shorter side): each singular value x becomes x (a + b x^2 + c x^4), which the default coefficients bring near 1.
+    The products are formed to float32's precision and the result is rounded once to the matrix's type; a matrix
+    of zeros stays one (for an eps above 0), and one with an infinity or NaN becomes NaN. ``out`` takes the results (each a contiguous
+    tensor of its matrix's shape and type, possibly the matrix itself). Other coefficients must keep values of
+    0 .. 1 below 3.5, and a + b x^2 + c x^4 below 15, at every step."""
+    matrices = list(matrices)
+    (a, b, c), steps = _polynomial(coefficients, steps)
+    eps = float(eps)
+    if not (math.isfinite(eps) and eps >= 0.0):
+        raise ValueError("eps must be finite and not negative")
+    views = [_matrix(value, "a matrix") for value in matrices]
+    if out is None:
+        out = [torch.empty_like(value, memory_format=torch.contiguous_format) for value in matrices]
+    else:
+        out = list(out)
+        if len(out) != len(matrices):
+            raise ValueError("out must hold a tensor for each matrix")
+        for value, to in zip(matrices, out):
+            if not (isinstance(to, torch.Tensor) and to.is_cuda and to.dtype is value.dtype and to.shape == value.shape
+                    and to.is_contiguous()):
+                raise ValueError("out must hold contiguous GPU tensors of the matrices' shapes and types")
+    native._on_current_device(*matrices, *out)
+    rows = {}
+    for view, to in zip(views, out):
+        if view.numel():
+            rows.setdefault(view.dtype, []).append((view, to))
+    for dtype, pairs in rows.items():
+        shapes = tuple(tuple(view.shape) for view, _ in pairs)
+        table = (native.OrthogonalMatrix * len(pairs))(*(
+            (view.data_ptr(), to.data_ptr(), view.stride(0) if view.shape[0] > 1 else view.shape[1], view.shape[1], *view.shape)
+            for view, to in pairs))
+        workspace, held = native.byte_workspace(_workspace(shapes))
+        native._call("mfh_orthogonalize", table, len(pairs), native.TYPE_CODES[dtype], steps, a, b, c, eps, workspace, held,
+                     native._stream())
+    return out
+
+
+def orthogonalize(matrix, *, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7, out=None):
+    """``orthogonalize_many`` of one matrix."""
+    return orthogonalize_many([matrix], steps=steps, coefficients=coefficients, eps=eps, out=None if out is None else [out])[0]

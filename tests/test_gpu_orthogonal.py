@@ -1,0 +1,191 @@
+"""Matrices orthogonalised by Newton-Schulz products, against the definition in 64 bits.
+
+Tolerance. The steps raise an error in a small singular direction by up to a = 3.4 each, whatever the arithmetic, so
+the error is measured against that of the same steps in float32 on the CPU. A value held as two float16 has an error
+of 2^-23 of it, twice float32's half step; a product leaves out lo lo, 2^-24 of it at most; its sums are float32. So
+each product has at most three times the error of a float32 one, and the order of the sums may differ: in the
+Frobenius norm the result is within 4 times float32's error, plus 2^-20 of the result for matrices so small that
+float32's own error happens to be near 0, plus half a step of the type (of a float16 result below 2^-14, half of 2^-24).
+"""
+
+import pytest
+import torch
+
+import myflows_amd as mf
+from myflows_amd import orthogonal as ops
+
+TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+gpu = pytest.mark.gpu
+
+
+def _steps(matrix, dtype, steps=5, coefficients=ops.COEFFICIENTS, eps=1e-7):
+    a, b, c = coefficients
+    x = matrix.detach().cpu().to(dtype).reshape(matrix.shape[0], -1)
+    tall = x.shape[0] > x.shape[1]
+    x = x.T if tall else x
+    x = x / (x.double().square().sum().sqrt() + eps).to(dtype)
+    for _ in range(steps):
+        g = x @ x.T
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return (x.T if tall else x).reshape(matrix.shape)
+
+
+def _check(got, matrix, **options):
+    want = _steps(matrix, torch.float64, **options)
+    size = float(want.norm())
+    rounding = torch.finfo(matrix.dtype).eps / 2 * size
+    if matrix.dtype is torch.float16:
+        rounding += 2.0 ** -25 * want.numel() ** 0.5
+    bound = 4 * float((_steps(matrix, torch.float32, **options).double() - want).norm()) + 2.0 ** -20 * size + rounding
+    off = float((got.detach().cpu().double() - want).norm())
+    print(f"off {off / size if size else off:.2e}, bound {bound / size if size else bound:.2e}", flush=True)
+    assert got.dtype is matrix.dtype and got.shape == matrix.shape and off <= bound
+
+
+def _matrix(rows, cols, dtype, seed, spectrum="noise"):
+    g = torch.Generator().manual_seed(seed)
+    if spectrum == "noise":
+        x = torch.randn((rows, cols), generator=g)
+    else:  # singular values that fall over four orders of magnitude
+        short = min(rows, cols)
+        u, _ = torch.linalg.qr(torch.randn((rows, short), generator=g, dtype=torch.float64))
+        v, _ = torch.linalg.qr(torch.randn((cols, short), generator=g, dtype=torch.float64))
+        x = (u * 10.0 ** (-4.0 * torch.arange(short) / short) @ v.T).float()
+    return (x * 0.01).to(TYPES[dtype]).cuda()
+
+
+SIZES = [(1, 1), (1, 7), (9, 1), (4, 5), (24, 25), (64, 64), (65, 63), (64, 576), (500, 2), (128, 600), (130, 500), (255, 256),
+         (256, 256), (257, 300), (256, 2304), (1000, 333), (777, 1500), (64, 5000)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_orthogonalised_matrices_match_the_definition(rows, cols, dtype):
+    print("orthogonalize", rows, cols, dtype, flush=True)
+    for spectrum in ("noise", "falling"):
+        matrix = _matrix(rows, cols, dtype, rows + cols, spectrum)
+        got = ops.orthogonalize(matrix)
+        _check(got, matrix)
+        assert torch.equal(ops.orthogonalize(matrix), got)
+
+
+@gpu
+def test_a_list_of_unlike_matrices_gives_the_bits_of_each_alone():
+    shapes = [(64, 147), (64, 576), (128, 64), (300, 700), (700, 300), (2, 512), (1, 1), (0, 4), (257, 257)] * 5
+    matrices = [_matrix(r, c, list(TYPES)[i % 3], i) if r else torch.zeros((r, c), device="cuda") for i, (r, c) in enumerate(shapes)]
+    got = ops.orthogonalize_many(matrices)
+    assert len(got) == len(matrices) and ops.orthogonalize_many([]) == []
+    for value, to in zip(matrices, got):
+        assert to.dtype is value.dtype and to.shape == value.shape
+        if value.numel():
+            assert torch.equal(ops.orthogonalize(value), to)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_kernels_strides_and_results_in_place(dtype):
+    kernel = _matrix(40, 27, dtype, 1).reshape(40, 3, 3, 3)
+    got = ops.orthogonalize(kernel)
+    _check(got, kernel)
+    assert torch.equal(ops.orthogonalize(kernel.reshape(40, 27)), got.reshape(40, 27))
+    wide = _matrix(70, 300, dtype, 2)
+    part = wide[:, 11:211]
+    _check(ops.orthogonalize(part), part)
+    assert torch.equal(ops.orthogonalize(part.contiguous()), ops.orthogonalize(part))
+    assert torch.equal(ops.orthogonalize(part.t()), ops.orthogonalize(part.t().contiguous()))
+    _check(ops.orthogonalize(part.t()), part.t())
+    want = ops.orthogonalize(wide)
+    assert ops.orthogonalize(wide, out=wide) is wide and torch.equal(wide, want)
+
+
+@gpu
+def test_other_polynomials_and_steps():
+    matrix = _matrix(90, 200, "float32", 3)
+    for steps, coefficients in ((1, ops.COEFFICIENTS), (2, ops.COEFFICIENTS), (12, (1.5, -0.5, 0.0)), (6, (15 / 8, -10 / 8, 3 / 8))):
+        options = dict(steps=steps, coefficients=coefficients)
+        _check(ops.orthogonalize(matrix, **options), matrix, **options)
+    orthogonal = ops.orthogonalize(matrix, steps=30, coefficients=(1.5, -0.5, 0.0)).double()
+    assert float((orthogonal @ orthogonal.T - torch.eye(90, device="cuda")).abs().max()) < 1e-5
+
+
+@gpu
+def test_sizes_of_the_values_do_not_matter():
+    base = _matrix(100, 170, "float32", 4)
+    want = ops.orthogonalize(base, eps=0.0)
+    for factor in (2.0 ** 100, 2.0 ** -100, 2.0 ** -126):  # the last leaves values below the normal range: not compared
+        got = ops.orthogonalize(base * factor, eps=0.0)
+        assert bool(got.isfinite().all())
+        if factor > 2.0 ** -110:
+            assert torch.equal(got, want)
+    spike = torch.zeros((100, 170), device="cuda")
+    spike[3, 5] = 1e30
+    _check(ops.orthogonalize(spike), spike)
+    tiny = _matrix(64, 100, "float32", 5) * 1e-9  # eps counts here
+    _check(ops.orthogonalize(tiny), tiny)
+
+
+@gpu
+def test_zeros_infinities_and_nan():
+    zeros = torch.zeros((70, 90), device="cuda")
+    assert torch.equal(ops.orthogonalize(zeros), zeros)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        matrix = torch.randn((70, 90), device="cuda")
+        matrix[69, 89] = bad
+        other = torch.randn((80, 30), device="cuda")
+        got = ops.orthogonalize_many([matrix, other])
+        assert bool(got[0].isnan().all()) and torch.equal(got[1], ops.orthogonalize(other))
+
+
+@gpu
+def test_streams_and_captured_graphs_have_workspaces_of_their_own():
+    first, second = _matrix(300, 500, "float32", 6), _matrix(256, 800, "float32", 7)
+    alone = [ops.orthogonalize(first), ops.orthogonalize(second)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        got = []
+        for stream, matrix in zip(streams, (first, second)):
+            with torch.cuda.stream(stream):
+                got.append(ops.orthogonalize(matrix))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))
+    graphs, held = [], []
+    for matrix in (first, second):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(ops.orthogonalize(matrix))
+        graphs.append(graph)
+    for _ in range(3):
+        for stream, graph in zip(streams, graphs):  # side by side
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, alone))
+        assert torch.equal(ops.orthogonalize(first), alone[0])
+
+
+def test_refusals_without_a_gpu():
+    with pytest.raises(TypeError, match="on the GPU"):
+        ops.orthogonalize(torch.zeros((3, 4)))
+    for options in (dict(steps=0), dict(steps=65), dict(coefficients=(1.0, 2.0)), dict(coefficients=(1.0, float("nan"), 0.0)),
+                    dict(coefficients=(4.0, 0.0, 0.0)), dict(coefficients=(2.0, 0.0, 0.0), steps=4), dict(eps=-1.0),
+                    dict(eps=float("inf"))):
+        with pytest.raises(ValueError):
+            ops.orthogonalize_many([], **options)
+
+
+@gpu
+def test_refusals():
+    matrix = torch.zeros((3, 4), device="cuda")
+    for bad in (matrix.double(), matrix.int(), [[1.0]]):
+        with pytest.raises(TypeError):
+            ops.orthogonalize(bad)
+    for bad in (matrix[0], matrix[0, 0], torch.zeros((1, 1), device="cuda").expand(1, (1 << 20) + 1)):
+        with pytest.raises(ValueError):
+            ops.orthogonalize(bad)
+    for out in (matrix.half(), matrix.t(), matrix.cpu(), torch.zeros((3, 8), device="cuda")[:, :4]):
+        with pytest.raises(ValueError, match="out"):
+            ops.orthogonalize(matrix, out=out)
+    with pytest.raises(ValueError, match="out"):
+        ops.orthogonalize_many([matrix], out=[])
