@@ -1444,7 +1444,8 @@ MFH_API std::int64_t mfh_orthogonalize_workspace(const mfh_orthogonal_matrix* ma
 }
 
 MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, int type, int steps, float a, float b, float c,
-                              float eps, std::uint64_t workspace, std::int64_t workspace_bytes, std::uint64_t stream) {
+                              float eps, std::uint64_t workspace, std::int64_t workspace_bytes, std::uint64_t counters,
+                              std::uint64_t stream) {
     MFH_TRY(require_ready());
     MFH_REQUIRE(type_valid(type), "unknown element type");
     MFH_REQUIRE(steps > 0 && steps <= ORTHOGONAL_STEPS_MAX, "number of steps out of range");
@@ -1452,10 +1453,10 @@ MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, 
     std::vector<OrthogonalMatrix> table;
     MFH_TRY(require_orthogonal(matrices, count, table));
     for (const OrthogonalMatrix& m : table) MFH_REQUIRE(m.in && m.out, "orthogonalisation received a null buffer");
-    MFH_REQUIRE(count == 0 || (workspace && workspace_bytes >= orthogonal_workspace(table.data(), count)),
+    MFH_REQUIRE(count == 0 || (counters && workspace && workspace_bytes >= orthogonal_workspace(table.data(), count)),
                 "orthogonalisation workspace too small");
-    return launch_orthogonal(table.data(), count, type, OrthogonalSteps{steps, a, b, c, eps}, as_ptr<void>(workspace),
-                             as_stream(stream));
+    return launch_orthogonal(table.data(), count, type, OrthogonalSteps{steps, a, b, c, eps, as_ptr<unsigned>(counters)},
+                             as_ptr<void>(workspace), as_stream(stream));
 }
 
 }  // extern "C"

@@ -667,6 +667,7 @@ struct OrthogonalMatrix {  // out has the shape and type of in, and may be in
 struct OrthogonalSteps {
     int steps;
     float a, b, c, eps;
+    unsigned* counters;  // LOGIT_COUNTERS
 };
 std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count);  // bytes
 int launch_orthogonal(const OrthogonalMatrix* matrices, int count, int type, const OrthogonalSteps& o, void* workspace,

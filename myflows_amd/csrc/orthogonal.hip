@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "common.h"
+#include "hand_over.h"
 #include "typed.h"
 
 namespace mfh {
@@ -40,6 +41,7 @@ constexpr int SCALE_LOG = 12;
 constexpr float SCALE = 1 << SCALE_LOG, UNSCALE = 1.0f / SCALE;
 constexpr int GROUP = 32;  // matrices of a launch: their descriptors travel in its arguments
 constexpr int XCD_COUNT = 8;
+constexpr std::int64_t PARTS_BYTES = 48 << 20;  // workspace of split tiles' sums
 
 // out = alpha A B^T + beta add, or the caller's matrix in its type.
 struct Product {
@@ -50,8 +52,11 @@ struct Product {
     _Float16* out_t;        // optional, transposed
     void* final;
     std::int64_t final_stride;
+    float* parts;        // where the steps of a tile are split over workgroups: their sums,
+    unsigned* arrived;   // and how many have come, a tile
     float alpha, beta;
     int ksteps, m_tiles, n_tiles;  // tiles of its own side
+    int splits;
     int rows, cols;                // of the caller's matrix, the shorter side as rows
     bool symmetric, small, tall;   // tall: the caller's matrix is the transposed result
 };
@@ -135,48 +140,110 @@ __device__ __forceinline__ void write_piece(const Product& p, const float16v& su
     }
 }
 
-// One SIDE x SIDE tile by four waves of SIDE / 2 x SIDE / 2, two steps in LDS: while a step is multiplied the next
-// one's rows are on their way.
+// The sums of a tile's parts, in their order, by the workgroup that comes last; false for the others.
+template <int SUMS>
+__device__ __forceinline__ bool join_parts(const Product& p, int tile, int part, float (&sum)[SUMS]) {
+    __shared__ unsigned last;
+    static_assert(SUMS % 2 == 0, "two sums a store");
+    using Two = unsigned long long;
+    Two* parts = reinterpret_cast<Two*>(p.parts) + static_cast<std::int64_t>(tile) * p.splits * (SUMS / 2) * THREADS + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < SUMS / 2; ++i) {
+        const float two[2] = {sum[2 * i], sum[2 * i + 1]};
+        hand_over(parts + (static_cast<std::int64_t>(part) * (SUMS / 2) + i) * THREADS, __builtin_bit_cast(Two, two));
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the sums are where every die sees them
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(p.arrived + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<unsigned>(p.splits);
+        if (last) hand_over(p.arrived + tile, 0u);
+    }
+    __syncthreads();
+    if (!last) return false;
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) sum[i] = 0.0f;
+    for (int other = 0; other < p.splits; ++other) {
+        Two two[SUMS / 2];
+#pragma unroll
+        for (int i = 0; i < SUMS / 2; ++i) two[i] = handed_over(parts + (static_cast<std::int64_t>(other) * (SUMS / 2) + i) * THREADS);
+#pragma unroll
+        for (int i = 0; i < SUMS / 2; ++i) {
+            sum[2 * i] += __uint_as_float(static_cast<unsigned>(two[i]));
+            sum[2 * i + 1] += __uint_as_float(static_cast<unsigned>(two[i] >> 32));
+        }
+    }
+    return true;
+}
+
+// One SIDE x SIDE tile, or the steps of one part of it, by four waves of SIDE / 2 x SIDE / 2. Two steps lie in LDS, a
+// step has two halves of 16 k. While one half is multiplied the other's operands are read from LDS, and the step
+// after next is on its way to LDS from the moment that all waves have read the one whose place it takes: one
+// barrier a step.
 template <int SIDE, typename T>
-__device__ __forceinline__ void tile_product(const Product& p, int tile_i, int tile_j, _Float16* lds) {
+__device__ __forceinline__ void tile_product(const Product& p, int tile_i, int tile_j, int tile, int part, _Float16* lds) {
     constexpr int PIECES = SIDE / 64, STAGE = SIDE * ROW_STEP;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wave_i = wave / 2 * (SIDE / 2), wave_j = wave % 2 * (SIDE / 2);
     const std::int64_t pitch = static_cast<std::int64_t>(p.ksteps) * ROW_STEP;
     const _Float16* a = p.a + static_cast<std::int64_t>(tile_i) * SIDE * pitch;
     const _Float16* b = p.b + static_cast<std::int64_t>(tile_j) * SIDE * pitch;
+    const int begin = static_cast<int>(static_cast<long long>(p.ksteps) * part / p.splits);
+    const int end = static_cast<int>(static_cast<long long>(p.ksteps) * (part + 1) / p.splits);
     float16v sum[PIECES][PIECES] = {};
-    stage_rows<SIDE>(a, pitch, 0, lds);
-    stage_rows<SIDE>(b, pitch, 0, lds + STAGE);
-    for (int step = 0; step < p.ksteps; ++step) {
-        const _Float16* at = lds + (step & 1) * 2 * STAGE;
-        // This wave's rows of the step have arrived, and with the barrier everyone's; and everyone has read the step before.
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    struct Operands {
+        half8 x[PIECES][2], y[PIECES][2];  // hi and lo
+    };
+    const auto stage = [&](int step) {  // beyond the last step that one again, into the place that nobody reads any more
+        _Float16* to = lds + ((step - begin) & 1) * 2 * STAGE;
+        const int from = min(step, end - 1);
+        stage_rows<SIDE>(a, pitch, from, to);
+        stage_rows<SIDE>(b, pitch, from, to + STAGE);
+    };
+    const auto read = [&](int step, int half) {
+        const _Float16* at = lds + ((step - begin) & 1) * 2 * STAGE;
+        Operands o;
+#pragma unroll
+        for (int piece = 0; piece < PIECES; ++piece)
+#pragma unroll
+            for (int low = 0; low < 2; ++low) {
+                o.x[piece][low] = operand(at, wave_i + piece * 32 + (lane & 31), low * 4 + half * 2 + lane / 32);
+                o.y[piece][low] = operand(at + STAGE, wave_j + piece * 32 + (lane & 31), low * 4 + half * 2 + lane / 32);
+            }
+        return o;
+    };
+    const auto multiply = [&](const Operands& o) {
+#pragma unroll
+        for (int term = 0; term < 3; ++term)
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j)
+                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.x[i][term == 2], o.y[j][term == 1], sum[i][j], 0, 0, 0);
+    };
+    stage(begin);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows have arrived; with the barrier, everyone's
+    __syncthreads();
+    stage(begin + 1);
+    Operands first = read(begin, 0);
+    for (int step = begin; step < end; ++step) {
+        const Operands second = read(step, 1);
+        multiply(first);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): the next step has arrived, and this one is read
         __syncthreads();
-        half8 x[2][PIECES][2], y[2][PIECES][2];
+        first = read(step + 1, 0);
+        stage(step + 2);
+        multiply(second);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    if (p.splits > 1) {
+        float flat[PIECES * PIECES * 16];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int e = 0; e < PIECES * PIECES * 16; ++e) flat[e] = sum[e / 16 / PIECES][e / 16 % PIECES][e % 16];
+        if (!join_parts(p, tile, part, flat)) return;
 #pragma unroll
-            for (int piece = 0; piece < PIECES; ++piece)
-#pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    x[k][piece][part] = operand(at, wave_i + piece * 32 + (lane & 31), part * 4 + k * 2 + lane / 32);
-                    y[k][piece][part] = operand(at + STAGE, wave_j + piece * 32 + (lane & 31), part * 4 + k * 2 + lane / 32);
-                }
-        if (step + 1 < p.ksteps) {
-            _Float16* next = lds + ((step + 1) & 1) * 2 * STAGE;
-            stage_rows<SIDE>(a, pitch, step + 1, next);
-            stage_rows<SIDE>(b, pitch, step + 1, next + STAGE);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int term = 0; term < 3; ++term)
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-                    for (int j = 0; j < PIECES; ++j)
-                        sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[k][i][term == 2], y[k][j][term == 1], sum[i][j], 0, 0, 0);
+        for (int e = 0; e < PIECES * PIECES * 16; ++e) sum[e / 16 / PIECES][e / 16 % PIECES][e % 16] = flat[e];
     }
     const bool mirrored = p.out && (!p.symmetric || tile_i != tile_j);
 #pragma unroll
@@ -186,16 +253,17 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
             write_piece<T>(p, sum[i][j], tile_i * SIDE + wave_i + i * 32, tile_j * SIDE + wave_j + j * 32, SIDE, mirrored);
 }
 
-template <typename T>
+// LARGEST: the side of the launch's largest tiles, for which LDS is held.
+template <int LARGEST, typename T>
 __global__ __launch_bounds__(THREADS, 2) void product_kernel(ProductGroup group) {
-    __shared__ __align__(1024) _Float16 lds[4 * LARGE * ROW_STEP];
+    __shared__ __align__(1024) _Float16 lds[4 * LARGEST * ROW_STEP];
     // Neighbouring units go to the same die: workgroups are dealt to the dies in turn.
     const int units = gridDim.x, die = blockIdx.x % XCD_COUNT, share = units / XCD_COUNT, more = units % XCD_COUNT;
     const int unit = die * share + min(die, more) + blockIdx.x / XCD_COUNT;
     int item = 0;
     while (unit >= group.first_unit[item + 1]) ++item;
     const Product& p = group.p[item];
-    const int t = unit - group.first_unit[item];
+    const int within = unit - group.first_unit[item], t = within / p.splits, part = within - t * p.splits;
     int i, j;
     if (p.symmetric) {  // the tiles on and below the diagonal, row by row
         i = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
@@ -203,11 +271,11 @@ __global__ __launch_bounds__(THREADS, 2) void product_kernel(ProductGroup group)
         while ((i + 1) * (i + 2) / 2 <= t) ++i;
         j = t - i * (i + 1) / 2;
     } else {  // columns of eight tiles, so that a die's tiles share rows of both operands
-        const int width = 8 * p.n_tiles, first = t / width * 8, rows = min(8, p.m_tiles - first), within = t % width;
-        i = first + within % rows, j = within / rows;
+        const int width = 8 * p.n_tiles, first = t / width * 8, rows = min(8, p.m_tiles - first), place = t % width;
+        i = first + place % rows, j = place / rows;
     }
-    if (p.small) tile_product<SMALL, T>(p, i, j, lds);
-    else tile_product<LARGE, T>(p, i, j, lds);
+    if (LARGEST == SMALL || p.small) tile_product<SMALL, T>(p, i, j, t, part, lds);
+    else tile_product<LARGEST, T>(p, i, j, t, part, lds);
 }
 
 // ---- before the products ----------------------------------------------------------------------
@@ -318,7 +386,15 @@ __global__ __launch_bounds__(THREADS) void split_kernel(SourceGroup group) {
 // ---- the plan of one matrix -------------------------------------------------------------------
 // Large tiles need half the loads of small ones a product; small ones fill more of the GPU with a small matrix and
 // pad it less.
-int side_of(int shorter) { return shorter >= 256 ? LARGE : SMALL; }
+int side_of(int shorter) { return shorter >= 1024 ? LARGE : SMALL; }
+
+// Parts of a tile's steps, for the products of a launch that would leave CUs idle: as many as fill `slots` workgroups,
+// but no more than about the root of the steps, since the last workgroup reads all parts' sums.
+int splits_of(int ksteps, std::int64_t launch_steps, std::int64_t slots, bool small) {
+    const std::int64_t share = std::max<std::int64_t>(launch_steps / slots, 4);
+    const int most = static_cast<int>(std::sqrt(ksteps * (small ? 1.5 : 0.5)));
+    return static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(ksteps / share, most)));
+}
 
 struct Plan {
     int side, s, l;              // padded
@@ -358,6 +434,7 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         buffers.emplace_back(plans[i], workspace);
         workspace += plans[i].bytes();
     }
+    char* const parts = workspace;
     SourceGroup sources{};
     sources.count = count, sources.eps = o.eps;
     for (int i = 0; i < count; ++i) {
@@ -377,9 +454,14 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         sources.first_block[i + 1] = sources.first_block[i] + sources.s[i].padded_rows / 64 * (sources.s[i].padded_cols / 64);
     launch(split_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
     MFH_TRY(MFH_CHECK_LAUNCH("orthogonal split", stream));
+    bool all_small = true;
+    for (const Plan& plan : plans) all_small = all_small && plan.side == SMALL;
+    const std::int64_t slots = static_cast<std::int64_t>(device_cu_count()) * (all_small ? 4 : 2);
     const auto products = [&](auto&& describe) {
         ProductGroup group{};
         group.count = count;
+        std::int64_t steps = 0;
+        const auto tiles = [](const Product& p) { return p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles; };
         for (int i = 0; i < count; ++i) {
             Product& p = group.p[i];
             const Plan& plan = plans[i];
@@ -388,9 +470,23 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
             p.rows = std::min(m.rows, m.cols), p.cols = std::max(m.rows, m.cols);
             describe(i, p);
             p.m_tiles = plan.s / plan.side, p.n_tiles = p.symmetric ? p.m_tiles : plan.l / plan.side;
-            group.first_unit[i + 1] = group.first_unit[i] + (p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles);
+            steps += static_cast<std::int64_t>(tiles(p)) * p.ksteps;
         }
-        launch(product_kernel<T>, dim3(group.first_unit[count]), dim3(THREADS), 0, stream, group);
+        char* part = parts;
+        int split_tiles = 0;
+        for (int i = 0; i < count; ++i) {
+            Product& p = group.p[i];
+            const std::int64_t bytes = static_cast<std::int64_t>(plans[i].side) * plans[i].side * 4;
+            p.splits = splits_of(p.ksteps, steps, slots, p.small);
+            if (p.splits > 1 && (split_tiles + tiles(p) > LOGIT_COUNTERS || part + bytes * p.splits * tiles(p) > parts + PARTS_BYTES)) p.splits = 1;
+            if (p.splits > 1) {
+                p.parts = reinterpret_cast<float*>(part), p.arrived = o.counters + split_tiles;
+                part += bytes * p.splits * tiles(p), split_tiles += tiles(p);
+            }
+            group.first_unit[i + 1] = group.first_unit[i] + tiles(p) * p.splits;
+        }
+        launch(all_small ? product_kernel<SMALL, T> : product_kernel<LARGE, T>, dim3(group.first_unit[count]), dim3(THREADS), 0,
+               stream, group);
         return MFH_CHECK_LAUNCH("orthogonal product", stream);
     };
     for (int step = 0; step < o.steps; ++step) {
@@ -421,7 +517,7 @@ std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count) {
     for (int i = 0; i < count; i += GROUP) {
         std::int64_t bytes = 0;
         for (int k = i; k < std::min(count, i + GROUP); ++k) bytes += Plan(matrices[k]).bytes();
-        most = std::max(most, bytes);
+        most = std::max(most, bytes + PARTS_BYTES);
     }
     return most;
 }

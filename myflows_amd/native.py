@@ -157,7 +157,7 @@ _SIGNATURES = {
     "mfh_group_norm_forward": ("i", "piqiii" + "ppif" + "ppp" + "pqp"),
     "mfh_group_norm_backward": ("i", "ppiqiii" + "pppp" + "i" + "ppp" + "iii" + "pqp"),
     "mfh_orthogonalize_workspace": ("q", "mi"),
-    "mfh_orthogonalize": ("i", "mii" + "iffff" + "pqp"),
+    "mfh_orthogonalize": ("i", "mii" + "iffff" + "pqpp"),
     "mfh_embedding": ("i", "piqiq" + "piqq" + "fpqp"),
     "mfh_embedding_workspace": ("q", "qqii"),
     "mfh_embedding_backward": ("i", "piqiq" + "piqqf" + "piqi" + "pqp"),

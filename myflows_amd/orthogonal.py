@@ -106,7 +106,7 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
             for view, to in pairs))
         workspace, held = native.byte_workspace(_workspace(shapes))
         native._call("mfh_orthogonalize", table, len(pairs), native.TYPE_CODES[dtype], steps, a, b, c, eps, workspace, held,
-                     native._stream())
+                     native.stream_counters(), native._stream())
     return out
 
 
