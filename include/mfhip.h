@@ -667,6 +667,23 @@ MFH_API int64_t mfh_orthogonalize_workspace(const mfh_orthogonal_matrix* matrice
 MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, int type, int steps, float a, float b, float c,
                               float eps, uint64_t workspace, int64_t workspace_bytes, uint64_t counters, uint64_t stream);
 
+/* One parameter of a Muon step: parameter, gradient and momentum (rows x cols contiguous floats each). */
+typedef struct mfh_muon_tensor {
+    uint64_t param, grad, momentum;
+    int32_t rows, cols;
+    float keep, rate;
+} mfh_muon_tensor;
+
+/* Bytes of workspace of mfh_muon_step, -1 when a size is out of range. */
+MFH_API int64_t mfh_muon_workspace(const mfh_muon_tensor* tensors, int count);
+
+/* For each tensor, with g = grad * grad_scale: m = momentum * m + g, d = g + momentum * m (nesterov != 0) or m,
+ * param = keep * param - rate * (d as mfh_orthogonalize makes it). The table is host memory, read during the call;
+ * no two of its arrays overlap. No counterpart in the reference. */
+MFH_API int mfh_muon_step(const mfh_muon_tensor* tensors, int count, float momentum, int nesterov, float grad_scale, int steps,
+                          float a, float b, float c, float eps, uint64_t workspace, int64_t workspace_bytes,
+                          uint64_t counters, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,7 +20,7 @@ from .ops_basic import LINEAR_BACKENDS, Add, ChannelNormalize_Op, Dropout_Op, Le
 from .ops_conv import (BACKENDS, NATIVE_BACKENDS, Conv2D_AddReLU_Op, Conv2D_LeakyReLU_Op, Conv2D_Op, Conv2D_ReLU_Op,
                        Flatten_Op, MaxPool2d_Op)
 from .ops_norm import BatchNorm2d_Op, BatchNormActivation, BatchNormReLUPool, GlobalAvgPool2d_Op
-from .optim import MBGD, Adam, Optimizer, ParameterGroups
+from .optim import MBGD, Adam, Muon, Optimizer, ParameterGroups
 from .resnet import BasicBlock, BatchNorm2d, GlobalAvgPool2d, ResNet18
 
 __all__ = [
@@ -28,7 +28,7 @@ __all__ = [
     "BatchNormReLUPool", "CapturedStep", "ChannelNormalize_Op", "Conv2D", "Dropout", "Dropout_Op",
     "Conv2D_AddReLU_Op", "Conv2D_LeakyReLU_Op", "Conv2D_Op", "Conv2D_ReLU_Op", "CrossEntropyLoss", "Dense", "DistillationLoss", "Embedding", "Embedding_Op",
     "Flatten", "Flatten_Op", "GlobalAvgPool2d", "GlobalAvgPool2d_Op", "GradientOp", "Graph", "GroupNorm", "GroupNorm_Op", "LINEAR_BACKENDS", "Layer", "LeakyReLU", "Linear", "MBGD",
-    "MSELoss", "MaxPool2d", "MaxPool2d_Op", "NATIVE_BACKENDS", "Node", "Optimizer", "ParameterGroups",
+    "MSELoss", "MaxPool2d", "MaxPool2d_Op", "Muon", "NATIVE_BACKENDS", "Node", "Optimizer", "ParameterGroups",
     "RecordedStep", "ReLU", "ResNet18", "Variable",
     "apply_graph_optimizations", "cuda_available", "embedding", "fused", "get_device", "group_norm", "logits",
     "make_initializer", "native", "orthogonal", "set_device",

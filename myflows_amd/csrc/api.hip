@@ -1459,4 +1459,39 @@ MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, 
                              as_ptr<void>(workspace), as_stream(stream));
 }
 
+static_assert(sizeof(mfh_muon_tensor) == sizeof(MuonTensor), "the C table is read as MuonTensor rows");
+
+static int require_muon(const mfh_muon_tensor* tensors, int count, std::vector<MuonTensor>& table) {
+    MFH_REQUIRE(count >= 0 && (count == 0 || tensors), "a Muon step received a null table");
+    for (int i = 0; i < count; ++i) {
+        const mfh_muon_tensor& t = tensors[i];
+        MFH_REQUIRE(t.rows > 0 && t.cols > 0 && t.rows <= ORTHOGONAL_SIDE_LIMIT && t.cols <= ORTHOGONAL_SIDE_LIMIT &&
+                        fits_index(static_cast<std::int64_t>(t.rows) * t.cols),
+                    "sides of a parameter out of range");
+        table.push_back({as_ptr<float>(t.param), as_ptr<const float>(t.grad), as_ptr<float>(t.momentum), t.rows, t.cols, t.keep, t.rate});
+    }
+    return OK;
+}
+
+MFH_API std::int64_t mfh_muon_workspace(const mfh_muon_tensor* tensors, int count) {
+    std::vector<MuonTensor> table;
+    if (require_muon(tensors, count, table) != OK) return -1;
+    return muon_workspace(table.data(), count);
+}
+
+MFH_API int mfh_muon_step(const mfh_muon_tensor* tensors, int count, float momentum, int nesterov, float grad_scale, int steps,
+                          float a, float b, float c, float eps, std::uint64_t workspace, std::int64_t workspace_bytes,
+                          std::uint64_t counters, std::uint64_t stream) {
+    MFH_TRY(require_ready());
+    MFH_REQUIRE(steps > 0 && steps <= ORTHOGONAL_STEPS_MAX, "number of steps out of range");
+    MFH_REQUIRE(eps >= 0.0f, "eps must not be negative");
+    std::vector<MuonTensor> table;
+    MFH_TRY(require_muon(tensors, count, table));
+    for (const MuonTensor& t : table) MFH_REQUIRE(t.param && t.grad && t.momentum, "a Muon step received a null buffer");
+    MFH_REQUIRE(count == 0 || (counters && workspace && workspace_bytes >= muon_workspace(table.data(), count)),
+                "Muon workspace too small");
+    const MuonSteps o{OrthogonalSteps{steps, a, b, c, eps, as_ptr<unsigned>(counters)}, momentum, grad_scale, nesterov != 0};
+    return launch_muon(table.data(), count, o, as_ptr<void>(workspace), as_stream(stream));
+}
+
 }  // extern "C"

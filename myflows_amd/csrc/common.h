@@ -673,4 +673,20 @@ std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count); 
 int launch_orthogonal(const OrthogonalMatrix* matrices, int count, int type, const OrthogonalSteps& o, void* workspace,
                       hipStream_t stream);
 
+// One parameter of a Muon step: m = momentum m + g; p = keep p - rate orthogonalised(g + momentum m, or m).
+struct MuonTensor {
+    float* param;
+    const float* grad;
+    float* momentum;
+    int rows, cols;
+    float keep, rate;
+};
+struct MuonSteps {
+    OrthogonalSteps orthogonal;
+    float momentum, grad_scale;
+    bool nesterov;
+};
+std::int64_t muon_workspace(const MuonTensor* tensors, int count);  // bytes
+int launch_muon(const MuonTensor* tensors, int count, const MuonSteps& o, void* workspace, hipStream_t stream);
+
 }  // namespace mfh

@@ -302,9 +302,9 @@ constexpr int SQUARES_EACH = 16384;  // elements of a workgroup, while they are 
 constexpr int SQUARES_BLOCKS = 256;
 
 template <typename Group>
-__device__ __forceinline__ int item_of(const Group& group, int block) {
+__device__ __forceinline__ int item_of(const Group& group, unsigned block) {
     int item = 0;
-    while (block >= group.first_block[item + 1]) ++item;
+    while (block >= static_cast<unsigned>(group.first_block[item + 1])) ++item;
     return item;
 }
 
@@ -510,15 +510,102 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
     return OK;
 }
 
+// ---- the optimiser's step around it -----------------------------------------------------------
+struct MomentumGroup {
+    MuonTensor t[GROUP];
+    float* direction[GROUP];
+    unsigned first_block[GROUP + 1];
+    float momentum, grad_scale;
+    int nesterov;
+};
+static_assert(sizeof(MomentumGroup) <= 4096, "descriptors must fit the kernel arguments");
+
+constexpr int ELEMENTWISE = 4;  // elements of a thread
+
+template <typename F>
+__device__ __forceinline__ void each_element(const MomentumGroup& group, F&& f) {
+    const int item = item_of(group, blockIdx.x);
+    const MuonTensor& t = group.t[item];
+    const std::int64_t size = static_cast<std::int64_t>(t.rows) * t.cols;
+    const std::int64_t first = static_cast<std::int64_t>(blockIdx.x - group.first_block[item]) * THREADS * ELEMENTWISE + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < ELEMENTWISE; ++k)
+        if (first + k * THREADS < size) f(t, group.direction[item], first + k * THREADS);
+}
+
+// m = momentum m + g; the direction is g + momentum m (Nesterov's), or m.
+__global__ __launch_bounds__(THREADS) void momentum_kernel(MomentumGroup group) {
+    each_element(group, [&](const MuonTensor& t, float* direction, std::int64_t at) {
+        const float g = t.grad[at] * group.grad_scale, m = group.momentum * t.momentum[at] + g;
+        t.momentum[at] = m;
+        direction[at] = group.nesterov ? g + group.momentum * m : m;
+    });
+}
+
+// p = keep p - rate direction, of the direction made orthogonal.
+__global__ __launch_bounds__(THREADS) void descend_kernel(MomentumGroup group) {
+    each_element(group, [&](const MuonTensor& t, const float* direction, std::int64_t at) {
+        t.param[at] = t.keep * t.param[at] - t.rate * direction[at];
+    });
+}
+
+std::int64_t group_bytes(const OrthogonalMatrix* matrices, int count) {
+    std::int64_t bytes = PARTS_BYTES;
+    for (int i = 0; i < count; ++i) bytes += Plan(matrices[i]).bytes();
+    return bytes;
+}
+
+OrthogonalMatrix direction_of(const MuonTensor& t, float* direction) {
+    return {direction, direction, t.cols, t.cols, t.rows, t.cols};
+}
+
+std::int64_t direction_bytes(const MuonTensor& t) { return (static_cast<std::int64_t>(t.rows) * t.cols * 4 + 255) / 256 * 256; }
+
+int run_muon_group(const MuonTensor* tensors, int count, const MuonSteps& o, char* workspace, hipStream_t stream) {
+    MomentumGroup group{};
+    group.momentum = o.momentum, group.grad_scale = o.grad_scale, group.nesterov = o.nesterov;
+    std::vector<OrthogonalMatrix> directions;
+    for (int i = 0; i < count; ++i) {
+        group.t[i] = tensors[i];
+        group.direction[i] = reinterpret_cast<float*>(workspace);
+        workspace += direction_bytes(tensors[i]);
+        directions.push_back(direction_of(tensors[i], group.direction[i]));
+        group.first_block[i + 1] =
+            group.first_block[i] + blocks_for(static_cast<std::int64_t>(tensors[i].rows) * tensors[i].cols, THREADS * ELEMENTWISE);
+    }
+    launch(momentum_kernel, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
+    MFH_TRY(MFH_CHECK_LAUNCH("muon momentum", stream));
+    MFH_TRY(run_group<float>(directions.data(), count, o.orthogonal, workspace, stream));
+    launch(descend_kernel, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
+    return MFH_CHECK_LAUNCH("muon step", stream);
+}
+
 }  // namespace
+
+std::int64_t muon_workspace(const MuonTensor* tensors, int count) {
+    std::int64_t most = 0;
+    for (int i = 0; i < count; i += GROUP) {
+        const int here = std::min(count - i, GROUP);
+        std::vector<OrthogonalMatrix> directions;
+        std::int64_t bytes = 0;
+        for (int k = 0; k < here; ++k) {
+            directions.push_back(direction_of(tensors[i + k], nullptr));
+            bytes += direction_bytes(tensors[i + k]);
+        }
+        most = std::max(most, bytes + group_bytes(directions.data(), here));
+    }
+    return most;
+}
+
+int launch_muon(const MuonTensor* tensors, int count, const MuonSteps& o, void* workspace, hipStream_t stream) {
+    for (int i = 0; i < count; i += GROUP)
+        MFH_TRY(run_muon_group(tensors + i, std::min(GROUP, count - i), o, static_cast<char*>(workspace), stream));
+    return OK;
+}
 
 std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count) {
     std::int64_t most = 0;
-    for (int i = 0; i < count; i += GROUP) {
-        std::int64_t bytes = 0;
-        for (int k = i; k < std::min(count, i + GROUP); ++k) bytes += Plan(matrices[k]).bytes();
-        most = std::max(most, bytes + PARTS_BYTES);
-    }
+    for (int i = 0; i < count; i += GROUP) most = std::max(most, group_bytes(matrices + i, std::min(GROUP, count - i)));
     return most;
 }
 

@@ -82,11 +82,18 @@ class OrthogonalMatrix(ctypes.Structure):
                 ("out_stride", ctypes.c_int64), ("rows", ctypes.c_int32), ("cols", ctypes.c_int32)]
 
 
+class MuonTensor(ctypes.Structure):
+    """One row of the mfh_muon_step table (include/mfhip.h)."""
+    _fields_ = [("param", ctypes.c_uint64), ("grad", ctypes.c_uint64), ("momentum", ctypes.c_uint64),
+                ("rows", ctypes.c_int32), ("cols", ctypes.c_int32), ("keep", ctypes.c_float), ("rate", ctypes.c_float)]
+
+
 # Argument codes: p device pointer / stream (uint64), i int32, q int64, f float, d double,
-# t pointer to an AdamTensor table, m pointer to an OrthogonalMatrix table, P pointer to int32 (host array), U pointer to uint64 (host array),
+# t pointer to an AdamTensor table, m pointer to an OrthogonalMatrix table,
+# u pointer to a MuonTensor table, P pointer to int32 (host array), U pointer to uint64 (host array),
 # L pointer to int64.
 _CTYPE = {"p": ctypes.c_uint64, "i": ctypes.c_int, "q": ctypes.c_int64, "f": ctypes.c_float, "d": ctypes.c_double,
-          "t": ctypes.POINTER(AdamTensor), "m": ctypes.POINTER(OrthogonalMatrix), "P": ctypes.POINTER(ctypes.c_int), "s": ctypes.c_char_p, "-": None,
+          "t": ctypes.POINTER(AdamTensor), "m": ctypes.POINTER(OrthogonalMatrix), "u": ctypes.POINTER(MuonTensor), "P": ctypes.POINTER(ctypes.c_int), "s": ctypes.c_char_p, "-": None,
           "U": ctypes.POINTER(ctypes.c_uint64), "L": ctypes.POINTER(ctypes.c_int64)}
 _CONV = "i" * 13
 # symbol: (result code, argument codes); mirrors include/mfhip.h.
@@ -158,6 +165,8 @@ _SIGNATURES = {
     "mfh_group_norm_backward": ("i", "ppiqiii" + "pppp" + "i" + "ppp" + "iii" + "pqp"),
     "mfh_orthogonalize_workspace": ("q", "mi"),
     "mfh_orthogonalize": ("i", "mii" + "iffff" + "pqpp"),
+    "mfh_muon_workspace": ("q", "ui"),
+    "mfh_muon_step": ("i", "ui" + "fifi" + "ffff" + "pqpp"),
     "mfh_embedding": ("i", "piqiq" + "piqq" + "fpqp"),
     "mfh_embedding_workspace": ("q", "qqii"),
     "mfh_embedding_backward": ("i", "piqiq" + "piqqf" + "piqi" + "pqp"),

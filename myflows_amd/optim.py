@@ -6,7 +6,9 @@ the interface of the reference's ``train/opt.py:11-281`` and ``train/param_group
 clears the accumulators. Parameter groups give their parameters an absolute learning rate or a
 multiple of the optimiser's, and a weight decay. Adam keeps zero-initialised moments and a step
 count per parameter and runs as one multi-tensor libmfhip launch per 48 tensors with the
-reference's float32 rounding order (``fused.adam_update_many``).
+reference's float32 rounding order (``fused.adam_update_many``). Muon (no counterpart in the reference) makes the
+momentum of each matrix orthogonal, all matrices together (``orthogonal.muon_update_many``), and leaves the other
+parameters to Adam.
 """
 
 from __future__ import annotations
@@ -16,6 +18,7 @@ import os
 
 from .fused import adam_update, adam_update_many
 from .graph import Variable
+from .orthogonal import muon_update_many
 
 
 def _non_negative(value, field):
@@ -183,21 +186,75 @@ class Adam(Optimizer):
 
     def _update(self):
         self.t += 1
-        # The averaging over the accumulated steps rides in the kernel as a gradient scale.
-        scale = 1.0 if self.acc_no in (0, 1) else 1.0 / self.acc_no
+        self._adam(self._updated())
+
+    def _updated(self):
+        """The trainable parameters with a gradient, in the graph's order."""
+        return [node for node in self.graph.nodes if isinstance(node, Variable) and node.trainable
+                and self.acc_gradient.get(node) is not None]
+
+    def _grad_scale(self):
+        """The averaging over the accumulated steps, which rides in the kernels."""
+        return 1.0 if self.acc_no in (0, 1) else 1.0 / self.acc_no
+
+    def _adam(self, nodes, learning_rate=None):
         updates = []
-        for node in self.graph.nodes:
-            if not (isinstance(node, Variable) and node.trainable):
-                continue
-            gradient = self.acc_gradient.get(node)
-            if gradient is not None:
-                lr, decay = self.groups.options(node, self.learning_rate)
-                first, second, step = self._state_of(node)
-                updates.append((node.value, gradient, first, second, lr, decay, step))
+        for node in nodes:
+            lr, decay = self.groups.options(node, self.learning_rate if learning_rate is None else learning_rate)
+            first, second, step = self._state_of(node)
+            updates.append((node.value, self.acc_gradient[node], first, second, lr, decay, step))
         options = dict(beta1=self.beta_1, beta2=self.beta_2, eps=self.eps)
+        scale = self._grad_scale()
         if self.multi_tensor:
             adam_update_many(updates, grad_scale=scale, **options)
             return
         for param, gradient, first, second, lr, decay, step in updates:
             adam_update(param, gradient, first, second, lr=lr, step=step, grad_scale=scale, weight_decay=decay,
                         **options)
+
+
+class Muon(Adam):
+    """Momentum made orthogonal (Jordan et al., 2024) for the matrices, Adam for the other parameters.
+
+    For a matrix: b = momentum b + g, and p = (1 - lr decay) p - lr s O, where O is the orthogonalised
+    g + momentum b (b without ``nesterov``; ``orthogonal.orthogonalize``), s = sqrt(max(1, outputs / inputs)) and
+    g the averaged gradient. Unlike Adam's, the group's weight decay acts on p itself. Matrices are the
+    parameters of two dimensions or more with no side of 1 (a Dense weight, inputs by outputs; a convolution's
+    kernel, outputs by the rest), but for those in ``adam_params``: usually the first layer's and the head's. The rest
+    are Adam's, with ``adam_learning_rate`` where no group names one. ``buffers`` holds the momenta."""
+
+    def __init__(self, graph, learning_rate=0.02, momentum=0.95, *, nesterov=True, steps=5, adam_params=(),
+                 adam_learning_rate=1e-3, beta_1=0.9, beta_2=0.999, eps=1e-8, param_groups=None, multi_tensor=None):
+        super().__init__(graph, learning_rate, beta_1, beta_2, eps, param_groups=param_groups, multi_tensor=multi_tensor)
+        self.momentum, self.nesterov, self.steps = float(momentum), bool(nesterov), int(steps)
+        if not 0.0 <= self.momentum < 1.0:
+            raise ValueError("momentum must lie in [0, 1)")
+        if not 1 <= self.steps <= 64:
+            raise ValueError("steps must lie between 1 and 64")
+        self.adam_learning_rate = _non_negative(adam_learning_rate, "adam_learning_rate")
+        self.adam_params = frozenset(adam_params)
+        if not self.adam_params <= set(graph.nodes):
+            raise ValueError("adam_params must be parameters of the graph")
+        self.buffers = {}
+
+    def _is_matrix(self, node):
+        shape = node.value.shape
+        return node not in self.adam_params and len(shape) >= 2 and shape[0] > 1 and math.prod(shape[1:]) > 1
+
+    def _update(self):
+        import torch
+        self.t += 1
+        nodes = self._updated()
+        self._adam([node for node in nodes if not self._is_matrix(node)], self.adam_learning_rate)
+        updates = []
+        for node in nodes:
+            if not self._is_matrix(node):
+                continue
+            lr, decay = self.groups.options(node, self.learning_rate)
+            if node not in self.buffers:
+                self.buffers[node] = torch.zeros_like(node.value)
+            shape = node.value.shape
+            outputs, inputs = (shape[1], shape[0]) if len(shape) == 2 else (shape[0], math.prod(shape[1:]))
+            updates.append((node.value, self.acc_gradient[node], self.buffers[node], lr * math.sqrt(max(1.0, outputs / inputs)),
+                            lr * decay))
+        muon_update_many(updates, momentum=self.momentum, nesterov=self.nesterov, grad_scale=self._grad_scale(), steps=self.steps)

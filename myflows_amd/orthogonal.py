@@ -113,3 +113,41 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
 def orthogonalize(matrix, *, steps=STEPS, coefficients=COEFFICIENTS, eps=1e-7, out=None):
     """``orthogonalize_many`` of one matrix."""
     return orthogonalize_many([matrix], steps=steps, coefficients=coefficients, eps=eps, out=None if out is None else [out])[0]
+
+
+@lru_cache(maxsize=64)
+def _muon_workspace(shapes):
+    table = (native.MuonTensor * len(shapes))(*((0, 0, 0, rows, cols, 0.0, 0.0) for rows, cols in shapes))
+    return native.workspace_bytes("mfh_muon_workspace", table, len(shapes))
+
+
+def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, steps=STEPS, coefficients=COEFFICIENTS,
+                     eps=1e-7):
+    """One Muon step, in place, for (param, grad, buffer, rate, decay) tuples of float32 tensors of a shape with two
+    dimensions or more: with g = grad * grad_scale, buffer = momentum * buffer + g; the parameter becomes
+    (1 - decay) param - rate O, with O the orthogonalised g + momentum * buffer (buffer without nesterov). A strided
+    param or buffer is updated through a contiguous copy that is written back; no two of the tensors may overlap."""
+    (a, b, c), steps = _polynomial(coefficients, steps)
+    rows, held, back = [], [], []
+    for param, grad, buffer, rate, decay in updates:
+        tensors = [native._device_f32(t, name) for t, name in ((param, "param"), (grad, "grad"), (buffer, "buffer"))]
+        if any(t.shape != param.shape for t in tensors):
+            raise ValueError("Muon updates tensors of the parameter's shape")
+        shape = tuple(_matrix(tensors[0], "param").shape)
+        native._on_current_device(*tensors)
+        if not param.numel():
+            continue
+        held.append(tensors)
+        back += [(old, new) for old, new in ((param, tensors[0]), (buffer, tensors[2])) if old is not new]
+        rows.append((*(t.data_ptr() for t in tensors), *shape, 1.0 - decay, float(rate)))
+    if not rows:
+        return
+    spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for tensors in held for t in tensors)
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+        raise ValueError("the tensors of a Muon step must not overlap")
+    table = (native.MuonTensor * len(rows))(*rows)
+    workspace, size = native.byte_workspace(_muon_workspace(tuple(row[3:5] for row in rows)))
+    native._call("mfh_muon_step", table, len(rows), float(momentum), int(bool(nesterov)), float(grad_scale), steps, a, b, c,
+                 float(eps), workspace, size, native.stream_counters(), native._stream())
+    for old, new in back:
+        old.copy_(new)
