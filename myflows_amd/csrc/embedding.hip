@@ -12,6 +12,7 @@
 
 #include "common.h"
 #include "typed.h"
+#include "wave.h"
 
 namespace mfh {
 namespace {
@@ -96,9 +97,6 @@ struct Sorted {
 __host__ __device__ __forceinline__ int slot_of(const Sorted& s, int token) {
     return (token & ((1 << s.classes_log) - 1)) * s.slice + (token >> s.classes_log);
 }
-
-// What one lane of a wave wrote to LDS is there for the others' next read: the wave's accesses run in order.
-__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // each(whether the token is of the class, its place there, position) for the positions begin .. end - 1, a wave's
 // width at a time; adds this lane's positions of lower classes to `below`.

@@ -11,7 +11,7 @@
 // matrix cores' float32 rate is below it. X and B are at most a few: values are held 2^12 times as large,
 // which keeps hi out of float16's subnormals and lo's steps below 2^-36.
 //
-// Layout. A matrix lies in rows padded to whole tiles, zeros there; a row's 32 neighbouring values are 64 bytes of
+// Layout. A matrix lies in memory with both sides padded to whole tiles, zeros behind the last value; a row's 32 neighbouring values are 64 bytes of
 // hi and 64 of lo, so that one step of a product reads a cache line of each row. Every product is of the form A B^T
 // with rows of both read along k: X is kept as X and as X^T. Symmetric products form the tiles on and below the
 // diagonal and write them to both places.
@@ -23,6 +23,7 @@
 #include "common.h"
 #include "hand_over.h"
 #include "typed.h"
+#include "wave.h"
 
 namespace mfh {
 namespace {
@@ -45,7 +46,7 @@ constexpr std::int64_t PARTS_BYTES = 48 << 20;  // workspace of split tiles' sum
 
 // out = alpha A B^T + beta add, or the caller's matrix in its type.
 struct Product {
-    const _Float16* a;  // rows of A and of B, ksteps * ROW_STEP halves each
+    const _Float16* a;  // rows of A and of B
     const _Float16* b;
     const _Float16* add_t;  // optional, transposed (a symmetric one is its own)
     _Float16* out;          // optional
@@ -55,10 +56,11 @@ struct Product {
     float* parts;        // where the steps of a tile are split over workgroups: their sums,
     unsigned* arrived;   // and how many have come, a tile
     float alpha, beta;
-    int ksteps, m_tiles, n_tiles;  // tiles of its own side
+    int ksteps, m_tiles, n_tiles;  // what holds values, in steps and in tiles of its own side
+    int k_padded, m_padded, n_padded;  // the sides as they lie in memory
     int splits;
     int rows, cols;                // of the caller's matrix, the shorter side as rows
-    bool symmetric, small, tall;   // tall: the caller's matrix is the transposed result
+    bool over_longer, symmetric, small, tall;  // the sums' side; tall: the caller's matrix is the transposed result
 };
 
 struct ProductGroup {
@@ -86,58 +88,127 @@ __device__ __forceinline__ half8 operand(const _Float16* lds, int row, int part)
     return *reinterpret_cast<const half8*>(lds + row * ROW_STEP + (part ^ (row & 7)) * 8);
 }
 
-// Value and place of the split halves of 4 values, neighbours along i, in row j of a matrix of `pitch` halves a row.
-__device__ __forceinline__ void write_four(_Float16* to, std::int64_t row, std::int64_t pitch, int i, const float (&v)[4]) {
-    half4 hi, lo;
+// A wave's scratch in LDS: 32 rows of a matrix as they lie in memory, 64 bytes of hi and 64 of lo each, their eight
+// 16-byte parts stored as the operands' are; or 32 x 33 floats. Through it the lanes read and write whole lines of
+// memory: straight from the registers, where a lane has four neighbours of one column, a line took 8 stores of 8
+// bytes, or 64 of two.
+constexpr int SCRATCH = 32 * 33 * 2;  // halves
+
+__device__ __forceinline__ _Float16* scratch_at(_Float16* scratch, int row, int value, int low) {
+    return scratch + row * ROW_STEP + ((value / 8 + 4 * low) ^ (row & 7)) * 8 + value % 8;
+}
+
+// Part lane % 8 of rows lane / 8 + 8 r: of the scratch, or of the 32 x 32 piece at `at` of a matrix.
+__device__ __forceinline__ half8* scratch_part(_Float16* scratch, int r) {
+    const int lane = threadIdx.x & 63, row = 8 * r + lane / 8;
+    return reinterpret_cast<half8*>(scratch + row * ROW_STEP + ((lane & 7) ^ (row & 7)) * 8);
+}
+template <typename Half>
+__device__ __forceinline__ Half* piece_part(Half* matrix, int row0, int col0, std::int64_t pitch, int r) {
+    const int lane = threadIdx.x & 63;
+    return matrix + (row0 + 8 * r + lane / 8) * pitch + col0 / K_STEP * ROW_STEP + (lane & 7) * 8;
+}
+
+__device__ __forceinline__ void write_scratch(_Float16* scratch, _Float16* matrix, int row0, int col0, std::int64_t pitch) {
+    wave_order();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        hi[k] = static_cast<_Float16>(v[k]);
-        lo[k] = static_cast<_Float16>(v[k] - static_cast<float>(hi[k]));
+    for (int r = 0; r < 4; ++r) *reinterpret_cast<half8*>(piece_part(matrix, row0, col0, pitch, r)) = *scratch_part(scratch, r);
+    wave_order();
+}
+
+template <typename T>
+__device__ __forceinline__ void write_final(const Product& p, const float (&v)[16], int i0, int j0, _Float16* scratch) {
+    const int lane = threadIdx.x & 63;
+    T* out = static_cast<T*>(p.final);
+    if (!p.tall) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int i = i0 + e / 4 * 8 + lane / 32 * 4 + e % 4, j = j0 + (lane & 31);
+            if (i < p.rows && j < p.cols) out[i * p.final_stride + j] = static_cast<T>(v[e]);
+        }
+        return;
     }
-    _Float16* at = to + row * pitch + i / K_STEP * ROW_STEP + i % K_STEP;
-    *reinterpret_cast<half4*>(at) = hi;
-    *reinterpret_cast<half4*>(at + K_STEP) = lo;
+    float* tile = reinterpret_cast<float*>(scratch);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) tile[(lane & 31) * 33 + e / 4 * 8 + lane / 32 * 4 + e % 4] = v[e];
+    wave_order();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int row = e * 2 + lane / 32, i = i0 + (lane & 31), j = j0 + row;
+        if (i < p.rows && j < p.cols) out[j * p.final_stride + i] = static_cast<T>(tile[row * 33 + (lane & 31)]);
+    }
+    wave_order();
 }
 
-template <typename T>
-__device__ __forceinline__ void write_final(const Product& p, int i, int j, float v) {
-    if (i >= p.rows || j >= p.cols) return;
-    static_cast<T*>(p.final)[(p.tall ? j * p.final_stride + i : i * p.final_stride + j)] = static_cast<T>(v);
-}
-
-// One 32 x 32 piece of a tile: this lane's column j and rows i0 + 8 q + 4 (lane / 32) + 0 .. 3.
-template <typename T>
-__device__ __forceinline__ void write_piece(const Product& p, const float16v& sum, int i0, int j0, int side, bool mirrored) {
-    const int lane = threadIdx.x & 63, j = j0 + (lane & 31);
-    const std::int64_t pitch = static_cast<std::int64_t>(p.n_tiles) * side * 2, pitch_t = static_cast<std::int64_t>(p.m_tiles) * side * 2;
+// A wave's pieces of 32 x 32 from (i0, j0) on. A lane has column lane % 32 of a piece and its rows 8 q + 4 (lane / 32)
+// + 0 .. 3.
+template <int PIECES, typename T>
+__device__ __forceinline__ void write_pieces(const Product& p, const float16v (&sum)[PIECES][PIECES], int i_first, int j_first,
+                                             bool mirrored, _Float16* scratch) {
+    const int lane = threadIdx.x & 63, column = lane & 31, high = lane / 32;
+    const std::int64_t pitch = p.n_padded * 2, pitch_t = p.m_padded * 2;
     const float alpha = p.alpha * UNSCALE;
+    half8 add[PIECES][PIECES][4];
+    if (p.add_t) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int i = i0 + 8 * q + 4 * (lane / 32);
-        float v[4];
+        for (int pi = 0; pi < PIECES; ++pi)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = sum[4 * q + k] * alpha;
-        if (p.add_t) {
-            const _Float16* at = p.add_t + j * pitch_t + i / K_STEP * ROW_STEP + i % K_STEP;
-            const half4 hi = *reinterpret_cast<const half4*>(at), lo = *reinterpret_cast<const half4*>(at + K_STEP);
+            for (int pj = 0; pj < PIECES; ++pj)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] += p.beta * (static_cast<float>(hi[k]) + static_cast<float>(lo[k]));
-        }
-        if (p.final) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) write_final<T>(p, i + k, j, v[k] * UNSCALE);
-            continue;
-        }
-        if (p.out_t) write_four(p.out_t, j, pitch_t, i, v);
-        if (!mirrored) continue;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const _Float16 hi = static_cast<_Float16>(v[k]);
-            _Float16* at = p.out + (i + k) * pitch + j / K_STEP * ROW_STEP + j % K_STEP;
-            at[0] = hi;
-            at[K_STEP] = static_cast<_Float16>(v[k] - static_cast<float>(hi));
-        }
+                for (int r = 0; r < 4; ++r)
+                    add[pi][pj][r] = *reinterpret_cast<const half8*>(piece_part(p.add_t, j_first + 32 * pj, i_first + 32 * pi, pitch_t, r));
     }
+#pragma unroll
+    for (int pi = 0; pi < PIECES; ++pi)
+#pragma unroll
+        for (int pj = 0; pj < PIECES; ++pj) {
+            const int i0 = i_first + 32 * pi, j0 = j_first + 32 * pj;
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = sum[pi][pj][e] * alpha;
+            if (p.add_t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) *scratch_part(scratch, r) = add[pi][pj][r];
+                wave_order();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const half4 hi = *reinterpret_cast<const half4*>(scratch_at(scratch, column, 8 * q + 4 * high, 0));
+                    const half4 lo = *reinterpret_cast<const half4*>(scratch_at(scratch, column, 8 * q + 4 * high, 1));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[4 * q + k] += p.beta * (static_cast<float>(hi[k]) + static_cast<float>(lo[k]));
+                }
+                wave_order();
+            }
+            if (p.final) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] *= UNSCALE;
+                write_final<T>(p, v, i0, j0, scratch);
+                continue;
+            }
+            half4 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                hi[e / 4][e % 4] = static_cast<_Float16>(v[e]);
+                lo[e / 4][e % 4] = static_cast<_Float16>(v[e] - static_cast<float>(hi[e / 4][e % 4]));
+            }
+            if (p.out_t) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    *reinterpret_cast<half4*>(scratch_at(scratch, column, 8 * q + 4 * high, 0)) = hi[q];
+                    *reinterpret_cast<half4*>(scratch_at(scratch, column, 8 * q + 4 * high, 1)) = lo[q];
+                }
+                write_scratch(scratch, p.out_t, j0, i0, pitch_t);
+            }
+            if (mirrored) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = e / 4 * 8 + 4 * high + e % 4;
+                    *scratch_at(scratch, row, column, 0) = hi[e / 4][e % 4];
+                    *scratch_at(scratch, row, column, 1) = lo[e / 4][e % 4];
+                }
+                write_scratch(scratch, p.out, i0, j0, pitch);
+            }
+        }
 }
 
 // The sums of a tile's parts, in their order, by the workgroup that comes last; false for the others.
@@ -184,7 +255,7 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
     constexpr int PIECES = SIDE / 64, STAGE = SIDE * ROW_STEP;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wave_i = wave / 2 * (SIDE / 2), wave_j = wave % 2 * (SIDE / 2);
-    const std::int64_t pitch = static_cast<std::int64_t>(p.ksteps) * ROW_STEP;
+    const std::int64_t pitch = p.k_padded * 2;
     const _Float16* a = p.a + static_cast<std::int64_t>(tile_i) * SIDE * pitch;
     const _Float16* b = p.b + static_cast<std::int64_t>(tile_j) * SIDE * pitch;
     const int begin = static_cast<int>(static_cast<long long>(p.ksteps) * part / p.splits);
@@ -236,7 +307,8 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
         multiply(second);
         __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the rows that were staged beyond the last step have arrived too:
+    __syncthreads();                     // LDS is free
     if (p.splits > 1) {
         float flat[PIECES * PIECES * 16];
 #pragma unroll
@@ -245,12 +317,8 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
 #pragma unroll
         for (int e = 0; e < PIECES * PIECES * 16; ++e) sum[e / 16 / PIECES][e / 16 % PIECES][e % 16] = flat[e];
     }
-    const bool mirrored = p.out && (!p.symmetric || tile_i != tile_j);
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j)
-            write_piece<T>(p, sum[i][j], tile_i * SIDE + wave_i + i * 32, tile_j * SIDE + wave_j + j * 32, SIDE, mirrored);
+    write_pieces<PIECES, T>(p, sum, tile_i * SIDE + wave_i, tile_j * SIDE + wave_j, p.out && (!p.symmetric || tile_i != tile_j),
+                            lds + wave * SCRATCH);
 }
 
 // LARGEST: the side of the launch's largest tiles, for which LDS is held.
@@ -397,11 +465,11 @@ int splits_of(int ksteps, std::int64_t launch_steps, std::int64_t slots, bool sm
 }
 
 struct Plan {
-    int side, s, l;              // padded
+    int side, s, l;              // sides as they lie in memory
+    int shorter, longer;         // and as they are
     std::int64_t x, square;      // bytes of X and of a square matrix
     int square_blocks;
-    explicit Plan(const OrthogonalMatrix& m) {
-        const int shorter = std::min(m.rows, m.cols), longer = std::max(m.rows, m.cols);
+    explicit Plan(const OrthogonalMatrix& m) : shorter(std::min(m.rows, m.cols)), longer(std::max(m.rows, m.cols)) {
         side = side_of(shorter);
         s = (shorter + side - 1) / side * side, l = (longer + side - 1) / side * side;
         x = static_cast<std::int64_t>(s) * l * 4, square = static_cast<std::int64_t>(s) * s * 4;
@@ -469,7 +537,11 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
             p.alpha = 1.0f, p.small = plan.side == SMALL, p.tall = m.rows > m.cols;
             p.rows = std::min(m.rows, m.cols), p.cols = std::max(m.rows, m.cols);
             describe(i, p);
-            p.m_tiles = plan.s / plan.side, p.n_tiles = p.symmetric ? p.m_tiles : plan.l / plan.side;
+            p.k_padded = p.over_longer ? plan.l : plan.s;
+            p.ksteps = ((p.over_longer ? plan.longer : plan.shorter) + K_STEP - 1) / K_STEP;
+            p.m_padded = plan.s, p.n_padded = p.symmetric ? plan.s : plan.l;
+            p.m_tiles = (plan.shorter + plan.side - 1) / plan.side;
+            p.n_tiles = p.symmetric ? p.m_tiles : (plan.longer + plan.side - 1) / plan.side;
             steps += static_cast<std::int64_t>(tiles(p)) * p.ksteps;
         }
         char* part = parts;
@@ -493,16 +565,16 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         const int from = step & 1;
         MFH_TRY(products([&](int i, Product& p) {
             const Buffers& at = buffers[i];
-            p.symmetric = true, p.a = p.b = at.x, p.out = p.out_t = at.g, p.ksteps = plans[i].l / K_STEP;
+            p.symmetric = true, p.a = p.b = at.x, p.out = p.out_t = at.g, p.over_longer = true;
         }));
         MFH_TRY(products([&](int i, Product& p) {
             const Buffers& at = buffers[i];
-            p.symmetric = true, p.a = p.b = p.add_t = at.g, p.out = p.out_t = at.p, p.ksteps = plans[i].s / K_STEP;
+            p.symmetric = true, p.a = p.b = p.add_t = at.g, p.out = p.out_t = at.p;
             p.alpha = o.c, p.beta = o.b;
         }));
         MFH_TRY(products([&](int i, Product& p) {
             const Buffers& at = buffers[i];
-            p.a = at.p, p.b = p.add_t = at.x_t[from], p.ksteps = plans[i].s / K_STEP, p.beta = o.a;
+            p.a = at.p, p.b = p.add_t = at.x_t[from], p.beta = o.a;
             if (step + 1 == o.steps) p.final = matrices[i].out, p.final_stride = matrices[i].out_stride;
             else p.out = at.x, p.out_t = at.x_t[from ^ 1];
         }));

@@ -1,4 +1,4 @@
-// Reductions over the 64 lanes of a wave, in a fixed order: four cross-lane steps within each row of 16 lanes
+// The 64 lanes of a wave. Reductions over them, in a fixed order: four cross-lane steps within each row of 16 lanes
 // (quad permutes and mirrors, no LDS), then the four rows through scalar registers. Every lane gets the result.
 #pragma once
 
@@ -28,5 +28,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ float wave_max(float v) {
     return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
+
+// What one lane of a wave wrote to LDS is there for the others' next read: the wave's accesses run in order.
+__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 }  // namespace mfh
