@@ -31,8 +31,6 @@ namespace {
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(1))) void GlobalBytes;
-typedef __attribute__((address_space(3))) void LocalBytes;
 
 constexpr int THREADS = 256;
 constexpr int K_STEP = 32;          // values of a row in one step: 128 bytes, hi and lo
@@ -70,22 +68,38 @@ struct ProductGroup {
 };
 static_assert(sizeof(ProductGroup) <= 4096, "descriptors must fit the kernel arguments");
 
-// Copies ROWS rows of one step to LDS, 16 bytes a lane. A row's eight 16-byte parts are stored in the order
-// part ^ (row % 8), so that neighbouring rows' equal parts lie in other banks.
-template <int ROWS>
-__device__ __forceinline__ void stage_rows(const _Float16* __restrict__ rows, std::int64_t pitch, int step, _Float16* lds) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    constexpr int EACH = ROWS / 8 / (THREADS / 64);  // instructions of a wave, 8 rows each
-    const _Float16* from = rows + (wave * EACH * 8 + lane / 8) * pitch + step * ROW_STEP + ((lane & 7) ^ (lane / 8)) * 8;
+// Rows lie in LDS 128 bytes apart, half of its 64 banks, their eight 16-byte parts in the order part ^ key: a 16-byte read
+// is served 16 lanes at a time, of neighbouring rows or, as the hardware pairs them, of four groups of four, and the
+// key gives those of one parity other parts.
+__device__ __forceinline__ int key_of(int row) { return row >> 1 & 7; }
+
+// One step of a tile's rows on their way through registers to LDS, 16 bytes a lane. (Loads straight to LDS would spare
+// the registers, but the compiler lets no LDS read pass one that is under way.)
+template <int SIDE>
+struct StagedRows {
+    static constexpr int EACH = SIDE / 8 / (THREADS / 64);  // instructions of a wave, 8 rows each
+    half8 v[EACH];
+
+    __device__ __forceinline__ void load(const _Float16* __restrict__ lane_rows, std::int64_t pitch, int step) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i)
-        __builtin_amdgcn_global_load_lds((const GlobalBytes*)(from + i * 8 * pitch), (LocalBytes*)(lds + (wave * EACH + i) * 8 * ROW_STEP),
-                                         16, 0, 0);
-}
+        for (int i = 0; i < EACH; ++i) v[i] = *reinterpret_cast<const half8*>(lane_rows + i * 8 * pitch + step * ROW_STEP);
+    }
+    __device__ __forceinline__ void store(_Float16* lds) const {
+        const int lane = threadIdx.x & 63, row = threadIdx.x / 64 * EACH * 8 + lane / 8;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            *reinterpret_cast<half8*>(lds + (row + i * 8) * ROW_STEP + ((lane & 7) ^ key_of(row + i * 8)) * 8) = v[i];
+    }
+    // This lane's first part of the tile's rows.
+    static __device__ __forceinline__ const _Float16* lane_rows(const _Float16* rows, std::int64_t pitch) {
+        const int lane = threadIdx.x & 63;
+        return rows + (threadIdx.x / 64 * EACH * 8 + lane / 8) * pitch + (lane & 7) * 8;
+    }
+};
 
 // The lane's 8 values of a 32 x 16 operand at LDS row `row` (its own lane % 32 included): part p of hi, or of lo.
 __device__ __forceinline__ half8 operand(const _Float16* lds, int row, int part) {
-    return *reinterpret_cast<const half8*>(lds + row * ROW_STEP + (part ^ (row & 7)) * 8);
+    return *reinterpret_cast<const half8*>(lds + row * ROW_STEP + (part ^ key_of(row)) * 8);
 }
 
 // A wave's scratch in LDS: 32 rows of a matrix as they lie in memory, 64 bytes of hi and 64 of lo each, their eight
@@ -95,13 +109,13 @@ __device__ __forceinline__ half8 operand(const _Float16* lds, int row, int part)
 constexpr int SCRATCH = 32 * 33 * 2;  // halves
 
 __device__ __forceinline__ _Float16* scratch_at(_Float16* scratch, int row, int value, int low) {
-    return scratch + row * ROW_STEP + ((value / 8 + 4 * low) ^ (row & 7)) * 8 + value % 8;
+    return scratch + row * ROW_STEP + ((value / 8 + 4 * low) ^ key_of(row)) * 8 + value % 8;
 }
 
 // Part lane % 8 of rows lane / 8 + 8 r: of the scratch, or of the 32 x 32 piece at `at` of a matrix.
 __device__ __forceinline__ half8* scratch_part(_Float16* scratch, int r) {
     const int lane = threadIdx.x & 63, row = 8 * r + lane / 8;
-    return reinterpret_cast<half8*>(scratch + row * ROW_STEP + ((lane & 7) ^ (row & 7)) * 8);
+    return reinterpret_cast<half8*>(scratch + row * ROW_STEP + ((lane & 7) ^ key_of(row)) * 8);
 }
 template <typename Half>
 __device__ __forceinline__ Half* piece_part(Half* matrix, int row0, int col0, std::int64_t pitch, int r) {
@@ -233,23 +247,31 @@ __device__ __forceinline__ bool join_parts(const Product& p, int tile, int part,
     if (!last) return false;
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) sum[i] = 0.0f;
-    for (int other = 0; other < p.splits; ++other) {
-        Two two[SUMS / 2];
+    constexpr int TOGETHER = 64 / SUMS > 1 ? 64 / SUMS : 2;  // parts whose sums are on their way at once
+    for (int first = 0; first < p.splits; first += TOGETHER) {
+        Two two[TOGETHER][SUMS / 2];
 #pragma unroll
-        for (int i = 0; i < SUMS / 2; ++i) two[i] = handed_over(parts + (static_cast<std::int64_t>(other) * (SUMS / 2) + i) * THREADS);
+        for (int k = 0; k < TOGETHER; ++k) {
+            const Two* from = parts + static_cast<std::int64_t>(min(first + k, p.splits - 1)) * (SUMS / 2) * THREADS;
 #pragma unroll
-        for (int i = 0; i < SUMS / 2; ++i) {
-            sum[2 * i] += __uint_as_float(static_cast<unsigned>(two[i]));
-            sum[2 * i + 1] += __uint_as_float(static_cast<unsigned>(two[i] >> 32));
+            for (int i = 0; i < SUMS / 2; ++i) two[k][i] = handed_over(from + i * THREADS);
+        }
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) {
+            if (first + k >= p.splits) break;
+#pragma unroll
+            for (int i = 0; i < SUMS / 2; ++i) {
+                sum[2 * i] += __uint_as_float(static_cast<unsigned>(two[k][i]));
+                sum[2 * i + 1] += __uint_as_float(static_cast<unsigned>(two[k][i] >> 32));
+            }
         }
     }
     return true;
 }
 
 // One SIDE x SIDE tile, or the steps of one part of it, by four waves of SIDE / 2 x SIDE / 2. Two steps lie in LDS, a
-// step has two halves of 16 k. While one half is multiplied the other's operands are read from LDS, and the step
-// after next is on its way to LDS from the moment that all waves have read the one whose place it takes: one
-// barrier a step.
+// step has two halves of 16 k. While one half is multiplied the other's operands are read from LDS and the next step's
+// rows are stored there, in the place of the step before, which all waves have read: one barrier a step.
 template <int SIDE, typename T>
 __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int tile_j, int tile, int part, _Float16* lds) {
     constexpr int PIECES = SIDE / 64, STAGE = SIDE * ROW_STEP;
@@ -264,11 +286,18 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
     struct Operands {
         half8 x[PIECES][2], y[PIECES][2];  // hi and lo
     };
-    const auto stage = [&](int step) {  // beyond the last step that one again, into the place that nobody reads any more
+    // AHEAD steps are in registers, or on their way there.
+    constexpr int AHEAD = SIDE == SMALL ? 3 : 1;
+    StagedRows<SIDE> rows_a[AHEAD], rows_b[AHEAD];
+    const _Float16 *lane_a = StagedRows<SIDE>::lane_rows(a, pitch), *lane_b = StagedRows<SIDE>::lane_rows(b, pitch);
+    const auto load = [&](int place, int step) {  // beyond the last step, that one again
+        rows_a[place].load(lane_a, pitch, min(step, end - 1));
+        rows_b[place].load(lane_b, pitch, min(step, end - 1));
+    };
+    const auto store = [&](int place, int step) {
         _Float16* to = lds + ((step - begin) & 1) * 2 * STAGE;
-        const int from = min(step, end - 1);
-        stage_rows<SIDE>(a, pitch, from, to);
-        stage_rows<SIDE>(b, pitch, from, to + STAGE);
+        rows_a[place].store(to);
+        rows_b[place].store(to + STAGE);
     };
     const auto read = [&](int step, int half) {
         const _Float16* at = lds + ((step - begin) & 1) * 2 * STAGE;
@@ -291,24 +320,27 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
                 for (int j = 0; j < PIECES; ++j)
                     sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.x[i][term == 2], o.y[j][term == 1], sum[i][j], 0, 0, 0);
     };
-    stage(begin);
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's rows have arrived; with the barrier, everyone's
+    load(0, begin);
+    store(0, begin);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) load(k, begin + 1 + k);
     __syncthreads();
-    stage(begin + 1);
     Operands first = read(begin, 0);
-    for (int step = begin; step < end; ++step) {
-        const Operands second = read(step, 1);
-        multiply(first);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): the next step has arrived, and this one is read
-        __syncthreads();
-        first = read(step + 1, 0);
-        stage(step + 2);
-        multiply(second);
-        __builtin_amdgcn_sched_barrier(0);
+    for (int base = begin; base < end; base += AHEAD) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int step = base + k;
+            if (step >= end) break;
+            const Operands second = read(step, 1);
+            store(k, step + 1);  // where the step before this one was, which all waves have read
+            load(k, step + 1 + AHEAD);
+            multiply(first);
+            __syncthreads();
+            first = read(step + 1, 0);
+            multiply(second);
+        }
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // the rows that were staged beyond the last step have arrived too:
-    __syncthreads();                     // LDS is free
+    __syncthreads();  // LDS is free
     if (p.splits > 1) {
         float flat[PIECES * PIECES * 16];
 #pragma unroll
@@ -454,7 +486,8 @@ __global__ __launch_bounds__(THREADS) void split_kernel(SourceGroup group) {
 // ---- the plan of one matrix -------------------------------------------------------------------
 // Large tiles need half the loads of small ones a product; small ones fill more of the GPU with a small matrix and
 // pad it less.
-int side_of(int shorter) { return shorter >= 1024 ? LARGE : SMALL; }
+int padding_of(int shorter) { return shorter >= 256 ? LARGE : SMALL; }
+int side_of(int shorter, bool symmetric) { return shorter >= (symmetric ? 1024 : 256) ? LARGE : SMALL; }
 
 // Parts of a tile's steps, for the products of a launch that would leave CUs idle: as many as fill `slots` workgroups,
 // but no more than about the root of the steps, since the last workgroup reads all parts' sums.
@@ -465,13 +498,13 @@ int splits_of(int ksteps, std::int64_t launch_steps, std::int64_t slots, bool sm
 }
 
 struct Plan {
-    int side, s, l;              // sides as they lie in memory
+    int s, l;                    // sides as they lie in memory
     int shorter, longer;         // and as they are
     std::int64_t x, square;      // bytes of X and of a square matrix
     int square_blocks;
     explicit Plan(const OrthogonalMatrix& m) : shorter(std::min(m.rows, m.cols)), longer(std::max(m.rows, m.cols)) {
-        side = side_of(shorter);
-        s = (shorter + side - 1) / side * side, l = (longer + side - 1) / side * side;
+        const int padding = padding_of(shorter);
+        s = (shorter + padding - 1) / padding * padding, l = (longer + padding - 1) / padding * padding;
         x = static_cast<std::int64_t>(s) * l * 4, square = static_cast<std::int64_t>(s) * s * 4;
         const std::int64_t blocks = (static_cast<std::int64_t>(m.rows) * m.cols + SQUARES_EACH - 1) / SQUARES_EACH;
         square_blocks = static_cast<int>(std::min<std::int64_t>(blocks, SQUARES_BLOCKS));
@@ -522,33 +555,34 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         sources.first_block[i + 1] = sources.first_block[i] + sources.s[i].padded_rows / 64 * (sources.s[i].padded_cols / 64);
     launch(split_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
     MFH_TRY(MFH_CHECK_LAUNCH("orthogonal split", stream));
-    bool all_small = true;
-    for (const Plan& plan : plans) all_small = all_small && plan.side == SMALL;
-    const std::int64_t slots = static_cast<std::int64_t>(device_cu_count()) * (all_small ? 4 : 2);
     const auto products = [&](auto&& describe) {
         ProductGroup group{};
         group.count = count;
         std::int64_t steps = 0;
+        bool all_small = true;
         const auto tiles = [](const Product& p) { return p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles; };
         for (int i = 0; i < count; ++i) {
             Product& p = group.p[i];
             const Plan& plan = plans[i];
             const OrthogonalMatrix& m = matrices[i];
-            p.alpha = 1.0f, p.small = plan.side == SMALL, p.tall = m.rows > m.cols;
+            p.alpha = 1.0f, p.tall = m.rows > m.cols;
             p.rows = std::min(m.rows, m.cols), p.cols = std::max(m.rows, m.cols);
             describe(i, p);
             p.k_padded = p.over_longer ? plan.l : plan.s;
             p.ksteps = ((p.over_longer ? plan.longer : plan.shorter) + K_STEP - 1) / K_STEP;
             p.m_padded = plan.s, p.n_padded = p.symmetric ? plan.s : plan.l;
-            p.m_tiles = (plan.shorter + plan.side - 1) / plan.side;
-            p.n_tiles = p.symmetric ? p.m_tiles : (plan.longer + plan.side - 1) / plan.side;
+            const int side = side_of(plan.shorter, p.symmetric);
+            p.small = side == SMALL, all_small = all_small && p.small;
+            p.m_tiles = (plan.shorter + side - 1) / side;
+            p.n_tiles = p.symmetric ? p.m_tiles : (plan.longer + side - 1) / side;
             steps += static_cast<std::int64_t>(tiles(p)) * p.ksteps;
         }
+        const std::int64_t slots = static_cast<std::int64_t>(device_cu_count()) * (all_small ? 4 : 2);
         char* part = parts;
         int split_tiles = 0;
         for (int i = 0; i < count; ++i) {
             Product& p = group.p[i];
-            const std::int64_t bytes = static_cast<std::int64_t>(plans[i].side) * plans[i].side * 4;
+            const std::int64_t bytes = p.small ? SMALL * SMALL * 4 : LARGE * LARGE * 4;
             p.splits = splits_of(p.ksteps, steps, slots, p.small);
             if (p.splits > 1 && (split_tiles + tiles(p) > LOGIT_COUNTERS || part + bytes * p.splits * tiles(p) > parts + PARTS_BYTES)) p.splits = 1;
             if (p.splits > 1) {
