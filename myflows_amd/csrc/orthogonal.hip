@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <numeric>
 #include <vector>
 
 #include "common.h"
@@ -38,7 +39,7 @@ constexpr int ROW_STEP = 2 * K_STEP;  // halves
 constexpr int LARGE = 128, SMALL = 64;  // sides of a workgroup's tile
 constexpr int SCALE_LOG = 12;
 constexpr float SCALE = 1 << SCALE_LOG, UNSCALE = 1.0f / SCALE;
-constexpr int GROUP = 32;  // matrices of a launch: their descriptors travel in its arguments
+constexpr int GROUP = 30;  // matrices of a launch: their descriptors travel in its arguments
 constexpr int XCD_COUNT = 8;
 constexpr std::int64_t PARTS_BYTES = 48 << 20;  // workspace of split tiles' sums
 
@@ -56,7 +57,7 @@ struct Product {
     float alpha, beta;
     int ksteps, m_tiles, n_tiles;  // what holds values, in steps and in tiles of its own side
     int k_padded, m_padded, n_padded;  // the sides as they lie in memory
-    int splits;
+    int whole, splits;  // tiles of one workgroup each, and the parts of each tile behind them
     int rows, cols;                // of the caller's matrix, the shorter side as rows
     bool over_longer, symmetric, small, tall;  // the sums' side; tall: the caller's matrix is the transposed result
 };
@@ -64,7 +65,7 @@ struct Product {
 struct ProductGroup {
     Product p[GROUP];
     int first_unit[GROUP + 1];
-    int count;
+    int round;  // the first units, which are dealt to the dies in runs
 };
 static_assert(sizeof(ProductGroup) <= 4096, "descriptors must fit the kernel arguments");
 
@@ -273,15 +274,15 @@ __device__ __forceinline__ bool join_parts(const Product& p, int tile, int part,
 // step has two halves of 16 k. While one half is multiplied the other's operands are read from LDS and the next step's
 // rows are stored there, in the place of the step before, which all waves have read: one barrier a step.
 template <int SIDE, typename T>
-__device__ __forceinline__ void tile_product(const Product& p, int tile_i, int tile_j, int tile, int part, _Float16* lds) {
+__device__ __forceinline__ void tile_product(const Product& p, int tile_i, int tile_j, int tile, int part, int parts, _Float16* lds) {
     constexpr int PIECES = SIDE / 64, STAGE = SIDE * ROW_STEP;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wave_i = wave / 2 * (SIDE / 2), wave_j = wave % 2 * (SIDE / 2);
     const std::int64_t pitch = p.k_padded * 2;
     const _Float16* a = p.a + static_cast<std::int64_t>(tile_i) * SIDE * pitch;
     const _Float16* b = p.b + static_cast<std::int64_t>(tile_j) * SIDE * pitch;
-    const int begin = static_cast<int>(static_cast<long long>(p.ksteps) * part / p.splits);
-    const int end = static_cast<int>(static_cast<long long>(p.ksteps) * (part + 1) / p.splits);
+    const int begin = static_cast<int>(static_cast<long long>(p.ksteps) * part / parts);
+    const int end = static_cast<int>(static_cast<long long>(p.ksteps) * (part + 1) / parts);
     float16v sum[PIECES][PIECES] = {};
     struct Operands {
         half8 x[PIECES][2], y[PIECES][2];  // hi and lo
@@ -334,18 +335,23 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
             const Operands second = read(step, 1);
             store(k, step + 1);  // where the step before this one was, which all waves have read
             load(k, step + 1 + AHEAD);
+            // The compiler would sink the reads to their uses, and wait for each there.
+            __builtin_amdgcn_sched_barrier(0);
             multiply(first);
+            __builtin_amdgcn_sched_barrier(0);
             __syncthreads();
             first = read(step + 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
             multiply(second);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     __syncthreads();  // LDS is free
-    if (p.splits > 1) {
+    if (parts > 1) {
         float flat[PIECES * PIECES * 16];
 #pragma unroll
         for (int e = 0; e < PIECES * PIECES * 16; ++e) flat[e] = sum[e / 16 / PIECES][e / 16 % PIECES][e % 16];
-        if (!join_parts(p, tile, part, flat)) return;
+        if (!join_parts(p, tile - p.whole, part, flat)) return;
 #pragma unroll
         for (int e = 0; e < PIECES * PIECES * 16; ++e) sum[e / 16 / PIECES][e / 16 % PIECES][e % 16] = flat[e];
     }
@@ -357,13 +363,18 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
 template <int LARGEST, typename T>
 __global__ __launch_bounds__(THREADS, 2) void product_kernel(ProductGroup group) {
     __shared__ __align__(1024) _Float16 lds[4 * LARGEST * ROW_STEP];
-    // Neighbouring units go to the same die: workgroups are dealt to the dies in turn.
-    const int units = gridDim.x, die = blockIdx.x % XCD_COUNT, share = units / XCD_COUNT, more = units % XCD_COUNT;
-    const int unit = die * share + min(die, more) + blockIdx.x / XCD_COUNT;
+    // Neighbouring units of the first round go to the same die: workgroups are dealt to the dies in turn.
+    int unit = blockIdx.x;
+    if (unit < group.round) {
+        const int die = unit % XCD_COUNT, share = group.round / XCD_COUNT, more = group.round % XCD_COUNT;
+        unit = die * share + min(die, more) + unit / XCD_COUNT;
+    }
     int item = 0;
     while (unit >= group.first_unit[item + 1]) ++item;
     const Product& p = group.p[item];
-    const int within = unit - group.first_unit[item], t = within / p.splits, part = within - t * p.splits;
+    const int within = unit - group.first_unit[item], beyond = within - p.whole;
+    const int t = beyond < 0 ? within : p.whole + beyond / p.splits, part = beyond < 0 ? 0 : beyond % p.splits;
+    const int parts = beyond < 0 ? 1 : p.splits;
     int i, j;
     if (p.symmetric) {  // the tiles on and below the diagonal, row by row
         i = static_cast<int>((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
@@ -374,8 +385,8 @@ __global__ __launch_bounds__(THREADS, 2) void product_kernel(ProductGroup group)
         const int width = 8 * p.n_tiles, first = t / width * 8, rows = min(8, p.m_tiles - first), place = t % width;
         i = first + place % rows, j = place / rows;
     }
-    if (LARGEST == SMALL || p.small) tile_product<SMALL, T>(p, i, j, t, part, lds);
-    else tile_product<LARGEST, T>(p, i, j, t, part, lds);
+    if (LARGEST == SMALL || p.small) tile_product<SMALL, T>(p, i, j, t, part, parts, lds);
+    else tile_product<LARGEST, T>(p, i, j, t, part, parts, lds);
 }
 
 // ---- before the products ----------------------------------------------------------------------
@@ -484,17 +495,12 @@ __global__ __launch_bounds__(THREADS) void split_kernel(SourceGroup group) {
 }
 
 // ---- the plan of one matrix -------------------------------------------------------------------
-// Large tiles need half the loads of small ones a product; small ones fill more of the GPU with a small matrix and
-// pad it less.
+// The padding allows large tiles from here on.
 int padding_of(int shorter) { return shorter >= 256 ? LARGE : SMALL; }
-int side_of(int shorter, bool symmetric) { return shorter >= (symmetric ? 1024 : 256) ? LARGE : SMALL; }
 
-// Parts of a tile's steps, for the products of a launch that would leave CUs idle: as many as fill `slots` workgroups,
-// but no more than about the root of the steps, since the last workgroup reads all parts' sums.
-int splits_of(int ksteps, std::int64_t launch_steps, std::int64_t slots, bool small) {
-    const std::int64_t share = std::max<std::int64_t>(launch_steps / slots, 4);
-    const int most = static_cast<int>(std::sqrt(ksteps * (small ? 1.5 : 0.5)));
-    return static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(ksteps / share, most)));
+int tiles_of(int shorter, int longer, bool symmetric, int side) {
+    const int m = (shorter + side - 1) / side;
+    return symmetric ? m * (m + 1) / 2 : m * ((longer + side - 1) / side);
 }
 
 struct Plan {
@@ -555,42 +561,63 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         sources.first_block[i + 1] = sources.first_block[i] + sources.s[i].padded_rows / 64 * (sources.s[i].padded_cols / 64);
     launch(split_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
     MFH_TRY(MFH_CHECK_LAUNCH("orthogonal split", stream));
+    const int cus = device_cu_count();
     const auto products = [&](auto&& describe) {
         ProductGroup group{};
-        group.count = count;
-        std::int64_t steps = 0;
-        bool all_small = true;
-        const auto tiles = [](const Product& p) { return p.symmetric ? p.m_tiles * (p.m_tiles + 1) / 2 : p.m_tiles * p.n_tiles; };
+        // Large tiles need half the loads of small ones a product, where there are enough of them.
+        int large_tiles = 0, tiles[GROUP], units[GROUP];
         for (int i = 0; i < count; ++i) {
             Product& p = group.p[i];
-            const Plan& plan = plans[i];
             const OrthogonalMatrix& m = matrices[i];
             p.alpha = 1.0f, p.tall = m.rows > m.cols;
             p.rows = std::min(m.rows, m.cols), p.cols = std::max(m.rows, m.cols);
             describe(i, p);
+            if (padding_of(plans[i].shorter) == LARGE) large_tiles += tiles_of(plans[i].shorter, plans[i].longer, p.symmetric, LARGE);
+        }
+        const bool use_large = large_tiles >= (group.p[0].symmetric ? 64 : 2 * cus);
+        bool all_small = true;
+        std::int64_t steps = 0;
+        for (int i = 0; i < count; ++i) {
+            Product& p = group.p[i];
+            const Plan& plan = plans[i];
+            p.small = !use_large || padding_of(plan.shorter) == SMALL, all_small = all_small && p.small;
+            const int side = p.small ? SMALL : LARGE;
             p.k_padded = p.over_longer ? plan.l : plan.s;
             p.ksteps = ((p.over_longer ? plan.longer : plan.shorter) + K_STEP - 1) / K_STEP;
             p.m_padded = plan.s, p.n_padded = p.symmetric ? plan.s : plan.l;
-            const int side = side_of(plan.shorter, p.symmetric);
-            p.small = side == SMALL, all_small = all_small && p.small;
             p.m_tiles = (plan.shorter + side - 1) / side;
             p.n_tiles = p.symmetric ? p.m_tiles : (plan.longer + side - 1) / side;
-            steps += static_cast<std::int64_t>(tiles(p)) * p.ksteps;
+            tiles[i] = tiles_of(plan.shorter, plan.longer, p.symmetric, side);
+            steps += static_cast<std::int64_t>(tiles[i]) * p.ksteps;
         }
-        const std::int64_t slots = static_cast<std::int64_t>(device_cu_count()) * (all_small ? 4 : 2);
+        const int slots = cus * (all_small ? 4 : 2);
+        // Tiles whose steps are shared by several workgroups: all of them where they would leave CUs idle, as many parts as
+        // fill the GPU but no more than about the root of the steps, since the last workgroup reads all parts' sums; else
+        // those that a last, short round would hold.
+        const int all = std::accumulate(tiles, tiles + count, 0);
+        int rest = all >= slots ? all % slots : all;
+        const std::int64_t share = all >= slots ? 1 : std::max<std::int64_t>(steps / slots, 4);
+        if (all >= slots && 2 * rest > slots) rest = 0;
         char* part = parts;
         int split_tiles = 0;
-        for (int i = 0; i < count; ++i) {
+        for (int i = count - 1; i >= 0; --i) {
             Product& p = group.p[i];
             const std::int64_t bytes = p.small ? SMALL * SMALL * 4 : LARGE * LARGE * 4;
-            p.splits = splits_of(p.ksteps, steps, slots, p.small);
-            if (p.splits > 1 && (split_tiles + tiles(p) > LOGIT_COUNTERS || part + bytes * p.splits * tiles(p) > parts + PARTS_BYTES)) p.splits = 1;
+            const int here = std::min(rest, tiles[i]), most = static_cast<int>(std::sqrt(p.ksteps * (p.small ? 1.5 : 0.5)));
+            rest -= here;
+            std::int64_t splits = std::min<std::int64_t>(all >= slots ? p.ksteps / 4 : p.ksteps / share, most);
+            if (all >= slots) splits = std::min<std::int64_t>(splits, slots / std::max(1, all % slots));
+            if (split_tiles + here > LOGIT_COUNTERS || part + bytes * splits * here > parts + PARTS_BYTES) splits = 1;
+            p.splits = static_cast<int>(std::max<std::int64_t>(splits, 1));
+            p.whole = p.splits > 1 ? tiles[i] - here : tiles[i];
             if (p.splits > 1) {
                 p.parts = reinterpret_cast<float*>(part), p.arrived = o.counters + split_tiles;
-                part += bytes * p.splits * tiles(p), split_tiles += tiles(p);
+                part += bytes * p.splits * here, split_tiles += here;
             }
-            group.first_unit[i + 1] = group.first_unit[i] + tiles(p) * p.splits;
+            units[i] = p.whole + (tiles[i] - p.whole) * p.splits;
         }
+        for (int i = 0; i < count; ++i) group.first_unit[i + 1] = group.first_unit[i] + units[i];
+        group.round = all >= slots ? all / slots * slots : group.first_unit[count];
         launch(all_small ? product_kernel<SMALL, T> : product_kernel<LARGE, T>, dim3(group.first_unit[count]), dim3(THREADS), 0,
                stream, group);
         return MFH_CHECK_LAUNCH("orthogonal product", stream);
