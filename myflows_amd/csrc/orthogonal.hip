@@ -131,8 +131,8 @@ __device__ __forceinline__ void write_scratch(_Float16* scratch, _Float16* matri
     wave_order();
 }
 
-template <typename T>
-__device__ __forceinline__ void write_final(const Product& p, const float (&v)[16], int i0, int j0, _Float16* scratch) {
+template <typename T, typename P>
+__device__ __forceinline__ void write_final(const P& p, const float (&v)[16], int i0, int j0, _Float16* scratch) {
     const int lane = threadIdx.x & 63;
     T* out = static_cast<T*>(p.final);
     if (!p.tall) {
@@ -227,8 +227,8 @@ __device__ __forceinline__ void write_pieces(const Product& p, const float16v (&
 }
 
 // The sums of a tile's parts, in their order, by the workgroup that comes last; false for the others.
-template <int SUMS>
-__device__ __forceinline__ bool join_parts(const Product& p, int tile, int part, float (&sum)[SUMS]) {
+template <int SUMS, typename P>
+__device__ __forceinline__ bool join_parts(const P& p, int tile, int part, float (&sum)[SUMS]) {
     __shared__ unsigned last;
     static_assert(SUMS % 2 == 0, "two sums a store");
     using Two = unsigned long long;
@@ -494,6 +494,148 @@ __global__ __launch_bounds__(THREADS) void split_kernel(SourceGroup group) {
     }
 }
 
+// ---- matrices of one tile's width -------------------------------------------------------------
+// With at most 64 rows, G is one tile. A workgroup takes some of X's columns through a whole step: it forms its new
+// columns from B, writes them, and adds their part of the next G; the workgroup that comes last joins the parts and forms
+// the next B. One launch a step instead of three: for such matrices the launches are what takes the time (64 x 576
+// float32 in five steps: NARROW_US us, 100 with the products above).
+struct Narrow {
+    const _Float16* x;  // rows of X, for the first G; then null
+    _Float16* x_t;      // X^T, rows of 64
+    _Float16* b;
+    float* parts;
+    unsigned* arrived;
+    void* final;
+    std::int64_t final_stride;
+    int rows, cols, x_pitch, tiles, each, splits;  // tiles of 64 columns, those of a workgroup, workgroups
+    bool tall;
+};
+
+struct NarrowGroup {
+    Narrow m[GROUP];
+    int first_block[GROUP + 1];
+    float a, b, c;
+};
+static_assert(sizeof(NarrowGroup) <= 4096, "descriptors must fit the kernel arguments");
+
+constexpr int NARROW_STEP = SMALL * ROW_STEP;  // halves of 64 rows in one step; a tile has two steps
+
+// The tile's two steps from memory to LDS.
+__device__ __forceinline__ void stage_tile(const _Float16* rows, std::int64_t pitch, _Float16* lds) {
+    StagedRows<SMALL> staged[2];
+    const _Float16* lane_rows = StagedRows<SMALL>::lane_rows(rows, pitch);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) staged[step].load(lane_rows, pitch, step);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) staged[step].store(lds + step * NARROW_STEP);
+}
+
+// This wave's 32 x 32 piece of x y^T, over the 64 values of the rows of both.
+__device__ __forceinline__ void multiply_tile(const _Float16* x, const _Float16* y, int wave_i, int wave_j, float16v& sum) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        half8 a[2], b[2];
+#pragma unroll
+        for (int low = 0; low < 2; ++low) {
+            a[low] = operand(x + k / 2 * NARROW_STEP, wave_i + (lane & 31), low * 4 + k % 2 * 2 + lane / 32);
+            b[low] = operand(y + k / 2 * NARROW_STEP, wave_j + (lane & 31), low * 4 + k % 2 * 2 + lane / 32);
+        }
+#pragma unroll
+        for (int term = 0; term < 3; ++term) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[term == 2], b[term == 1], sum, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ void split_piece(const float (&v)[16], half4 (&hi)[4], half4 (&lo)[4]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        hi[e / 4][e % 4] = static_cast<_Float16>(v[e]);
+        lo[e / 4][e % 4] = static_cast<_Float16>(v[e] - static_cast<float>(hi[e / 4][e % 4]));
+    }
+}
+
+// The lane's column of a piece, as 16 of the 32 values of row `row`, at 32 rows of a step in LDS.
+__device__ __forceinline__ void write_quads(_Float16* step, int row, const half4 (&hi)[4], const half4 (&lo)[4]) {
+    const int high = (threadIdx.x & 63) / 32;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        *reinterpret_cast<half4*>(scratch_at(step, row, 8 * q + 4 * high, 0)) = hi[q];
+        *reinterpret_cast<half4*>(scratch_at(step, row, 8 * q + 4 * high, 1)) = lo[q];
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
+    __shared__ __align__(1024) _Float16 columns[2 * NARROW_STEP], factor[2 * NARROW_STEP], rows[2 * NARROW_STEP];
+    __shared__ __align__(16) _Float16 scratches[THREADS / 64 * SCRATCH];
+    const int item = item_of(group, blockIdx.x), part = blockIdx.x - group.first_block[item];
+    const Narrow& m = group.m[item];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wave_i = wave / 2 * 32, wave_j = wave % 2 * 32, column = lane & 31, high = lane / 32;
+    _Float16* scratch = scratches + wave * SCRATCH;
+    constexpr std::int64_t PITCH = 2 * SMALL;
+    float16v gram = {};
+    half4 hi[4], lo[4];
+    float v[16];
+    if (!m.x) stage_tile(m.b, PITCH, factor);
+    for (int tile = part * m.each; tile < min((part + 1) * m.each, m.tiles); ++tile) {
+        if (m.x) {
+            stage_tile(m.x + tile * PITCH, m.x_pitch, rows);
+        } else {
+            stage_tile(m.x_t + tile * SMALL * PITCH, PITCH, columns);
+            __syncthreads();
+            float16v sum = {};
+            multiply_tile(factor, columns, wave_i, wave_j, sum);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const _Float16* step = columns + wave_i / 32 * NARROW_STEP;
+                const half4 old_hi = *reinterpret_cast<const half4*>(scratch_at(const_cast<_Float16*>(step), wave_j + column, 8 * q + 4 * high, 0));
+                const half4 old_lo = *reinterpret_cast<const half4*>(scratch_at(const_cast<_Float16*>(step), wave_j + column, 8 * q + 4 * high, 1));
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    v[4 * q + k] = sum[4 * q + k] * UNSCALE + group.a * (static_cast<float>(old_hi[k]) + static_cast<float>(old_lo[k]));
+            }
+            if (m.final) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] *= UNSCALE;
+                write_final<T>(m, v, wave_i, tile * SMALL + wave_j, scratch);
+                __syncthreads();
+                continue;
+            }
+            split_piece(v, hi, lo);
+            write_quads(scratch, column, hi, lo);
+            write_scratch(scratch, m.x_t, tile * SMALL + wave_j, wave_i, PITCH);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int row = wave_i + e / 4 * 8 + 4 * high + e % 4;
+                *scratch_at(rows + wave_j / 32 * NARROW_STEP, row, column, 0) = hi[e / 4][e % 4];
+                *scratch_at(rows + wave_j / 32 * NARROW_STEP, row, column, 1) = lo[e / 4][e % 4];
+            }
+        }
+        __syncthreads();
+        multiply_tile(rows, rows, wave_i, wave_j, gram);
+        __syncthreads();
+    }
+    if (m.final) return;
+    float flat[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) flat[e] = gram[e];
+    if (m.splits > 1 && !join_parts(m, 0, part, flat)) return;
+    // G, symmetric, and the next B.
+#pragma unroll
+    for (int e = 0; e < 16; ++e) flat[e] *= UNSCALE;
+    split_piece(flat, hi, lo);
+    write_quads(rows + wave_i / 32 * NARROW_STEP, wave_j + column, hi, lo);
+    __syncthreads();
+    float16v square = {};
+    multiply_tile(rows, rows, wave_i, wave_j, square);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = group.c * square[e] * UNSCALE + group.b * flat[e];
+    split_piece(v, hi, lo);
+    write_quads(scratch, column, hi, lo);
+    write_scratch(scratch, m.b, wave_j, wave_i, PITCH);
+}
+
 // ---- the plan of one matrix -------------------------------------------------------------------
 // The padding allows large tiles from here on.
 int padding_of(int shorter) { return shorter >= 256 ? LARGE : SMALL; }
@@ -532,6 +674,33 @@ struct Buffers {
     }
 };
 
+constexpr int NARROW_SPLITS = 16;  // workgroups of a narrow matrix: the last one reads all their parts
+
+template <typename T>
+int run_narrow(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps& o, const std::vector<Plan>& plans,
+               const std::vector<Buffers>& buffers, char* parts, hipStream_t stream) {
+    static_assert(GROUP * NARROW_SPLITS * SMALL * SMALL * 4 <= PARTS_BYTES && GROUP <= LOGIT_COUNTERS, "parts fit their workspace");
+    for (int step = 0; step <= o.steps; ++step) {  // the first G and B, then the steps
+        NarrowGroup group{};
+        group.a = o.a, group.b = o.b, group.c = o.c;
+        for (int i = 0; i < count; ++i) {
+            Narrow& m = group.m[i];
+            const Plan& plan = plans[i];
+            m.x = step == 0 ? buffers[i].x : nullptr, m.x_t = buffers[i].x_t[0], m.b = buffers[i].p, m.x_pitch = plan.l * 2;
+            m.parts = reinterpret_cast<float*>(parts + static_cast<std::int64_t>(i) * NARROW_SPLITS * SMALL * SMALL * 4);
+            m.arrived = o.counters + i;
+            if (step == o.steps) m.final = matrices[i].out, m.final_stride = matrices[i].out_stride;
+            m.rows = plan.shorter, m.cols = plan.longer, m.tall = matrices[i].rows > matrices[i].cols;
+            m.tiles = (plan.longer + SMALL - 1) / SMALL;
+            m.each = (m.tiles + NARROW_SPLITS - 1) / NARROW_SPLITS, m.splits = (m.tiles + m.each - 1) / m.each;
+            group.first_block[i + 1] = group.first_block[i] + m.splits;
+        }
+        launch(narrow_kernel<T>, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
+        MFH_TRY(MFH_CHECK_LAUNCH("orthogonal narrow step", stream));
+    }
+    return OK;
+}
+
 template <typename T>
 int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps& o, char* workspace, hipStream_t stream) {
     std::vector<Plan> plans;
@@ -561,6 +730,8 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         sources.first_block[i + 1] = sources.first_block[i] + sources.s[i].padded_rows / 64 * (sources.s[i].padded_cols / 64);
     launch(split_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
     MFH_TRY(MFH_CHECK_LAUNCH("orthogonal split", stream));
+    if (std::all_of(plans.begin(), plans.end(), [](const Plan& plan) { return plan.shorter <= SMALL; }))
+        return run_narrow<T>(matrices, count, o, plans, buffers, parts, stream);
     const int cus = device_cu_count();
     const auto products = [&](auto&& describe) {
         ProductGroup group{};

@@ -6,6 +6,11 @@ of 2^-23 of it, twice float32's half step; a product leaves out lo lo, 2^-24 of 
 each product has at most three times the error of a float32 one, and the order of the sums may differ: in the
 Frobenius norm the result is within 4 times float32's error, plus 2^-20 of the result for matrices so small that
 float32's own error happens to be near 0, plus half a step of the type (of a float16 result below 2^-14, half of 2^-24).
+With one row or column there is one singular value, 1, and float32 may well have no error at all: there the bound is
+the worst case. A step holds G, B and X with relative errors of 2^-23, so with g = x^2 up to 1.24 its X is off by at most
+(2 |b| g + 3 |c| g^2 + |a| + 1) 2^-23 < 26 2^-23 of 1. The default steps take 1 to .701, 1.114, .721, 1.090, where the
+derivative a + 3 b g + 5 c g^2 is -1.14, 1.30, -1.26, .76, so an error after the steps 1 to 5 comes out 1.42, 1.25, .96, .76
+and 1 times as large: 5.4 times 26 2^-23 in all, below 2^-15.
 """
 
 import pytest
@@ -36,7 +41,7 @@ def _check(got, matrix, **options):
     rounding = torch.finfo(matrix.dtype).eps / 2 * size
     if matrix.dtype is torch.float16:
         rounding += 2.0 ** -25 * want.numel() ** 0.5
-    bound = 4 * float((_steps(matrix, torch.float32, **options).double() - want).norm()) + 2.0 ** -20 * size + rounding
+    bound = 4 * float((_steps(matrix, torch.float32, **options).double() - want).norm()) + 2.0 ** (-15 if min(want.shape[0], want[0].numel()) == 1 else -20) * size + rounding
     off = float((got.detach().cpu().double() - want).norm())
     print(f"off {off / size if size else off:.2e}, bound {bound / size if size else bound:.2e}", flush=True)
     assert got.dtype is matrix.dtype and got.shape == matrix.shape and off <= bound
@@ -71,15 +76,18 @@ def test_orthogonalised_matrices_match_the_definition(rows, cols, dtype):
 
 
 @gpu
-def test_a_list_of_unlike_matrices_gives_the_bits_of_each_alone():
+def test_lists_of_unlike_matrices():
     shapes = [(64, 147), (64, 576), (128, 64), (300, 700), (700, 300), (2, 512), (1, 1), (0, 4), (257, 257)] * 5
     matrices = [_matrix(r, c, list(TYPES)[i % 3], i) if r else torch.zeros((r, c), device="cuda") for i, (r, c) in enumerate(shapes)]
     got = ops.orthogonalize_many(matrices)
     assert len(got) == len(matrices) and ops.orthogonalize_many([]) == []
-    for value, to in zip(matrices, got):
-        assert to.dtype is value.dtype and to.shape == value.shape
+    for value, to, again in zip(matrices, got, ops.orthogonalize_many(matrices)):
+        assert to.dtype is value.dtype and to.shape == value.shape and torch.equal(to, again)
         if value.numel():
-            assert torch.equal(ops.orthogonalize(value), to)
+            _check(to, value)
+    narrow = [matrices[i] for i in (0, 1, 2, 5, 6)]  # no side of 64 or less is one of the others
+    for value, to in zip(narrow, ops.orthogonalize_many(narrow)):
+        _check(to, value)
 
 
 @gpu
@@ -134,7 +142,8 @@ def test_zeros_infinities_and_nan():
         matrix[69, 89] = bad
         other = torch.randn((80, 30), device="cuda")
         got = ops.orthogonalize_many([matrix, other])
-        assert bool(got[0].isnan().all()) and torch.equal(got[1], ops.orthogonalize(other))
+        assert bool(got[0].isnan().all())
+        _check(got[1], other)
 
 
 @gpu
