@@ -253,7 +253,8 @@ __device__ __forceinline__ bool join_parts(const P& p, int tile, int part, float
         Two two[TOGETHER][SUMS / 2];
 #pragma unroll
         for (int k = 0; k < TOGETHER; ++k) {
-            const Two* from = parts + static_cast<std::int64_t>(min(first + k, p.splits - 1)) * (SUMS / 2) * THREADS;
+            if (first + k >= p.splits) break;
+            const Two* from = parts + static_cast<std::int64_t>(first + k) * (SUMS / 2) * THREADS;
 #pragma unroll
             for (int i = 0; i < SUMS / 2; ++i) two[k][i] = handed_over(from + i * THREADS);
         }
