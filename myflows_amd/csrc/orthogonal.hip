@@ -746,6 +746,8 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
             describe(i, p);
             if (padding_of(plans[i].shorter) == LARGE) large_tiles += tiles_of(plans[i].shorter, plans[i].longer, p.symmetric, LARGE);
         }
+        // From 64 symmetric ones on they win split (1024 x 4096 and 4096 x 1024: 72), others from a whole round on
+        // (1999 x 517 and 771 x 1003, 136 of them: 33 us, 22 with small ones).
         const bool use_large = large_tiles >= (group.p[0].symmetric ? 64 : 2 * cus);
         bool all_small = true;
         std::int64_t steps = 0;
@@ -764,8 +766,9 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         }
         const int slots = cus * (all_small ? 4 : 2);
         // Tiles whose steps are shared by several workgroups: all of them where they would leave CUs idle, as many parts as
-        // fill the GPU but no more than about the root of the steps, since the last workgroup reads all parts' sums; else
-        // those that a last, short round would hold.
+        // fill the GPU but no more than half the root of the steps, since the last workgroup reads all parts' sums (1999 x 517
+        // and 771 x 1003 float16, G: 18 us, 24 with up to 1.2 times the root); else those that a last, short round would
+        // hold (4096 x 4096, 528 tiles for 512 places: 222 us, 292 with whole tiles).
         const int all = std::accumulate(tiles, tiles + count, 0);
         int rest = all >= slots ? all % slots : all;
         const std::int64_t share = all >= slots ? 1 : std::max<std::int64_t>(steps / slots, 4);
@@ -775,7 +778,7 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         for (int i = count - 1; i >= 0; --i) {
             Product& p = group.p[i];
             const std::int64_t bytes = p.small ? SMALL * SMALL * 4 : LARGE * LARGE * 4;
-            const int here = std::min(rest, tiles[i]), most = static_cast<int>(std::sqrt(p.ksteps * (p.small ? 1.5 : 0.5)));
+            const int here = std::min(rest, tiles[i]), most = static_cast<int>(std::sqrt(p.ksteps * 0.25));
             rest -= here;
             std::int64_t splits = std::min<std::int64_t>(all >= slots ? p.ksteps / 4 : p.ksteps / share, most);
             if (all >= slots) splits = std::min<std::int64_t>(splits, slots / std::max(1, all % slots));
