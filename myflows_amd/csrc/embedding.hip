@@ -304,6 +304,35 @@ __device__ __forceinline__ void walk_tasks(const SumPlan& plan, const EmbeddingG
     }
 }
 
+// A wave's share of the pieces: `lanes` lanes to a row, and 64 / lanes groups of them that take neighbouring ranges of the
+// rows that are summed, whose sums are then added in a fixed order. each(row, the lane's column, whether it is one, group).
+template <int N, typename F>
+__device__ __forceinline__ void walk_waves(const SumPlan& plan, const EmbeddingGradient& g, unsigned blocks, std::int64_t rows, F&& each) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    for (std::int64_t task = static_cast<std::int64_t>(blockIdx.x) * (THREADS / 64) + wave; task < rows * plan.columns;
+         task += static_cast<std::int64_t>(blocks) * (THREADS / 64)) {
+        const int row = static_cast<int>(task / plan.columns);
+        const int column = (static_cast<int>(task - static_cast<std::int64_t>(row) * plan.columns) * plan.lanes + lane % plan.lanes) * N;
+        each(row, min(column, g.dim - 1), column < g.dim, lane / plan.lanes);
+    }
+}
+
+struct Range {
+    int begin, end;
+    // The group's part of begin .. end - 1.
+    __device__ __forceinline__ Range part(int group, int groups) const {
+        const int each = (end - begin + groups - 1) / groups, from = min(begin + group * each, end);
+        return {from, min(from + each, end)};
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void add_groups(float (&sum)[N], int lanes) {
+    for (int o = lanes; o < 64; o *= 2)
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum[e] += __shfl_xor(sum[e], o);
+}
+
 template <bool WAVE, typename T, typename Out>
 __global__ __launch_bounds__(THREADS) void sum_kernel(const T* __restrict__ grad, Out* __restrict__ out, EmbeddingGradient g,
                                                       SumPlan plan, Sorted s, float* __restrict__ parts) {
@@ -311,16 +340,18 @@ __global__ __launch_bounds__(THREADS) void sum_kernel(const T* __restrict__ grad
     if (blockIdx.x < plan.part_blocks) {
         const int given = shared_by<WAVE>(s.starts[s.slice << s.classes_log]);
         const int chunks = (given + plan.chunk - 1) / plan.chunk;
-        walk_tasks<WAVE, N>(plan, g, 0, plan.part_blocks, chunks, [&](int chunk, int column, bool there) {
+        walk_waves<N>(plan, g, plan.part_blocks, chunks, [&](int chunk, int column, bool there, int group) {
             const int begin = chunk * plan.chunk, end = min(begin + plan.chunk, given);
 #pragma unroll 1
             for (int last = 0; last < 2; ++last) {
-                const int slot = shared_by<WAVE>(s.slots[last ? end - 1 : begin]);
-                const int from = shared_by<WAVE>(s.starts[slot]), to = shared_by<WAVE>(s.starts[slot + 1]);
+                const int slot = __builtin_amdgcn_readfirstlane(s.slots[last ? end - 1 : begin]);
+                const int from = __builtin_amdgcn_readfirstlane(s.starts[slot]), to = __builtin_amdgcn_readfirstlane(s.starts[slot + 1]);
                 if (to - from <= plan.chunk || (last && from <= begin)) continue;
+                const Range piece{max(from, begin), min(to, end)}, mine = WAVE ? piece : piece.part(group, 64 / plan.lanes);
                 float sum[N] = {};
-                add_positions<WAVE, T, N>(sum, grad, g, s.order, max(from, begin), min(to, end), column);
-                if (!there) continue;
+                add_positions<WAVE, T, N>(sum, grad, g, s.order, mine.begin, mine.end, column);
+                if (!WAVE) add_groups(sum, plan.lanes);
+                if (!there || group) continue;
                 float* to_part = parts + (2 * static_cast<std::int64_t>(chunk) + last) * plan.part_width + column;
 #pragma unroll
                 for (int e = 0; e < N; ++e) to_part[e] = sum[e];
@@ -342,16 +373,19 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Out* __restrict__ out, Em
                                                        const float* __restrict__ parts) {
     const int given = s.starts[s.slice << s.classes_log];
     const int chunks = (given + plan.chunk - 1) / plan.chunk;
-    walk_tasks<false, N>(plan, g, 0, gridDim.x, chunks, [&](int chunk, int column, bool) {
-        const int begin = chunk * plan.chunk, slot = s.slots[min(begin + plan.chunk, given) - 1];
-        const int from = s.starts[slot], to = s.starts[slot + 1];
+    walk_waves<N>(plan, g, gridDim.x, chunks, [&](int chunk, int column, bool there, int group) {
+        const int begin = chunk * plan.chunk, slot = __builtin_amdgcn_readfirstlane(s.slots[min(begin + plan.chunk, given) - 1]);
+        const int from = __builtin_amdgcn_readfirstlane(s.starts[slot]), to = __builtin_amdgcn_readfirstlane(s.starts[slot + 1]);
         if (to - from <= plan.chunk || from < begin) return;
         // The first piece ends its chunk, unless it begins there; every further one begins its chunk.
         float sum[N] = {};
-        add_rows<Pack<float, N>>(sum, chunk, (to - 1) / plan.chunk + 1, [&](int c) {
+        const Range mine = Range{chunk, (to - 1) / plan.chunk + 1}.part(group, 64 / plan.lanes);
+        add_rows<Pack<float, N>>(sum, mine.begin, mine.end, [&](int c) {
             const int ends = c == chunk && from != begin;
-            return load_pack<float, N>(parts + (2 * static_cast<std::int64_t>(c) + ends) * plan.part_width + column);
+            return load_pack<float, N>(parts + (2 * static_cast<std::int64_t>(c) + ends) * plan.part_width + column / N * N);
         });
+        add_groups(sum, plan.lanes);
+        if (!there || group) return;
         const int token_class = slot / s.slice;
         write_sum(out, sum, g, ((slot - token_class * s.slice) << s.classes_log) + token_class, column);
     });
@@ -379,7 +413,7 @@ SumPlan sum_plan(const EmbeddingGradient& g, int type) {
     SumPlan plan{chunk_of(g.count), 1, 1, packs * n, 0};
     while (plan.lanes < 64 && plan.lanes < packs) plan.lanes *= 2;
     plan.columns = (packs + plan.lanes - 1) / plan.lanes;
-    plan.part_blocks = wave_blocks(chunks_of(g, plan), plan);
+    plan.part_blocks = static_cast<unsigned>(std::min<std::int64_t>((chunks_of(g, plan) * plan.columns + THREADS / 64 - 1) / (THREADS / 64), BLOCKS_MAX));
     return plan;
 }
 
