@@ -648,7 +648,7 @@ MFH_API int mfh_embedding_backward(uint64_t grad, int type, int64_t count, int d
 
 /* ---- orthogonal matrices --------------------------------------------------------------------- */
 
-/* One matrix of mfh_orthogonalize: rows x cols elements (sides of at most 2^20, at most 2^31 - 1 elements), rows of
+/* One matrix of mfh_orthogonalize (at most 65536 of a call, as of mfh_muon_step's): rows x cols elements (sides of at most 2^20, at most 2^31 - 1 elements), rows of
  * contiguous elements their stride apart. out may be in; it overlaps no other matrix of the call. */
 typedef struct mfh_orthogonal_matrix {
     uint64_t in, out;

@@ -1425,7 +1425,8 @@ MFH_API int mfh_embedding_backward(std::uint64_t grad, int type, std::int64_t co
 static_assert(sizeof(mfh_orthogonal_matrix) == sizeof(OrthogonalMatrix), "the C table is read as OrthogonalMatrix rows");
 
 static int require_orthogonal(const mfh_orthogonal_matrix* matrices, int count, std::vector<OrthogonalMatrix>& table) {
-    MFH_REQUIRE(count >= 0 && (count == 0 || matrices), "orthogonalisation received a null table");
+    MFH_REQUIRE(count >= 0 && count <= ORTHOGONAL_COUNT_LIMIT, "number of matrices out of range");
+    MFH_REQUIRE(count == 0 || matrices, "orthogonalisation received a null table");
     for (int i = 0; i < count; ++i) {
         const mfh_orthogonal_matrix& m = matrices[i];
         MFH_REQUIRE(m.rows > 0 && m.cols > 0 && m.rows <= ORTHOGONAL_SIDE_LIMIT && m.cols <= ORTHOGONAL_SIDE_LIMIT &&
@@ -1462,7 +1463,8 @@ MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, 
 static_assert(sizeof(mfh_muon_tensor) == sizeof(MuonTensor), "the C table is read as MuonTensor rows");
 
 static int require_muon(const mfh_muon_tensor* tensors, int count, std::vector<MuonTensor>& table) {
-    MFH_REQUIRE(count >= 0 && (count == 0 || tensors), "a Muon step received a null table");
+    MFH_REQUIRE(count >= 0 && count <= ORTHOGONAL_COUNT_LIMIT, "number of parameters out of range");
+    MFH_REQUIRE(count == 0 || tensors, "a Muon step received a null table");
     for (int i = 0; i < count; ++i) {
         const mfh_muon_tensor& t = tensors[i];
         MFH_REQUIRE(t.rows > 0 && t.cols > 0 && t.rows <= ORTHOGONAL_SIDE_LIMIT && t.cols <= ORTHOGONAL_SIDE_LIMIT &&

@@ -657,6 +657,7 @@ int launch_embedding_backward(const void* grad, int type, void* out, int out_typ
 // ---- orthogonal.hip ---------------------------------------------------------------------------
 constexpr int ORTHOGONAL_SIDE_LIMIT = 1 << 20;
 constexpr int ORTHOGONAL_STEPS_MAX = 64;
+constexpr int ORTHOGONAL_COUNT_LIMIT = 1 << 16;  // matrices of a call
 
 struct OrthogonalMatrix {  // out has the shape and type of in, and may be in
     const void* in;

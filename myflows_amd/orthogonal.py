@@ -10,6 +10,7 @@ its only optimisers with a state are elementwise.
 from __future__ import annotations
 
 import math
+from bisect import bisect_right
 from functools import lru_cache
 
 import torch
@@ -21,6 +22,7 @@ STEPS = 5
 STEPS_MAX = 64
 SIDE_LIMIT = 1 << 20
 ELEMENTS_LIMIT = 2 ** 31 - 1
+COUNT_LIMIT = 1 << 16  # matrices of a call
 
 
 def _matrix(value, name):
@@ -37,6 +39,31 @@ def _matrix(value, name):
     if rows and cols and ((cols > 1 and value.stride(1) != 1) or (rows > 1 and value.stride(0) < cols)):
         value = value.contiguous()
     return value
+
+
+def _span(value):
+    """The addresses from a tensor's first byte to behind its last one."""
+    last = sum((size - 1) * stride for size, stride in zip(value.shape, value.stride()))
+    return value.data_ptr(), value.data_ptr() + (last + 1) * value.element_size()
+
+
+def _overlap(written, read):
+    """Whether one of the tensors written shares memory with another of them, or with a tensor read that is not its own:
+    ``read`` holds (tensor, the index in ``written`` of the tensor that may lie on it, or None)."""
+    spans = sorted((*_span(value), index) for index, value in enumerate(written) if value.numel())
+    if any(end > start for (_, end, _), (start, _, _) in zip(spans, spans[1:])):
+        return True
+    starts = [start for start, _, _ in spans]
+    for value, own in read:
+        if not value.numel():
+            continue
+        first, end = _span(value)
+        at = max(0, bisect_right(starts, first) - 1)
+        while at < len(spans) and spans[at][0] < end:
+            if spans[at][1] > first and spans[at][2] != own:
+                return True
+            at += 1
+    return False
 
 
 @lru_cache(maxsize=64)
@@ -78,13 +105,15 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
     of zeros stays one (for an eps above 0), and one with an infinity or NaN becomes NaN. The same call
     gives the same bits each time; which order a matrix's sums are added in may depend on the call's other matrices.
     ``out`` takes the results (each a contiguous
-    tensor of its matrix's shape and type, possibly the matrix itself). Other coefficients must keep values of
+    tensor of its matrix's shape and type, possibly the matrix itself but no other one's memory). Other coefficients must keep values of
     0 .. 1 below 3.5, and a + b x^2 + c x^4 below 15, at every step."""
     matrices = list(matrices)
     (a, b, c), steps = _polynomial(coefficients, steps)
     eps = float(eps)
     if not (math.isfinite(eps) and eps >= 0.0):
         raise ValueError("eps must be finite and not negative")
+    if len(matrices) > COUNT_LIMIT:
+        raise ValueError(f"a call takes at most {COUNT_LIMIT} matrices")
     views = [_matrix(value, "a matrix") for value in matrices]
     if out is None:
         out = [torch.empty_like(value, memory_format=torch.contiguous_format) for value in matrices]
@@ -96,6 +125,8 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
             if not (isinstance(to, torch.Tensor) and to.is_cuda and to.dtype is value.dtype and to.shape == value.shape
                     and to.is_contiguous()):
                 raise ValueError("out must hold contiguous GPU tensors of the matrices' shapes and types")
+        if _overlap(out, [(view, i) for i, view in enumerate(views)]):
+            raise ValueError("out must share no memory but with its own matrix")
     native._on_current_device(*matrices, *out)
     rows = {}
     for view, to in zip(views, out):
@@ -128,7 +159,8 @@ def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, s
     """One Muon step, in place, for (param, grad, buffer, rate, decay) tuples of float32 tensors of a shape with two
     dimensions or more: with g = grad * grad_scale, buffer = momentum * buffer + g; the parameter becomes
     (1 - decay) param - rate O, with O the orthogonalised g + momentum * buffer (buffer without nesterov). A strided
-    param or buffer is updated through a contiguous copy that is written back; no two of the tensors may overlap."""
+    param or buffer is updated through a contiguous copy that is written back; neither may overlap another of the
+    call's tensors."""
     (a, b, c), steps = _polynomial(coefficients, steps)
     rows, held, back = [], [], []
     for param, grad, buffer, rate, decay in updates:
@@ -144,9 +176,10 @@ def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, s
         rows.append((*(t.data_ptr() for t in tensors), *shape, 1.0 - decay, float(rate)))
     if not rows:
         return
-    spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for tensors in held for t in tensors)
-    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
-        raise ValueError("the tensors of a Muon step must not overlap")
+    if len(rows) > COUNT_LIMIT:
+        raise ValueError(f"a Muon step takes at most {COUNT_LIMIT} parameters")
+    if _overlap([t for param, _, buffer in held for t in (param, buffer)], [(grad, None) for _, grad, _ in held]):
+        raise ValueError("the params and buffers of a Muon step must not overlap, nor its gradients any of them")
     table = (native.MuonTensor * len(rows))(*rows)
     workspace, size = native.byte_workspace(_muon_workspace(tuple(row[3:5] for row in rows)))
     native._call("mfh_muon_step", table, len(rows), float(momentum), int(bool(nesterov)), float(grad_scale), steps, a, b, c,

@@ -50,7 +50,7 @@ SIZES = [
     # tokens (more than 64 rows), one token only, more positions than a chunk, slices of every size
     (1, 1, 1), (0, 5, 3), (3, 2, 2), (7, 1000, 8), (64, 100, 31), (65, 3, 64), (200, 1, 33), (129, 2, 513),
     (1000, 70000, 5), (1000, 50, 771), (5000, 1000, 512), (4096, 300000, 16), (33000, 130, 24), (40000, 8, 9),
-    (140000, 3000, 4), (777, 65537, 1030),
+    (140000, 3000, 4), (777, 65537, 1030), (300, 262144, 3), (66000, 5, 20),
 ]
 
 
@@ -206,6 +206,23 @@ def test_recorded_and_captured_steps_repeat_the_eager_bits():
             torch.cuda.synchronize()
         results.append(layer.W.value.clone())
     assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+
+
+@gpu
+def test_an_optimized_graph_gives_the_plain_graphs_gradients():
+    mf.set_device("cuda")
+    ids = mf.Variable(torch.arange(50, device="cuda") % 7, requires_grad=False)
+    labels = mf.Variable(torch.arange(50, device="cuda") % 9, requires_grad=False)
+    grads = []
+    for optimize in (False, True):
+        layer = mf.Embedding(7, 12, initializer=mf.make_initializer("normal", seed=1, std=0.5))
+        hidden = mf.Dense(12, 16, activation=mf.ReLU, initializer=mf.make_initializer(seed=2))
+        head = mf.Dense(16, 9, initializer=mf.make_initializer(seed=3))
+        graph = mf.Graph(mf.CrossEntropyLoss(head(hidden(layer(ids))), labels), optimize=optimize)
+        graph.forward()
+        graph.backward()
+        grads.append(layer.W.grad)
+    assert torch.equal(grads[0], grads[1])
 
 
 @gpu

@@ -136,5 +136,7 @@ def test_refusals():
     for bad in ((p.half(), g, b), (p, g.cpu(), b), (p, g, b.double())):
         with pytest.raises(TypeError):
             orthogonal.muon_update_many([(*bad, 0.1, 0.0)])
+    same = torch.ones((4, 5), device="cuda")  # one gradient of two parameters is no overlap
+    orthogonal.muon_update_many([(p.clone(), same, b.clone(), 0.1, 0.0), (p.clone(), same, b.clone(), 0.1, 0.0)])
     with pytest.raises(ValueError, match="overlap"):
         orthogonal.muon_update_many([(p, g, b, 0.1, 0.0), (g, torch.ones_like(p), torch.ones_like(p), 0.1, 0.0)])

@@ -198,3 +198,14 @@ def test_refusals():
             ops.orthogonalize(matrix, out=out)
     with pytest.raises(ValueError, match="out"):
         ops.orthogonalize_many([matrix], out=[])
+    held = torch.randn(40, device="cuda")
+    first, second = held[:12].view(3, 4), held[20:32].view(3, 4)
+    for out in ([first, first], [second, first], [held[16:28].view(3, 4), first], [held[10:22].view(3, 4), second]):
+        with pytest.raises(ValueError, match="share no memory"):
+            ops.orthogonalize_many([first, second], out=out)
+    want = [ops.orthogonalize(first.clone()), ops.orthogonalize(second.clone())]
+    moved = held.clone()  # a result that lies across its own matrix: all are read before any result is written
+    assert torch.equal(ops.orthogonalize(moved[:12].view(3, 4), out=moved[5:17].view(3, 4)), want[0])
+    got = ops.orthogonalize_many([first, second], out=[first, second])
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b, rtol=0.0, atol=1e-5)
