@@ -25,7 +25,7 @@ constexpr float NOT_A_NUMBER = __builtin_nanf("");
 // ---- lookup -----------------------------------------------------------------------------------
 // Bound by HBM (each row looked up is read and written once) or, for few rows, by the two dependent loads of an
 // id and its row. A workgroup takes a few neighbouring rows, whose packs its threads share whatever the rows'
-// length is; four packs a thread are in flight. 65536 rows of 2048 bfloat16: 73 us (7 TB/s, rows of frequent tokens
+// length is; four packs a thread are in flight. 65536 rows of 2048 bfloat16: 69 us (7.7 TB/s, rows of frequent tokens
 // from the caches).
 constexpr int LOOKUP_PACKS = 4;
 
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_kernel(EmbeddingGradient g,
 // of that many, and a chunk holds a piece of at most two such tokens, the one that it begins with and the one that
 // it ends with. sum_kernel's first workgroups sum the pieces, the others the rows of each other token; join_kernel
 // sums the pieces of a token, of which at most one begins in a chunk. Bound by HBM: each gradient row is read once,
-// the table's gradient written once. 65536 rows of 2048 bfloat16 into a table of 65536: 143 us and 9 (3.5 TB/s).
+// the table's gradient written once. 65536 rows of 2048 bfloat16 into a table of 65536: 140 us and 9 (3.6 TB/s).
 struct SumPlan {
     int chunk;       // positions of a piece
     int lanes;       // lanes (a power of two) that share a row's packs

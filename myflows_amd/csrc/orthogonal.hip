@@ -407,7 +407,6 @@ struct SourceGroup {
     Source s[GROUP];
     int first_block[GROUP + 1];
     int square_blocks[GROUP];
-    int count;
     float eps;
 };
 static_assert(sizeof(SourceGroup) <= 4096, "descriptors must fit the kernel arguments");
@@ -715,7 +714,7 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
     }
     char* const parts = workspace;
     SourceGroup sources{};
-    sources.count = count, sources.eps = o.eps;
+    sources.eps = o.eps;
     for (int i = 0; i < count; ++i) {
         const OrthogonalMatrix& m = matrices[i];
         const bool tall = m.rows > m.cols;
