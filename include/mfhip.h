@@ -662,7 +662,7 @@ MFH_API int64_t mfh_orthogonalize_workspace(const mfh_orthogonal_matrix* matrice
 /* out = the matrix M of an element type taken through `steps` (1..64) Newton-Schulz steps: with X = M / (|M| + eps)
  * (the Frobenius norm) and the shorter side as rows, X = a X + (b G + c G G) X with G = X X^T, so that each singular
  * value x becomes x (a + b x^2 + c x^4). Formed to the precision of float32 products and rounded once. The
- * polynomial must keep the values from 0 to 1 below 3.5, and a + b x^2 + c x^4 below 15, at every step. The table is
+ * polynomial must keep the values from 0 to 1 below 3.5, and b x^2 + c x^4 below 15.9, at every step. The table is
  * host memory, read during the call. counters as of the rows of logits. No counterpart in the reference. */
 MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, int type, int steps, float a, float b, float c,
                               float eps, uint64_t workspace, int64_t workspace_bytes, uint64_t counters, uint64_t stream);

@@ -68,14 +68,16 @@ def _overlap(written, read):
 
 @lru_cache(maxsize=64)
 def _checked_polynomial(coefficients, steps):
-    """The coefficients, once a sampling of 0 .. 1 shows that the steps keep every singular value below 3.5 and the
-    polynomial's factor below 15: the range that the kernels hold."""
+    """The coefficients, once it is shown that the steps keep every singular value below 3.5 and b x^2 + c x^4 below
+    15.9: the kernels hold X, G and B = b G + c G G 2^12 times as large in float16, which ends at 2^12 * 15.99. The
+    values that a step meets are all of 0 .. top (a continuous image of 0 .. 1 that holds 0); they are sampled."""
     a, b, c = coefficients
-    values = [i / 4096 for i in range(4097)]
+    top = 1.0
     for _ in range(steps):
-        factors = [a + b * x * x + c * x ** 4 for x in values]
-        values = [x * f for x, f in zip(values, factors)]
-        if not (max(map(abs, factors)) < 15.0 and max(map(abs, values)) < 3.5):
+        values = [top * i / 4096 for i in range(4097)]
+        factors = [b * x * x + c * x ** 4 for x in values]
+        top = max(abs(x * (a + f)) for x, f in zip(values, factors))
+        if not (max(map(abs, factors)) < 15.9 and top < 3.5):
             raise ValueError(f"the coefficients {coefficients} take singular values out of range in {steps} steps")
     return coefficients
 
@@ -106,7 +108,7 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
     gives the same bits each time; which order a matrix's sums are added in may depend on the call's other matrices.
     ``out`` takes the results (each a contiguous
     tensor of its matrix's shape and type, possibly the matrix itself but no other one's memory). Other coefficients must keep values of
-    0 .. 1 below 3.5, and a + b x^2 + c x^4 below 15, at every step."""
+    0 .. 1 below 3.5, and b x^2 + c x^4 below 15.9, at every step."""
     matrices = list(matrices)
     (a, b, c), steps = _polynomial(coefficients, steps)
     eps = float(eps)

@@ -184,6 +184,43 @@ def test_refusals_without_a_gpu():
             ops.orthogonalize_many([], **options)
 
 
+@pytest.mark.parametrize("steps,coefficients", [(1, (14.9, -44.5, 27.0)), (1, (12.0, -55.0, 46.0)), (1, (13.0, -30.0, 13.6)),
+                                                (2, (13.0, -30.0, 13.6))])
+def test_polynomials_whose_products_leave_the_range_are_refused(steps, coefficients):
+    # Each keeps the values below 3.5 and a + b x^2 + c x^4 below 15, but b x^2 + c x^4 passes 16 on 0 .. 1.
+    with pytest.raises(ValueError, match="out of range"):
+        ops.orthogonalize_many([], steps=steps, coefficients=coefficients)
+
+
+def test_polynomials_within_the_range_are_taken():
+    for steps, coefficients in ((64, ops.COEFFICIENTS), (1, (12.507, -49.235, 38.123)), (1, (13.424, -50.472, 40.054)),
+                                (5, (1.5, -0.5, 0.0)), (1, (2.0, 0.0, 0.0))):
+        assert ops._polynomial(coefficients, steps) == (coefficients, steps)
+
+
+@gpu
+@pytest.mark.parametrize("coefficients", [(12.507, -49.235, 38.123), (13.424, -50.472, 40.054), (5.0, -17.0, 12.0)])
+@pytest.mark.parametrize("side", [2, 130])
+def test_products_near_the_end_of_the_range(side, coefficients):
+    """Two singular values, one where |b x^2 + c x^4| is largest on 0 .. 1. With u = 2^-23, X is held to u, G = x^2 to 4 u
+    (twice X's, its product's and its own), b G + c G G to (6.5 |b| x^2 + 11.5 |c| x^4) u (G's errors, the product's, the
+    coefficients', two float32 roundings and its own), and with X's error and three roundings more the step's result to
+    x (3 |a| + 10 |b| x^2 + 15 |c| x^4) u."""
+    a, b, c = coefficients
+    grid = torch.arange(1, 4097, dtype=torch.float64) / 4096
+    x = float(grid[(b * grid ** 2 + c * grid ** 4).abs().argmax()])
+    values = torch.tensor([x, (1.0 - x * x) ** 0.5], dtype=torch.float64)
+    matrix = torch.zeros((side, side), device="cuda")
+    matrix[0, 0], matrix[1, 1] = values.float()
+    got = ops.orthogonalize(matrix, steps=1, coefficients=coefficients).cpu().double()
+    want = _steps(matrix, torch.float64, steps=1, coefficients=coefficients)
+    bound = values * (3 * abs(a) + 10 * abs(b) * values ** 2 + 15 * abs(c) * values ** 4) * 2.0 ** -23
+    off = (got - want).abs()
+    assert bool((off.diagonal()[:2] <= bound).all())
+    got[0, 0] = got[1, 1] = 0.0
+    assert not bool(got.any())
+
+
 @gpu
 def test_refusals():
     matrix = torch.zeros((3, 4), device="cuda")
