@@ -640,7 +640,8 @@ MFH_API int64_t mfh_embedding_workspace(int64_t count, int64_t vocab, int dim, i
 
 /* table_grad[v] (written, or added to with add) = scale * the sum of the rows grad[p] with ids[p] = v, in rising
  * order of p and float32, rounded once; grad is of `type`, table_grad (vocab x dim) of the same or float32. Tokens
- * outside of the table count nowhere. Every row is written; with add, rows that no token names stay as they are. */
+ * outside of the table count nowhere. Every row is written; with add, rows that no token names stay as they are.
+ * table_grad shares no memory with grad and ids. */
 MFH_API int mfh_embedding_backward(uint64_t grad, int type, int64_t count, int dim, int64_t grad_stride, uint64_t ids,
                                    int ids_int64, int64_t ids_stride, int64_t vocab, float scale, uint64_t table_grad,
                                    int table_grad_type, int64_t table_grad_stride, int add, uint64_t workspace,

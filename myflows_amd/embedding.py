@@ -17,6 +17,7 @@ from . import native
 from .graph import GradientOp
 from .init import make_initializer
 from .layers import Layer, _count, _parameter
+from .memory import share_memory
 
 COUNT_LIMIT = 1 << 30
 VOCAB_LIMIT = 1 << 24
@@ -82,15 +83,16 @@ def embedding_forward(table, ids, *, scale=1.0):
 def embedding_backward(grad, ids, vocab, *, scale=1.0, out=None, add=False):
     """The gradient (vocab, dim) of the table from that of embedding_forward's output (ids' shape, dim): scale
     times the sum of the rows of each token, in float32 and the order of the tokens, rounded once. It is written to
-    (or, with add, added to) out, of grad's type or float32 with contiguous rows; a row that no token names
-    is zeros (with add, left as it is). Tokens beyond the vocabulary count nowhere."""
+    (or, with add, added to) out, of grad's type or float32 with contiguous rows, which shares no memory with grad
+    and ids; a row that no token names is zeros (with add, left as it is). Tokens beyond the vocabulary count nowhere."""
     flat, wide, step = _tokens(ids)
     if not isinstance(grad, torch.Tensor) or grad.ndim != ids.ndim + 1 or grad.shape[:-1] != ids.shape:
         raise ValueError("grad must have the shape of ids and one more dimension")
     vocab, dim = int(vocab), int(grad.shape[-1])
     _table_sizes(vocab, dim)
     grad, grad_stride = _rows(grad if grad.ndim == 2 else grad.reshape(-1, dim), "grad")
-    if out is None:
+    given = out is not None
+    if not given:
         if add:
             raise ValueError("add needs an out tensor")
         out = torch.empty((vocab, dim), dtype=grad.dtype, device=grad.device)
@@ -99,6 +101,8 @@ def embedding_backward(grad, ids, vocab, *, scale=1.0, out=None, add=False):
               and (vocab <= 1 or out.stride(0) >= dim)):
         raise ValueError("out must be a (vocab, dim) GPU tensor of grad's type or float32 with contiguous rows")
     native._on_current_device(grad, flat, out)
+    if given and (share_memory(out, grad) or share_memory(out, flat)):
+        raise ValueError("out must share no memory with grad and ids")
     code = native.TYPE_CODES[grad.dtype]
     workspace, held = native.byte_workspace(_workspace(flat.numel(), vocab, dim, code))
     native._call("mfh_embedding_backward", grad.data_ptr(), code, flat.numel(), dim, grad_stride, flat.data_ptr(), wide,

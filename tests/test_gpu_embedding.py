@@ -281,3 +281,20 @@ def test_refusals():
                 torch.zeros((1, 3), device="cuda").expand(4, 3)):
         with pytest.raises(ValueError, match="out"):
             ops.embedding_backward(grad, ids, 4, out=out)
+
+
+@gpu
+def test_a_gradient_written_over_what_it_is_made_of_is_refused():
+    held = torch.zeros((30, 8), device="cuda")
+    ids = torch.zeros(10, dtype=torch.int64, device="cuda")
+    for grad, out in ((held[:10], held[:4]), (held[:10], held[9:13]), (held[5:15, :4], held[:6, 3:7]),
+                      (held[:10], held[10:14].view(-1).as_strided((4, 8), (8, 1), 79))):
+        for add in (False, True):
+            with pytest.raises(ValueError, match="share no memory"):
+                ops.embedding_backward(grad, ids, out.shape[0], out=out, add=add)
+    words = torch.zeros(40, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.embedding_backward(torch.zeros((10, 8), device="cuda"), words[20:30], 4, out=words[10:].view(torch.float32)[:32].view(4, 8))
+    grad = torch.randn((10, 8), device="cuda")
+    want = ops.embedding_backward(grad[:, :3].contiguous(), ids, 10)
+    assert torch.equal(ops.embedding_backward(grad[:, :3], ids, 10, out=grad[:, 4:7]), want)  # rows side by side
