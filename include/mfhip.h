@@ -565,7 +565,8 @@ MFH_API int mfh_log_probs_backward(uint64_t logits, int type, int64_t rows, int 
  *   bias_ids, bias_values: `biases` (at most 1024) of a row; values of equal ids add up in their order.
  *   allowed: bits, bit v % 32 of 32-bit word v / 32 of a row; a token without its bit gets -inf.
  * Tokens and ids outside of the vocabulary count nowhere. Computed in float32 and rounded once to the logits' type.
- * out is logits (with the same stride) or shares no memory with them. No counterpart in the reference. */
+ * out is logits (with the same stride) or shares no memory with them, and shares none with the rest. No counterpart in
+ * the reference. */
 MFH_API int mfh_adjust_logits(uint64_t logits, int type, int64_t rows, int vocab, int64_t row_stride, uint64_t tokens,
                               int tokens_int64, int64_t tokens_stride, int held, uint64_t prompt_lengths, int prompt_int64,
                               int64_t prompt_stride, uint64_t repetition, int64_t repetition_stride, float repetition_all,

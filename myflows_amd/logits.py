@@ -23,6 +23,7 @@ import torch
 
 from . import native
 from .graph import GradientOp
+from .memory import share_memory
 
 _TYPE_CODES = native.TYPE_CODES
 _WHOLE = {torch.int32: 0, torch.int64: 1}  # whether whole numbers are int64
@@ -245,19 +246,10 @@ def _rows_of(value, rows, name):
     return value
 
 
-def _disjoint(one, other, stride, other_stride):
-    """Whether two tensors of one shape and type, of contiguous rows at these strides, share no memory: one lies
-    behind the other, or their rows lie side by side."""
-    rows, length = one.shape
-    apart = (other.data_ptr() - one.data_ptr()) // one.element_size()
-    if apart >= (rows - 1) * stride + length or -apart >= (rows - 1) * other_stride + length:
-        return True
-    return stride == other_stride and length <= apart % stride <= stride - length
-
-
 def adjust_logits(logits, *, tokens=None, prompt_lengths=None, repetition=1.0, presence=0.0, frequency=0.0,
                   bias_ids=None, bias_values=None, allowed=None, out=None):
-    """The logits as an answer is drawn from them, of their type; out may be the logits themselves.
+    """The logits as an answer is drawn from them, of their type; out may be the logits themselves, and shares no
+    memory with anything else that the call reads.
 
     ``tokens`` (rows, held) are a row's history: its prompt, the first ``prompt_lengths[row]`` of them (none
     without), and its answer so far. A logit z of a token in the history becomes z / repetition where z > 0 and
@@ -307,12 +299,15 @@ def adjust_logits(logits, *, tokens=None, prompt_lengths=None, repetition=1.0, p
         if allowed.stride(1) != 1 and allowed.shape[1] > 1:
             allowed = allowed.contiguous()
         allowed_stride = allowed.stride(0)
+    given = out is not None
     out, out_stride = _gradient(out, False, logits)
-    if rows and (out.data_ptr() != logits.data_ptr() or out_stride != stride):
-        if not _disjoint(logits, out, stride, out_stride):
+    read = (tokens, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values, allowed)
+    native._on_current_device(logits, out, *read)
+    if given:
+        if (out.data_ptr() != logits.data_ptr() or out_stride != stride) and share_memory(out, logits):
             raise ValueError("out must be the logits themselves or share no memory with them")
-    native._on_current_device(logits, tokens, prompt_lengths, repetition, presence, frequency, bias_ids, bias_values,
-                              allowed, out)
+        if any(value is not None and share_memory(out, value) for value in read):
+            raise ValueError("out must share no memory with what the logits are adjusted by")
     native._call("mfh_adjust_logits", logits.data_ptr(), code, rows, vocab, stride, native._addr(tokens), wide,
                  tokens_stride, held, native._addr(prompt_lengths), prompt_wide, prompt_stride, native._addr(repetition),
                  repetition_stride, repetition_all, native._addr(presence), presence_stride, presence_all,

@@ -252,3 +252,26 @@ def test_refusals():
     _check(got, side[:, 3:53], tokens, presence=1.0)
     with pytest.raises(ValueError, match="share no memory"):
         ops.adjust_logits(side[:, 3:53], out=side[:, 52:102])
+
+
+@gpu
+def test_results_written_over_what_logits_are_adjusted_by_are_refused():
+    held = torch.zeros(1000, device="cuda")
+    z, out, words = torch.zeros((4, 50), device="cuda"), held[100:300].view(4, 50), held.view(torch.int32)
+    tokens = words[:200].view(4, 50)
+    for options in (dict(tokens=tokens), dict(tokens=tokens[:, :3], prompt_lengths=words[297:301]), dict(repetition=held[150:154]),
+                    dict(presence=held[299:303]), dict(frequency=held[97:101]), dict(bias_ids=tokens[:, :2], bias_values=z[:, :2]),
+                    dict(bias_ids=torch.zeros((4, 2), dtype=torch.int32, device="cuda"), bias_values=held[290:298].view(4, 2)),
+                    dict(allowed=words[292:300].view(4, 2)), dict(allowed=words[299:301])):
+        for logits in (z, out):
+            with pytest.raises(ValueError, match="share no memory"):
+                ops.adjust_logits(logits, out=out, **options)
+    # Rows of logits and what they are adjusted by side by side, adjusted in place.
+    rows = torch.randn((4, 54), device="cuda")
+    rows[:, 50:] = torch.tensor([1.5, 0.5, 0.25, 0.0], device="cuda")
+    rows[:, 53] = torch.arange(4, dtype=torch.int32, device="cuda").view(torch.float32)
+    at = rows.view(torch.int32)[:, 53:]
+    want = ops.adjust_logits(rows[:, :50].clone(), tokens=at.clone(), repetition=1.5, presence=0.5, frequency=0.25)
+    got = ops.adjust_logits(rows[:, :50], tokens=at, repetition=rows[:, 50], presence=rows[:, 51], frequency=rows[:, 52],
+                            out=rows[:, :50])
+    assert torch.equal(got, want)
