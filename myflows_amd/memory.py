@@ -8,6 +8,10 @@ matrix's columns): they share nothing, and are told apart exactly.
 from __future__ import annotations
 
 from functools import lru_cache
+from heapq import heappop, heappush
+from itertools import chain
+
+import torch
 
 
 def span(value):
@@ -66,3 +70,43 @@ def share_memory(one, other):
         return True
     return _runs_meet(_runs(tuple(one.shape), one.stride(), one.element_size()),
                       _runs(tuple(other.shape), other.stride(), other.element_size()), other_first - first)
+
+
+@lru_cache(maxsize=1024)
+def _folded(shape, strides):
+    """Whether two of the elements of these sizes and strides are one."""
+    reach = 1
+    for stride, count in sorted((stride, count) for stride, count in zip(strides, shape) if count > 1):
+        if stride < reach:
+            break
+        reach += stride * (count - 1)
+    else:
+        return False
+    offsets = torch.zeros((1,), dtype=torch.int64)
+    for stride, count in zip(strides, shape):
+        if count > 1 and not stride:
+            return True
+        offsets = (offsets[:, None] + torch.arange(count) * stride).reshape(-1)
+    return offsets.unique().numel() < offsets.numel()
+
+
+def overlap(written, read=()):
+    """Whether one of the tensors written shares memory with itself, with another of them, or with a tensor read that is
+    not its own: ``read`` holds (tensor, the index in ``written`` of the tensor that may lie on it, or None)."""
+    entries = [(*span(value), index, False, value) for index, value in enumerate(written) if value.numel()]
+    if any(not value.is_contiguous() and _folded(tuple(value.shape), value.stride()) for *_, value in entries):
+        return True
+    entries += [(*span(value), own, True, value) for value, own in read if value.numel()]
+    entries.sort(key=lambda entry: entry[:2])
+    writes, reads = [], []  # those whose spans have not ended, the one that ends first at the front
+    for order, (first, end, own, is_read, value) in enumerate(entries):
+        for held in (writes, reads):
+            while held and held[0][0] <= first:
+                heappop(held)
+        for _, _, other_own, other_is_read, other in writes if is_read else chain(writes, reads):
+            if (is_read or other_is_read) and own == other_own:
+                continue
+            if share_memory(value, other):
+                return True
+        heappush(reads if is_read else writes, (end, order, own, is_read, value))
+    return False

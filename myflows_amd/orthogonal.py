@@ -10,12 +10,12 @@ its only optimisers with a state are elementwise.
 from __future__ import annotations
 
 import math
-from bisect import bisect_right
 from functools import lru_cache
 
 import torch
 
 from . import native
+from .memory import overlap
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # steep at 0, and within 0.7 .. 1.2 for what began above 0.002, in five steps
 STEPS = 5
@@ -39,31 +39,6 @@ def _matrix(value, name):
     if rows and cols and ((cols > 1 and value.stride(1) != 1) or (rows > 1 and value.stride(0) < cols)):
         value = value.contiguous()
     return value
-
-
-def _span(value):
-    """The addresses from a tensor's first byte to behind its last one."""
-    last = sum((size - 1) * stride for size, stride in zip(value.shape, value.stride()))
-    return value.data_ptr(), value.data_ptr() + (last + 1) * value.element_size()
-
-
-def _overlap(written, read):
-    """Whether one of the tensors written shares memory with another of them, or with a tensor read that is not its own:
-    ``read`` holds (tensor, the index in ``written`` of the tensor that may lie on it, or None)."""
-    spans = sorted((*_span(value), index) for index, value in enumerate(written) if value.numel())
-    if any(end > start for (_, end, _), (start, _, _) in zip(spans, spans[1:])):
-        return True
-    starts = [start for start, _, _ in spans]
-    for value, own in read:
-        if not value.numel():
-            continue
-        first, end = _span(value)
-        at = max(0, bisect_right(starts, first) - 1)
-        while at < len(spans) and spans[at][0] < end:
-            if spans[at][1] > first and spans[at][2] != own:
-                return True
-            at += 1
-    return False
 
 
 @lru_cache(maxsize=64)
@@ -127,7 +102,7 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
             if not (isinstance(to, torch.Tensor) and to.is_cuda and to.dtype is value.dtype and to.shape == value.shape
                     and to.is_contiguous()):
                 raise ValueError("out must hold contiguous GPU tensors of the matrices' shapes and types")
-        if _overlap(out, [(view, i) for i, view in enumerate(views)]):
+        if overlap(out, [(view, i) for i, view in enumerate(views)]):
             raise ValueError("out must share no memory but with its own matrix")
     native._on_current_device(*matrices, *out)
     rows = {}
@@ -161,10 +136,11 @@ def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, s
     """One Muon step, in place, for (param, grad, buffer, rate, decay) tuples of float32 tensors of a shape with two
     dimensions or more: with g = grad * grad_scale, buffer = momentum * buffer + g; the parameter becomes
     (1 - decay) param - rate O, with O the orthogonalised g + momentum * buffer (buffer without nesterov). A strided
-    param or buffer is updated through a contiguous copy that is written back; neither may overlap another of the
-    call's tensors."""
+    param or buffer is updated through a contiguous copy that is written back; neither may overlap itself or another
+    of the call's tensors."""
     (a, b, c), steps = _polynomial(coefficients, steps)
-    rows, held, back = [], [], []
+    updates = list(updates)
+    rows, held, back = [], [], []  # held: the copies of strided tensors, until the call is issued
     for param, grad, buffer, rate, decay in updates:
         tensors = [native._device_f32(t, name) for t, name in ((param, "param"), (grad, "grad"), (buffer, "buffer"))]
         if any(t.shape != param.shape for t in tensors):
@@ -180,7 +156,8 @@ def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, s
         return
     if len(rows) > COUNT_LIMIT:
         raise ValueError(f"a Muon step takes at most {COUNT_LIMIT} parameters")
-    if _overlap([t for param, _, buffer in held for t in (param, buffer)], [(grad, None) for _, grad, _ in held]):
+    # The caller's tensors, not their copies: a copy is written back over what it was made of.
+    if overlap([t for param, _, buffer, _, _ in updates for t in (param, buffer)], [(grad, None) for _, grad, *_ in updates]):
         raise ValueError("the params and buffers of a Muon step must not overlap, nor its gradients any of them")
     table = (native.MuonTensor * len(rows))(*rows)
     workspace, size = native.byte_workspace(_muon_workspace(tuple(row[3:5] for row in rows)))

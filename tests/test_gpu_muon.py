@@ -140,3 +140,24 @@ def test_refusals():
     orthogonal.muon_update_many([(p.clone(), same, b.clone(), 0.1, 0.0), (p.clone(), same, b.clone(), 0.1, 0.0)])
     with pytest.raises(ValueError, match="overlap"):
         orthogonal.muon_update_many([(p, g, b, 0.1, 0.0), (g, torch.ones_like(p), torch.ones_like(p), 0.1, 0.0)])
+
+
+@gpu
+def test_overlap_is_that_of_the_tensors_given_not_of_their_copies():
+    make = lambda *shape: torch.randn(shape, device="cuda")  # noqa: E731
+    w, one = make(6, 6), torch.ones((6, 6), device="cuda")
+    alike = make(6, 12)
+    for updates in ([(w.t(), one, make(6, 6), 0.1, 0.0), (w, one, make(6, 6), 0.1, 0.0)],
+                    [(w.t(), one, w, 0.1, 0.0)], [(w.t(), one, w.t(), 0.1, 0.0)], [(w.t(), w, make(6, 6), 0.1, 0.0)],
+                    [(alike[:, :6], one, alike[:, 5:11], 0.1, 0.0)], [(make(1, 6).expand(6, 6), one, make(6, 6), 0.1, 0.0)],
+                    [(make(6, 6), one, make(6, 1).expand(6, 6), 0.1, 0.0)]):
+        before = [[t.clone() for t in update[:3]] for update in updates]
+        with pytest.raises(ValueError, match="overlap"):
+            orthogonal.muon_update_many(updates)
+        assert all(torch.equal(a, b) for update, held in zip(updates, before) for a, b in zip(update, held))
+    # Columns side by side are no overlap.
+    left, right, momentum = alike[:, :6], alike[:, 6:], torch.zeros((6, 12), device="cuda")
+    twins = [(t.clone(), torch.zeros((6, 6), device="cuda")) for t in (left, right)]
+    orthogonal.muon_update_many([(left, one, momentum[:, :6], 0.1, 0.0), (right, one, momentum[:, 6:], 0.1, 0.0)])
+    orthogonal.muon_update_many([(p, one, b, 0.1, 0.0) for p, b in twins])
+    assert torch.equal(alike, torch.cat([p for p, _ in twins], 1)) and torch.equal(momentum, torch.cat([b for _, b in twins], 1))
