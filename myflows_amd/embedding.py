@@ -55,8 +55,8 @@ def _table_sizes(vocab, dim):
 
 def _scale(value):
     value = float(value)
-    if not math.isfinite(value):
-        raise ValueError("scale must be finite")
+    if not math.isfinite(native._float32(value)):
+        raise ValueError("scale must be finite in float32")
     return value
 
 

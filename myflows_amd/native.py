@@ -379,6 +379,11 @@ def _on_current_device(*tensors):
             raise ValueError(f"a tensor lies on cuda:{tensor.get_device()}, the current device is cuda:{device}")
 
 
+def _float32(value):
+    """A number as the library receives it, rounded to float32: what is checked has to be that."""
+    return ctypes.c_float(float(value)).value
+
+
 def _within_int32(**counts):
     for name, count in counts.items():
         if int(count) > INT32_LIMIT:

@@ -298,3 +298,22 @@ def test_a_gradient_written_over_what_it_is_made_of_is_refused():
     grad = torch.randn((10, 8), device="cuda")
     want = ops.embedding_backward(grad[:, :3].contiguous(), ids, 10)
     assert torch.equal(ops.embedding_backward(grad[:, :3], ids, 10, out=grad[:, 4:7]), want)  # rows side by side
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 3.4028236e38, float("inf"), float("nan")])
+def test_scales_beyond_float32_are_refused(scale):
+    with pytest.raises(ValueError, match="finite"):
+        mf.Embedding(3, 3, scale=scale)
+
+
+@gpu
+def test_the_largest_scale_leaves_zeros_and_unnamed_rows():
+    scale = torch.finfo(torch.float32).max
+    ids = torch.tensor([1, -1], device="cuda")
+    y = ops.embedding_forward(torch.ones((3, 5), device="cuda"), ids, scale=scale)
+    assert bool((y[0] == scale).all()) and bool((y[1] == 0).all())
+    grad = ops.embedding_backward(torch.ones((2, 5), device="cuda"), ids, 3, scale=scale)
+    assert bool((grad[1] == scale).all()) and bool((grad[[0, 2]] == 0).all())
+    for call in (lambda: ops.embedding_forward(y, ids, scale=1e39), lambda: ops.embedding_backward(y, ids, 3, scale=1e39)):
+        with pytest.raises(ValueError, match="finite"):
+            call()
