@@ -231,9 +231,9 @@ def _penalty(value, rows, name, positive=False):
     """(tensor or None, stride, value for all rows) of a penalty: a number, or one float32 a row."""
     if isinstance(value, torch.Tensor):
         return *_row_floats(value, rows, name), 0.0
-    value = float(value)
+    value = native._float32(value)
     if not math.isfinite(value) or (positive and value <= 0.0):
-        raise ValueError(f"{name} must be finite{' and positive' if positive else ''}")
+        raise ValueError(f"{name} must be finite{' and positive' if positive else ''} in float32")
     return None, 0, value
 
 

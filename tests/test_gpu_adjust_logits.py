@@ -275,3 +275,29 @@ def test_results_written_over_what_logits_are_adjusted_by_are_refused():
     got = ops.adjust_logits(rows[:, :50], tokens=at, repetition=rows[:, 50], presence=rows[:, 51], frequency=rows[:, 52],
                             out=rows[:, :50])
     assert torch.equal(got, want)
+
+
+def test_penalties_that_float32_does_not_hold_are_refused():
+    for bad in (1e39, 3.4028236e38, 1e-46, 0.0, -1e-46):
+        with pytest.raises(ValueError, match="finite and positive"):
+            ops._penalty(bad, 4, "repetition", positive=True)
+    for bad in (1e39, -1e39, -3.4028236e38):
+        with pytest.raises(ValueError, match="finite"):
+            ops._penalty(bad, 4, "presence")
+    assert ops._penalty(1e-40, 4, "repetition", positive=True)[2] > 0.0 and ops._penalty(-1e-46, 4, "presence")[2] == 0.0
+
+
+@gpu
+def test_the_smallest_and_largest_penalties():
+    z = torch.tensor([[2.0 ** -30, -2.0 ** -30, 0.0, 1.0]], device="cuda")
+    tokens = torch.tensor([[0, 1, 2]], device="cuda")
+    tiny, huge = 2.0 ** -149, torch.finfo(torch.float32).max
+    lengths = torch.tensor([3], device="cuda")
+    got = ops.adjust_logits(z, tokens=tokens, prompt_lengths=lengths, repetition=tiny)
+    assert got.tolist() == [[2.0 ** 119, 0.0, 0.0, 1.0]]  # 2^-179 lies below float32
+    got = ops.adjust_logits(z, tokens=tokens, prompt_lengths=lengths, repetition=2.0 ** 127)
+    assert got.tolist() == [[0.0, -2.0 ** 97, 0.0, 1.0]]  # and so does 2^-157
+    assert ops.adjust_logits(z, tokens=tokens, presence=huge).tolist() == [[-huge, -huge, -huge, 1.0]]
+    for name in ("repetition", "presence", "frequency"):
+        with pytest.raises(ValueError, match="finite"):
+            ops.adjust_logits(z, tokens=tokens, **{name: 1e39})
