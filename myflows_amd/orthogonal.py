@@ -67,6 +67,13 @@ def _polynomial(coefficients, steps):
     return _checked_polynomial(coefficients, steps), steps
 
 
+def _eps(value):
+    value, held = float(value), native._float32(value)
+    if not (math.isfinite(held) and value >= 0.0 and (held > 0.0 or value == 0.0)):
+        raise ValueError("eps must be 0, or positive and finite in float32")
+    return held
+
+
 @lru_cache(maxsize=256)
 def _workspace(shapes):
     table = (native.OrthogonalMatrix * len(shapes))(*((0, 0, cols, cols, rows, cols) for rows, cols in shapes))
@@ -86,9 +93,7 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
     0 .. 1 below 3.5, and b x^2 + c x^4 below 15.9, at every step."""
     matrices = list(matrices)
     (a, b, c), steps = _polynomial(coefficients, steps)
-    eps = float(eps)
-    if not (math.isfinite(eps) and eps >= 0.0):
-        raise ValueError("eps must be finite and not negative")
+    eps = _eps(eps)
     if len(matrices) > COUNT_LIMIT:
         raise ValueError(f"a call takes at most {COUNT_LIMIT} matrices")
     views = [_matrix(value, "a matrix") for value in matrices]
@@ -139,6 +144,7 @@ def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, s
     param or buffer is updated through a contiguous copy that is written back; neither may overlap itself or another
     of the call's tensors."""
     (a, b, c), steps = _polynomial(coefficients, steps)
+    eps = _eps(eps)
     updates = list(updates)
     rows, held, back = [], [], []  # held: the copies of strided tensors, until the call is issued
     for param, grad, buffer, rate, decay in updates:
@@ -162,6 +168,6 @@ def muon_update_many(updates, *, momentum=0.95, nesterov=True, grad_scale=1.0, s
     table = (native.MuonTensor * len(rows))(*rows)
     workspace, size = native.byte_workspace(_muon_workspace(tuple(row[3:5] for row in rows)))
     native._call("mfh_muon_step", table, len(rows), float(momentum), int(bool(nesterov)), float(grad_scale), steps, a, b, c,
-                 float(eps), workspace, size, native.stream_counters(), native._stream())
+                 eps, workspace, size, native.stream_counters(), native._stream())
     for old, new in back:
         old.copy_(new)

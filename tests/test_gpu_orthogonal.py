@@ -246,3 +246,18 @@ def test_refusals():
     got = ops.orthogonalize_many([first, second], out=[first, second])
     for a, b in zip(got, want):
         assert torch.allclose(a, b, rtol=0.0, atol=1e-5)
+
+
+@pytest.mark.parametrize("eps", [1e-50, 1e39, -1e-50, -1.0, float("inf"), float("nan")])
+def test_an_eps_that_float32_does_not_hold_is_refused(eps):
+    for call in (lambda: ops.orthogonalize_many([], eps=eps), lambda: ops.muon_update_many([], eps=eps)):
+        with pytest.raises(ValueError, match="eps"):
+            call()
+
+
+@gpu
+def test_zeros_stay_zeros_for_the_smallest_eps():
+    zeros = torch.zeros((3, 70), device="cuda")
+    assert torch.equal(ops.orthogonalize(zeros, eps=2.0 ** -149), zeros)
+    matrix = _matrix(40, 70, "float32", 8)
+    assert torch.equal(ops.orthogonalize(matrix, eps=2.0 ** -149), ops.orthogonalize(matrix, eps=0.0))
