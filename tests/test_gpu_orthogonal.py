@@ -202,10 +202,11 @@ def test_polynomials_within_the_range_are_taken():
 @pytest.mark.parametrize("coefficients", [(12.507, -49.235, 38.123), (13.424, -50.472, 40.054), (5.0, -17.0, 12.0)])
 @pytest.mark.parametrize("side", [2, 130])
 def test_products_near_the_end_of_the_range(side, coefficients):
-    """Two singular values, one where |b x^2 + c x^4| is largest on 0 .. 1. With u = 2^-23, X is held to u, G = x^2 to 4 u
-    (twice X's, its product's and its own), b G + c G G to (6.5 |b| x^2 + 11.5 |c| x^4) u (G's errors, the product's, the
-    coefficients', two float32 roundings and its own), and with X's error and three roundings more the step's result to
-    x (3 |a| + 10 |b| x^2 + 15 |c| x^4) u."""
+    """Two singular values, one where |b x^2 + c x^4| is largest on 0 .. 1. With u = 2^-23, X is held to u and a product is
+    formed to 2.5 u: lo is up to 2^-11 of its value, so lo lo up to 2 u, and a float32 rounding. So G = x^2 is held to 5.5 u
+    (2 from X), b G + c G G to (8 |b| x^2 + 16 |c| x^4) u (5.5 and 11 from G, 2.5 for G G, half a u for a coefficient, its
+    product and the sum, 1 for holding it), and with X's error, the product's and two roundings more the step's result to
+    x (3 |a| + 13 |b| x^2 + 21 |c| x^4) u."""
     a, b, c = coefficients
     grid = torch.arange(1, 4097, dtype=torch.float64) / 4096
     x = float(grid[(b * grid ** 2 + c * grid ** 4).abs().argmax()])
@@ -214,7 +215,7 @@ def test_products_near_the_end_of_the_range(side, coefficients):
     matrix[0, 0], matrix[1, 1] = values.float()
     got = ops.orthogonalize(matrix, steps=1, coefficients=coefficients).cpu().double()
     want = _steps(matrix, torch.float64, steps=1, coefficients=coefficients)
-    bound = values * (3 * abs(a) + 10 * abs(b) * values ** 2 + 15 * abs(c) * values ** 4) * 2.0 ** -23
+    bound = values * (3 * abs(a) + 13 * abs(b) * values ** 2 + 21 * abs(c) * values ** 4) * 2.0 ** -23
     off = (got - want).abs()
     assert bool((off.diagonal()[:2] <= bound).all())
     got[0, 0] = got[1, 1] = 0.0
