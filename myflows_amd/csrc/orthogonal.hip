@@ -5,11 +5,13 @@
 //
 // Precision. The polynomial raises small singular values by up to a each step (485 times in five), and with them
 // whatever error the products have: in 16-bit products it would be a tenth of the result. So every matrix is held as
-// the sum of two float16 values, hi + lo, 22 bits, and a product is hi hi + hi lo + lo hi on the matrix cores, added in
-// float32 (the splitting of single-precision products that Ootomo and Yokota published in 2022): as near to the
-// definition as float32 products, at three times the cost of one float16 product instead of the sixteen that the
-// matrix cores' float32 rate is below it. X and B are at most a few: values are held 2^12 times as large,
-// which keeps hi out of float16's subnormals and lo's steps below 2^-36.
+// the sum of two float16 values, hi + lo, within 2^-23 of it, and a product is hi hi + (hi lo + lo hi) on the matrix
+// cores, added in float32 (the splitting of single-precision products that Ootomo and Yokota published in 2022; lo lo,
+// 2^-25 of hi hi as a rule, is left out): as near to the definition as float32 products, at three times the cost of one
+// float16 product instead of the sixteen that the matrix cores' float32 rate is below it. 1024 x 4096: the result is off by
+// 1.5e-6 of its norm; the same steps in float32 by 4.1e-6 with the library's products and by 1.4e-6 on the host.
+// Values are held 2^12 times as large, which keeps hi out of float16's subnormals and lo's steps below 2^-36; float16 ends
+// at 16 times that, so a polynomial must keep X below 3.5, G's largest root, and b x^2 + c x^4, B's, below 15.9.
 //
 // Layout. A matrix lies in memory with both sides padded to whole tiles, zeros behind the last value; a row's 32 neighbouring values are 64 bytes of
 // hi and 64 of lo, so that one step of a product reads a cache line of each row. Every product is of the form A B^T
@@ -101,6 +103,15 @@ struct StagedRows {
 // The lane's 8 values of a 32 x 16 operand at LDS row `row` (its own lane % 32 included): part p of hi, or of lo.
 __device__ __forceinline__ half8 operand(const _Float16* lds, int row, int part) {
     return *reinterpret_cast<const half8*>(lds + row * ROW_STEP + (part ^ key_of(row)) * 8);
+}
+
+// One term of a product of two pieces, hi and lo: hi hi, added to `sum`, or hi lo or lo hi, added to `cross`. These are
+// 2^-11 of hi hi: on their own they are added without a rounding of the whole sum each. With one sum for all three the
+// result's error was half as large again (4096 x 4096: 2.3e-6 of it for 1.3e-6, 1024 x 4096: 2.2e-6 for 1.5e-6), in
+// no less time.
+__device__ __forceinline__ void add_term(int term, const half8 (&x)[2], const half8 (&y)[2], float16v& sum, float16v& cross) {
+    float16v& to = term == 0 ? sum : cross;
+    to = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[term == 2], y[term == 1], to, 0, 0, 0);
 }
 
 // A wave's scratch in LDS: 32 rows of a matrix as they lie in memory, 64 bytes of hi and 64 of lo each, their eight
@@ -286,12 +297,12 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
     const _Float16* b = p.b + static_cast<std::int64_t>(tile_j) * SIDE * pitch;
     const int begin = static_cast<int>(static_cast<long long>(p.ksteps) * part / parts);
     const int end = static_cast<int>(static_cast<long long>(p.ksteps) * (part + 1) / parts);
-    float16v sum[PIECES][PIECES] = {};
+    float16v sum[PIECES][PIECES] = {}, cross[PIECES][PIECES] = {};
     struct Operands {
         half8 x[PIECES][2], y[PIECES][2];  // hi and lo
     };
     // AHEAD steps are in registers, or on their way there.
-    constexpr int AHEAD = SIDE == SMALL ? 3 : 1;
+    constexpr int AHEAD = SIDE == SMALL ? 2 : 1;  // as many as leave four small tiles or two large ones a CU
     StagedRows<SIDE> rows_a[AHEAD], rows_b[AHEAD];
     const _Float16 *lane_a = StagedRows<SIDE>::lane_rows(a, pitch), *lane_b = StagedRows<SIDE>::lane_rows(b, pitch);
     const auto load = [&](int place, int step) {  // beyond the last step, that one again
@@ -321,8 +332,7 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
 #pragma unroll
             for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-                for (int j = 0; j < PIECES; ++j)
-                    sum[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.x[i][term == 2], o.y[j][term == 1], sum[i][j], 0, 0, 0);
+                for (int j = 0; j < PIECES; ++j) add_term(term, o.x[i], o.y[j], sum[i][j], cross[i][j]);
     };
     load(0, begin);
     store(0, begin);
@@ -350,6 +360,10 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
         }
     }
     __syncthreads();  // LDS is free
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) sum[i][j] += cross[i][j];
     if (parts > 1) {
         float flat[PIECES * PIECES * 16];
 #pragma unroll
@@ -532,8 +546,9 @@ __device__ __forceinline__ void stage_tile(const _Float16* rows, std::int64_t pi
     for (int step = 0; step < 2; ++step) staged[step].store(lds + step * NARROW_STEP);
 }
 
-// This wave's 32 x 32 piece of x y^T, over the 64 values of the rows of both.
-__device__ __forceinline__ void multiply_tile(const _Float16* x, const _Float16* y, int wave_i, int wave_j, float16v& sum) {
+// This wave's 32 x 32 piece of x y^T, over the 64 values of the rows of both, added to sum + cross.
+__device__ __forceinline__ void multiply_tile(const _Float16* x, const _Float16* y, int wave_i, int wave_j, float16v& sum,
+                                              float16v& cross) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -544,7 +559,7 @@ __device__ __forceinline__ void multiply_tile(const _Float16* x, const _Float16*
             b[low] = operand(y + k / 2 * NARROW_STEP, wave_j + (lane & 31), low * 4 + k % 2 * 2 + lane / 32);
         }
 #pragma unroll
-        for (int term = 0; term < 3; ++term) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[term == 2], b[term == 1], sum, 0, 0, 0);
+        for (int term = 0; term < 3; ++term) add_term(term, a, b, sum, cross);
     }
 }
 
@@ -576,7 +591,7 @@ __global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
     const int wave_i = wave / 2 * 32, wave_j = wave % 2 * 32, column = lane & 31, high = lane / 32;
     _Float16* scratch = scratches + wave * SCRATCH;
     constexpr std::int64_t PITCH = 2 * SMALL;
-    float16v gram = {};
+    float16v gram = {}, gram_cross = {};
     half4 hi[4], lo[4];
     float v[16];
     if (!m.x) stage_tile(m.b, PITCH, factor);
@@ -586,8 +601,9 @@ __global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
         } else {
             stage_tile(m.x_t + tile * SMALL * PITCH, PITCH, columns);
             __syncthreads();
-            float16v sum = {};
-            multiply_tile(factor, columns, wave_i, wave_j, sum);
+            float16v sum = {}, cross = {};
+            multiply_tile(factor, columns, wave_i, wave_j, sum, cross);
+            sum += cross;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const _Float16* step = columns + wave_i / 32 * NARROW_STEP;
@@ -615,13 +631,13 @@ __global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
             }
         }
         __syncthreads();
-        multiply_tile(rows, rows, wave_i, wave_j, gram);
+        multiply_tile(rows, rows, wave_i, wave_j, gram, gram_cross);
         __syncthreads();
     }
     if (m.final) return;
     float flat[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) flat[e] = gram[e];
+    for (int e = 0; e < 16; ++e) flat[e] = gram[e] + gram_cross[e];
     if (m.splits > 1 && !join_parts(m, 0, part, flat)) return;
     // G, symmetric, and the next B.
 #pragma unroll
@@ -629,8 +645,9 @@ __global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
     split_piece(flat, hi, lo);
     write_quads(rows + wave_i / 32 * NARROW_STEP, wave_j + column, hi, lo);
     __syncthreads();
-    float16v square = {};
-    multiply_tile(rows, rows, wave_i, wave_j, square);
+    float16v square = {}, square_cross = {};
+    multiply_tile(rows, rows, wave_i, wave_j, square, square_cross);
+    square += square_cross;
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = group.c * square[e] * UNSCALE + group.b * flat[e];
     split_piece(v, hi, lo);

@@ -262,3 +262,19 @@ def test_zeros_stay_zeros_for_the_smallest_eps():
     assert torch.equal(ops.orthogonalize(zeros, eps=2.0 ** -149), zeros)
     matrix = _matrix(40, 70, "float32", 8)
     assert torch.equal(ops.orthogonalize(matrix, eps=2.0 ** -149), ops.orthogonalize(matrix, eps=0.0))
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols,count", [(500, 500, 4), (512, 4608, 2), (1024, 4096, 2)])
+def test_errors_of_long_sums_are_those_of_float32_steps(rows, cols, count):
+    """Root mean square over matrices. Of the errors of float32 steps, those of the sums are no larger here, which round a
+    sum once for 16 products; those of a value's rounding as hi + lo are as a rule the same (2^-24 of a power of two, and
+    2^-23 at most), and what is left out, lo lo, is as a rule 2^-25 of a product. Two independent errors for one: 2^.5."""
+    ours = theirs = 0.0
+    for seed in range(count):
+        matrix = _matrix(rows, cols, "float32", seed)
+        want = _steps(matrix, torch.float64)
+        ours += float((ops.orthogonalize(matrix).cpu().double() - want).square().sum())
+        theirs += float((_steps(matrix, torch.float32).double() - want).square().sum())
+    print(f"{rows} x {cols}: {(ours / theirs) ** 0.5:.2f} times float32's error", flush=True)
+    assert ours <= 2 * theirs
