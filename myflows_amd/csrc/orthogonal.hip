@@ -655,6 +655,161 @@ __global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
     write_scratch(scratch, m.b, wave_j, wave_i, PITCH);
 }
 
+// ---- matrices of a few rows -------------------------------------------------------------------
+// A step takes X to M X and G to M G M with M = a + b G + c G G, so that the result is T X of a T that follows from the
+// first G alone. With at most 8 rows these small matrices cost nothing in 64 bits, the result is rounded once, and two launches
+// serve for all steps: the first adds up G (its trace is the norm's square), the second forms T, once a workgroup, and T X. In split
+// float16 the few errors of such a matrix do not average out: 512 x 2 was off by 8.5e-7 of it, twice the float32 steps'
+// 4.2e-7. Taken for more rows it would need sums beyond the registers.
+constexpr int THIN = 8;
+constexpr int THIN_SUMS = THIN * (THIN + 1) / 2;  // of G, on and below the diagonal
+constexpr int THIN_SPLITS = 64;                   // workgroups that share a matrix's sums
+constexpr int THIN_COLUMNS = 4 * THREADS;         // columns of T X of a workgroup, and the fewest of the sums
+
+struct Thin {
+    const void* in;
+    void* out;
+    std::int64_t in_row, in_col, out_row, out_col;  // steps along the longer side's columns and the shorter one's rows
+    float* x;      // the values, rows of `cols`: out may lie across the matrix
+    double* sums;  // THIN_SUMS a workgroup of the first launch
+    int rows, cols, splits, each;
+};
+
+struct ThinGroup {
+    Thin m[GROUP];
+    int first_block[GROUP + 1];
+    int steps;
+    float a, b, c, eps;
+};
+static_assert(sizeof(ThinGroup) <= 4096, "descriptors must fit the kernel arguments");
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void thin_sums_kernel(ThinGroup group) {
+    __shared__ double parts[THREADS / 64][THIN_SUMS];
+    const int item = item_of(group, blockIdx.x), part = blockIdx.x - group.first_block[item];
+    const Thin& m = group.m[item];
+    const T* in = static_cast<const T*>(m.in);
+    double sums[THIN_SUMS] = {};
+    const int end = min((part + 1) * m.each, m.cols);
+    for (int column = part * m.each + threadIdx.x; column < end; column += THREADS) {
+        float v[THIN];
+#pragma unroll
+        for (int i = 0; i < THIN; ++i) v[i] = i < m.rows ? static_cast<float>(in[i * m.in_row + column * m.in_col]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < THIN; ++i) {
+            if (i >= m.rows) break;
+            m.x[static_cast<std::int64_t>(i) * m.cols + column] = v[i];
+#pragma unroll
+            for (int k = 0; k <= i; ++k) sums[i * (i + 1) / 2 + k] += static_cast<double>(v[i]) * static_cast<double>(v[k]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < THIN_SUMS; ++i) {
+        if (i >= m.rows * (m.rows + 1) / 2) break;
+        const double total = wave_total(sums[i]);
+        if ((threadIdx.x & 63) == 0) parts[threadIdx.x / 64][i] = total;
+    }
+    __syncthreads();
+    if (threadIdx.x < m.rows * (m.rows + 1) / 2)
+        m.sums[part * THIN_SUMS + threadIdx.x] =
+            (parts[0][threadIdx.x] + parts[1][threadIdx.x]) + (parts[2][threadIdx.x] + parts[3][threadIdx.x]);
+}
+
+using ThinMatrix = double[THIN][THIN];
+
+// The lane's element of a product; lane 8 i + j has element (i, j).
+__device__ __forceinline__ double thin_product(const ThinMatrix& a, const ThinMatrix& b) {
+    const int i = (threadIdx.x & 63) / THIN, j = threadIdx.x % THIN;
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < THIN; ++k) sum += a[i][k] * b[k][j];
+    return sum;
+}
+__device__ __forceinline__ void set_thin(ThinMatrix& to, double v) {
+    wave_order();
+    to[(threadIdx.x & 63) / THIN][threadIdx.x % THIN] = v;
+    wave_order();
+}
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void thin_apply_kernel(ThinGroup group) {
+    static_assert(THIN * THIN == 64, "a wave has a small matrix");
+    __shared__ ThinMatrix gram, factor, applied, held;
+    const int item = item_of(group, blockIdx.x), part = blockIdx.x - group.first_block[item];
+    const Thin& m = group.m[item];
+    if (threadIdx.x < 64) {
+        const int i = threadIdx.x / THIN, j = threadIdx.x % THIN, high = max(i, j), at = high * (high + 1) / 2 + min(i, j);
+        const bool there = high < m.rows;
+        double g = 0.0;
+        if (there)
+            for (int split = 0; split < m.splits; ++split) g += m.sums[split * THIN_SUMS + at];
+        const double squares = wave_total(i == j ? g : 0.0);
+        const double scale = 1.0 / (sqrt(squares) + static_cast<double>(group.eps));
+        const double unit = there && i == j ? 1.0 : 0.0;
+        set_thin(gram, there ? g * scale * scale : 0.0);
+        set_thin(applied, unit);
+        for (int step = 0; step < group.steps; ++step) {
+            const double own = gram[i][j];
+            set_thin(factor, group.a * unit + group.b * own + group.c * thin_product(gram, gram));
+            const double next = thin_product(factor, applied);
+            set_thin(held, thin_product(factor, gram));
+            set_thin(applied, next);
+            set_thin(gram, thin_product(held, factor));
+        }
+        set_thin(applied, applied[i][j] * scale);
+    }
+    __syncthreads();
+    T* out = static_cast<T*>(m.out);
+    const int end = min((part + 1) * THIN_COLUMNS, m.cols);
+    for (int column = part * THIN_COLUMNS + threadIdx.x; column < end; column += THREADS) {
+        double v[THIN];
+#pragma unroll
+        for (int k = 0; k < THIN; ++k) v[k] = k < m.rows ? m.x[static_cast<std::int64_t>(k) * m.cols + column] : 0.0f;
+        for (int i = 0; i < m.rows; ++i) {
+            double sum = 0.0;
+#pragma unroll
+            for (int k = 0; k < THIN; ++k)
+                if (k < m.rows) sum += applied[i][k] * v[k];
+            out[i * m.out_row + column * m.out_col] = static_cast<T>(static_cast<float>(sum));
+        }
+    }
+}
+
+bool is_thin(const OrthogonalMatrix& m) { return std::min(m.rows, m.cols) <= THIN; }
+
+std::int64_t aligned(std::int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+std::int64_t thin_bytes(const OrthogonalMatrix& m) {
+    return aligned(static_cast<std::int64_t>(m.rows) * m.cols * 4) + aligned(THIN_SPLITS * THIN_SUMS * 8);
+}
+
+template <typename T>
+int run_thin(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps& o, char* workspace, hipStream_t stream) {
+    ThinGroup group{};
+    group.steps = o.steps, group.a = o.a, group.b = o.b, group.c = o.c, group.eps = o.eps;
+    for (int i = 0; i < count; ++i) {
+        const OrthogonalMatrix& from = matrices[i];
+        const bool tall = from.rows > from.cols;
+        Thin& m = group.m[i];
+        m.in = from.in, m.out = from.out;
+        m.in_row = tall ? 1 : from.in_stride, m.in_col = tall ? from.in_stride : 1;
+        m.out_row = tall ? 1 : from.out_stride, m.out_col = tall ? from.out_stride : 1;
+        m.rows = std::min(from.rows, from.cols), m.cols = std::max(from.rows, from.cols);
+        m.x = reinterpret_cast<float*>(workspace);
+        m.sums = reinterpret_cast<double*>(workspace + aligned(static_cast<std::int64_t>(m.rows) * m.cols * 4));
+        workspace += thin_bytes(from);
+        m.each = std::max((m.cols + THIN_SPLITS - 1) / THIN_SPLITS, THIN_COLUMNS);
+        m.splits = (m.cols + m.each - 1) / m.each;
+        group.first_block[i + 1] = group.first_block[i] + m.splits;
+    }
+    launch(thin_sums_kernel<T>, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
+    MFH_TRY(MFH_CHECK_LAUNCH("orthogonal thin sums", stream));
+    for (int i = 0; i < count; ++i)
+        group.first_block[i + 1] = group.first_block[i] + (group.m[i].cols + THIN_COLUMNS - 1) / THIN_COLUMNS;
+    launch(thin_apply_kernel<T>, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
+    return MFH_CHECK_LAUNCH("orthogonal thin result", stream);
+}
+
 // ---- the plan of one matrix -------------------------------------------------------------------
 // The padding allows large tiles from here on.
 int padding_of(int shorter) { return shorter >= 256 ? LARGE : SMALL; }
@@ -836,6 +991,44 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
     return OK;
 }
 
+std::int64_t group_bytes(const OrthogonalMatrix* matrices, int count) {
+    std::int64_t bytes = PARTS_BYTES;
+    for (int i = 0; i < count; ++i) bytes += Plan(matrices[i]).bytes();
+    return bytes;
+}
+
+// Groups of a list, the thin matrices apart: thin(first, count) and others(first, count) until one fails.
+template <typename Few, typename Others>
+int each_group(const OrthogonalMatrix* matrices, int count, Few&& thin, Others&& others) {
+    std::vector<OrthogonalMatrix> held(matrices, matrices + count);
+    const int first = static_cast<int>(std::stable_partition(held.begin(), held.end(), is_thin) - held.begin());
+    for (int i = 0; i < first; i += GROUP) MFH_TRY(thin(held.data() + i, std::min(GROUP, first - i)));
+    for (int i = first; i < count; i += GROUP) MFH_TRY(others(held.data() + i, std::min(GROUP, count - i)));
+    return OK;
+}
+
+std::int64_t list_bytes(const OrthogonalMatrix* matrices, int count) {
+    std::int64_t most = 0;
+    const auto thin = [&](const OrthogonalMatrix* group, int here) {
+        std::int64_t bytes = 0;
+        for (int i = 0; i < here; ++i) bytes += thin_bytes(group[i]);
+        most = std::max(most, bytes);
+        return static_cast<int>(OK);
+    };
+    each_group(matrices, count, thin, [&](const OrthogonalMatrix* group, int here) {
+        most = std::max(most, group_bytes(group, here));
+        return static_cast<int>(OK);
+    });
+    return most;
+}
+
+template <typename T>
+int run_list(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps& o, char* workspace, hipStream_t stream) {
+    return each_group(
+        matrices, count, [&](const OrthogonalMatrix* group, int here) { return run_thin<T>(group, here, o, workspace, stream); },
+        [&](const OrthogonalMatrix* group, int here) { return run_group<T>(group, here, o, workspace, stream); });
+}
+
 // ---- the optimiser's step around it -----------------------------------------------------------
 struct MomentumGroup {
     MuonTensor t[GROUP];
@@ -875,17 +1068,11 @@ __global__ __launch_bounds__(THREADS) void descend_kernel(MomentumGroup group) {
     });
 }
 
-std::int64_t group_bytes(const OrthogonalMatrix* matrices, int count) {
-    std::int64_t bytes = PARTS_BYTES;
-    for (int i = 0; i < count; ++i) bytes += Plan(matrices[i]).bytes();
-    return bytes;
-}
-
 OrthogonalMatrix direction_of(const MuonTensor& t, float* direction) {
     return {direction, direction, t.cols, t.cols, t.rows, t.cols};
 }
 
-std::int64_t direction_bytes(const MuonTensor& t) { return (static_cast<std::int64_t>(t.rows) * t.cols * 4 + 255) / 256 * 256; }
+std::int64_t direction_bytes(const MuonTensor& t) { return aligned(static_cast<std::int64_t>(t.rows) * t.cols * 4); }
 
 int run_muon_group(const MuonTensor* tensors, int count, const MuonSteps& o, char* workspace, hipStream_t stream) {
     MomentumGroup group{};
@@ -901,7 +1088,7 @@ int run_muon_group(const MuonTensor* tensors, int count, const MuonSteps& o, cha
     }
     launch(momentum_kernel, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
     MFH_TRY(MFH_CHECK_LAUNCH("muon momentum", stream));
-    MFH_TRY(run_group<float>(directions.data(), count, o.orthogonal, workspace, stream));
+    MFH_TRY(run_list<float>(directions.data(), count, o.orthogonal, workspace, stream));
     launch(descend_kernel, dim3(group.first_block[count]), dim3(THREADS), 0, stream, group);
     return MFH_CHECK_LAUNCH("muon step", stream);
 }
@@ -918,7 +1105,7 @@ std::int64_t muon_workspace(const MuonTensor* tensors, int count) {
             directions.push_back(direction_of(tensors[i + k], nullptr));
             bytes += direction_bytes(tensors[i + k]);
         }
-        most = std::max(most, bytes + group_bytes(directions.data(), here));
+        most = std::max(most, bytes + list_bytes(directions.data(), here));
     }
     return most;
 }
@@ -929,19 +1116,11 @@ int launch_muon(const MuonTensor* tensors, int count, const MuonSteps& o, void* 
     return OK;
 }
 
-std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count) {
-    std::int64_t most = 0;
-    for (int i = 0; i < count; i += GROUP) most = std::max(most, group_bytes(matrices + i, std::min(GROUP, count - i)));
-    return most;
-}
+std::int64_t orthogonal_workspace(const OrthogonalMatrix* matrices, int count) { return list_bytes(matrices, count); }
 
 int launch_orthogonal(const OrthogonalMatrix* matrices, int count, int type, const OrthogonalSteps& o, void* workspace,
                       hipStream_t stream) {
-    return with_type(type, [&](auto element) {
-        for (int i = 0; i < count; i += GROUP)
-            MFH_TRY(run_group<decltype(element)>(matrices + i, std::min(GROUP, count - i), o, static_cast<char*>(workspace), stream));
-        return static_cast<int>(OK);
-    });
+    return with_type(type, [&](auto element) { return run_list<decltype(element)>(matrices, count, o, static_cast<char*>(workspace), stream); });
 }
 
 }  // namespace mfh

@@ -17,6 +17,7 @@ import pytest
 import torch
 
 import myflows_amd as mf
+from myflows_amd import native
 from myflows_amd import orthogonal as ops
 
 TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
@@ -278,3 +279,67 @@ def test_errors_of_long_sums_are_those_of_float32_steps(rows, cols, count):
         theirs += float((_steps(matrix, torch.float32).double() - want).square().sum())
     print(f"{rows} x {cols}: {(ours / theirs) ** 0.5:.2f} times float32's error", flush=True)
     assert ours <= 2 * theirs
+
+
+EXACT = dict(coefficients=(3.4375, -4.75, 2.03125))  # float32 holds them
+THIN = [(1, 1), (1, 7), (2, 2), (512, 2), (2, 513), (8, 8), (3, 1025), (8, 3000), (5000, 7), (6, 70001), (200003, 4), (1, 1 << 20)]
+
+
+def _check_thin(got, matrix, **options):
+    """A matrix of at most 8 rows or columns is formed in 64 bits: an element is off by its rounding to float32 and to its
+    type, and by 2^-40 of the largest for 64-bit steps on both sides, whose errors are raised 500 times at most."""
+    want = _steps(matrix, torch.float64, **{**EXACT, **options})
+    info = torch.finfo(matrix.dtype)
+    half_step = info.eps / 2 + (0.0 if matrix.dtype is torch.float32 else 2.0 ** -24)
+    bound = half_step * want.abs().clamp(min=info.smallest_normal) + 2.0 ** -40 * want.abs().max()
+    assert got.dtype is matrix.dtype and got.shape == matrix.shape
+    assert bool(((got.cpu().double() - want).abs() <= bound).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", THIN)
+def test_matrices_of_a_few_rows_are_rounded_once(rows, cols, dtype):
+    print("orthogonalize", rows, cols, dtype, flush=True)
+    for spectrum in ("noise", "falling"):
+        matrix = _matrix(rows, cols, dtype, rows + cols, spectrum)
+        got = ops.orthogonalize(matrix, **EXACT)
+        _check_thin(got, matrix)
+        _check_thin(ops.orthogonalize(matrix, steps=1, **EXACT), matrix, steps=1)
+        assert torch.equal(ops.orthogonalize(matrix, **EXACT), got)
+        wide = torch.full((rows, cols + 5), 7.0, dtype=TYPES[dtype], device="cuda")
+        wide[:, 3:3 + cols] = matrix
+        assert torch.equal(ops.orthogonalize(wide[:, 3:3 + cols], **EXACT), got)
+        assert ops.orthogonalize(matrix, out=matrix, **EXACT) is matrix and torch.equal(matrix, got)
+
+
+@gpu
+def test_matrices_of_a_few_rows_among_others():
+    shapes = [(512, 2), (64, 100), (3, 70), (130, 140), (8, 9), (9, 8), (9, 9), (1, 5)] * 12
+    matrices = [_matrix(r, c, list(TYPES)[i % 3], i) for i, (r, c) in enumerate(shapes)]
+    native.stream_workspace(1, torch.float64).view(torch.int64).fill_(-1)
+    for value, to in zip(matrices, ops.orthogonalize_many(matrices, **EXACT)):
+        if min(value.shape) <= 8:
+            _check_thin(to, value)
+            assert torch.equal(ops.orthogonalize(value, **EXACT), to)
+        else:
+            _check(to, value, **EXACT)
+    held = torch.randn(5000, device="cuda")  # a result that lies across its own matrix
+    want = ops.orthogonalize(held[:4000].clone().view(4, 1000))
+    assert torch.equal(ops.orthogonalize(held[:4000].view(4, 1000), out=held[777:4777].view(4, 1000)), want)
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(1, 9), (2, 512), (700, 8)])
+def test_zeros_infinities_nan_and_sizes_of_a_few_rows(rows, cols):
+    zeros = torch.zeros((rows, cols), device="cuda")
+    assert torch.equal(ops.orthogonalize(zeros), zeros)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        matrix = torch.randn((rows, cols), device="cuda")
+        matrix[-1, -1] = bad
+        assert bool(ops.orthogonalize(matrix).isnan().all())
+    base = _matrix(rows, cols, "float32", 4)
+    want = ops.orthogonalize(base, eps=0.0)
+    for factor in (2.0 ** 100, 2.0 ** -100):
+        assert torch.equal(ops.orthogonalize(base * factor, eps=0.0), want)
+    assert bool(ops.orthogonalize(base * 2.0 ** -126, eps=0.0).isfinite().all())
