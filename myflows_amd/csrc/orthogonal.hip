@@ -6,10 +6,12 @@
 // Precision. The polynomial raises small singular values by up to a each step (485 times in five), and with them
 // whatever error the products have: in 16-bit products it would be a tenth of the result. So every matrix is held as
 // the sum of two float16 values, hi + lo, within 2^-23 of it, and a product is hi hi + (hi lo + lo hi) on the matrix
-// cores, added in float32 (the splitting of single-precision products that Ootomo and Yokota published in 2022; lo lo,
-// 2^-25 of hi hi as a rule, is left out): as near to the definition as float32 products, at three times the cost of one
-// float16 product instead of the sixteen that the matrix cores' float32 rate is below it. 1024 x 4096: the result is off by
-// 1.5e-6 of its norm; the same steps in float32 by 4.1e-6 with the library's products and by 1.4e-6 on the host.
+// cores, added in float32 (the splitting of single-precision products that Ootomo and Yokota published in 2022): as near
+// to the definition as float32 products, at three times the cost of one float16 product instead of the sixteen that the
+// matrix cores' float32 rate is below it. Of at most 64 rows, where the matrix cores are not what counts, lo lo (2^-25 of
+// a product as a rule, of one sign in G's diagonal) is added too; of at most 8 rows all is in 64 bits. Off by, of the
+// result's norm: 1024 x 4096 1.5e-6 (the same steps in float32: 4.1e-6 with the library's products, 1.4e-6 on the host);
+// 64 x 576 1.4e-6 (1.7e-6 and 1.4e-6; without lo lo 1.8e-6).
 // Values are held 2^12 times as large, which keeps hi out of float16's subnormals and lo's steps below 2^-36; float16 ends
 // at 16 times that, so a polynomial must keep X below 3.5, G's largest root, and b x^2 + c x^4, B's, below 15.9.
 //
@@ -105,13 +107,13 @@ __device__ __forceinline__ half8 operand(const _Float16* lds, int row, int part)
     return *reinterpret_cast<const half8*>(lds + row * ROW_STEP + (part ^ key_of(row)) * 8);
 }
 
-// One term of a product of two pieces, hi and lo: hi hi, added to `sum`, or hi lo or lo hi, added to `cross`. These are
+// One term of a product of two pieces, hi and lo: hi hi, added to `sum`, or hi lo, lo hi or lo lo, added to `cross`. These are
 // 2^-11 of hi hi: on their own they are added without a rounding of the whole sum each. With one sum for all three the
 // result's error was half as large again (4096 x 4096: 2.3e-6 of it for 1.3e-6, 1024 x 4096: 2.2e-6 for 1.5e-6), in
 // no less time.
 __device__ __forceinline__ void add_term(int term, const half8 (&x)[2], const half8 (&y)[2], float16v& sum, float16v& cross) {
     float16v& to = term == 0 ? sum : cross;
-    to = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[term == 2], y[term == 1], to, 0, 0, 0);
+    to = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[term / 2], y[term % 2], to, 0, 0, 0);
 }
 
 // A wave's scratch in LDS: 32 rows of a matrix as they lie in memory, 64 bytes of hi and 64 of lo each, their eight
@@ -298,6 +300,7 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
     const int begin = static_cast<int>(static_cast<long long>(p.ksteps) * part / parts);
     const int end = static_cast<int>(static_cast<long long>(p.ksteps) * (part + 1) / parts);
     float16v sum[PIECES][PIECES] = {}, cross[PIECES][PIECES] = {};
+    const bool few = p.rows <= SMALL;  // products with lo lo
     struct Operands {
         half8 x[PIECES][2], y[PIECES][2];  // hi and lo
     };
@@ -328,11 +331,13 @@ __device__ __forceinline__ void tile_product(const Product& p, int tile_i, int t
     };
     const auto multiply = [&](const Operands& o) {
 #pragma unroll
-        for (int term = 0; term < 3; ++term)
+        for (int term = 0; term < 4; ++term) {
+            if (term == 3 && (SIDE != SMALL || !few)) break;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i)
 #pragma unroll
                 for (int j = 0; j < PIECES; ++j) add_term(term, o.x[i], o.y[j], sum[i][j], cross[i][j]);
+        }
     };
     load(0, begin);
     store(0, begin);
@@ -559,7 +564,7 @@ __device__ __forceinline__ void multiply_tile(const _Float16* x, const _Float16*
             b[low] = operand(y + k / 2 * NARROW_STEP, wave_j + (lane & 31), low * 4 + k % 2 * 2 + lane / 32);
         }
 #pragma unroll
-        for (int term = 0; term < 3; ++term) add_term(term, a, b, sum, cross);
+        for (int term = 0; term < 4; ++term) add_term(term, a, b, sum, cross);
     }
 }
 
@@ -643,6 +648,9 @@ __global__ __launch_bounds__(THREADS) void narrow_kernel(NarrowGroup group) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) flat[e] *= UNSCALE;
     split_piece(flat, hi, lo);
+    // B is formed from one G, as it is held: near G = 1 the errors of b G and c G G cancel but for a fiftieth.
+#pragma unroll
+    for (int e = 0; e < 16; ++e) flat[e] = static_cast<float>(hi[e / 4][e % 4]) + static_cast<float>(lo[e / 4][e % 4]);
     write_quads(rows + wave_i / 32 * NARROW_STEP, wave_j + column, hi, lo);
     __syncthreads();
     float16v square = {}, square_cross = {};

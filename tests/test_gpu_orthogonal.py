@@ -343,3 +343,20 @@ def test_zeros_infinities_nan_and_sizes_of_a_few_rows(rows, cols):
     for factor in (2.0 ** 100, 2.0 ** -100):
         assert torch.equal(ops.orthogonalize(base * factor, eps=0.0), want)
     assert bool(ops.orthogonalize(base * 2.0 ** -126, eps=0.0).isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols,count", [(40, 70, 16), (64, 147, 8), (64, 576, 8)])
+def test_errors_of_few_rows_are_those_of_float32_steps(rows, cols, count):
+    """Root mean square over matrices. In float32 steps a value held is rounded by .58 of 2^-24 of its power of two (the
+    standard deviation of a rounding), and the sums and the polynomial's three operations add at least as much again. Here a
+    value is held as hi + lo, rounded by .87 of that (lo has 11 bits of what hi leaves), and nothing else is lost:
+    ((.87^2 + .58^2) / (2 .58^2))^.5 < 1.3."""
+    ours = theirs = 0.0
+    for seed in range(count):
+        matrix = _matrix(rows, cols, "float32", seed)
+        want = _steps(matrix, torch.float64)
+        ours += float((ops.orthogonalize(matrix).cpu().double() - want).square().sum())
+        theirs += float((_steps(matrix, torch.float32).double() - want).square().sum())
+    print(f"{rows} x {cols}: {(ours / theirs) ** 0.5:.2f} times float32's error", flush=True)
+    assert ours <= 1.3 ** 2 * theirs
