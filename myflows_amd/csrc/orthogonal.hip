@@ -857,11 +857,14 @@ struct Buffers {
 };
 
 constexpr int NARROW_SPLITS = 16;  // workgroups of a narrow matrix: the last one reads all their parts
+constexpr std::int64_t NARROW_PARTS_BYTES = NARROW_SPLITS * SMALL * SMALL * 4;
+
+bool is_narrow(const Plan& plan) { return plan.shorter <= SMALL; }
 
 template <typename T>
 int run_narrow(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps& o, const std::vector<Plan>& plans,
                const std::vector<Buffers>& buffers, char* parts, hipStream_t stream) {
-    static_assert(GROUP * NARROW_SPLITS * SMALL * SMALL * 4 <= PARTS_BYTES && GROUP <= LOGIT_COUNTERS, "parts fit their workspace");
+    static_assert(GROUP <= LOGIT_COUNTERS, "a counter a matrix");
     for (int step = 0; step <= o.steps; ++step) {  // the first G and B, then the steps
         NarrowGroup group{};
         group.a = o.a, group.b = o.b, group.c = o.c;
@@ -869,7 +872,7 @@ int run_narrow(const OrthogonalMatrix* matrices, int count, const OrthogonalStep
             Narrow& m = group.m[i];
             const Plan& plan = plans[i];
             m.x = step == 0 ? buffers[i].x : nullptr, m.x_t = buffers[i].x_t[0], m.b = buffers[i].p, m.x_pitch = plan.l * 2;
-            m.parts = reinterpret_cast<float*>(parts + static_cast<std::int64_t>(i) * NARROW_SPLITS * SMALL * SMALL * 4);
+            m.parts = reinterpret_cast<float*>(parts + static_cast<std::int64_t>(i) * NARROW_PARTS_BYTES);
             m.arrived = o.counters + i;
             if (step == o.steps) m.final = matrices[i].out, m.final_stride = matrices[i].out_stride;
             m.rows = plan.shorter, m.cols = plan.longer, m.tall = matrices[i].rows > matrices[i].cols;
@@ -912,7 +915,7 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
         sources.first_block[i + 1] = sources.first_block[i] + sources.s[i].padded_rows / 64 * (sources.s[i].padded_cols / 64);
     launch(split_kernel<T>, dim3(sources.first_block[count]), dim3(THREADS), 0, stream, sources);
     MFH_TRY(MFH_CHECK_LAUNCH("orthogonal split", stream));
-    if (std::all_of(plans.begin(), plans.end(), [](const Plan& plan) { return plan.shorter <= SMALL; }))
+    if (std::all_of(plans.begin(), plans.end(), is_narrow))
         return run_narrow<T>(matrices, count, o, plans, buffers, parts, stream);
     const int cus = device_cu_count();
     const auto products = [&](auto&& describe) {
@@ -1000,9 +1003,13 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
 }
 
 std::int64_t group_bytes(const OrthogonalMatrix* matrices, int count) {
-    std::int64_t bytes = PARTS_BYTES;
-    for (int i = 0; i < count; ++i) bytes += Plan(matrices[i]).bytes();
-    return bytes;
+    std::int64_t bytes = 0;
+    bool narrow = true;
+    for (int i = 0; i < count; ++i) {
+        const Plan plan(matrices[i]);
+        bytes += plan.bytes(), narrow = narrow && is_narrow(plan);
+    }
+    return bytes + (narrow ? count * NARROW_PARTS_BYTES : PARTS_BYTES);
 }
 
 // Groups of a list, the thin matrices apart: thin(first, count) and others(first, count) until one fails.

@@ -360,3 +360,10 @@ def test_errors_of_few_rows_are_those_of_float32_steps(rows, cols, count):
         theirs += float((_steps(matrix, torch.float32).double() - want).square().sum())
     print(f"{rows} x {cols}: {(ours / theirs) ** 0.5:.2f} times float32's error", flush=True)
     assert ours <= 1.3 ** 2 * theirs
+
+
+@gpu
+def test_small_matrices_ask_for_little_workspace():
+    assert ops._workspace(((4, 4),)) < 1 << 16 and ops._muon_workspace(((4, 4), (2, 9))) < 1 << 17
+    assert ops._workspace(((64, 576),)) < 1 << 21 and ops._workspace(((64, 576),) * 40) < 30 << 21
+    assert ops._workspace(((1, 1 << 20),)) < 5 << 20
