@@ -639,8 +639,9 @@ MFH_API int mfh_embedding(uint64_t table, int type, int64_t vocab, int dim, int6
 /* Bytes of workspace of mfh_embedding_backward, -1 when the sizes are out of range. */
 MFH_API int64_t mfh_embedding_workspace(int64_t count, int64_t vocab, int dim, int type);
 
-/* table_grad[v] (written, or added to with add) = scale * the sum of the rows grad[p] with ids[p] = v, in rising
- * order of p and float32, rounded once; grad is of `type`, table_grad (vocab x dim) of the same or float32. Tokens
+/* table_grad[v] (written, or added to with add) = scale * the sum of the rows grad[p] with ids[p] = v, in float32 and
+ * an order that is the same each time (that of p for tokens that come at most 64 times; the others' rows are summed in
+ * pieces), rounded once. The time to sort the tokens grows with vocab beyond 262144; grad is of `type`, table_grad (vocab x dim) of the same or float32. Tokens
  * outside of the table count nowhere. Every row is written; with add, rows that no token names stay as they are.
  * table_grad shares no memory with grad and ids. */
 MFH_API int mfh_embedding_backward(uint64_t grad, int type, int64_t count, int dim, int64_t grad_stride, uint64_t ids,
@@ -650,8 +651,9 @@ MFH_API int mfh_embedding_backward(uint64_t grad, int type, int64_t count, int d
 
 /* ---- orthogonal matrices --------------------------------------------------------------------- */
 
-/* One matrix of mfh_orthogonalize (at most 65536 of a call, as of mfh_muon_step's): rows x cols elements (sides of at most 2^20, at most 2^31 - 1 elements), rows of
- * contiguous elements their stride apart. out may be in; it overlaps no other matrix of the call. */
+/* One matrix of mfh_orthogonalize (at most 65536 of a call, as of mfh_muon_step's): rows x cols elements (sides of at
+ * most 2^20, at most 2^31 - 1 elements), rows of contiguous elements their stride apart. out may be in; it overlaps no
+ * other matrix of the call. */
 typedef struct mfh_orthogonal_matrix {
     uint64_t in, out;
     int64_t in_stride, out_stride;
@@ -663,7 +665,8 @@ MFH_API int64_t mfh_orthogonalize_workspace(const mfh_orthogonal_matrix* matrice
 
 /* out = the matrix M of an element type taken through `steps` (1..64) Newton-Schulz steps: with X = M / (|M| + eps)
  * (the Frobenius norm) and the shorter side as rows, X = a X + (b G + c G G) X with G = X X^T, so that each singular
- * value x becomes x (a + b x^2 + c x^4). Formed to the precision of float32 products and rounded once. The
+ * value x becomes x (a + b x^2 + c x^4). Formed to the precision of float32 products (with at most 8 rows or columns,
+ * of 64-bit ones) and rounded once. The
  * polynomial must keep the values from 0 to 1 below 3.5, and b x^2 + c x^4 below 15.9, at every step. The table is
  * host memory, read during the call. counters as of the rows of logits. No counterpart in the reference. */
 MFH_API int mfh_orthogonalize(const mfh_orthogonal_matrix* matrices, int count, int type, int steps, float a, float b, float c,

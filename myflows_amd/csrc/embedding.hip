@@ -1,11 +1,12 @@
 // Embedding: rows of a table by token, scaled, and the table's gradient by sorted tokens.
 //
 //   y[p] = scale T[id[p]]            (zeros where id[p] < 0, NaN where id[p] >= vocab)
-//   dT[v] = scale sum over p with id[p] = v of dy[p], in rising order of p, in float32
+//   dT[v] = scale sum over p with id[p] = v of dy[p], in float32
 //
-// The gradient is dense: a row that no token names is zero (or left as it is, with add). No atomics: the
-// positions are sorted by token first, then each row's are summed in their order, so a gradient has the same
-// bits every time.
+// The gradient is dense: a row that no token names is zero (or left as it is, with add). No atomics: the positions are
+// sorted by token first. The rows of a token that comes seldom are added in rising order of p; those of a frequent one
+// in pieces, and in narrow rows by lanes that share a piece, whose sums are joined in a fixed order. So a gradient has
+// the same bits every time, but not those of one running sum.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -86,7 +87,8 @@ __global__ __launch_bounds__(THREADS) void lookup_kernel(const T* __restrict__ t
 // LDS; from the sums over the tokens and waves before it, it then places those it listed in their order, lanes with
 // the same token finding one another by ballots, a token at a time. A wave whose list overflows (a token of every
 // fourth position, say) reads its ids again instead. Bound by the instructions of the walk: 65536 ids of 65536
-// tokens, 1 / k of them the k-th, 21 us (44 with two walks, 370 with neighbouring tokens in one class).
+// tokens, 1 / k of them the k-th, 21 us (44 with two walks, 370 with neighbouring tokens in one class). A class has at most 1024 tokens:
+// beyond 262144 of them there are more classes than CUs, and their walks take turns.
 struct Sorted {
     int* order;
     int* slots;

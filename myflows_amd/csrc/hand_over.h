@@ -6,8 +6,8 @@
 namespace mfh {
 
 // Values that workgroups hand to one another within a launch. A fence over the whole GPU writes back and drops an
-// XCD's cache, which took 200 us for a thousand workgroups; instead these few values are written through to the
-// memory that all XCDs share, and read from there, as relaxed atomics of that scope. That a written-through value has
+// XCD's cache, which took 200 us for a thousand workgroups; instead these values (a row's statistics, the sums of a
+// split tile) are written through to the memory that all XCDs share, and read from there, as relaxed atomics of that scope. That a written-through value has
 // reached that memory once s_waitcnt has counted its store is how gfx950 works; the language's memory model, which knows
 // fences only, does not promise it.
 template <typename V>

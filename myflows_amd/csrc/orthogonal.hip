@@ -15,7 +15,9 @@
 // Values are held 2^12 times as large, which keeps hi out of float16's subnormals and lo's steps below 2^-36; float16 ends
 // at 16 times that, so a polynomial must keep X below 3.5, G's largest root, and b x^2 + c x^4, B's, below 15.9.
 //
-// Layout. A matrix lies in memory with both sides padded to whole tiles, zeros behind the last value; a row's 32 neighbouring values are 64 bytes of
+// Layout. A matrix lies in memory with both sides padded to whole tiles. Behind the last value there are zeros up to
+// the next multiple of 64; beyond it, in the padding to 128, a small tile leaves what was there, which only reaches rows and
+// columns that are padding themselves: no product reads that far along k. A row's 32 neighbouring values are 64 bytes of
 // hi and 64 of lo, so that one step of a product reads a cache line of each row. Every product is of the form A B^T
 // with rows of both read along k: X is kept as X and as X^T. Symmetric products form the tiles on and below the
 // diagonal and write them to both places.
@@ -519,7 +521,7 @@ __global__ __launch_bounds__(THREADS) void split_kernel(SourceGroup group) {
 // With at most 64 rows, G is one tile. A workgroup takes some of X's columns through a whole step: it forms its new
 // columns from B, writes them, and adds their part of the next G; the workgroup that comes last joins the parts and forms
 // the next B. One launch a step instead of three: for such matrices the launches are what takes the time (64 x 576
-// float32 in five steps: 58 us on the GPU, 89 with the products above).
+// float32 in five steps: a call takes 68 us, 100 with the products above).
 struct Narrow {
     const _Float16* x;  // rows of X, for the first G; then null
     _Float16* x_t;      // X^T, rows of 64

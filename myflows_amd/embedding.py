@@ -82,7 +82,8 @@ def embedding_forward(table, ids, *, scale=1.0):
 
 def embedding_backward(grad, ids, vocab, *, scale=1.0, out=None, add=False):
     """The gradient (vocab, dim) of the table from that of embedding_forward's output (ids' shape, dim): scale
-    times the sum of the rows of each token, in float32 and the order of the tokens, rounded once. It is written to
+    times the sum of the rows of each token, in float32 and an order that is the same each time (that of the tokens for
+    those that come at most 64 times; the others' rows are summed in pieces), rounded once. It is written to
     (or, with add, added to) out, of grad's type or float32 with contiguous rows, which shares no memory with grad
     and ids; a row that no token names is zeros (with add, left as it is). Tokens beyond the vocabulary count nowhere."""
     flat, wide, step = _tokens(ids)

@@ -85,7 +85,8 @@ def orthogonalize_many(matrices, *, steps=STEPS, coefficients=COEFFICIENTS, eps=
 
     With X = M / (|M| + eps), |M| the Frobenius norm, a step makes X = a X + (b G + c G G) X of X X^T = G (of the
     shorter side): each singular value x becomes x (a + b x^2 + c x^4), which the default coefficients bring near 1.
-    The products are formed to float32's precision and the result is rounded once to the matrix's type; a matrix
+    The products are formed to float32's precision (with at most 8 rows or columns, to 64 bits') and the result is
+    rounded once to the matrix's type; a matrix
     of zeros stays one (for an eps above 0), and one with an infinity or NaN becomes NaN. The same call
     gives the same bits each time; which order a matrix's sums are added in may depend on the call's other matrices.
     ``out`` takes the results (each a contiguous
