@@ -932,9 +932,12 @@ int run_group(const OrthogonalMatrix* matrices, int count, const OrthogonalSteps
             describe(i, p);
             if (padding_of(plans[i].shorter) == LARGE) large_tiles += tiles_of(plans[i].shorter, plans[i].longer, p.symmetric, LARGE);
         }
-        // From 64 symmetric ones on they win split (1024 x 4096 and 4096 x 1024: 72), others from a whole round on
-        // (1999 x 517 and 771 x 1003, 136 of them: 33 us, 22 with small ones).
-        const bool use_large = large_tiles >= (group.p[0].symmetric ? 64 : 2 * cus);
+        // Whole calls with large and with small ones, us, by their number on 256 CUs. Symmetric products: 66 of 1408 x 1408
+        // 472 and 420, 80 of eight 512 x 2048 555 and 467, 100 of ten 692 and 600, 108 of three 1000 x 3000 851 and 848,
+        // 136 of 2048 x 2048 856 and 891, 210 of 2560 x 2560 1463 and 1673. Others: 196 of 896 x 3584 425 and 408, 256 of 1024 x 4096
+        // 503 and 477, 256 of 2048 x 2048 833 and 856, 320 of five 512 x 2048 381 and 384, 324 of 1152 x 4608 611 and 666,
+        // 448 of seven 512 x 2048 524 and 569, 484 of 1408 x 5632 857 and 999, 576 of 3000 x 3000 2064 and 2244.
+        const bool use_large = large_tiles >= (group.p[0].symmetric ? cus / 2 : cus + cus / 4);
         bool all_small = true;
         std::int64_t steps = 0;
         for (int i = 0; i < count; ++i) {

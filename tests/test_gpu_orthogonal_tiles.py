@@ -1,7 +1,7 @@
 """Orthogonalised matrices of sizes whose products take each of the tile kernels' ways, against the definition in 64 bits.
 
-Tiles are of 64 x 64, or of 128 x 128 where a launch has enough of them (64 of a symmetric product, twice the CUs of
-another one, of matrices of at least 256 rows and columns); the steps of few tiles, or of those of a last short round,
+Tiles are of 64 x 64, or of 128 x 128 where a launch has enough of them (half as many as CUs of a symmetric product, five
+quarters of them of another one, of matrices of at least 256 rows and columns); the steps of few tiles, or of those of a last short round,
 are split over workgroups. What each list takes below is worked out for 256 CUs.
 
 The bound is that of the other sizes: 4 times the error of the same steps in float32, 2^-20 of the result, and half a step
@@ -20,8 +20,10 @@ TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.
 RESNET18 = ([(64, 147)] + [(64, 576)] * 4 + [(128, 576)] + [(128, 1152)] * 3 + [(128, 64), (256, 1152)] + [(256, 2304)] * 3 +
             [(256, 128), (512, 2304)] + [(512, 4608)] * 3 + [(512, 256), (512, 2)])
 LISTS = {
-    # G and B of 78 large tiles, split; B X of 529 small ones
+    # G and B of 276 small tiles, split; B X of 529 small ones
     "square": [(1425, 1425)],
+    # G and B of 171 small tiles, split; B X of 324 large ones, less than a round
+    "part_round": [(1152, 4608)],
     # G and B of 210 small tiles, split; B X of 530 large ones, a whole round and 18 that are split
     "wide": [(1217, 6700)],
     "tall": [(6700, 1217)],
@@ -33,9 +35,9 @@ LISTS = {
     "large_rounds": [(4100, 4100)],
     # B X of 821 tiles of both sizes in two rounds, none split
     "network": RESNET18,
-    # G and B of 103 tiles of both sizes, some split
-    "both_sizes": [(1425, 1425), (200, 3000), (70, 90), (90, 70), (300, 290)],
-    # exactly one round of large tiles
+    # G and B of 178 tiles of both sizes, some split
+    "both_sizes": [(2100, 2100), (200, 3000), (70, 90), (90, 70), (300, 290)],
+    # B X of exactly one round of large tiles
     "one_round": [(1024, 4096), (4096, 1024)],
 }
 
@@ -107,7 +109,7 @@ def test_strided_matrices_and_their_neighbours(name):
 
 
 def test_captured_graphs_side_by_side():
-    lists = [_matrices(LISTS[name], "float32", 3) for name in ("wide", "square")]
+    lists = [_matrices(LISTS[name], "float32", 3) for name in ("wide", "two_sizes")]
     alone = [ops.orthogonalize_many(matrices) for matrices in lists]
     torch.cuda.synchronize()
     graphs, held = [], []
