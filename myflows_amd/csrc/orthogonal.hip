@@ -11,7 +11,7 @@
 // matrix cores' float32 rate is below it. Of at most 64 rows, where the matrix cores are not what counts, lo lo (2^-25 of
 // a product as a rule, of one sign in G's diagonal) is added too; of at most 8 rows all is in 64 bits. Off by, of the
 // result's norm: 1024 x 4096 1.5e-6 (the same steps in float32: 4.1e-6 with the library's products, 1.4e-6 on the host);
-// 64 x 576 1.4e-6 (1.7e-6 and 1.4e-6; without lo lo 1.8e-6).
+// 64 x 576 of normal values 1.4e-6 (1.7e-6 and 1.4e-6; without lo lo 1.8e-6).
 // Values are held 2^12 times as large, which keeps hi out of float16's subnormals and lo's steps below 2^-36; float16 ends
 // at 16 times that, so a polynomial must keep X below 3.5, G's largest root, and b x^2 + c x^4, B's, below 15.9.
 //
