@@ -161,3 +161,25 @@ def test_overlap_is_that_of_the_tensors_given_not_of_their_copies():
     orthogonal.muon_update_many([(left, one, momentum[:, :6], 0.1, 0.0), (right, one, momentum[:, 6:], 0.1, 0.0)])
     orthogonal.muon_update_many([(p, one, b, 0.1, 0.0) for p, b in twins])
     assert torch.equal(alike, torch.cat([p for p, _ in twins], 1)) and torch.equal(momentum, torch.cat([b for _, b in twins], 1))
+
+
+@gpu
+def test_a_head_of_two_outputs_in_recorded_and_captured_steps():
+    mf.set_device("cuda")
+    results = []
+    for kind in (None, mf.RecordedStep, mf.CapturedStep):
+        hidden = mf.Dense(40, 70, activation=mf.ReLU, initializer=mf.make_initializer(seed=1))
+        head = mf.Dense(70, 2, initializer=mf.make_initializer(seed=2))  # a matrix of two columns beside one of 40 rows
+        x = mf.Variable(torch.zeros((30, 40), device="cuda"), requires_grad=False)
+        target = mf.Variable(torch.ones((30, 2), device="cuda"), requires_grad=False)
+        optimizer = mf.Muon(mf.Graph(mf.MSELoss(head(hidden(x)), target)), 0.02)
+        step = optimizer if kind is None else kind(optimizer)
+        for seed in range(5):
+            x.value.copy_(torch.randn((30, 40), generator=torch.Generator().manual_seed(seed)))
+            step.one_step()
+            step.update()
+            torch.cuda.synchronize()
+        assert set(optimizer.buffers) == {hidden.W, head.W}
+        results.append([p.value.clone() for p in (hidden.W, head.W, hidden.b, head.b)])
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))

@@ -367,3 +367,26 @@ def test_small_matrices_ask_for_little_workspace():
     assert ops._workspace(((4, 4),)) < 1 << 16 and ops._muon_workspace(((4, 4), (2, 9))) < 1 << 17
     assert ops._workspace(((64, 576),)) < 1 << 21 and ops._workspace(((64, 576),) * 40) < 30 << 21
     assert ops._workspace(((1, 1 << 20),)) < 5 << 20
+
+
+@gpu
+def test_few_rows_on_two_streams_and_in_graphs():
+    lists = [[_matrix(2, 3000, "float32", 1), _matrix(90, 80, "float32", 2)], [_matrix(70001, 5, "float32", 3)]]
+    alone = [ops.orthogonalize_many(matrices) for matrices in lists]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in lists]
+    graphs, held = [], []
+    for matrices in lists:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(ops.orthogonalize_many(matrices))
+        graphs.append(graph)
+    for _ in range(4):
+        eager = []
+        for stream, graph, matrices in zip(streams, graphs, lists):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                eager.append(ops.orthogonalize_many(matrices))
+        torch.cuda.synchronize()
+        for got, want in zip([*held, *eager], [*alone, *alone]):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
